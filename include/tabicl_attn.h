@@ -369,6 +369,61 @@ int tabicl_icl_cache_append(void* k_cache, void* v_cache, int64_t dst_sn, int64_
                             int64_t T, int64_t D, int32_t dtype, void* stream);
 
 /*
+ * Paged K/V cache: sequences of different lengths share one pool of pages. No counterpart in the reference, whose cache
+ * is one padded tensor per block.
+ *
+ * Pool of one block: k_pages, v_pages [pages, H, page_rows, D] (element stride page_sp between pages, a multiple of
+ * 16 bytes; the rest contiguous), page_rows a power of two >= 16, D in {32, 64, 128}. table [N, max_pages] int32 (row
+ * stride table_sn): row i of sequence n is row i % page_rows of page table[n, i / page_rows]. A page id outside
+ * [0, pages) holds no rows: they are neither read nor written, and no query attends to them. lengths [N] int32,
+ * clamped to [0, max_pages * page_rows]. All on the device; nothing is read back.
+ */
+
+/*
+ * Attention of q [N, Hq, Tq, D] over the first lengths[n] rows of each sequence, query head h over K/V head
+ * h / (Hq / H): softmax(scale q k^T) v in fp32 (bf16 probabilities are not rounded to bf16), written to out (element
+ * strides, contiguous last dim). Rows without a key, or whose every score is -inf, are 0. weights (or NULL): fp32
+ * [N, max_pages * page_rows] (row stride weights_sn), the probabilities summed over the query heads and rows are added
+ * to the first lengths[n] entries; the sums' order is fixed. For one query row to a few hundred.
+ * ws: tabicl_paged_attn_workspace_bytes(...) bytes, 16-byte aligned.
+ */
+int tabicl_paged_attn(const void* q, const void* k_pages, const void* v_pages, int64_t pages, int64_t page_sp,
+                      int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths,
+                      float* weights, int64_t weights_sn, void* out, int64_t N, int64_t Hq, int64_t H, int64_t Tq,
+                      int64_t D, int64_t q_sn, int64_t q_sh, int64_t q_st, int64_t o_sn, int64_t o_sh, int64_t o_st,
+                      float scale, int32_t dtype, void* ws, int64_t ws_bytes, void* stream);
+/* Workspace of tabicl_paged_attn for sequences of up to `rows` rows (max_pages * page_rows); <0 on bad arguments. */
+int64_t tabicl_paged_attn_workspace_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows,
+                                          int32_t with_weights, int32_t dtype);
+
+/*
+ * Writes rows t < count[n] (NULL: all T) of k, v [N, H, T, D] (element strides, contiguous last dim) to rows
+ * lengths[n] + t of each sequence; rows at or past max_pages * page_rows are dropped. lengths stays as it is (the
+ * other blocks append at the same rows). Two sequences must not share a page that is written.
+ */
+int tabicl_paged_append(void* k_pages, void* v_pages, int64_t pages, int64_t page_sp, int64_t page_rows,
+                        const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const void* k,
+                        const void* v, const int32_t* count, int64_t N, int64_t H, int64_t T, int64_t D, int64_t k_sn,
+                        int64_t k_sh, int64_t k_st, int64_t v_sn, int64_t v_sh, int64_t v_st, int32_t dtype, void* stream);
+
+/*
+ * Cuts each sequence to kept = min(lengths[n], keep) rows, keep = keep_n[n] (device, or NULL: keep_all), clamped to
+ * [0, K]. Kept are its last min(recent, kept) rows and, of the rows before them, those of the largest weights
+ * (ties: the lower row; NaN counts as -inf). Kept rows at or past `kept` move, in order, to the places below it whose
+ * rows are not kept, in order; no other row moves. All blocks (element stride block_sp) move alike. Written:
+ * index [N, K] (slot j holds the old row index[n, j]; -1 from kept on), kept_weights [N, max_pages * page_rows]
+ * (weights of the kept rows in their slots, 0 after), kept_lengths [N]. weights, table and lengths stay as they are.
+ * No two sequences may share a page. ws: tabicl_paged_evict_workspace_bytes(N, K) bytes, 16-byte aligned.
+ */
+int tabicl_paged_evict(void* k_pages, void* v_pages, int64_t blocks, int64_t block_sp, int64_t pages, int64_t page_sp,
+                       int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages,
+                       const int32_t* lengths, const float* weights, int64_t weights_sn, const int32_t* keep_n,
+                       int64_t keep_all, int64_t recent, int32_t* index, int64_t K, float* kept_weights,
+                       int32_t* kept_lengths, int64_t N, int64_t H, int64_t D, int32_t dtype, void* ws, int64_t ws_bytes,
+                       void* stream);
+int64_t tabicl_paged_evict_workspace_bytes(int64_t N, int64_t K);
+
+/*
  * Shape predicate, mirroring supported / hxq_supported / packed_supported
  * (reference scripts/tabicl_tpu_pallas_attn.py:319-320, 715-719, 762-764). Returns 1 if the op
  * accepts the shape, 0 otherwise. Lq/Lk are query/key lengths, E the merged width (ICL: head dim).

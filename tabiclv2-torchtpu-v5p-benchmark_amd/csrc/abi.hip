@@ -7,6 +7,7 @@
 #include "../../include/tabicl_attn.h"
 #include "common.h"
 #include "launch.h"
+#include "paged.h"
 
 namespace {
 
@@ -703,4 +704,168 @@ int tabicl_column_embed(const float* x, const int64_t* real_features, const void
   return launch_status(tabicl_launch_column_embed(x, real_features, weight, bias, out, B, T, H, reserve, skip, dtype,
                                                   (hipStream_t)stream),
                        "column_embed");
+}
+
+namespace {
+
+constexpr int64_t PAGED_MAX_ROWS = 1LL << 30;  // rows of a sequence: row numbers and their sums stay in 32 bits
+
+// The pool part of the paged entry points' arguments, checked and packed (status 0 or 1 with the message set).
+int paged_pool(const char* op, PagedPool* c, const void* k_pages, const void* v_pages, int64_t pages, int64_t page_sp,
+               int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths,
+               int64_t N, int64_t H, int64_t D, int32_t dtype) {
+  if (dtype != TABICL_DTYPE_BF16 && dtype != TABICL_DTYPE_F32) return fail(1, "%s: dtype code %d not supported", op, dtype);
+  if (D != 32 && D != 64 && D != 128) return fail(1, "%s: head dim must be 32, 64 or 128, got %lld", op, (long long)D);
+  if (page_rows < 16 || page_rows > (1 << 20) || (page_rows & (page_rows - 1)))
+    return fail(1, "%s: page_rows must be a power of two from 16 to 2^20, got %lld", op, (long long)page_rows);
+  if (N < 0 || N > 65535 || H < 1 || H > 1024) return fail(1, "%s: needs 0 <= N <= 65535 and 1 <= H <= 1024", op);
+  if (pages < 0 || pages > 0x7fffffffLL || max_pages < 0 || max_pages * page_rows > PAGED_MAX_ROWS || table_sn < 0 ||
+      max_pages > PAGED_MAX_ROWS)
+    return fail(1, "%s: bad page counts (pages %lld, max_pages %lld)", op, (long long)pages, (long long)max_pages);
+  if (page_sp < H * page_rows * D || !stride_ok(page_sp, dtype) || (pages && page_sp > (1LL << 60) / pages))
+    return fail(1, "%s: the page stride must be a multiple of 16 bytes and at least H * page_rows * D", op);
+  if (N > 0 && (!lengths || (max_pages > 0 && !table))) return fail(1, "%s: table and lengths are required", op);
+  if (!aligned16(k_pages) || !aligned16(v_pages)) return fail(1, "%s: pools must be 16-byte aligned", op);
+  if (pages > 0 && (!k_pages || !v_pages)) return fail(1, "%s: pools are required", op);
+  c->k = (void*)k_pages;
+  c->v = (void*)v_pages;
+  c->pages = pages;
+  c->page_sp = page_sp;
+  c->H = (int)H;
+  c->D = (int)D;
+  c->shift = __builtin_ctzll((unsigned long long)page_rows);
+  c->table = table;
+  c->table_sn = table_sn;
+  c->max_pages = (int)max_pages;
+  c->lengths = lengths;
+  return 0;
+}
+
+int paged_attn_sizes(const char* op, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows) {
+  if (N < 0 || N > 65535 || H < 1 || H > 1024 || Hq < 1 || Hq > 1024 || Hq % H || Tq < 0 || rows < 0 ||
+      rows > PAGED_MAX_ROWS || (D != 32 && D != 64 && D != 128))
+    return fail(1, "%s: bad sizes N=%lld Hq=%lld H=%lld Tq=%lld D=%lld rows=%lld (Hq must be a multiple of H)", op,
+                (long long)N, (long long)Hq, (long long)H, (long long)Tq, (long long)D, (long long)rows);
+  if (Tq > (1LL << 22) || N * Hq * Tq > (1LL << 22)) return fail(1, "%s: more than 2^22 query rows", op);
+  return 0;
+}
+
+}  // namespace
+
+int64_t tabicl_paged_attn_workspace_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows,
+                                          int32_t with_weights, int32_t dtype) {
+  if (dtype != TABICL_DTYPE_BF16 && dtype != TABICL_DTYPE_F32)
+    return -fail(1, "paged_attn_workspace_bytes: dtype code %d not supported", dtype);
+  if (int st = paged_attn_sizes("paged_attn_workspace_bytes", N, Hq, H, Tq, D, rows)) return -st;
+  if (N == 0 || Tq == 0) return 0;
+  return tabicl_launch_paged_attn_ws_bytes(N, Hq, H, Tq, D, rows, with_weights, dtype);
+}
+
+int tabicl_paged_attn(const void* q, const void* k_pages, const void* v_pages, int64_t pages, int64_t page_sp,
+                      int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths,
+                      float* weights, int64_t weights_sn, void* out, int64_t N, int64_t Hq, int64_t H, int64_t Tq,
+                      int64_t D, int64_t q_sn, int64_t q_sh, int64_t q_st, int64_t o_sn, int64_t o_sh, int64_t o_st,
+                      float scale, int32_t dtype, void* ws, int64_t ws_bytes, void* stream) {
+  PagedAttn a = {};
+  int st = paged_pool("paged_attn", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+                      lengths, N, H, D, dtype);
+  if (st) return st;
+  st = paged_attn_sizes("paged_attn", N, Hq, H, Tq, D, max_pages * page_rows);
+  if (st) return st;
+  if (N == 0 || Tq == 0) return 0;
+  if (!q || !out || !aligned16(q) || !aligned16(out)) return fail(1, "paged_attn: q and out must be 16-byte aligned");
+  const int64_t s[6] = {q_sn, q_sh, q_st, o_sn, o_sh, o_st};
+  for (int i = 0; i < 6; ++i)
+    if (s[i] < 0 || !stride_ok(s[i], dtype))
+      return fail(1, "paged_attn: strides must be non-negative multiples of 16 bytes");
+  if (!(scale > -1e30f && scale < 1e30f)) return fail(1, "paged_attn: scale must be finite");
+  if (weights && (((uintptr_t)weights & 3) || weights_sn < max_pages * page_rows))
+    return fail(1, "paged_attn: weights needs rows of max_pages * page_rows values");
+  const int64_t need = tabicl_launch_paged_attn_ws_bytes(N, Hq, H, Tq, D, max_pages * page_rows, weights != nullptr, dtype);
+  if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need))
+    return fail(1, "paged_attn: workspace of %lld bytes (16-byte aligned) required", (long long)need);
+  a.q = q;
+  a.q_sn = q_sn;
+  a.q_sh = q_sh;
+  a.q_st = q_st;
+  a.out = out;
+  a.o_sn = o_sn;
+  a.o_sh = o_sh;
+  a.o_st = o_st;
+  a.weights = weights;
+  a.weights_sn = weights_sn;
+  a.N = (int)N;
+  a.Hq = (int)Hq;
+  a.Tq = (int)Tq;
+  a.scale = scale;
+  return launch_status(tabicl_launch_paged_attn(a, dtype, ws, (hipStream_t)stream), "paged_attn");
+}
+
+int tabicl_paged_append(void* k_pages, void* v_pages, int64_t pages, int64_t page_sp, int64_t page_rows,
+                        const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const void* k,
+                        const void* v, const int32_t* count, int64_t N, int64_t H, int64_t T, int64_t D, int64_t k_sn,
+                        int64_t k_sh, int64_t k_st, int64_t v_sn, int64_t v_sh, int64_t v_st, int32_t dtype, void* stream) {
+  PagedAppend a = {};
+  int st = paged_pool("paged_append", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+                      lengths, N, H, D, dtype);
+  if (st) return st;
+  if (T < 0 || T > PAGED_MAX_ROWS) return fail(1, "paged_append: bad row count %lld", (long long)T);
+  if (N == 0 || T == 0) return 0;
+  if (!k || !v || !aligned16(k) || !aligned16(v)) return fail(1, "paged_append: k and v must be 16-byte aligned");
+  const int64_t s[6] = {k_sn, k_sh, k_st, v_sn, v_sh, v_st};
+  for (int i = 0; i < 6; ++i)
+    if (s[i] < 0 || !stride_ok(s[i], dtype))
+      return fail(1, "paged_append: strides must be non-negative multiples of 16 bytes");
+  a.k = k;
+  a.v = v;
+  a.k_sn = k_sn;
+  a.k_sh = k_sh;
+  a.k_st = k_st;
+  a.v_sn = v_sn;
+  a.v_sh = v_sh;
+  a.v_st = v_st;
+  a.count = count;
+  a.N = (int)N;
+  a.T = (int)T;
+  return launch_status(tabicl_launch_paged_append(a, dtype, (hipStream_t)stream), "paged_append");
+}
+
+int64_t tabicl_paged_evict_workspace_bytes(int64_t N, int64_t K) {
+  if (N < 0 || N > 65535 || K < 0 || K > PAGED_MAX_ROWS) return -fail(1, "paged_evict_workspace_bytes: bad sizes");
+  return tabicl_launch_paged_evict_ws_bytes(N, K);
+}
+
+int tabicl_paged_evict(void* k_pages, void* v_pages, int64_t blocks, int64_t block_sp, int64_t pages, int64_t page_sp,
+                       int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages,
+                       const int32_t* lengths, const float* weights, int64_t weights_sn, const int32_t* keep_n,
+                       int64_t keep_all, int64_t recent, int32_t* index, int64_t K, float* kept_weights,
+                       int32_t* kept_lengths, int64_t N, int64_t H, int64_t D, int32_t dtype, void* ws, int64_t ws_bytes,
+                       void* stream) {
+  PagedEvict a = {};
+  int st = paged_pool("paged_evict", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+                      lengths, N, H, D, dtype);
+  if (st) return st;
+  const int64_t cap = max_pages * page_rows;
+  if (blocks < 0 || blocks > 65535 || block_sp < 0 || !stride_ok(block_sp, dtype))
+    return fail(1, "paged_evict: bad block count or stride");
+  if (recent < 0 || keep_all < 0 || K < 0 || K > cap) return fail(1, "paged_evict: needs recent, keep >= 0 and 0 <= K <= the capacity %lld", (long long)cap);
+  if (N == 0) return 0;
+  if (!kept_lengths || (K > 0 && !index) || (cap > 0 && (!weights || !kept_weights)) || weights_sn < cap)
+    return fail(1, "paged_evict: weights and kept_weights need rows of max_pages * page_rows values");
+  if (N * K > 0 && (!ws || !aligned16(ws) || ws_bytes < tabicl_launch_paged_evict_ws_bytes(N, K)))
+    return fail(1, "paged_evict: workspace of %lld bytes (16-byte aligned) required",
+                (long long)tabicl_launch_paged_evict_ws_bytes(N, K));
+  a.blocks = blocks;
+  a.block_sp = block_sp;
+  a.weights = weights;
+  a.weights_sn = weights_sn;
+  a.keep = keep_n;
+  a.keep_all = (int)(keep_all < K ? keep_all : K);
+  a.recent = (int)(recent < cap ? recent : cap);
+  a.index = index;
+  a.K = (int)K;
+  a.kept_weights = kept_weights;
+  a.kept_lengths = kept_lengths;
+  a.N = (int)N;
+  return launch_status(tabicl_launch_paged_evict(a, dtype, ws, (hipStream_t)stream), "paged_evict");
 }

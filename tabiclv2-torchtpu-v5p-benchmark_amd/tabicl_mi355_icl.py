@@ -457,7 +457,11 @@ class IclKVCache:
         into heads and written to rows [row0, row0 + T) of the block. One GEMM [E T, width] x [width,
         2 width] (torch / hipBLASLt) produces K|V interleaved per row; the append kernel reads the heads
         out of it through strides, so no permuted copy is made."""
-        E, NB, H, cap, D = self.keys.shape
+        self.append(block, *self._project_kv(x, in_proj_weight, in_proj_bias), row0)
+
+    def _project_kv(self, x: Tensor, in_proj_weight: Tensor, in_proj_bias: Optional[Tensor]):
+        """The head-split K and V [E, H, T, D] of rows x in the cache's dtype, views of one projection's output."""
+        E, NB, H, cap, D = self.shape
         width = H * D
         if x.dim() != 3 or x.shape[0] != E or x.shape[2] != width:
             raise ValueError(f"append_projected expects x [{E}, T, {width}], got {tuple(x.shape)}")
@@ -466,12 +470,11 @@ class IclKVCache:
         if in_proj_bias is not None and tuple(in_proj_bias.shape) != (3 * width,):
             raise ValueError(f"in_proj_bias must be [{3 * width}], got {tuple(in_proj_bias.shape)}")
         _nat.require_device(x, in_proj_weight)
-        T = x.shape[1]
         kv = F.linear(x, in_proj_weight[width:], None if in_proj_bias is None else in_proj_bias[width:])
         if kv.dtype != self.keys.dtype:
             kv = kv.to(self.keys.dtype)  # the reference stores k_l.to(cache_dtype) (tabicl_tpu_bucketed.py:676, 688)
-        kv = kv.view(E, T, 2, H, D)
-        self.append(block, kv[:, :, 0].permute(0, 2, 1, 3), kv[:, :, 1].permute(0, 2, 1, 3), row0)
+        kv = kv.view(E, x.shape[1], 2, H, D)
+        return kv[:, :, 0].permute(0, 2, 1, 3), kv[:, :, 1].permute(0, 2, 1, 3)
 
     def attention_layer(self, block: int, x: Tensor, in_proj_weight: Tensor, in_proj_bias: Optional[Tensor],
                         out_proj_weight: Tensor, out_proj_bias: Optional[Tensor],
@@ -485,7 +488,7 @@ class IclKVCache:
         (diff:314-317), heads merged and the
         out-projection applied (diff:383-393). Returns [E, Tq, width] in the promoted dtype; the residual and the
         feed-forward part of the block stay with the caller."""
-        E, NB, H, cap, D = self.keys.shape
+        E, NB, H, cap, D = self.shape
         width = H * D
         if x.dim() != 3 or x.shape[0] != E or x.shape[2] != width:
             raise ValueError(f"attention_layer expects x [{E}, Tq, {width}], got {tuple(x.shape)}")
@@ -511,11 +514,11 @@ class IclKVCache:
         blocks: one IclBlockWeights per cache block, in order. The GEMMs run in the weights' dtype (bf16
         weights: the reference's bf16 autocast of the ICL stage) and the residual stream keeps x's dtype.
         q_transform (RoPE / SSMax on q: upstream modules) is applied to every block's head-split q."""
-        if len(blocks) > self.keys.shape[1]:
-            raise ValueError(f"{len(blocks)} blocks of weights for a cache of {self.keys.shape[1]} blocks")
+        if len(blocks) > self.shape[1]:
+            raise ValueError(f"{len(blocks)} blocks of weights for a cache of {self.shape[1]} blocks")
         # the fused layers read their operands through pointers: any other x or cache goes to attention_layer, which
         # refuses what does not fit
-        E, _, H, _, D = self.keys.shape
+        E, _, H, _, D = self.shape
         fits = self.keys.dtype == torch.bfloat16 and H * D == 512 and x.dim() == 3 and x.shape[0] == E
         for b, w in enumerate(blocks):
             if fits and _linear_native(x, w, activation):
@@ -531,7 +534,7 @@ class IclKVCache:
         """One block of query_blocks on the library's fused linear layers (tabicl_ln_linear,
         tabicl_linear_residual): the same layer with the projections' sums kept in fp32 up to the residual
         stream and the GELU."""
-        E, NB, H, cap, D = self.keys.shape
+        E, NB, H, cap, D = self.shape
         Tq, width = x.shape[1], H * D
         q = _ln_linear(x, w.ln1_w, w.ln1_b, w.eps, w.in_w, w.in_b, False, width)  # the q rows of the in-projection
         q = q.view(E, Tq, H, D).transpose(1, 2)

@@ -75,6 +75,14 @@ SIGNATURES = {
     "tabicl_icl_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i32],
     "tabicl_icl_cache_append": [_c_p, _c_p, _i64, _i64, _i64, _i64, _c_p, _c_p, _i64, _i64, _i64, _i64, _i64,
                                 _i64, _i64, _i32, _c_p],
+    "tabicl_paged_attn": [_c_p] * 3 + [_i64] * 3 + [_c_p, _i64, _i64, _c_p, _c_p, _i64, _c_p] + [_i64] * 11
+                         + [_f32, _i32, _c_p, _i64, _c_p],
+    "tabicl_paged_attn_workspace_bytes": [_i64] * 6 + [_i32] * 2,
+    "tabicl_paged_append": [_c_p] * 2 + [_i64] * 3 + [_c_p, _i64, _i64, _c_p, _c_p, _c_p, _c_p] + [_i64] * 10
+                           + [_i32, _c_p],
+    "tabicl_paged_evict": [_c_p] * 2 + [_i64] * 5 + [_c_p, _i64, _i64, _c_p, _c_p, _i64, _c_p, _i64, _i64, _c_p, _i64,
+                                                     _c_p, _c_p, _i64, _i64, _i64, _i32, _c_p, _i64, _c_p],
+    "tabicl_paged_evict_workspace_bytes": [_i64] * 2,
     "tabicl_attn_supported": [_i32, _i64, _i64, _i64, _i32, _i32],
     "tabicl_attn_last_error": [],
     "tabicl_attn_version": [],
@@ -83,7 +91,8 @@ _RESTYPES = {"tabicl_attn_last_error": ctypes.c_char_p, "tabicl_attn_version": c
              "tabicl_icl_workspace_bytes": ctypes.c_int64, "tabicl_hxq_workspace_bytes": ctypes.c_int64,
              "tabicl_smallhead_bwd_workspace_bytes": ctypes.c_int64, "tabicl_hxf_workspace_bytes": ctypes.c_int64,
              "tabicl_icl_noalloc_scratch_bytes": ctypes.c_int64, "tabicl_icl_bwd_workspace_bytes": ctypes.c_int64,
-             "tabicl_layer_workspace_bytes": ctypes.c_int64}
+             "tabicl_layer_workspace_bytes": ctypes.c_int64, "tabicl_paged_attn_workspace_bytes": ctypes.c_int64,
+             "tabicl_paged_evict_workspace_bytes": ctypes.c_int64}
 
 
 class NativeLibraryError(RuntimeError):

@@ -1,0 +1,495 @@
+"""A paged K/V cache of the ICL stage on MI355X: tables of different sizes share one pool of pages, a test row or a few
+attend over the cached train rows of their table, and a cache over its budget keeps the rows the queries attended to.
+
+IclKVCache (tabicl_mi355_icl.py) gives every estimator of a cache the same capacity; a service that holds many tables at
+once, that gets its train rows over time or answers one test row at a time keeps them here instead:
+  * paged_attention(q, k_pages, v_pages, table, lengths, weights) (op tabicl::paged_attn): attention of few query rows
+    over the cached rows, optionally adding up the attention weight that each cached row drew;
+  * paged_append (op tabicl::paged_append): new rows into the pages;
+  * paged_evict (op tabicl::paged_evict): cuts sequences to their rows of largest weight, in place;
+  * PagedIclKVCache: the pool, the page table and the lengths, with the surface of IclKVCache (append, query,
+    attention_layer, query_blocks, usable as cached_query's icl_cache), and evict.
+
+A pool is [pages, H, page_rows, D] per block for K and V (bf16 or fp32, head dim 32, 64 or 128, page_rows a power of two
+from 16 on): a (page, head) is page_rows contiguous rows. Row i of sequence n is row i % page_rows of page
+table[n, i // page_rows]; table and lengths are int32 on the GPU and never read back, so a call can be captured in a
+graph. A page id outside the pool holds no rows. The order of a sequence's rows carries no meaning (a train row's
+position is not part of its key), which is what lets eviction fill the places of evicted rows with rows from the end.
+No counterpart in the reference, whose cache is one padded tensor per block (scripts/tabicl_tpu_bucketed.py:413-435)."""
+from __future__ import annotations
+
+from typing import Optional, Sequence, Union
+
+import torch
+from torch import Tensor
+
+import tabicl_mi355_icl as _icl
+import tabicl_mi355_native as _nat
+
+
+def _rows16(t: Tensor) -> Tensor:
+    """t when its last dim is contiguous and it starts, and its other dims step, in multiples of 16 bytes (what the
+    kernels' loads need), else a contiguous copy."""
+    es = t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+            t.shape[i] == 1 or t.stride(i) * es % 16 == 0 for i in range(t.dim() - 1)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _steps(t: Tensor):
+    """(n, h, row) element strides of a [N, H, T, D] view; 0 for a dim of one entry, whose stride says nothing."""
+    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(3))
+
+
+def _check_pool(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor) -> None:
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+        raise ValueError(f"k_pages and v_pages must be [pages, H, page_rows, D] of one layout, got {tuple(k_pages.shape)} "
+                         f"and {tuple(v_pages.shape)}")
+    P, H, R, D = k_pages.shape
+    if P > 0 and (k_pages.stride(3) != 1 or k_pages.stride(2) != D or (H > 1 and k_pages.stride(1) != R * D)):
+        raise ValueError("a page [H, page_rows, D] must be contiguous")
+    if k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must share a dtype")
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be an int32 [N, max_pages] tensor with contiguous rows")
+    if lengths.dtype != torch.int32 or lengths.shape != (table.shape[0],) or not lengths.is_contiguous():
+        raise ValueError(f"lengths must be a contiguous int32 tensor of {table.shape[0]} entries")
+    if any(t.device != k_pages.device for t in (v_pages, table, lengths)):
+        raise ValueError("the pool, table and lengths must be on one device")
+
+
+def _pool_args(k_pages: Tensor, table: Tensor):
+    """(pages, page stride, page_rows, table, table stride, max_pages) as the entry points take them."""
+    P, H, R, D = k_pages.shape
+    return (P, k_pages.stride(0) if P > 1 else H * R * D, R, table.data_ptr(),
+            table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1])
+
+
+def _check_weights(weights: Tensor, table: Tensor, R: int, what: str) -> None:
+    if weights.dtype != torch.float32 or weights.dim() != 2 or weights.shape[0] != table.shape[0] \
+            or weights.shape[1] < table.shape[1] * R or (weights.shape[1] > 1 and weights.stride(1) != 1) \
+            or weights.device != table.device:
+        raise ValueError(f"{what} must be a float32 [{table.shape[0]}, >= {table.shape[1] * R}] tensor with contiguous "
+                         f"rows on the table's device, got {weights.dtype} {tuple(weights.shape)}")
+
+
+class _On:
+    """Launches on a tensor's device: a HIP launch goes by the current one."""
+
+    def __init__(self, t: Tensor):
+        self.guard = None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+_WS_BYTES: dict = {}
+
+
+def _attn_launch(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Optional[Tensor],
+                 scale: float, out: Tensor) -> None:
+    _check_pool(k_pages, v_pages, table, lengths)
+    P, H, R, D = k_pages.shape
+    if q.dim() != 4 or q.shape[0] != table.shape[0] or q.shape[3] != D or q.shape[1] % H:
+        raise ValueError(f"q must be [{table.shape[0]}, a multiple of {H} heads, Tq, {D}], got {tuple(q.shape)}")
+    if out.shape != q.shape or out.dtype != q.dtype or q.dtype != k_pages.dtype:
+        raise ValueError("out must match q, and both the pool's dtype (cast q to the cache dtype first)")
+    if q.device != k_pages.device or out.device != q.device:
+        raise ValueError("q, out and the pool must be on one device")
+    if weights is not None:
+        _check_weights(weights, table, R, "weights")
+    _nat.require_device(q)
+    N, Hq, Tq, _ = q.shape
+    code = _nat.dtype_code(q.dtype)
+    q = _rows16(q)
+    with _On(q):
+        key = (N, Hq, H, Tq, D, table.shape[1] * R, weights is None, code, q.get_device())
+        nbytes = _WS_BYTES.get(key)
+        if nbytes is None:
+            nbytes = int(_nat.load().tabicl_paged_attn_workspace_bytes(N, Hq, H, Tq, D, table.shape[1] * R,
+                                                                       int(weights is not None), code))
+            if nbytes < 0:
+                raise _nat.UnsupportedShapeError(f"tabicl_paged_attn: {_nat.last_error()}")
+            if len(_WS_BYTES) >= 4096:  # lengths that grow row by row bring new keys for ever
+                _WS_BYTES.clear()
+            _WS_BYTES[key] = nbytes
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        _nat.call("tabicl_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), *_pool_args(k_pages, table),
+                  lengths.data_ptr(), _nat.ptr(weights), 0 if weights is None else max(weights.stride(0), weights.shape[1]),
+                  out.data_ptr(), N, Hq, H, Tq, D, *_steps(q), *_steps(out), float(scale), code, _nat.ptr(ws), nbytes,
+                  _nat.stream_of(q))
+
+
+@torch.library.custom_op("tabicl::paged_attn", mutates_args=("weights",))
+def _paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Optional[Tensor],
+                scale: float) -> Tensor:
+    """See paged_attention; weights is added to in place."""
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, out)
+    return out
+
+
+@_paged_attn.register_fake
+def _(q, k_pages, v_pages, table, lengths, weights, scale):  # noqa: ANN001
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("tabicl::paged_attn_out", mutates_args=("out", "weights"))
+def _paged_attn_out(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Optional[Tensor],
+                    scale: float, out: Tensor) -> None:
+    """tabicl::paged_attn written into `out`, any [N, Hq, Tq, D] view with a contiguous last dim."""
+    _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, out)
+
+
+@_paged_attn_out.register_fake
+def _(q, k_pages, v_pages, table, lengths, weights, scale, out):  # noqa: ANN001
+    return None
+
+
+def _no_grad(what: str, *ts: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise ValueError(f"{what} has no gradient (a serving operator): detach its inputs or call it under no_grad")
+
+
+def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor,
+                    weights: Optional[Tensor] = None, scale: Optional[float] = None, out: Optional[Tensor] = None) -> Tensor:
+    """softmax(q k^T scale) v of q [N, Hq, Tq, D] over the first lengths[n] rows of each sequence n of a paged pool
+    (k_pages, v_pages [pages, H, page_rows, D]; Hq a multiple of H, query head h reads K/V head h // (Hq // H); table
+    [N, max_pages] and lengths [N] int32; scale defaults to D^-0.5). Returns [N, Hq, Tq, D] in q's dtype, the pool's;
+    rows of an empty sequence, or whose every score is -inf, are 0. Scores, softmax and the value products are fp32
+    sums. weights: an optional fp32 [N, >= max_pages page_rows] tensor; the probabilities of each cached row, summed over
+    query heads and rows, are added to it in place (entries past the length are left as they are), always in the same
+    order of sums. out: written in place of a new tensor, any [N, Hq, Tq, D] view whose last dim is contiguous and whose
+    rows start on 16 bytes.
+
+    The work is split over the cached rows, so one test row over one long table fills the GPU; a table slice
+    table[:, :w] that covers the longest sequence spares the workgroups of pages nobody holds. For up to a few hundred
+    query rows (each group of 64 reads the cache again). No gradient."""
+    _no_grad("paged_attention", q, k_pages, v_pages)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if _nat.direct(q, k_pages, v_pages, table, lengths, weights, out):
+        o = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+        _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, o)
+        for t in (out, weights):
+            if t is not None:
+                torch.autograd.graph.increment_version(t)
+        return o
+    if out is None:
+        return torch.ops.tabicl.paged_attn(q, k_pages, v_pages, table, lengths, weights, scale)
+    torch.ops.tabicl.paged_attn_out(q, k_pages, v_pages, table, lengths, weights, scale, out)
+    return out
+
+
+def _append_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: Tensor, v: Tensor,
+                   count: Optional[Tensor]) -> None:
+    _check_pool(k_pages, v_pages, table, lengths)
+    P, H, R, D = k_pages.shape
+    N = table.shape[0]
+    if k.dim() != 4 or k.shape != v.shape or k.shape[:2] != (N, H) or k.shape[3] != D:
+        raise ValueError(f"k and v must be [{N}, {H}, T, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
+        raise ValueError(f"paged_append expects {k_pages.dtype} (cast before appending)")
+    if count is not None and (count.dtype != torch.int32 or count.shape != (N,) or not count.is_contiguous()):
+        raise ValueError(f"count must be a contiguous int32 tensor of {N} entries")
+    if any(t is not None and t.device != k_pages.device for t in (k, v, count)):
+        raise ValueError("k, v, count and the pool must be on one device")
+    _nat.require_device(k)
+    k, v = _rows16(k), _rows16(v)
+    with _On(k):
+        _nat.call("tabicl_paged_append", k_pages.data_ptr(), v_pages.data_ptr(), *_pool_args(k_pages, table),
+                  lengths.data_ptr(), k.data_ptr(), v.data_ptr(), _nat.ptr(count), N, H, k.shape[2], D, *_steps(k),
+                  *_steps(v), _nat.dtype_code(k.dtype), _nat.stream_of(k))
+
+
+@torch.library.custom_op("tabicl::paged_append", mutates_args=("k_pages", "v_pages"))
+def _paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: Tensor, v: Tensor,
+                  count: Optional[Tensor] = None) -> None:
+    """See paged_append."""
+    _append_launch(k_pages, v_pages, table, lengths, k, v, count)
+
+
+@_paged_append.register_fake
+def _(k_pages, v_pages, table, lengths, k, v, count=None):  # noqa: ANN001
+    return None
+
+
+def paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: Tensor, v: Tensor,
+                 count: Optional[Tensor] = None) -> None:
+    """Rows t < count[n] (int32 [N]; default all) of k, v [N, H, T, D] into rows lengths[n] + t of each sequence of the
+    pool (any strides with a contiguous last dim, e.g. the heads of a K|V projection). lengths is read, not changed: the
+    other blocks of a model append at the same rows. Rows that the table has no page for are dropped. Two sequences
+    must not share a page that is written."""
+    _no_grad("paged_append", k_pages, v_pages, k, v)
+    if _nat.direct(k_pages, v_pages, table, lengths, k, v, count):
+        _append_launch(k_pages, v_pages, table, lengths, k, v, count)
+        torch.autograd.graph.increment_version(k_pages)
+        torch.autograd.graph.increment_version(v_pages)
+    else:
+        torch.ops.tabicl.paged_append(k_pages, v_pages, table, lengths, k, v, count)
+
+
+def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int,
+                  recent: int, keep_n: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+    if k_pages.dim() != 5 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+        raise ValueError(f"k_pages and v_pages must be [blocks, pages, H, page_rows, D] of one layout, got "
+                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    B, P, H, R, D = k_pages.shape
+    if B > 0:
+        _check_pool(k_pages[0], v_pages[0], table, lengths)
+    N, cap = table.shape[0], table.shape[1] * R
+    _check_weights(weights, table, R, "weights")
+    if keep < 0 or recent < 0:
+        raise ValueError(f"keep and recent must not be negative, got {keep} and {recent}")
+    if keep_n is not None and (keep_n.dtype != torch.int32 or keep_n.shape != (N,) or not keep_n.is_contiguous()
+                               or keep_n.device != table.device):
+        raise ValueError(f"keep must be a number or a contiguous int32 tensor of {N} entries on the table's device")
+    _nat.require_device(table)
+    K = min(keep, cap)
+    with _On(table):
+        index = torch.empty(N, K, dtype=torch.int32, device=table.device)
+        kept_weights = torch.empty(N, cap, dtype=torch.float32, device=table.device)
+        kept = torch.empty(N, dtype=torch.int32, device=table.device)
+        nbytes = int(_nat.load().tabicl_paged_evict_workspace_bytes(N, K))
+        if nbytes < 0:
+            raise _nat.UnsupportedShapeError(f"tabicl_paged_evict: {_nat.last_error()}")
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=table.device)
+        pool = _pool_args(k_pages[0], table) if B > 0 else (0, H * R * D, R, table.data_ptr(), cap, table.shape[1])
+        _nat.call("tabicl_paged_evict", k_pages.data_ptr(), v_pages.data_ptr(), B, k_pages.stride(0) if B > 1 else 0, *pool,
+                  lengths.data_ptr(), weights.data_ptr(), max(weights.stride(0), weights.shape[1]), _nat.ptr(keep_n), keep,
+                  recent, index.data_ptr(), K, kept_weights.data_ptr(), kept.data_ptr(), N, H, D,
+                  _nat.dtype_code(k_pages.dtype), ws.data_ptr(), ws.numel(), _nat.stream_of(table))
+    return index, kept_weights, kept
+
+
+@torch.library.custom_op("tabicl::paged_evict", mutates_args=("k_pages", "v_pages"))
+def _paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int, recent: int,
+                 keep_n: Optional[Tensor] = None) -> tuple[Tensor, Tensor, Tensor]:
+    """See paged_evict; keep_n is its tensor keep (keep then bounds it)."""
+    return _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n)
+
+
+@_paged_evict.register_fake
+def _(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n=None):  # noqa: ANN001
+    N, cap = table.shape[0], table.shape[1] * k_pages.shape[3]
+    return (table.new_empty(N, min(keep, cap)), weights.new_empty(N, cap), table.new_empty(N))
+
+
+def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor,
+                keep: Union[int, Tensor], recent: int = 0) -> tuple[Tensor, Tensor, Tensor]:
+    """Cuts each sequence to kept = min(lengths[n], keep) rows (keep: a number, or int32 [N] on the GPU) in all blocks of
+    k_pages, v_pages [blocks, pages, H, page_rows, D] (or one block [pages, H, page_rows, D]), in place. Kept are its last
+    min(recent, kept) rows and, of those before them, the rows of the largest weights [N, >= max_pages page_rows] (fp32;
+    ties: the lower row; NaN counts as -inf). Kept rows past the cut move, in order, to the places of the evicted ones
+    below it; nothing else moves. Returns index [N, K] int32 (slot j holds the old row index[n, j], -1 from kept on; K =
+    keep, or the capacity for a tensor), the weights in their new slots [N, max_pages page_rows] (0 past the cut) and
+    kept [N] int32. weights, table and lengths are not changed: take over the new ones. No two sequences may share a
+    page."""
+    _no_grad("paged_evict", k_pages, v_pages, weights)
+    if k_pages.dim() == 4:
+        k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
+    keep_n = None
+    if isinstance(keep, Tensor):
+        keep, keep_n = table.shape[1] * k_pages.shape[3], keep
+    if _nat.direct(k_pages, v_pages, table, lengths, weights, keep_n):
+        r = _evict_launch(k_pages, v_pages, table, lengths, weights, int(keep), int(recent), keep_n)
+        torch.autograd.graph.increment_version(k_pages)
+        torch.autograd.graph.increment_version(v_pages)
+        return r
+    return torch.ops.tabicl.paged_evict(k_pages, v_pages, table, lengths, weights, int(keep), int(recent), keep_n)
+
+
+class PagedIclKVCache(_icl.IclKVCache):
+    """The ICL stage's K/V cache in pages: `sequences` (tables, or estimators of tables) of up to max_rows rows each, in
+    `pages` pages of page_rows rows that every block holds one of ([blocks, pages, heads, page_rows, head_dim] for K and
+    V). append, append_projected, query, attention_layer, query_blocks and query_chunked as in IclKVCache (rows go behind
+    each sequence's last one, and a sequence may get fewer rows than the others of a call); cached_query takes it as its
+    icl_cache.
+
+    track=True adds up, over every query of every block, the attention weight that each cached row draws (`weights`, fp32
+    [sequences, capacity]); evict(keep) cuts the sequences to their heaviest rows and returns the emptied pages.
+
+    Pages are given out on the host; the page table and the lengths live on the GPU, so a query costs no host sync. Calls
+    follow each other on one stream. Only queries can be captured in a graph (the others keep books on the host)."""
+
+    def __init__(self, sequences: int, blocks: int, heads: int, head_dim: int, max_rows: int, pages: int,
+                 page_rows: int = 64, dtype: torch.dtype = torch.bfloat16, device: Union[str, torch.device] = "cuda",
+                 track: bool = False):
+        if page_rows < 16 or page_rows & (page_rows - 1):
+            raise ValueError(f"page_rows must be a power of two from 16 on, got {page_rows}")
+        width = -(-max_rows // page_rows)
+        self.keys = torch.empty(blocks, pages, heads, page_rows, head_dim, dtype=dtype, device=device)
+        self.values = torch.empty_like(self.keys)
+        self.page_rows = page_rows
+        self.capacity = width * page_rows
+        self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(blocks, sequences, dtype=torch.int32, device=device)
+        self.weights = torch.zeros(sequences, self.capacity, dtype=torch.float32, device=device) if track else None
+        self._pages = torch.full((sequences, width), -1, dtype=torch.int32)  # the table's host copy
+        self._held = [0] * sequences  # pages a sequence holds
+        self._rows = [[0] * sequences for _ in range(blocks)]  # the lengths' host copy
+        self._free = list(range(pages - 1, -1, -1))
+        self._owner = True
+
+    @property
+    def shape(self):
+        """(sequences, blocks, heads, capacity, head_dim), as of IclKVCache."""
+        B, _, H, _, D = self.keys.shape
+        return (self.table.shape[0], B, H, self.capacity, D)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, block: int, sequence: int = 0) -> int:
+        return self._rows[block][sequence]
+
+    def default_valid(self, block: int) -> Tensor:
+        """The block's filled lengths as the int32 device tensor the kernels take."""
+        if not any(self._rows[block]):
+            raise ValueError(f"block {block} of the cache has no rows: append before querying")
+        return self.lengths[block]
+
+    def _own(self, what: str) -> None:
+        if not self._owner:
+            raise ValueError(f"{what}: a view of some of a cache's estimators answers queries only")
+
+    def reserve(self, rows: Union[int, Sequence[int]]) -> None:
+        """Pages for sequences of up to `rows` rows (a number, or one per sequence), given out now rather than by the
+        appends that fill them."""
+        self._own("reserve")
+        S, R = self.table.shape[0], self.page_rows
+        rows = [int(rows)] * S if isinstance(rows, int) else [int(r) for r in rows]
+        if len(rows) != S:
+            raise ValueError(f"{len(rows)} row counts for {S} sequences")
+        if max(rows, default=0) > self.capacity:
+            raise ValueError(f"{max(rows)} rows exceed the capacity {self.capacity}")
+        want = [max(0, -(-r // R) - h) for r, h in zip(rows, self._held)]
+        if sum(want) > len(self._free):
+            raise ValueError(f"{sum(want)} pages wanted, {len(self._free)} free: evict, release or build a larger pool")
+        for s, n in enumerate(want):
+            for _ in range(n):
+                self._pages[s, self._held[s]] = self._free.pop()
+                self._held[s] += 1
+        if any(want):
+            self.table.copy_(self._pages)
+
+    def append(self, block: int, k: Tensor, v: Tensor, rows: Optional[Sequence[int]] = None) -> None:  # noqa: ANN001
+        """Rows t < rows[s] (default all) of k, v [sequences, H, T, d] behind each sequence's last row of `block`."""
+        self._own("append")
+        S, NB, H, cap, D = self.shape
+        if k.shape != v.shape or k.dim() != 4 or k.shape[0] != S or k.shape[1] != H or k.shape[3] != D:
+            raise ValueError(f"append expects k/v [{S}, {H}, T, {D}], got {tuple(k.shape)} / {tuple(v.shape)}")
+        if k.dtype != self.keys.dtype or v.dtype != self.keys.dtype:
+            raise ValueError(f"append expects {self.keys.dtype} (cast before appending)")
+        if not 0 <= block < NB:
+            raise ValueError(f"block {block} out of range [0, {NB})")
+        _nat.require_device(k, v, self.keys)
+        T = k.shape[2]
+        new = [T] * S if rows is None else [int(r) for r in rows]
+        if len(new) != S or any(not 0 <= r <= T for r in new):
+            raise ValueError(f"rows must be {S} counts from 0 to {T}, got {new}")
+        ends = [a + n for a, n in zip(self._rows[block], new)]
+        self.reserve(ends)
+        count = None if rows is None else torch.tensor(new, dtype=torch.int32, device=self.table.device)
+        paged_append(self.keys[block], self.values[block], self.table, self.lengths[block], k, v, count)
+        self.lengths[block] += T if count is None else count
+        self._rows[block] = ends
+
+    def append_projected(self, block: int, x: Tensor, in_proj_weight: Tensor, in_proj_bias: Optional[Tensor] = None,
+                         rows: Optional[Sequence[int]] = None) -> None:
+        """append of the rows x [sequences, T, width] through the K|V thirds of a block's packed in-projection (one
+        GEMM; the append reads the heads out of it through strides)."""
+        self.append(block, *self._project_kv(x, in_proj_weight, in_proj_bias), rows)
+
+    def query(self, block: int, q: Tensor, valid_kv_len: Optional[Union[int, Tensor]] = None,
+              out: Optional[Tensor] = None) -> Tensor:
+        """Attention of q [sequences, H, Tq, d] over `block` of the cache: each sequence's own rows, of those the ones
+        below valid_kv_len if given (a number, or one per sequence). q in the cache's dtype or one that widens to it."""
+        lengths = self.default_valid(block)
+        longest = max(self._rows[block])
+        if isinstance(valid_kv_len, Tensor):
+            lengths = torch.minimum(valid_kv_len.to(device=lengths.device, dtype=torch.int32).reshape(-1).expand_as(lengths),
+                                    lengths)
+        elif valid_kv_len is not None and int(valid_kv_len) < longest:
+            longest = max(0, int(valid_kv_len))
+            lengths = lengths.clamp(max=longest)
+        dt = self.keys.dtype
+        if torch.promote_types(q.dtype, dt) != dt:
+            raise ValueError(f"q is {q.dtype}, wider than the {dt} cache: cast it")
+        w = max(1, -(-longest // self.page_rows))
+        weights = None if self.weights is None else self.weights[:, :w * self.page_rows]
+        return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out)
+
+    def evict(self, keep: Union[int, Sequence[int]], recent: int = 0) -> Tensor:
+        """Cuts each sequence to at most keep rows (a number, or one per sequence), in every block alike: its `recent`
+        last rows and the heaviest of the others (paged_evict by the tracked weights, which follow their rows). Emptied
+        pages go back to the pool. Returns index [sequences, K] int32: slot j now holds the old row index[s, j]."""
+        self._own("evict")
+        if self.weights is None:
+            raise ValueError("evict needs a cache built with track=True")
+        S = self.table.shape[0]
+        if any(r != self._rows[0] for r in self._rows):
+            raise ValueError("the blocks hold different rows: append to every block before evicting")
+        keeps = [int(keep)] * S if isinstance(keep, int) else [int(n) for n in keep]
+        if len(keeps) != S or min(keeps, default=0) < 0:
+            raise ValueError(f"keep must be one count of at least 0, or {S} of them")
+        have = self._rows[0]
+        w = max(1, -(-max(have, default=0) // self.page_rows))
+        kept = [min(h, n) for h, n in zip(have, keeps)]
+        keep_n = None if isinstance(keep, int) else torch.tensor(kept, dtype=torch.int32, device=self.table.device)
+        index, weights, lengths = paged_evict(self.keys, self.values, self.table[:, :w], self.lengths[0], self.weights,
+                                              max(kept, default=0) if keep_n is None else keep_n, recent)
+        index = index[:, :max(kept, default=0)]
+        self.weights[:, :weights.shape[1]] = weights
+        self.lengths.copy_(lengths.expand_as(self.lengths))
+        self._rows = [list(kept) for _ in self._rows]
+        self._give_back(kept)
+        return index
+
+    def release(self, sequence: int) -> None:
+        """Forgets a sequence: its pages go back to the pool, its place can be filled anew."""
+        self._own("release")
+        for rows in self._rows:
+            rows[sequence] = 0
+        self.lengths[:, sequence] = 0
+        if self.weights is not None:
+            self.weights[sequence] = 0.0
+        self._give_back([max(r[s] for r in self._rows) if s != sequence else 0 for s in range(len(self._held))])
+
+    def _give_back(self, rows) -> None:  # noqa: ANN001
+        """Pages past each sequence's first `rows` rows back to the pool."""
+        changed = False
+        for s, r in enumerate(rows):
+            need = -(-r // self.page_rows)
+            for p in range(self._held[s] - 1, need - 1, -1):
+                self._free.append(int(self._pages[s, p]))
+                self._pages[s, p] = -1
+                changed = True
+            self._held[s] = min(self._held[s], need)
+        if changed:
+            self.table.copy_(self._pages)
+
+    def estimators(self, start: int, stop: int) -> "PagedIclKVCache":
+        """Sequences [start, stop) as a cache of their own that answers queries (query_chunked): views of the pool, the
+        table, the lengths and the tracked weights."""
+        S = self.table.shape[0]
+        if not 0 <= start < stop <= S:
+            raise ValueError(f"estimators [{start}, {stop}) out of range [0, {S})")
+        view = object.__new__(PagedIclKVCache)
+        view.__dict__.update(self.__dict__)
+        view.table = self.table[start:stop]
+        view.lengths = self.lengths[:, start:stop]
+        view.weights = None if self.weights is None else self.weights[start:stop]
+        view._rows = [r[start:stop] for r in self._rows]
+        view._owner = False
+        return view
+
+    def block_kv(self, block: int):
+        """The block's pools [pages, H, page_rows, d]."""
+        return self.keys[block], self.values[block]

@@ -1,0 +1,568 @@
+"""GPU tests of the paged K/V cache (tabicl_mi355_paged) against the plain float64 forms of paged_ref.py: attention of
+few rows with and without the weights it adds up, append and eviction, at lengths around the tiles' and pages' edges, on
+strided inputs, with pages that hold no rows, with non-finite values in and around the live rows, on other streams, in
+captured graphs, far into a large pool, and run together as PagedIclKVCache runs them.
+
+Everything the kernels must not read (rows past a length, pages nobody holds) is NaN; everything they must not write is
+compared. Bounds: paged_ref.attention derives them; append and eviction copy, so they are compared bit for bit."""
+import pytest
+import torch
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _case(dev, seed, lengths, H=8, G=1, D=64, R=64, T=1, dtype=BF, spare=5, slack=0, blocks=None, sharp=1.0):
+    """A pool whose pages lie in random order, NaN wherever no sequence has a row."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    N = len(lengths)
+    M = max(1, max(-(-n // R) for n in lengths)) + slack
+    P = N * M + spare
+    table = torch.randperm(P, generator=g, device=dev)[:N * M].to(torch.int32).view(N, M).contiguous()
+    lead = () if blocks is None else (blocks,)
+    kp, vp = (torch.randn(*lead, P, H, R, D, generator=g, device=dev).to(dtype) for _ in range(2))
+    dead = torch.ones(P, R, dtype=torch.bool, device=dev)
+    for n, length in enumerate(lengths):
+        _, page, row = ref.rows_of(table[n], length, R, P)
+        dead[page, row] = False
+    for t in (kp, vp):
+        t.masked_fill_(dead[:, None, :, None], float("nan"))
+    q = (torch.randn(N, H * G, T, D, generator=g, device=dev) * sharp).to(dtype)
+    return q, kp, vp, table, torch.tensor(lengths, dtype=torch.int32, device=dev), g
+
+
+def _attend(q, kp, vp, table, lengths, weights=None, scale=None, what=""):
+    import tabicl_mi355_paged as paged
+    before = None if weights is None else weights.clone()
+    keep = [t.clone() for t in (q, kp, vp, table, lengths)]
+    print(f"[paged] {what} q {tuple(q.shape)} pool {tuple(kp.shape)} {q.dtype}", flush=True)
+    out = paged.paged_attention(q, kp, vp, table, lengths, weights, scale)
+    torch.cuda.synchronize()
+    assert out.shape == q.shape and out.dtype == q.dtype
+    for t, k in zip((q, kp, vp, table, lengths), keep):
+        assert torch.equal(t.view(torch.uint8) if t.is_contiguous() else t, k.view(torch.uint8) if t.is_contiguous() else k)
+    want, w, tol, wtol = ref.attention(q, kp, vp, table, lengths, q.shape[-1] ** -0.5 if scale is None else scale, before)
+    ref.near(out, want, tol, what + " out")
+    if weights is not None:
+        ref.near(weights, w, wtol, what + " weights")
+        for n in range(len(lengths)):  # past the length: left alone
+            assert torch.equal(weights[n, max(0, int(lengths[n])):], before[n, max(0, int(lengths[n])):])
+    return out
+
+
+EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1000, 1023, 1025]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("R", [16, 64, 256])
+@pytest.mark.parametrize("weighted", [False, True], ids=["", "weights"])
+def test_lengths(dev, dtype, R, weighted):
+    q, kp, vp, table, n, g = _case(dev, R, EDGES, H=2, R=R, dtype=dtype, sharp=2.0)
+    w = torch.rand(len(EDGES), table.shape[1] * R, generator=g, device=dev) if weighted else None
+    out = _attend(q, kp, vp, table, n, w, what="lengths")
+    assert (out[0] == 0).all()  # no cached row
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("T,G", [(1, 1), (1, 4), (3, 1), (5, 3), (16, 1), (17, 1), (33, 2), (64, 1), (65, 1), (130, 1)])
+def test_query_rows_and_head_dims(dev, dtype, D, T, G):
+    q, kp, vp, table, n, g = _case(dev, 7 * D + T, [300, 77, 1], H=3, G=G, D=D, R=32, T=T, dtype=dtype, sharp=1.5)
+    w = torch.rand(3, table.shape[1] * 32, generator=g, device=dev)
+    _attend(q, kp, vp, table, n, None, what="plain")
+    _attend(q, kp, vp, table, n, w, what="weights")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lengths,T", [([45001], 1), ([20011, 3, 9999, 0, 12345], 2), ([6007] * 3, 40)])
+def test_long_and_ragged(dev, dtype, lengths, T):
+    q, kp, vp, table, n, g = _case(dev, T, lengths, R=64, T=T, dtype=dtype, slack=3, sharp=2.5)
+    w = torch.zeros(len(lengths), table.shape[1] * 64, device=dev)
+    _attend(q, kp, vp, table, n, None, what="long")
+    _attend(q, kp, vp, table, n, w, what="long weights")
+    # probabilities of every row sum to one
+    total = w.double().sum(1)
+    for i, length in enumerate(lengths):
+        assert abs(float(total[i]) - (8 * T if length else 0)) < 1e-3 * 8 * T
+
+
+def test_one_sequence_per_many(dev):
+    # 300 sequences of a few rows
+    q, kp, vp, table, n, g = _case(dev, 5, [(i * 7) % 40 for i in range(300)], H=1, R=16, T=2)
+    _attend(q, kp, vp, table, n, torch.zeros(300, table.shape[1] * 16, device=dev), what="many")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_pages_without_rows(dev, dtype):
+    # page ids outside the pool inside and past the length, lengths below 0 and past the table
+    q, kp, vp, table, n, g = _case(dev, 11, [200, 150, 90, 64], H=2, R=16, dtype=dtype, T=2)
+    table[0, 3], table[0, 7], table[1, :] = -1, kp.shape[0], -5
+    table[2, 0], table[2, 6:] = 2 ** 31 - 1, -1
+    n[3] = -7
+    w = torch.rand(4, table.shape[1] * 16, generator=g, device=dev)
+    out = _attend(q, kp, vp, table, n, w, what="holes")
+    assert (out[1] == 0).all() and (out[3] == 0).all()
+    q, kp, vp, table, n, g = _case(dev, 12, [48, 48], H=2, R=16, dtype=dtype)
+    want = _attend(q, kp, vp, table, n, what="full")
+    n[:] = torch.tensor([2 ** 31 - 1, 49], dtype=torch.int32)  # clamped to the table
+    assert torch.equal(_attend(q, kp, vp, table, n, what="past the table"), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_strided_views(dev, dtype):
+    import tabicl_mi355_paged as paged
+    N, H, T, D, R = 3, 4, 5, 64, 32
+    q, kp, vp, table, n, g = _case(dev, 21, [100, 65, 33], H=H, T=T, R=R, dtype=dtype)
+    want = _attend(q, kp, vp, table, n, what="contiguous")
+    # heads of a projection, an unaligned view, a strided last dim, a broadcast query
+    proj = torch.zeros(N, T, 3 * H * D, dtype=dtype, device=dev)
+    proj.view(N, T, 3, H, D)[:, :, 1] = q.transpose(1, 2)
+    odd = torch.zeros(q.numel() + 3, dtype=dtype, device=dev)[3:].view(q.shape).copy_(q)
+    wide = torch.zeros(N, H, T, 2 * D, dtype=dtype, device=dev)[..., ::2].copy_(q)
+    for view in (proj.view(N, T, 3, H, D)[:, :, 1].transpose(1, 2), odd, wide):
+        assert torch.equal(paged.paged_attention(view, kp, vp, table, n), want)
+    one = q[:1].expand(N, H, T, D)
+    assert torch.equal(paged.paged_attention(one, kp, vp, table, n),
+                       paged.paged_attention(one.contiguous(), kp, vp, table, n))
+    # output in merged-head order, beside values that stay
+    out = torch.full((N, T, H, 2 * D), 7.0, dtype=dtype, device=dev)
+    o = paged.paged_attention(q, kp, vp, table, n, None, None, out[..., :D].transpose(1, 2))
+    assert o.data_ptr() == out.data_ptr()
+    assert torch.equal(out[..., :D].transpose(1, 2), want) and (out[..., D:] == 7).all()
+    # a slice of a wider table, pages of a larger pool, weights with a row stride
+    wide_t = torch.full((N, table.shape[1] + 4), -1, dtype=torch.int32, device=dev)
+    wide_t[:, :table.shape[1]] = table
+    big = torch.full((2, kp.shape[0], 3, *kp.shape[1:]), float("nan"), dtype=dtype, device=dev)
+    big[0, :, 1], big[1, :, 2] = kp, vp
+    w = torch.zeros(N, table.shape[1] * R + 9, device=dev)
+    got = paged.paged_attention(q, big[0, :, 1], big[1, :, 2], wide_t[:, :table.shape[1]], n, w)
+    assert torch.equal(got, want) and (w[:, table.shape[1] * R:] == 0).all()
+    assert abs(float(w.sum()) - N * H * T) < 1e-2
+    with pytest.raises(ValueError):
+        paged.paged_attention(q, kp, vp, table, n, None, None, torch.zeros_like(wide)[..., ::1][..., :D][..., ::2])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_non_finite_values(dev, dtype):
+    # infinities and NaN in live rows reach what they should and nothing else
+    lengths = [70, 70, 70, 70, 70, 700]
+    q, kp, vp, table, n, g = _case(dev, 31, lengths, H=2, R=16, T=3, dtype=dtype)
+    q = q.abs() + 0.1
+    at = lambda s, r: (table[s, r // 16].long(), slice(None), r % 16)  # noqa: E731
+    kp[at(0, 5)] = float("-inf")    # a key of score -inf: weight 0
+    kp[at(1, 40)] = float("inf")    # a score of +inf: inf - inf
+    kp[at(2, 69)] = float("nan")
+    vp[at(3, 3)] = float("inf")
+    vp[at(4, 64)] = float("nan")
+    for r in range(600):            # whole tiles of -inf before the first finite score
+        kp[at(5, r)] = float("-inf")
+    w = torch.zeros(6, table.shape[1] * 16, device=dev)
+    import tabicl_mi355_paged as paged
+    out = paged.paged_attention(q, kp, vp, table, n, w)
+    want, ww, tol, wtol = ref.attention(q, kp, vp, table, n, 0.125, torch.zeros_like(w))
+    inf = torch.isinf(want)
+    assert inf[3].all() and torch.equal(out.double()[inf], want[inf])
+    ref.near(torch.where(inf, 0, out.double()), torch.where(inf, 0, want), torch.where(inf, 1, tol), "non-finite out")
+    ref.near(w, ww, wtol, "non-finite weights")
+    # every key at -inf: no weight anywhere, 0
+    kp[table[0, :5].long()] = float("-inf")
+    assert (paged.paged_attention(q, kp, vp, table, n)[0] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("scale", [0.125, 4.0, -2.0, 0.0])
+def test_sharp_scores(dev, dtype, scale):
+    # scores that rise along the cache (every tile moves the running maximum) and fall along it, large scales
+    q, kp, vp, table, n, g = _case(dev, 41, [3000, 3000], H=2, R=64, T=2, dtype=dtype)
+    for s, sign in ((0, 1.0), (1, -1.0)):
+        _, page, row = ref.rows_of(table[s], 3000, 64, kp.shape[0])
+        kp[page, :, row] = (kp[page, :, row].float() + sign * torch.linspace(-4, 4, 3000, device=dev).view(-1, 1, 1)
+                            ).to(dtype)
+    q = (q.float().abs() * 0.5).to(dtype)
+    _attend(q, kp, vp, table, n, torch.zeros(2, table.shape[1] * 64, device=dev), scale, "sharp")
+
+
+def test_values_near_the_largest(dev):
+    # fp32 values near the largest float survive the weighting; far negative scores with no others stay a softmax
+    q, kp, vp, table, n, g = _case(dev, 43, [900, 40], H=1, R=16, T=1, dtype=F32)
+    import tabicl_mi355_paged as paged
+    vp[:] = torch.where(torch.isnan(vp), vp, torch.full_like(vp, 3e38))
+    out = paged.paged_attention(q, kp, vp, table, n)
+    assert torch.isfinite(out).all() and float((out / 3e38 - 1).abs().max()) < 1e-5
+    _, page, row = ref.rows_of(table[1], 40, 16, kp.shape[0])
+    kp[page, :, row] = -1e33
+    q[1] = 1e3
+    vp[page, :, row] = torch.arange(40.0, device=dev).view(40, 1, 1)
+    assert torch.allclose(paged.paged_attention(q, kp, vp, table, n)[1], torch.tensor(19.5, device=dev))
+
+
+def test_repeatable_and_concurrent(dev):
+    # the same bits every time, on two streams at once and beside a default stream at work
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, 51, [9000, 4001, 200], T=4)
+    w0 = torch.rand(3, table.shape[1] * 64, generator=g, device=dev)
+
+    def once():
+        w = w0.clone()
+        return paged.paged_attention(q, kp, vp, table, n, w), w
+
+    want = once()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(once())
+        got.append(once())
+    torch.cuda.synchronize()
+    for o, w in got:
+        assert torch.equal(o, want[0]) and torch.equal(w, want[1])
+
+
+def test_large_offsets(dev):
+    # pages more than 2^32 elements apart in one pool
+    import tabicl_mi355_paged as paged
+    P, H, R, D = 2200, 8, 4096, 64  # 2200 x 2 Mi elements
+    kp, vp = (torch.empty(P, H, R, D, dtype=BF, device=dev) for _ in range(2))
+    ids = torch.tensor([[2199, 0], [2100, 2198]], dtype=torch.int32, device=dev)
+    g = torch.Generator(device=dev).manual_seed(1)
+    k, v = (torch.randn(2, H, 5000, D, generator=g, device=dev).to(BF) for _ in range(2))
+    zero, n = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([0, 0], [5000, 5000]))
+    paged.paged_append(kp, vp, ids, zero, k, v)
+    for s in range(2):
+        for t, want in ((kp, k), (vp, v)):
+            got = torch.cat([t[ids[s, 0].long()], t[ids[s, 1].long(), :, :904]], 1)
+            assert torch.equal(got, want[s])
+    q = torch.randn(2, H, 2, D, generator=g, device=dev).to(BF)
+    w = torch.zeros(2, 2 * R, device=dev)
+    out = paged.paged_attention(q, kp, vp, ids, n, w)
+    want, ww, tol, wtol = ref.attention(q, kp, vp, ids, n, D ** -0.5, torch.zeros_like(w))
+    ref.near(out, want, tol, "far pages")
+    ref.near(w, ww, wtol, "far pages weights")
+    index, kw, kept = paged.paged_evict(kp, vp, ids, n, w, 4500, 16)
+    assert kept.tolist() == [4500, 4500]
+    for s in range(2):
+        got = torch.cat([kp[ids[s, 0].long()], kp[ids[s, 1].long(), :, :404]], 1)
+        assert torch.equal(got, k[s][:, index[s].long()])
+    del kp, vp
+
+
+# ---------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("start,T", [([0, 0, 0], 1), ([5, 16, 31], 1), ([0, 7, 100], 77), ([90, 112, 200], 30), ([-3, 0, 1], 0)])
+@pytest.mark.parametrize("counted", [False, True], ids=["", "count"])
+def test_append(dev, dtype, D, start, T, counted):
+    # starts inside a page, rows past the table dropped, pages the pool does not have dropped
+    import tabicl_mi355_paged as paged
+    H, R = 3, 16
+    g = torch.Generator(device=dev).manual_seed(T + D)
+    kp, vp = (torch.randn(30, H, R, D, generator=g, device=dev).to(dtype) for _ in range(2))
+    table = torch.randperm(30, generator=g, device=dev)[:24].to(torch.int32).view(3, 8).contiguous()
+    table[1, 2], table[2, 7] = -1, 30
+    n = torch.tensor(start, dtype=torch.int32, device=dev)
+    kv = torch.randn(3, T, 2, H, D, generator=g, device=dev).to(dtype)  # heads of a K|V projection
+    k, v = kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+    count = torch.tensor([T, T // 2, -1], dtype=torch.int32, device=dev) if counted else None
+    want = ref.append(kp.cpu(), vp.cpu(), table.cpu(), n.cpu(), k.cpu(), v.cpu(), count)
+    print(f"[paged] append {dtype} D={D} start={start} T={T} counted={counted}", flush=True)
+    paged.paged_append(kp, vp, table, n, k, v, count)
+    torch.cuda.synchronize()
+    assert torch.equal(kp.cpu(), want[0]) and torch.equal(vp.cpu(), want[1]) and n.tolist() == start
+
+
+def test_append_layouts(dev):
+    # contiguous, unaligned and strided sources, a pool with gaps between its pages, a count past T
+    import tabicl_mi355_paged as paged
+    g = torch.Generator(device=dev).manual_seed(3)
+    H, R, D, T = 2, 32, 64, 50
+    k, v = (torch.randn(2, H, T, D, generator=g, device=dev).to(BF) for _ in range(2))
+    table = torch.tensor([[4, 1], [0, 3]], dtype=torch.int32, device=dev)
+    n = torch.tensor([3, 14], dtype=torch.int32, device=dev)
+    odd = torch.zeros(k.numel() + 1, dtype=BF, device=dev)[1:].view(k.shape).copy_(k)
+    wide = torch.zeros(2, H, T, 2 * D, dtype=BF, device=dev)[..., ::2].copy_(v)
+    count = torch.tensor([1000, 50], dtype=torch.int32, device=dev)
+    for a, b, c in ((k, v, None), (odd, wide, None), (k, wide, count)):
+        pool = torch.full((5, 3, H, R, D), 9.0, dtype=BF, device=dev)
+        kp, vp = pool[:, 0], pool[:, 2]
+        want = ref.append(kp.cpu(), vp.cpu(), table.cpu(), n.cpu(), k.cpu(), v.cpu(), c)
+        paged.paged_append(kp, vp, table, n, a, b, c)
+        torch.cuda.synchronize()
+        assert torch.equal(kp.cpu(), want[0]) and torch.equal(vp.cpu(), want[1]) and (pool[:, 1] == 9).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# eviction
+# ---------------------------------------------------------------------------------------------
+def _evict(kp, vp, table, n, w, keep, recent, what):
+    import tabicl_mi355_paged as paged
+    cpu = [t.cpu() for t in (kp, vp, table, n, w)]
+    want = ref.evict(*cpu, keep.cpu() if torch.is_tensor(keep) else keep, recent)
+    print(f"[paged] evict {what} pool {tuple(kp.shape)} keep {keep if not torch.is_tensor(keep) else keep.tolist()[:8]} "
+          f"recent {recent}", flush=True)
+    index, kw, kept = paged.paged_evict(kp, vp, table, n, w, keep, recent)
+    torch.cuda.synchronize()
+    assert torch.equal(kept.cpu(), want[4]), what
+    assert torch.equal(index.cpu(), want[2]), what
+    assert torch.equal(kw.cpu().view(torch.int32), want[3].view(torch.int32)), what
+    for got, ref_pool in ((kp, want[0]), (vp, want[1])):
+        assert torch.equal(got.cpu().view(torch.uint8), ref_pool.view(torch.uint8)), what
+    for t, c in zip((table, n, w), cpu[2:]):  # read, not changed
+        assert torch.equal(t.cpu().view(torch.int32), c.view(torch.int32))
+
+
+LENGTHS = [0, 1, 2, 40, 63, 64, 65, 300, 1000, 1023, 1024, 1025, 2500]
+
+
+@pytest.mark.parametrize("keep,recent", [(0, 0), (1, 0), (1, 5), (40, 0), (40, 7), (512, 32), (900, 900), (2499, 1), (2500, 0),
+                                         (10000, 3)])
+def test_evict(dev, keep, recent):
+    q, kp, vp, table, n, g = _case(dev, keep + recent, LENGTHS, H=2, R=16, D=32, blocks=2)
+    _evict(kp, vp, table, n, torch.exp(torch.randn(len(LENGTHS), table.shape[1] * 16, generator=g, device=dev) * 2), keep,
+           recent, "log-normal")
+
+
+@pytest.mark.parametrize("dtype,D,blocks", [(F32, 64, 1), (BF, 64, 3), (BF, 128, 1), (F32, 128, 2)])
+def test_evict_types(dev, dtype, D, blocks):
+    q, kp, vp, table, n, g = _case(dev, D, [700, 123, 64], H=3, R=64, D=D, dtype=dtype, blocks=blocks, slack=1)
+    _evict(kp, vp, table, n, torch.rand(3, table.shape[1] * 64, generator=g, device=dev), 100, 10, "types")
+
+
+def test_evict_ties_and_special_weights(dev):
+    # equal weights, a few distinct ones, zeros of both signs, infinities, NaN, negative weights
+    L = [1500] * 8
+    q, kp, vp, table, n, g = _case(dev, 9, L, H=1, R=16, D=32, blocks=1)
+    C = table.shape[1] * 16
+    w = torch.zeros(8, C, device=dev)
+    w[1] = 0.25
+    w[2] = torch.randint(0, 3, (C,), generator=g, device=dev).float()
+    w[3] = torch.where(torch.rand(C, generator=g, device=dev) < 0.5, -0.0, 0.0)
+    w[4] = torch.randn(C, generator=g, device=dev)
+    w[4, ::3], w[4, 1::7], w[4, 5::11] = float("nan"), float("inf"), float("-inf")
+    w[5] = float("nan")
+    w[6] = 1.0 + torch.arange(C, device=dev) * 2.0 ** -23  # neighbours in fp32, rising
+    w[7] = torch.finfo(F32).tiny * 2.0 ** -10 * torch.randint(0, 2000, (C,), generator=g, device=dev)  # subnormal
+    for keep, recent in ((1, 0), (700, 0), (700, 50), (1499, 0)):
+        q, kp, vp, table, n, _ = _case(dev, 9, L, H=1, R=16, D=32, blocks=1)
+        _evict(kp, vp, table, n, w, keep, recent, "ties")
+
+
+def test_evict_budgets_and_layouts(dev):
+    # a budget per sequence (negative and past the length too), weights with a row stride, one block without its dim,
+    # pages the pool does not have, a pool whose blocks lie apart
+    q, kp, vp, table, n, g = _case(dev, 13, [400, 400, 400, 50, 0], H=2, R=32, D=64)
+    C = table.shape[1] * 32
+    w = torch.rand(5, C + 5, generator=g, device=dev)[:, :C + 1]
+    table[1, 2], table[2, 12] = -1, kp.shape[0]
+    keep = torch.tensor([100, 399, 256, -4, 7], dtype=torch.int32, device=dev)
+    import tabicl_mi355_paged as paged
+    want = ref.evict(kp[None].cpu(), vp[None].cpu(), table.cpu(), n.cpu(), w.cpu(), keep.cpu(), 20)
+    index, kw, kept = paged.paged_evict(kp, vp, table, n, w, keep, 20)
+    torch.cuda.synchronize()
+    assert index.shape == (5, C) and torch.equal(index.cpu(), want[2]) and torch.equal(kept.cpu(), want[4])
+    assert torch.equal(kw.cpu(), want[3])
+    for got, r in ((kp, want[0][0]), (vp, want[1][0])):
+        assert torch.equal(got.cpu().view(torch.uint8), r.view(torch.uint8))
+    pool = torch.randn(kp.shape[0], 3, 2, *kp.shape[1:], generator=g, device=dev).to(BF)
+    _evict(pool[:, :, 0].transpose(0, 1), pool[:, :, 1].transpose(0, 1), table, n, w, 111, 0, "pages of all blocks")
+
+
+@pytest.mark.parametrize("length,keep", [(70001, 30000), (45000, 44000)])
+def test_evict_long(dev, length, keep):
+    q, kp, vp, table, n, g = _case(dev, 17, [length, length // 3], H=1, R=256, D=32, blocks=1)
+    w = torch.exp(torch.randn(2, table.shape[1] * 256, generator=g, device=dev))
+    w = torch.where(torch.rand(w.shape, generator=g, device=dev) < 0.3, torch.zeros_like(w), w)
+    _evict(kp, vp, table, n, w, keep, 100, "long")
+
+
+# ---------------------------------------------------------------------------------------------
+# graphs, ops, and the operators together
+# ---------------------------------------------------------------------------------------------
+def test_graph(dev):
+    # one graph of append, attention with weights and eviction: replayed with other inputs, lengths and pages
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, 61, [3000, 900, 20], T=2, blocks=2, slack=2, spare=0)
+    k, v = (torch.randn(3, 8, 10, 64, generator=g, device=dev).to(BF) for _ in range(2))
+    w = torch.zeros(3, table.shape[1] * 64, device=dev)
+    grown = n + 10
+
+    def step():
+        for b in range(2):
+            paged.paged_append(kp[b], vp[b], table, n, k, v)
+        out = paged.paged_attention(q, kp[0], vp[0], table, grown, w)
+        return (out, *paged.paged_evict(kp, vp, table, grown, w, 800, 16))
+
+    start = [t.clone() for t in (kp, vp, w)]
+
+    def reset():
+        for t, s in zip((kp, vp, w), start):
+            t.copy_(s)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    with torch.cuda.graph(other):  # a second graph of the same calls, replayed between the first one's replays
+        got2 = step()
+    for i in range(3):
+        q.copy_(torch.randn(q.shape, generator=g, device=dev).to(BF))
+        k.copy_(torch.randn(k.shape, generator=g, device=dev).to(BF))
+        n.copy_(torch.tensor([3000 - 700 * i, 900 + i, 20 * i], dtype=torch.int32))
+        grown.copy_(n + 10)
+        table.copy_(table.flip(0) if i == 1 else table)
+        for t in start[:2]:
+            t.copy_(torch.randn(t.shape, generator=g, device=dev).to(BF))
+        results = []
+        for run in (lambda: (graph.replay(), got)[1], lambda: (other.replay(), got2)[1], step):
+            reset()
+            torch.cuda.synchronize()
+            r = run()
+            torch.cuda.synchronize()
+            results.append([t.clone() for t in (*r, kp, vp, w)])
+        for a in results[:2]:
+            for x, y in zip(a, results[2]):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), f"replay {i}"
+
+
+def test_ops_equal_direct_calls(dev):
+    import tabicl_mi355_paged as paged
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        names: list = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    results = []
+    for mode in (None, Seen()):
+        q, kp, vp, table, n, g = _case(dev, 71, [500, 77], blocks=2)
+        w = torch.zeros(2, table.shape[1] * 64, device=dev)
+        out2 = torch.empty_like(q)
+
+        def step():
+            paged.paged_append(kp[1], vp[1], table, n - 3, q, q)
+            out = paged.paged_attention(q, kp[1], vp[1], table, n, w)
+            paged.paged_attention(q, kp[0], vp[0], table, n, None, None, out2)
+            return (out, out2, w, *paged.paged_evict(kp, vp, table, n, w, 60, 3), kp, vp)
+
+        if mode is None:
+            results.append(step())
+        else:
+            with mode:
+                results.append(step())
+    for name in ("paged_append", "paged_attn.", "paged_attn_out", "paged_evict"):
+        assert any(name in s for s in Seen.names), (name, Seen.names)
+    for a, b in zip(*results):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_gradient_refused(dev):
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, 73, [50])
+    with pytest.raises(ValueError, match="no gradient"):
+        paged.paged_attention(q.requires_grad_(), kp, vp, table, n)
+    with torch.no_grad():
+        paged.paged_attention(q, kp, vp, table, n)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_cache_together(dev, dtype):
+    # tables of different sizes appended block by block, queried with the weights tracked, cut, grown and queried again:
+    # what it answers is attention over the rows it says it holds
+    import tabicl_mi355_paged as paged
+    g = torch.Generator(device=dev).manual_seed(81)
+    S, NB, H, D = 3, 2, 8, 64
+    c = paged.PagedIclKVCache(S, NB, H, D, 1000, 40, 64, dtype, dev, track=True)
+    c.keys.fill_(float("nan"))
+    c.values.fill_(float("nan"))
+    held = [[torch.zeros(0, H, D, dtype=dtype, device=dev)] * S for _ in range(2 * NB)]
+
+    def grow(T, rows):
+        for b in range(NB):
+            k, v = (torch.randn(S, H, T, D, generator=g, device=dev).to(dtype) for _ in range(2))
+            c.append(b, k, v, rows)
+            for s in range(S):
+                r = T if rows is None else rows[s]
+                for i, x in ((2 * b, k), (2 * b + 1, v)):
+                    held[i][s] = torch.cat([held[i][s], x[s, :, :r].transpose(0, 1)])
+
+    def ask(T):
+        before = c.weights.double().clone()
+        total, tols = before.clone(), torch.zeros_like(before)
+        for b in range(NB):
+            q = (torch.randn(S, H, T, D, generator=g, device=dev) * 1.5).to(dtype)
+            out = c.query(b, q)
+            for s in range(S):
+                k, v = held[2 * b][s], held[2 * b + 1][s]
+                pool = [x.transpose(0, 1)[None].contiguous() for x in (k, v)]
+                one = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+                n = torch.tensor([len(k)], dtype=torch.int32, device=dev)
+                want, w, tol, wt = ref.attention(q[s:s + 1], *pool, one, n, D ** -0.5, torch.zeros(1, len(k), device=dev))
+                ref.near(out[s:s + 1], want, tol, f"block {b} sequence {s}")
+                total[s, :len(k)] += w[0]
+                tols[s, :len(k)] += wt[0]
+        ref.near(c.weights, total, tols + total.abs() * NB * 2.0 ** -23 + 2.0 ** -100, "tracked weights")
+
+    grow(300, None)
+    grow(400, [400, 100, 1])
+    ask(1)
+    ask(3)
+    free = c.free_pages
+    index = c.evict(256, recent=10)
+    assert c.free_pages > free and [c.length(0, s) for s in range(S)] == [256, 256, 256]
+    for i in range(2 * NB):
+        held[i] = [held[i][s][index[s].long()] for s in range(S)]
+    ask(2)
+    grow(200, [200, 0, 100])
+    ask(1)
+    c.evict([300, 256, 1])
+    c.release(1)
+    assert [c.length(1, s) for s in range(S)] == [300, 0, 1]
+
+
+def test_cached_query_on_pages(dev):
+    # the whole cached query of two tables on the paged cache against the dense one: the same rows, so logits as far
+    # apart as two roundings of the bf16 attention output allow (parity.py's bf16 bars)
+    import tabicl_mi355_icl as icl
+    import tabicl_mi355_paged as paged
+    import tabicl_mi355_query as Q
+    from parity import check
+    from query_ref import C, E, ICLH, NI, Rope, model, to_device
+    w, g = model(F32)
+    wd = to_device(w, dev)
+    B, T, NF, train = 2, 3, 20, 600
+    X = torch.randn(B, T, NF, generator=g).to(dev)
+    col = Q.ColumnKVCache(3, B, NF + C, NI, E, F32, dev)
+    for b in range(3):
+        col.append_projected(b, torch.randn(B, NF + C, NI, E, generator=g).to(dev), wd.column.blocks[b])
+    dense = icl.IclKVCache(B, 2, ICLH, train, 64, BF, dev)
+    pages = paged.PagedIclKVCache(B, 2, ICLH, 64, 1024, 30, 64, BF, dev, track=True)
+    for b in range(2):
+        x = torch.randn(B, train, 512, generator=g).to(BF).to(dev)
+        dense.append_projected(b, x, wd.icl_blocks[b].in_w, wd.icl_blocks[b].in_b)
+        pages.append_projected(b, x[:, :400], wd.icl_blocks[b].in_w, wd.icl_blocks[b].in_b)
+        pages.append_projected(b, x[:, 400:], wd.icl_blocks[b].in_w, wd.icl_blocks[b].in_b)
+    for valid in (train, 250, torch.tensor([300], device=dev)):
+        with torch.no_grad():
+            want = Q.cached_query(X, None, col, dense, wd, valid, Rope())
+            got = Q.cached_query(X, None, col, pages, wd, valid, Rope())
+        torch.cuda.synchronize()
+        check(got, want, BF, f"logits, valid {valid}", abs_tol=2e-2 * max(1.0, float(want.abs().max())))
+    total = pages.weights.sum(1)
+    assert torch.allclose(total, torch.full_like(total, 3 * 2 * ICLH * T), rtol=1e-4)
+    with torch.no_grad():
+        x = torch.randn(B, T, 512, generator=g).to(dev)
+        a = pages.query_blocks(x, wd.icl_blocks)
+        parts = pages.query_chunked(x, wd.icl_blocks, [(0, 1), (1, 2)])
+    check(parts, a, BF, "chunked", abs_tol=2e-2 * max(1.0, float(a.abs().max())))

@@ -1,0 +1,281 @@
+"""CPU tests of the paged K/V cache: what the wrappers and the C ABI refuse, and PagedIclKVCache's books (pages, lengths,
+weights) with the plain forms in the kernels' place."""
+import pytest
+import torch
+
+import paged_ref as ref
+
+
+def _pool(P=6, H=2, R=16, D=64, dtype=torch.float32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return tuple(torch.randn(P, H, R, D, generator=g).to(dtype) for _ in range(2))
+
+
+def _table(N=2, M=3):
+    return torch.arange(N * M, dtype=torch.int32).view(N, M)
+
+
+def test_no_cpu_path():
+    import tabicl_mi355_native as nat
+    import tabicl_mi355_paged as paged
+    k, v = _pool()
+    t, n, q = _table(), torch.tensor([5, 9], dtype=torch.int32), torch.randn(2, 2, 1, 64)
+    with pytest.raises(nat.NativeLibraryError):
+        paged.paged_attention(q, k, v, t, n)
+    with pytest.raises(nat.NativeLibraryError):
+        paged.paged_append(k, v, t, n, q, q)
+    with pytest.raises(nat.NativeLibraryError):
+        paged.paged_evict(k, v, t, n, torch.zeros(2, 48), 4)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(q=torch.zeros(2, 3, 1, 64)), "multiple of 2 heads"),
+    (dict(q=torch.zeros(3, 2, 1, 64)), "must be"),
+    (dict(q=torch.zeros(2, 2, 1, 32)), "must be"),
+    (dict(q=torch.zeros(2, 2, 64)), "must be"),
+    (dict(q=torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16)), "cast q"),
+    (dict(table=torch.zeros(2, 3, dtype=torch.int64)), "int32"),
+    (dict(table=torch.zeros(6, dtype=torch.int32)), "int32"),
+    (dict(lengths=torch.zeros(2, dtype=torch.int64)), "lengths"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths"),
+    (dict(v=torch.zeros(6, 2, 16, 32)), "one layout"),
+    (dict(k=torch.zeros(6, 16, 2, 64).transpose(1, 2), v=torch.zeros(6, 16, 2, 64).transpose(1, 2)), "contiguous"),
+    (dict(weights=torch.zeros(2, 47)), "weights"),
+    (dict(weights=torch.zeros(2, 48, dtype=torch.float64)), "weights"),
+    (dict(weights=torch.zeros(48, 2).t()), "weights"),
+    (dict(out=torch.zeros(2, 2, 2, 64)), "out"),
+    (dict(q=torch.zeros(2, 2, 1, 64, requires_grad=True)), "no gradient"),
+])
+def test_attention_refuses(change, word):
+    import tabicl_mi355_paged as paged
+    k, v = _pool()
+    a = dict(q=torch.zeros(2, 2, 1, 64), k=k, v=v, table=_table(), lengths=torch.tensor([5, 9], dtype=torch.int32),
+             weights=None, out=None)
+    a.update(change)
+    with pytest.raises(ValueError, match=word):
+        paged.paged_attention(a["q"], a["k"], a["v"], a["table"], a["lengths"], a["weights"], None, a["out"])
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(k=torch.zeros(2, 2, 4, 32), v=torch.zeros(2, 2, 4, 32)), "must be"),
+    (dict(v=torch.zeros(2, 2, 3, 64)), "must be"),
+    (dict(k=torch.zeros(2, 2, 4, 64, dtype=torch.bfloat16)), "cast"),
+    (dict(count=torch.zeros(2, dtype=torch.int64)), "count"),
+    (dict(count=torch.zeros(1, dtype=torch.int32)), "count"),
+    (dict(k=torch.zeros(2, 2, 4, 64, requires_grad=True)), "no gradient"),
+])
+def test_append_refuses(change, word):
+    import tabicl_mi355_paged as paged
+    kp, vp = _pool()
+    a = dict(k=torch.zeros(2, 2, 4, 64), v=torch.zeros(2, 2, 4, 64), count=None)
+    a.update(change)
+    with pytest.raises(ValueError, match=word):
+        paged.paged_append(kp, vp, _table(), torch.zeros(2, dtype=torch.int32), a["k"], a["v"], a["count"])
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(keep=-1), "negative"),
+    (dict(recent=-1), "negative"),
+    (dict(keep=torch.zeros(3, dtype=torch.int32)), "keep"),
+    (dict(keep=torch.zeros(2, dtype=torch.int64)), "keep"),
+    (dict(weights=torch.zeros(2, 40)), "weights"),
+])
+def test_evict_refuses(change, word):
+    import tabicl_mi355_paged as paged
+    kp, vp = _pool()
+    a = dict(weights=torch.zeros(2, 48), keep=4, recent=0)
+    a.update(change)
+    with pytest.raises(ValueError, match=word):
+        paged.paged_evict(kp, vp, _table(), torch.zeros(2, dtype=torch.int32), a["weights"], a["keep"], a["recent"])
+
+
+def test_abi_refuses_before_launch():
+    import tabicl_mi355_native as nat
+    lib = nat.load()
+    a = 0x1000  # 16-byte aligned placeholder address: refused before any use
+
+    def attn(D=64, R=64, H=8, Hq=8, pages=10, sp=None, dtype=0, q=a, scale=0.125, table=a, M=4, w=None, wsn=0, N=2, Tq=1,
+             qs=(512, 64, 512), ws=a, wsb=1 << 40):
+        return lib.tabicl_paged_attn(q, a, a, pages, H * R * D if sp is None else sp, R, table, M, M, a, w, wsn, a, N, Hq,
+                                     H, Tq, D, *qs, 512, 64, 512, scale, dtype, ws, wsb, None)
+
+    for kw, word in ((dict(D=48), "head dim"), (dict(R=24), "power of two"), (dict(R=8), "power of two"),
+                     (dict(Hq=12), "multiple of H"), (dict(dtype=2), "dtype"), (dict(sp=512), "page stride"),
+                     (dict(sp=8 * 64 * 64 + 4), "page stride"), (dict(q=a + 2), "aligned"), (dict(q=None), "aligned"),
+                     (dict(scale=float("nan")), "scale"), (dict(table=None), "table"), (dict(M=1 << 30), "page counts"),
+                     (dict(w=a, wsn=255), "weights"), (dict(qs=(512, 63, 512)), "strides"), (dict(N=70000), "65535"),
+                     (dict(Tq=1 << 23), "query rows"), (dict(w=a, wsn=256, wsb=8), "workspace"),
+                     (dict(pages=-1), "page counts")):
+        assert attn(**kw) == 1 and word in nat.last_error(), (kw, nat.last_error())
+    assert attn(N=0) == 0 and attn(Tq=0, q=None) == 0
+    assert lib.tabicl_paged_attn_workspace_bytes(2, 8, 8, 1, 48, 1000, 0, 0) < 0
+    assert lib.tabicl_paged_attn_workspace_bytes(2, 8, 8, 1, 64, 1000, 1, 0) > 0
+    assert lib.tabicl_paged_evict_workspace_bytes(-1, 4) < 0
+
+    def append(T=3, k=a, ks=(64, 64, 64), N=2):
+        return lib.tabicl_paged_append(a, a, 10, 8 * 64 * 64, 64, a, 4, 4, a, k, a, None, N, 8, T, 64, *ks, 64, 64, 64, 0,
+                                       None)
+
+    for kw, word in ((dict(T=-1), "row count"), (dict(k=a + 8), "aligned"), (dict(ks=(64, 64, 4)), "strides")):
+        assert append(**kw) == 1 and word in nat.last_error(), (kw, nat.last_error())
+    assert append(T=0) == 0 and append(N=0) == 0
+
+    def evict(K=100, recent=0, ws=a, wsb=1 << 40, bsp=0, w=a, N=2):
+        return lib.tabicl_paged_evict(a, a, 1, bsp, 10, 8 * 64 * 64, 64, a, 4, 4, a, w, 256, None, 100, recent, a, K, a, a, N,
+                                      8, 64, 0, ws, wsb, None)
+
+    for kw, word in ((dict(K=257), "capacity"), (dict(recent=-1), "recent"), (dict(ws=None), "workspace"),
+                     (dict(wsb=64), "workspace"), (dict(bsp=4), "block"), (dict(w=None), "weights")):
+        assert evict(**kw) == 1 and word in nat.last_error(), (kw, nat.last_error())
+    assert evict(N=0) == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# PagedIclKVCache
+# ---------------------------------------------------------------------------------------------
+@pytest.fixture
+def plain(monkeypatch):
+    """The plain forms in place of the kernels."""
+    import tabicl_mi355_native as nat
+    import tabicl_mi355_paged as paged
+
+    def attention(q, kp, vp, table, lengths, weights=None, scale=None, out=None):
+        o, w, _, _ = ref.attention(q, kp, vp, table, lengths, q.shape[-1] ** -0.5 if scale is None else scale, weights)
+        if weights is not None:
+            weights.copy_(w)
+        return o.to(q.dtype) if out is None else out.copy_(o)
+
+    def append(kp, vp, table, lengths, k, v, count=None):
+        a, b = ref.append(kp, vp, table, lengths, k, v, count)
+        kp.copy_(a)
+        vp.copy_(b)
+
+    def evict(kp, vp, table, lengths, weights, keep, recent=0):
+        a, b, *rest = ref.evict(kp, vp, table, lengths, weights, keep, recent)
+        kp.copy_(a)
+        vp.copy_(b)
+        return tuple(rest)
+
+    monkeypatch.setattr(nat, "require_device", lambda *t: None)
+    for name, f in (("paged_attention", attention), ("paged_append", append), ("paged_evict", evict)):
+        monkeypatch.setattr(paged, name, f)
+    return paged
+
+
+def _cache(paged, S=3, blocks=2, H=2, D=32, max_rows=100, pages=12, track=True):
+    c = paged.PagedIclKVCache(S, blocks, H, D, max_rows, pages, 16, torch.float32, "cpu", track)
+    c.keys.fill_(float("nan"))
+    c.values.fill_(float("nan"))
+    return c
+
+
+def _rows(c, b, s):
+    n = c.length(b, s)
+    _, page, row = ref.rows_of(c.table[s], n, c.page_rows, c.keys.shape[1])
+    return c.keys[b][page, :, row], c.values[b][page, :, row]
+
+
+def test_cache_appends_and_queries(plain):
+    g = torch.Generator().manual_seed(1)
+    c = _cache(plain)
+    assert c.shape == (3, 2, 2, 112, 32) and c.free_pages == 12
+    want = {b: [(torch.zeros(0, 2, 32),) * 2 for _ in range(3)] for b in range(2)}
+    with pytest.raises(ValueError, match="append before"):
+        c.query(0, torch.zeros(3, 2, 1, 32))
+    for rows in ([20, 1, 0], [1, 1, 1], [15, 40, 16], [0, 0, 0]):
+        T = max(rows)
+        for b in range(2):
+            k, v = (torch.randn(3, 2, T, 32, generator=g) for _ in range(2))
+            c.append(b, k, v, rows)
+            for s in range(3):
+                want[b][s] = tuple(torch.cat([o, x[s, :, :rows[s]].transpose(0, 1)]) for o, x in zip(want[b][s], (k, v)))
+    for b in range(2):
+        for s in range(3):
+            for got, w in zip(_rows(c, b, s), want[b][s]):
+                assert torch.equal(got, w)
+        assert c.lengths[b].tolist() == [36, 42, 17] == [c.length(b, s) for s in range(3)]
+    assert c.free_pages == 12 - 3 - 3 - 2
+    assert (c.table >= 0).sum() == 8 and len(set(c.table[c.table >= 0].tolist())) == 8
+    q = torch.randn(3, 2, 4, 32, generator=g)
+    out = c.query(1, q)
+    for s in range(3):
+        k, v = want[1][s]
+        p = torch.softmax(torch.einsum("htd,rhd->htr", q[s], k) * 32 ** -0.5, -1)
+        assert torch.allclose(out[s], torch.einsum("htr,rhd->htd", p, v), atol=1e-5)
+        assert torch.allclose(c.weights[s, :len(k)], p.sum((0, 1)), atol=1e-5)
+    # a valid length, as a number and per sequence, and an output view
+    for valid in (5, torch.tensor([5, 5, 5]), torch.tensor(5)):
+        o = torch.zeros(3, 4, 2, 32)
+        c.query(1, q, valid, out=o.transpose(1, 2))
+        for s in range(3):
+            k, v = want[1][s][0][:5], want[1][s][1][:5]
+            p = torch.softmax(torch.einsum("htd,rhd->htr", q[s], k) * 32 ** -0.5, -1)
+            assert torch.allclose(o[s], torch.einsum("htr,rhd->thd", p, v), atol=1e-5)
+    view = c.estimators(1, 3)
+    assert torch.allclose(view.query(1, q[1:]), out[1:], atol=1e-6)
+    with pytest.raises(ValueError, match="queries only"):
+        view.append(0, torch.zeros(2, 2, 1, 32), torch.zeros(2, 2, 1, 32))
+
+
+def test_cache_evicts_and_reuses_pages(plain):
+    g = torch.Generator().manual_seed(2)
+    c = _cache(plain)
+    k, v = (torch.randn(3, 2, 60, 32, generator=g) for _ in range(2))
+    for b in range(2):
+        c.append(b, k + b, v - b, [60, 33, 5])
+    assert c.free_pages == 12 - 4 - 3 - 1
+    c.query(0, torch.randn(3, 2, 3, 32, generator=g))
+    before = c.weights.clone()
+    index = c.evict(20, recent=2)
+    assert index.shape == (3, 20) and c.free_pages == 12 - 2 - 2 - 1
+    assert [c.length(1, s) for s in range(3)] == [20, 20, 5] and c.lengths.tolist() == [[20, 20, 5]] * 2
+    for s, n in enumerate((20, 20, 5)):
+        idx = index[s, :n].long()
+        assert (index[s, n:] == -1).all() and len(set(idx.tolist())) == n
+        for b in range(2):
+            kb, vb = _rows(c, b, s)
+            assert torch.equal(kb, (k[s] + b)[:, idx].transpose(0, 1)) and torch.equal(vb, (v[s] - b)[:, idx].transpose(0, 1))
+        assert torch.equal(c.weights[s, :n], before[s, idx]) and (c.weights[s, n:] == 0).all()
+    assert {58, 59} <= set(index[0].tolist())
+    # the freed pages serve the next appends; a per-sequence budget; release
+    for b in range(2):
+        c.append(b, k[:, :, :30], v[:, :, :30], [30, 0, 30])
+    assert c.free_pages == 12 - 4 - 2 - 3
+    c.evict([50, 7, 0])
+    assert [c.length(0, s) for s in range(3)] == [50, 7, 0] and c.free_pages == 12 - 4 - 1
+    c.release(0)
+    assert c.free_pages == 11 and c.length(0, 0) == 0 and (c.table[0] == -1).all() and (c.weights[0] == 0).all()
+
+
+def test_cache_refuses(plain):
+    c = _cache(plain, track=False)
+    z = torch.zeros(3, 2, 4, 32)
+    with pytest.raises(ValueError, match="power of two"):
+        plain.PagedIclKVCache(1, 1, 2, 32, 100, 4, 24, device="cpu")
+    with pytest.raises(ValueError, match="append expects"):
+        c.append(0, z[:2], z[:2])
+    with pytest.raises(ValueError, match="out of range"):
+        c.append(2, z, z)
+    with pytest.raises(ValueError, match="counts from 0"):
+        c.append(0, z, z, [1, 2, 5])
+    with pytest.raises(ValueError, match="cast"):
+        c.append(0, z.bfloat16(), z.bfloat16())
+    with pytest.raises(ValueError, match="capacity"):
+        c.reserve(113)
+    with pytest.raises(ValueError, match="pages wanted"):
+        c.reserve(100)
+    assert c.free_pages == 12 and (c.table == -1).all()  # a refused call changes nothing
+    c.append(0, z, z)
+    with pytest.raises(ValueError, match="track"):
+        c.evict(2)
+    with pytest.raises(ValueError, match="wider"):
+        c.query(0, torch.zeros(3, 2, 1, 32, dtype=torch.float64))
+    t = _cache(plain)
+    t.append(0, z, z)
+    with pytest.raises(ValueError, match="different rows"):
+        t.evict(2)
+    t.append(1, z, z)
+    with pytest.raises(ValueError, match="keep"):
+        t.evict([1, 2])
+    with pytest.raises(ValueError, match="keep"):
+        t.evict(-1)
