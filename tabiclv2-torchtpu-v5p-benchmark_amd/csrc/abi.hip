@@ -781,6 +781,7 @@ int tabicl_paged_attn(const void* q, const void* k_pages, const void* v_pages, i
   if (!(scale > -1e30f && scale < 1e30f)) return fail(1, "paged_attn: scale must be finite");
   if (weights && (((uintptr_t)weights & 3) || weights_sn < max_pages * page_rows))
     return fail(1, "paged_attn: weights needs rows of max_pages * page_rows values");
+  if (weights && N * max_pages * page_rows > (1LL << 29)) return fail(1, "paged_attn: weights for more than 2^29 rows");
   const int64_t need = tabicl_launch_paged_attn_ws_bytes(N, Hq, H, Tq, D, max_pages * page_rows, weights != nullptr, dtype);
   if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need))
     return fail(1, "paged_attn: workspace of %lld bytes (16-byte aligned) required", (long long)need);
