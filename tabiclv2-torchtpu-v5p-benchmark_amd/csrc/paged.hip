@@ -442,90 +442,162 @@ __device__ __forceinline__ EvictSizes evict_sizes(const PagedEvict& a, int n) {
   return z;
 }
 
-// The number of set flags before this thread's, and the workgroup's total.
-__device__ __forceinline__ int block_rank(bool flag, int* sh, int* total) {
-  const uint64_t b = __ballot(flag);
+// Selection, one workgroup per sequence: the threshold code by three digits (11, 11 and 10 bits) of a histogram in LDS,
+// then ranks. Wave w holds the rows [w seg, (w + 1) seg), lane l of step i row w seg + 64 i + l, so that a rank is the
+// count of earlier flags of the wave (ballots) and of the waves before it: two barriers per rank, none per step. Up to
+// PE_HELD steps the codes stay in registers from the first pass on; longer sequences read their weights again (from L2)
+// in each of the six passes.
+constexpr int PE_NW = PE_NT / 64, PE_HELD = 16, PE_BINS = 2048;
+
+// The exclusive sums over the waves of three counts each, in sh; returns this wave's, total in *all.
+__device__ __forceinline__ int wave_scan(int count, int* sh, int* all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __syncthreads();
-  if (lane == 0) sh[wave] = __popcll(b);
+  if (lane == 0) sh[wave] = count;
   __syncthreads();
-  int before = __popcll(b & ((1ull << lane) - 1)), sum = 0;
-  for (int w = 0; w < PE_NT / 64; ++w) {
-    before += w < wave ? sh[w] : 0;
-    sum += sh[w];
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < PE_NW; ++w) {
+    const int x = sh[w];
+    before += w < wave ? x : 0;
+    sum += x;
   }
-  *total = sum;
+  *all = sum;
   return before;
 }
 
-// pairs [N, K]: (source row << 32 | place) of the rows that move, count in npairs[n].
-__global__ __launch_bounds__(PE_NT) void paged_select_kernel(PagedEvict a, int64_t* pairs, int32_t* npairs) {
-  __shared__ int hist[256], sh[PE_NT / 64], pick[2];
-  const int n = blockIdx.x, tid = threadIdx.x;
-  const EvictSizes z = evict_sizes(a, n);
+template <bool HELD>
+__device__ __forceinline__ void evict_select(const PagedEvict& a, int n, const EvictSizes z, int64_t* pairs, int32_t* npairs,
+                                             int* hist, int* sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* w = a.weights + n * a.weights_sn;
   const int64_t cap = (int64_t)a.pool.max_pages << a.pool.shift;
-  const int free_rows = z.len - z.recent;
-  int want = z.kept - z.recent;  // of the rows [0, free_rows)
-  // threshold code: the want-th largest, one digit of 8 bits at a time
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int r = tid; r < free_rows; r += PE_NT) {
-      const uint32_t c = weight_code(w[r]);
-      if (shift == 24 || (c >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(c >> shift) & 255], 1);
+  const int free_rows = z.len - z.recent;  // the rows that compete
+  const int steps = ((z.len + PE_NT - 1) / PE_NT), base = wave * steps * 64 + lane;
+  uint32_t held[HELD ? PE_HELD : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int i = 0; i < PE_HELD; ++i) {
+      const int r = base + i * 64;
+      held[i] = i < steps && r < free_rows ? weight_code(w[r]) : 0;
     }
-    __syncthreads();
-    if (tid == 0) {
-      int left = want, b = 255;
-      for (; b > 0 && hist[b] < left; --b) left -= hist[b];
-      pick[0] = b;
-      pick[1] = left;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)pick[0] << shift;
-    want = pick[1];
-    __syncthreads();
   }
-  // want: rows of exactly the threshold's weight that are kept, the lowest ones
-  const bool any = z.kept > z.recent;
-  int64_t* pr = pairs + (int64_t)n * a.K;
+  // f(step, row, code) over this lane's rows in order
+  auto each = [&](auto f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int i = 0; i < PE_HELD; ++i)
+        if (i < steps) f(base + i * 64, held[i]);
+    } else {
+      for (int i = 0; i < steps; i += 8) {
+        uint32_t c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = base + (i + j) * 64;
+          c[j] = i + j < steps && r < free_rows ? weight_code(w[r]) : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (i + j < steps) f(base + (i + j) * 64, c[j]);
+      }
+    }
+  };
+  int want = z.kept - z.recent;  // of the rows [0, free_rows); in the end, of those of the threshold's weight
+  const bool any = want > 0;
+  uint32_t prefix = 0;
+  if (any) {
+#pragma unroll
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
+      for (int i = tid; i < PE_BINS; i += PE_NT) hist[i] = 0;
+      __syncthreads();
+      each([&](int r, uint32_t c) {
+        const bool in = r < free_rows && (digit == 0 || (c >> (shift + bits)) == (prefix >> (shift + bits)));
+        if (in) atomicAdd(&hist[(c >> shift) & ((1u << bits) - 1)], 1);
+      });
+      __syncthreads();
+      // thread t sums the bins 2 t' and 2 t' + 1 with t' counted from the top: the first digit whose count from above
+      // reaches `want`
+      const int top = PE_BINS - 2 * tid - 1;
+      const int h1 = hist[top], h0 = hist[top - 1];
+      int incl = h0 + h1;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(incl, d, 64);
+        if (lane >= d) incl += y;
+      }
+      int all;
+      const int before = wave_scan(__shfl(incl, 63, 64), sh, &all) + incl - h0 - h1;
+      __syncthreads();
+      if (before < want && before + h0 + h1 >= want) {  // one thread
+        const bool first = before + h1 >= want;
+        sh[0] = first ? top : top - 1;
+        sh[1] = want - before - (first ? 0 : h1);
+      }
+      __syncthreads();
+      prefix |= (uint32_t)sh[0] << shift;
+      want = sh[1];
+      __syncthreads();
+    }
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  int ties = 0, all;
+  each([&](int r, uint32_t c) { ties += __popcll(__ballot(any && r < free_rows && c == prefix)); });
+  const int tie0 = wave_scan(ties, sh, &all);
+  auto kept = [&](int r, uint32_t c, int& at) {
+    const bool tie = any && r < free_rows && c == prefix;
+    const uint64_t b = __ballot(tie);
+    const bool k = r < z.len && (r >= free_rows || (any && c > prefix) || (tie && at + __popcll(b & below) < want));
+    at += __popcll(b);
+    return k;
+  };
+  int holes = 0, tails = 0, at = tie0;
+  each([&](int r, uint32_t c) {
+    const bool k = kept(r, c, at);
+    holes += __popcll(__ballot(r < z.kept && !k));
+    tails += __popcll(__ballot(r >= z.kept && k));
+  });
+  int hole = wave_scan(holes, sh, &all), tail = wave_scan(tails, sh, &all);
+  const int moves = all;
+  int32_t* pr = (int32_t*)(pairs + (int64_t)n * a.K);
   int32_t* index = a.index + (int64_t)n * a.K;
   float* kw = a.kept_weights + n * cap;
-  int ties = 0, holes = 0, tails = 0;
-  for (int r0 = 0; r0 < z.len; r0 += PE_NT) {
-    const int r = r0 + tid;
-    const uint32_t c = r < free_rows ? weight_code(w[r]) : 0;
-    int total;
-    const bool tie = any && r < free_rows && c == prefix;
-    const int tie_rank = ties + block_rank(tie, sh, &total);
-    ties += total;
-    const bool keep = r < z.len && (r >= free_rows || (any && c > prefix) || (tie && tie_rank < want));
-    const bool hole = r < z.kept && !keep, tail = r >= z.kept && keep;
-    const int hole_rank = holes + block_rank(hole, sh, &total);
-    holes += total;
-    const int tail_rank = tails + block_rank(tail, sh, &total);
-    tails += total;
-    if (hole) ((int32_t*)(pr + hole_rank))[0] = r;
-    if (tail) ((int32_t*)(pr + tail_rank))[1] = r;
-    if (keep && r < z.kept) {
+  at = tie0;
+  each([&](int r, uint32_t c) {
+    const bool k = kept(r, c, at), is_hole = r < z.kept && !k, is_tail = r >= z.kept && k;
+    const uint64_t bh = __ballot(is_hole), bt = __ballot(is_tail);
+    if (is_hole) pr[2 * (hole + __popcll(bh & below))] = r;
+    if (is_tail) pr[2 * (tail + __popcll(bt & below)) + 1] = r;
+    hole += __popcll(bh);
+    tail += __popcll(bt);
+    if (k && r < z.kept) {
       index[r] = r;
       kw[r] = w[r];
     }
-  }
+  });
   __syncthreads();
-  for (int i = tid; i < holes; i += PE_NT) {
-    const int to = ((int32_t*)(pr + i))[0], from = ((int32_t*)(pr + i))[1];
+  for (int i = tid; i < moves; i += PE_NT) {
+    const int to = pr[2 * i], from = pr[2 * i + 1];
     index[to] = from;
     kw[to] = w[from];
   }
   for (int r = z.kept + tid; r < a.K; r += PE_NT) index[r] = -1;
   for (int64_t r = z.kept + tid; r < cap; r += PE_NT) kw[r] = 0.f;
   if (tid == 0) {
-    npairs[n] = holes;
+    npairs[n] = moves;
     a.kept_lengths[n] = z.kept;
   }
+}
+
+// pairs [N, K]: (place, source row) of the rows that move, their count in npairs[n].
+__global__ __launch_bounds__(PE_NT) void paged_select_kernel(PagedEvict a, int64_t* pairs, int32_t* npairs) {
+  __shared__ int hist[PE_BINS], sh[PE_NW];
+  const int n = blockIdx.x;
+  const EvictSizes z = evict_sizes(a, n);
+  if (z.len <= PE_HELD * PE_NT)
+    evict_select<true>(a, n, z, pairs, npairs, hist, sh);
+  else
+    evict_select<false>(a, n, z, pairs, npairs, hist, sh);
 }
 
 __global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a, const int64_t* pairs, const int32_t* npairs, int es) {

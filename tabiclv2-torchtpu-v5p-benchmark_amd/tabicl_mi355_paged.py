@@ -27,103 +27,103 @@ import tabicl_mi355_icl as _icl
 import tabicl_mi355_native as _nat
 
 
-def _rows16(t: Tensor) -> Tensor:
-    """t when its last dim is contiguous and it starts, and its other dims step, in multiples of 16 bytes (what the
-    kernels' loads need), else a contiguous copy."""
-    es = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-            t.shape[i] == 1 or t.stride(i) * es % 16 == 0 for i in range(t.dim() - 1)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+# A call of few rows is over in 10 us on the GPU; the checks below cost 4 us on a CPU core of the box (12 as one test and
+# one generator expression per property).
+def _rows16(t: Tensor, es: int):
+    """(t, its (n, h, row) element strides) of [N, H, T, D] when its last dim is contiguous and it starts, and its other
+    dims step, in multiples of 16 bytes (what the kernels' loads need), else of a contiguous copy. A dim of one entry,
+    whose stride says nothing, counts as stride 0."""
+    n, h, r, d = t.stride()
+    shape = t.shape
+    n, h, r = n if shape[0] > 1 else 0, h if shape[1] > 1 else 0, r if shape[2] > 1 else 0
+    if (d == 1 or shape[3] == 1) and ((n | h | r) * es | t.data_ptr()) & 15 == 0:
+        return t, n, h, r
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3]
 
 
-def _steps(t: Tensor):
-    """(n, h, row) element strides of a [N, H, T, D] view; 0 for a dim of one entry, whose stride says nothing."""
-    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(3))
-
-
-def _check_pool(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor) -> None:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
-        raise ValueError(f"k_pages and v_pages must be [pages, H, page_rows, D] of one layout, got {tuple(k_pages.shape)} "
-                         f"and {tuple(v_pages.shape)}")
-    P, H, R, D = k_pages.shape
-    if P > 0 and (k_pages.stride(3) != 1 or k_pages.stride(2) != D or (H > 1 and k_pages.stride(1) != R * D)):
+def _pool_args(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, lead: int = 0):
+    """Checks a pool [pages, H, page_rows, D] (behind `lead` more dims) with its table and lengths; returns (pages, page
+    stride, page_rows, table, table stride, max_pages) as the entry points take them, then H, D, N, device index, dtype
+    code."""
+    shape, st = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 + lead or v_pages.shape != shape or v_pages.stride() != st:
+        raise ValueError(f"k_pages and v_pages must be [{'blocks, ' * lead}pages, H, page_rows, D] of one layout, got "
+                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
+    P, H, R, D = shape[lead:]
+    if st[-1] != 1 or st[-2] != D or (st[-3] != R * D and H > 1):
         raise ValueError("a page [H, page_rows, D] must be contiguous")
-    if k_pages.dtype != v_pages.dtype:
+    if k_pages.dtype is not v_pages.dtype:
         raise ValueError("k_pages and v_pages must share a dtype")
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+    ts = table.shape
+    if table.dtype is not torch.int32 or len(ts) != 2 or (table.stride(1) != 1 and ts[1] > 1):
         raise ValueError("table must be an int32 [N, max_pages] tensor with contiguous rows")
-    if lengths.dtype != torch.int32 or lengths.shape != (table.shape[0],) or not lengths.is_contiguous():
-        raise ValueError(f"lengths must be a contiguous int32 tensor of {table.shape[0]} entries")
-    if any(t.device != k_pages.device for t in (v_pages, table, lengths)):
+    N, M = ts
+    if lengths.dtype is not torch.int32 or lengths.shape != (N,) or (N > 1 and lengths.stride(0) != 1):
+        raise ValueError(f"lengths must be a contiguous int32 tensor of {N} entries")
+    dev = k_pages.get_device()
+    if v_pages.get_device() != dev or table.get_device() != dev or lengths.get_device() != dev:
         raise ValueError("the pool, table and lengths must be on one device")
+    return (P, st[lead] if P > 1 else H * R * D, R, table.data_ptr(), table.stride(0) if N > 1 else M, M), H, D, N, dev, \
+        _nat.dtype_code(k_pages.dtype)
 
 
-def _pool_args(k_pages: Tensor, table: Tensor):
-    """(pages, page stride, page_rows, table, table stride, max_pages) as the entry points take them."""
-    P, H, R, D = k_pages.shape
-    return (P, k_pages.stride(0) if P > 1 else H * R * D, R, table.data_ptr(),
-            table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1])
-
-
-def _check_weights(weights: Tensor, table: Tensor, R: int, what: str) -> None:
-    if weights.dtype != torch.float32 or weights.dim() != 2 or weights.shape[0] != table.shape[0] \
-            or weights.shape[1] < table.shape[1] * R or (weights.shape[1] > 1 and weights.stride(1) != 1) \
-            or weights.device != table.device:
-        raise ValueError(f"{what} must be a float32 [{table.shape[0]}, >= {table.shape[1] * R}] tensor with contiguous "
-                         f"rows on the table's device, got {weights.dtype} {tuple(weights.shape)}")
-
-
-class _On:
-    """Launches on a tensor's device: a HIP launch goes by the current one."""
-
-    def __init__(self, t: Tensor):
-        self.guard = None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _check_weights(weights: Tensor, N: int, cap: int, dev: int) -> int:
+    """The row stride of weights [N, >= cap]."""
+    shape = weights.shape
+    if weights.dtype is not torch.float32 or len(shape) != 2 or shape[0] != N or shape[1] < cap \
+            or (shape[1] > 1 and weights.stride(1) != 1) or weights.get_device() != dev:
+        raise ValueError(f"weights must be a float32 [{N}, >= {cap}] tensor with contiguous rows on the table's device, got "
+                         f"{weights.dtype} {tuple(shape)}")
+    return weights.stride(0) if N > 1 else shape[1]
 
 
 _WS_BYTES: dict = {}
 
 
+def _ws_bytes(key: tuple, N: int, Hq: int, H: int, Tq: int, D: int, rows: int, weighted: int, code: int) -> int:
+    nbytes = int(_nat.load().tabicl_paged_attn_workspace_bytes(N, Hq, H, Tq, D, rows, weighted, code))
+    if nbytes < 0:
+        raise _nat.UnsupportedShapeError(f"tabicl_paged_attn: {_nat.last_error()}")
+    if len(_WS_BYTES) >= 4096:  # lengths that grow row by row bring new keys for ever
+        _WS_BYTES.clear()
+    _WS_BYTES[key] = nbytes
+    return nbytes
+
+
 def _attn_launch(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Optional[Tensor],
                  scale: float, out: Tensor) -> None:
-    _check_pool(k_pages, v_pages, table, lengths)
-    P, H, R, D = k_pages.shape
-    if q.dim() != 4 or q.shape[0] != table.shape[0] or q.shape[3] != D or q.shape[1] % H:
-        raise ValueError(f"q must be [{table.shape[0]}, a multiple of {H} heads, Tq, {D}], got {tuple(q.shape)}")
-    if out.shape != q.shape or out.dtype != q.dtype or q.dtype != k_pages.dtype:
+    pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths)
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != N or shape[3] != D or shape[1] % max(1, H):
+        raise ValueError(f"q must be [{N}, a multiple of {H} heads, Tq, {D}], got {tuple(shape)}")
+    if out.shape != shape or out.dtype is not q.dtype or q.dtype is not k_pages.dtype:
         raise ValueError("out must match q, and both the pool's dtype (cast q to the cache dtype first)")
-    if q.device != k_pages.device or out.device != q.device:
+    if q.get_device() != dev or out.get_device() != dev:
         raise ValueError("q, out and the pool must be on one device")
+    rows = pool[5] * pool[2]
+    w_ptr = w_sn = 0
     if weights is not None:
-        _check_weights(weights, table, R, "weights")
-    _nat.require_device(q)
-    N, Hq, Tq, _ = q.shape
-    code = _nat.dtype_code(q.dtype)
-    q = _rows16(q)
-    with _On(q):
-        key = (N, Hq, H, Tq, D, table.shape[1] * R, weights is None, code, q.get_device())
-        nbytes = _WS_BYTES.get(key)
-        if nbytes is None:
-            nbytes = int(_nat.load().tabicl_paged_attn_workspace_bytes(N, Hq, H, Tq, D, table.shape[1] * R,
-                                                                       int(weights is not None), code))
-            if nbytes < 0:
-                raise _nat.UnsupportedShapeError(f"tabicl_paged_attn: {_nat.last_error()}")
-            if len(_WS_BYTES) >= 4096:  # lengths that grow row by row bring new keys for ever
-                _WS_BYTES.clear()
-            _WS_BYTES[key] = nbytes
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _nat.call("tabicl_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), *_pool_args(k_pages, table),
-                  lengths.data_ptr(), _nat.ptr(weights), 0 if weights is None else max(weights.stride(0), weights.shape[1]),
-                  out.data_ptr(), N, Hq, H, Tq, D, *_steps(q), *_steps(out), float(scale), code, _nat.ptr(ws), nbytes,
-                  _nat.stream_of(q))
+        w_sn = _check_weights(weights, N, rows, dev)
+        w_ptr = weights.data_ptr()
+    if dev != torch.cuda.current_device() if dev >= 0 else True:  # a HIP launch goes by the current device
+        _nat.require_device(q)
+        with torch.cuda.device(dev):
+            return _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, out)
+    _, Hq, Tq, _ = shape
+    q, qn, qh, qr = _rows16(q, q.element_size())
+    on, oh, orow, od = out.stride()
+    if od != 1:
+        raise ValueError("out needs a contiguous last dim")
+    on, oh, orow = on if N > 1 else 0, oh if Hq > 1 else 0, orow if Tq > 1 else 0
+    key = (N, Hq, H, Tq, D, rows, w_ptr != 0, code, dev)
+    nbytes = _WS_BYTES.get(key)
+    if nbytes is None:
+        nbytes = _ws_bytes(key, N, Hq, H, Tq, D, rows, w_ptr != 0, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _nat.call("tabicl_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), *pool, lengths.data_ptr(),
+              w_ptr or None, w_sn, out.data_ptr(), N, Hq, H, Tq, D, qn, qh, qr, on, oh, orow, scale, code,
+              None if ws is None else ws.data_ptr(), nbytes, _nat.stream_of(q))
 
 
 @torch.library.custom_op("tabicl::paged_attn", mutates_args=("weights",))
@@ -171,15 +171,16 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     The work is split over the cached rows, so one test row over one long table fills the GPU; a table slice
     table[:, :w] that covers the longest sequence spares the workgroups of pages nobody holds. For up to a few hundred
     query rows (each group of 64 reads the cache again). No gradient."""
-    _no_grad("paged_attention", q, k_pages, v_pages)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, table, lengths, weights, out):
-        o = torch.empty(q.shape, device=q.device, dtype=q.dtype) if out is None else out
+        o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
         _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, o)
-        for t in (out, weights):
-            if t is not None:
-                torch.autograd.graph.increment_version(t)
+        if out is not None:
+            torch.autograd.graph.increment_version(out)
+        if weights is not None:
+            torch.autograd.graph.increment_version(weights)
         return o
+    _no_grad("paged_attention", q, k_pages, v_pages, weights, out)
     if out is None:
         return torch.ops.tabicl.paged_attn(q, k_pages, v_pages, table, lengths, weights, scale)
     torch.ops.tabicl.paged_attn_out(q, k_pages, v_pages, table, lengths, weights, scale, out)
@@ -188,23 +189,27 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
 
 def _append_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: Tensor, v: Tensor,
                    count: Optional[Tensor]) -> None:
-    _check_pool(k_pages, v_pages, table, lengths)
-    P, H, R, D = k_pages.shape
-    N = table.shape[0]
-    if k.dim() != 4 or k.shape != v.shape or k.shape[:2] != (N, H) or k.shape[3] != D:
-        raise ValueError(f"k and v must be [{N}, {H}, T, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
+    pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths)
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or shape[0] != N or shape[1] != H or shape[3] != D:
+        raise ValueError(f"k and v must be [{N}, {H}, T, {D}], got {tuple(shape)} and {tuple(v.shape)}")
+    if k.dtype is not k_pages.dtype or v.dtype is not k_pages.dtype:
         raise ValueError(f"paged_append expects {k_pages.dtype} (cast before appending)")
-    if count is not None and (count.dtype != torch.int32 or count.shape != (N,) or not count.is_contiguous()):
-        raise ValueError(f"count must be a contiguous int32 tensor of {N} entries")
-    if any(t is not None and t.device != k_pages.device for t in (k, v, count)):
-        raise ValueError("k, v, count and the pool must be on one device")
-    _nat.require_device(k)
-    k, v = _rows16(k), _rows16(v)
-    with _On(k):
-        _nat.call("tabicl_paged_append", k_pages.data_ptr(), v_pages.data_ptr(), *_pool_args(k_pages, table),
-                  lengths.data_ptr(), k.data_ptr(), v.data_ptr(), _nat.ptr(count), N, H, k.shape[2], D, *_steps(k),
-                  *_steps(v), _nat.dtype_code(k.dtype), _nat.stream_of(k))
+    if count is not None and (count.dtype is not torch.int32 or count.shape != (N,) or not count.is_contiguous()
+                              or count.get_device() != dev):
+        raise ValueError(f"count must be a contiguous int32 tensor of {N} entries on the pool's device")
+    if k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("k, v and the pool must be on one device")
+    if dev != torch.cuda.current_device() if dev >= 0 else True:
+        _nat.require_device(k)
+        with torch.cuda.device(dev):
+            return _append_launch(k_pages, v_pages, table, lengths, k, v, count)
+    es = k.element_size()
+    k, kn, kh, kr = _rows16(k, es)
+    v, vn, vh, vr = _rows16(v, es)
+    _nat.call("tabicl_paged_append", k_pages.data_ptr(), v_pages.data_ptr(), *pool, lengths.data_ptr(), k.data_ptr(),
+              v.data_ptr(), None if count is None else count.data_ptr(), N, H, shape[2], D, kn, kh, kr, vn, vh, vr, code,
+              _nat.stream_of(k))
 
 
 @torch.library.custom_op("tabicl::paged_append", mutates_args=("k_pages", "v_pages"))
@@ -225,45 +230,44 @@ def paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tenso
     pool (any strides with a contiguous last dim, e.g. the heads of a K|V projection). lengths is read, not changed: the
     other blocks of a model append at the same rows. Rows that the table has no page for are dropped. Two sequences
     must not share a page that is written."""
-    _no_grad("paged_append", k_pages, v_pages, k, v)
     if _nat.direct(k_pages, v_pages, table, lengths, k, v, count):
         _append_launch(k_pages, v_pages, table, lengths, k, v, count)
-        torch.autograd.graph.increment_version(k_pages)
-        torch.autograd.graph.increment_version(v_pages)
+        torch.autograd.graph.increment_version((k_pages, v_pages))
     else:
+        _no_grad("paged_append", k_pages, v_pages, k, v)
         torch.ops.tabicl.paged_append(k_pages, v_pages, table, lengths, k, v, count)
 
 
 def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int,
                   recent: int, keep_n: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
-    if k_pages.dim() != 5 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
-        raise ValueError(f"k_pages and v_pages must be [blocks, pages, H, page_rows, D] of one layout, got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    B, P, H, R, D = k_pages.shape
-    if B > 0:
-        _check_pool(k_pages[0], v_pages[0], table, lengths)
-    N, cap = table.shape[0], table.shape[1] * R
-    _check_weights(weights, table, R, "weights")
+    pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths, 1)
+    w_sn = _check_weights(weights, N, pool[2] * pool[5], dev)
     if keep < 0 or recent < 0:
         raise ValueError(f"keep and recent must not be negative, got {keep} and {recent}")
-    if keep_n is not None and (keep_n.dtype != torch.int32 or keep_n.shape != (N,) or not keep_n.is_contiguous()
-                               or keep_n.device != table.device):
+    if keep_n is not None and (keep_n.dtype is not torch.int32 or keep_n.shape != (N,) or not keep_n.is_contiguous()
+                               or keep_n.get_device() != dev):
         raise ValueError(f"keep must be a number or a contiguous int32 tensor of {N} entries on the table's device")
-    _nat.require_device(table)
+    if dev != torch.cuda.current_device() if dev >= 0 else True:
+        _nat.require_device(table)
+        with torch.cuda.device(dev):
+            return _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n)
+    B, cap = k_pages.shape[0], pool[2] * pool[5]
     K = min(keep, cap)
-    with _On(table):
-        index = torch.empty(N, K, dtype=torch.int32, device=table.device)
-        kept_weights = torch.empty(N, cap, dtype=torch.float32, device=table.device)
-        kept = torch.empty(N, dtype=torch.int32, device=table.device)
+    index = table.new_empty(N, K)
+    kept_weights = weights.new_empty(N, cap)
+    kept = table.new_empty(N)
+    key = (N, K)
+    nbytes = _WS_BYTES.get(key)
+    if nbytes is None:
         nbytes = int(_nat.load().tabicl_paged_evict_workspace_bytes(N, K))
         if nbytes < 0:
             raise _nat.UnsupportedShapeError(f"tabicl_paged_evict: {_nat.last_error()}")
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=table.device)
-        pool = _pool_args(k_pages[0], table) if B > 0 else (0, H * R * D, R, table.data_ptr(), cap, table.shape[1])
-        _nat.call("tabicl_paged_evict", k_pages.data_ptr(), v_pages.data_ptr(), B, k_pages.stride(0) if B > 1 else 0, *pool,
-                  lengths.data_ptr(), weights.data_ptr(), max(weights.stride(0), weights.shape[1]), _nat.ptr(keep_n), keep,
-                  recent, index.data_ptr(), K, kept_weights.data_ptr(), kept.data_ptr(), N, H, D,
-                  _nat.dtype_code(k_pages.dtype), ws.data_ptr(), ws.numel(), _nat.stream_of(table))
+        _WS_BYTES[key] = nbytes = max(nbytes, 16)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=table.device)
+    _nat.call("tabicl_paged_evict", k_pages.data_ptr(), v_pages.data_ptr(), B, k_pages.stride(0) if B > 1 else 0, *pool,
+              lengths.data_ptr(), weights.data_ptr(), w_sn, None if keep_n is None else keep_n.data_ptr(), keep, recent,
+              index.data_ptr(), K, kept_weights.data_ptr(), kept.data_ptr(), N, H, D, code, ws.data_ptr(), nbytes,
+              _nat.stream_of(table))
     return index, kept_weights, kept
 
 
@@ -290,17 +294,16 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
     keep, or the capacity for a tensor), the weights in their new slots [N, max_pages page_rows] (0 past the cut) and
     kept [N] int32. weights, table and lengths are not changed: take over the new ones. No two sequences may share a
     page."""
-    _no_grad("paged_evict", k_pages, v_pages, weights)
-    if k_pages.dim() == 4:
+    if k_pages.dim() == 4 and v_pages.dim() == 4:
         k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
     keep_n = None
     if isinstance(keep, Tensor):
         keep, keep_n = table.shape[1] * k_pages.shape[3], keep
     if _nat.direct(k_pages, v_pages, table, lengths, weights, keep_n):
         r = _evict_launch(k_pages, v_pages, table, lengths, weights, int(keep), int(recent), keep_n)
-        torch.autograd.graph.increment_version(k_pages)
-        torch.autograd.graph.increment_version(v_pages)
+        torch.autograd.graph.increment_version((k_pages, v_pages))
         return r
+    _no_grad("paged_evict", k_pages, v_pages, weights)
     return torch.ops.tabicl.paged_evict(k_pages, v_pages, table, lengths, weights, int(keep), int(recent), keep_n)
 
 
