@@ -27,9 +27,9 @@ __device__ __forceinline__ int64_t pool_row(const PagedPool& c, int n, int h, in
 // attention
 // ---------------------------------------------------------------------------------------------
 // Bound by the bytes of K and V, which are read once: a workgroup takes `chunk` rows of one (sequence, K/V head) and up
-// to 16 QT of its query rows (the heads of a group and the query rows together), its four waves take turns of KS rows.
+// to 16 QT of its query rows (the heads of a group and the query rows together), its NW waves take turns of KS rows.
 // Nothing of K and V is shared between waves, so they go from memory straight into the registers of the matrix products,
-// a turn ahead of their use; LDS only joins the four waves at the end.
+// a turn ahead of their use; LDS only joins the waves at the end.
 //   S^T = K Q^T  (16 keys x 16 queries): the A operand is 16 bytes of a K row per lane, the result holds query l % 16,
 //                keys 4 (l / 16) + i, which is the B operand of
 //   O^T = V^T P^T with the keys in that order: the A operand holds the values of column group l % 16 (D / 16 columns, one
@@ -38,18 +38,104 @@ __device__ __forceinline__ int64_t pool_row(const PagedPool& c, int n, int h, in
 // alone; the second product costs nothing beside the loads. fp32 runs on the fp32 matrix unit.
 // Softmax: p = 2^(s - ref) with ref the running maximum + PA_SHIFT, moved only when a score passes it by more than 2^8
 // (one test per turn); the shift keeps sums of 2^30 products with values near the largest float finite.
-constexpr int PA_NW = 4;
 constexpr float PA_SHIFT = 24.f, PA_SLACK = 8.f;
 constexpr float PA_REF0 = -3.4028234663852886e38f;
 
+// The work is cut on the device, by the lengths as they are: a unit is PA_UNIT rows of one item (sequence, K/V head, query
+// tile), units are counted item after item, and workgroup w of G takes the units [w T / G, (w + 1) T / G) of all T: an equal
+// share whatever the lengths, with G two per CU. An item that one workgroup covers is
+// written at once; of the others each workgroup leaves a partial (at most two: one of an item begun before it, one of an
+// item it begins), which pa_merge_kernel joins. (A fixed number of rows per workgroup: 64 sequences of 500 to 10,000 rows
+// took 97 us at 8 workgroups per CU and 146 at 2, one sequence of 45,000 rows 39 and 27.)
+constexpr int PA_UNIT = 128, PA_WHOLE = 1024;
+
 struct PagedSplit {
-  int chunk, splits, qtiles;
-  int turn;      // (split turn + blockIdx) % 8 advances by one from split to split
-  float* part;   // [N H][splits][rows][D] unnormalised outputs
-  float2* ml;    // [N H][splits][rows] (ref, sum)
-  float2* stat;  // [N H][rows] (ref, 1 / sum), for the weights
-  float* score;  // [N H][rows][score_sn] scores in log2 units, for the weights
+  int groups;    // G, or 0: a workgroup of eight waves for each item
+  int least;     // units a workgroup takes at least
+  int qtiles;
+  float* part;   // [2 G][16 QT][D] unnormalised outputs
+  float2* ml;    // [2 G][16 QT] (ref, sum)
+  float2* stat;  // [N Hq Tq] (ref, 1 / sum), for the weights
+  float* score;  // [N Hq Tq][score_sn] scores in log2 units, for the weights
   int64_t score_sn;
+};
+
+__device__ __forceinline__ int pa_len(const PagedAttn& a, int n) { return a.pool.pages > 0 ? pool_length(a.pool, n) : 0; }
+
+__device__ __forceinline__ int pa_units(int len) { return (len + PA_UNIT - 1) / PA_UNIT; }
+
+// Inclusive sum over the lanes of a wave, in the registers.
+__device__ __forceinline__ int wave_sum_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8 within 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
+// The units of the sequences, 64 sequences at a time, one per lane.
+struct PagedUnits {
+  const PagedAttn& a;
+  int per, lane;  // items of a sequence
+  int own, upto;  // sequence `lane`: its units, and theirs up to it
+  int total;      // of all sequences
+  __device__ __forceinline__ int load(int base) const {
+    const int n = base + lane;
+    return n < a.N ? pa_units(pa_len(a, n)) * per : 0;
+  }
+  __device__ __forceinline__ PagedUnits(const PagedAttn& args, int items, int l) : a(args), per(items), lane(l) {
+    own = load(0);
+    upto = wave_sum_scan(own);
+    total = __builtin_amdgcn_readlane(upto, 63);
+    for (int base = 64; base < a.N; base += 64) total += __builtin_amdgcn_readlane(wave_sum_scan(load(base)), 63);
+  }
+  // the sequence that unit t < total belongs to, and its first unit
+  __device__ __forceinline__ int find(int t, int* first) const {
+    int u = own, s = upto;
+    for (int base = 0;;) {
+      const uint64_t past = __ballot(s > t);
+      if (past) {
+        const int k = __builtin_ctzll(past);
+        *first = __builtin_amdgcn_readlane(s - u, k);
+        return base + k;
+      }
+      base += 64;
+      if (base >= a.N) return *first = 0;  // not reached
+      const int before = __builtin_amdgcn_readlane(s, 63);
+      u = load(base);
+      s = wave_sum_scan(u) + before;
+    }
+  }
+  // the first unit of sequence n
+  __device__ __forceinline__ int before(int n) const {
+    int u = own, s = upto;
+    for (int base = 64; base <= n; base += 64) {
+      const int sum = __builtin_amdgcn_readlane(s, 63);
+      u = load(base);
+      s = wave_sum_scan(u) + sum;
+    }
+    return __builtin_amdgcn_readlane(s - u, n & 63);
+  }
+};
+
+// Equal shares: `groups` workgroups (fewer, if they would get less than `least` units) of `share` units, the first `more`
+// of them one more.
+struct PagedShares {
+  int groups, share, more;
+  __device__ __forceinline__ PagedShares(const PagedSplit& z, int total) {
+    groups = total / z.least;
+    groups = groups < 1 ? 1 : groups < z.groups ? groups : z.groups;
+    share = total / groups;
+    more = total - share * groups;
+  }
+  __device__ __forceinline__ int first(int w) const { return w * share + (w < more ? w : more); }
+  // the workgroup that holds unit t
+  __device__ __forceinline__ int holder(int t) const {
+    const int big = more * (share + 1);
+    return t < big ? t / (share + 1) : more + (t - big) / share;
+  }
 };
 
 template <typename T, int D>
@@ -61,18 +147,20 @@ struct PagedTile {
   uint32_t v[SUB][4][DW];
 };
 
+typedef uint32_t u32v2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32v4 __attribute__((ext_vector_type(4)));
 template <int DW>
-__device__ __forceinline__ void load_dwords(uint32_t* d, const char* p) {
+__device__ __forceinline__ void load_dwords(uint32_t* d, __amdgpu_buffer_rsrc_t r, uint32_t off) {
   if constexpr (DW == 1) {
-    d[0] = *(const uint32_t*)p;
+    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
   } else if constexpr (DW == 2) {
-    const uint2 x = *(const uint2*)p;
-    d[0] = x.x, d[1] = x.y;
+    const u32v2 x = __builtin_bit_cast(u32v2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    d[0] = x[0], d[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < DW; i += 4) {
-      const uint4 x = *(const uint4*)(p + 4 * i);
-      d[i] = x.x, d[i + 1] = x.y, d[i + 2] = x.z, d[i + 3] = x.w;
+      const u32v4 x = __builtin_bit_cast(u32v4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, 0));
+      d[i] = x[0], d[i + 1] = x[1], d[i + 2] = x[2], d[i + 3] = x[3];
     }
   }
 }
@@ -133,24 +221,46 @@ __device__ __forceinline__ void paged_values(const PagedTile<float, D>& t, const
   }
 }
 
-template <typename T, int D, int QT, bool W>
-__global__ __launch_bounds__(64 * PA_NW, 2) void pa_kernel(PagedAttn a, PagedSplit z) {
+template <typename T, int D, int QT, bool W, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void pa_kernel(PagedAttn a, PagedSplit z) {
   typedef PagedTile<T, D> Tile;
   constexpr int SUB = Tile::SUB, KS = Tile::KS, NC = Tile::NC, DE = Tile::DE, ES = Tile::ES;
-  __shared__ float sh_o[PA_NW / 2][16 * QT][D + 4];
-  __shared__ float2 sh_ml[PA_NW / 2][16 * QT];
+  __shared__ float sh_o[NW / 2][16 * QT][D + 4];
+  __shared__ float2 sh_ml[NW / 2][16 * QT];
   const PagedPool& c = a.pool;
-  // Workgroup b runs on XCD b % 8. The splits of a sequence and the first splits of all sequences go to all XCDs alike
-  // (short sequences leave the later splits empty: with the splits of a sequence in a row, 16 of them, 64 sequences of 500
-  // to 10,000 rows took 160 us, this way 87).
-  const int items = a.N * c.H * z.qtiles, split = blockIdx.x / items;
-  const int item = (blockIdx.x % items + items - split % items * (int)z.turn % items) % items;
-  const int qt0 = item % z.qtiles, nh = item / z.qtiles;
-  const int n = nh / c.H, h = nh % c.H, G = a.Hq / c.H, rows = G * a.Tq;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
-  const int len = c.pages > 0 ? pool_length(c, n) : 0;
-  const int c0 = split * z.chunk, c1 = c0 + z.chunk < len ? c0 + z.chunk : len;
-  if (c0 >= c1 && split) return;  // nothing here, and the merge knows
+  const int G = a.Hq / c.H, rows = G * a.Tq;
+  const float sc = a.scale * TA_LOG2E;
+  const uint32_t koff = lr * D * ES + lg * 16, voff = lg * 4 * D * ES + lr * DE * ES;
+  const int per = c.H * z.qtiles;
+  int unit = 0, end = 1, n = 0, first = 0;
+  const PagedUnits units(a, per, lane);
+  if (z.groups) {
+    const PagedShares shares(z, units.total);
+    if ((int)blockIdx.x >= shares.groups) return;
+    unit = shares.first(blockIdx.x);
+    end = shares.first(blockIdx.x + 1);
+  }
+  while (unit < end) {
+  // the segment: rows [c0, c1) of an item
+  int item, c0, c1, slot = -1;
+  if (z.groups) {
+    n = units.find(unit, &first);
+    const int len = __builtin_amdgcn_readfirstlane(pa_len(a, n)), each = pa_units(len);
+    item = (unit - first) / each;
+    const int u0 = unit - first - item * each, u1 = u0 + end - unit < each ? u0 + end - unit : each;
+    c0 = u0 * PA_UNIT;
+    c1 = u1 * PA_UNIT < len ? u1 * PA_UNIT : len;
+    if (u1 - u0 < each) slot = 2 * blockIdx.x + (u0 == 0);
+    unit += u1 - u0;
+  } else {
+    n = blockIdx.x / per;
+    item = blockIdx.x % per;
+    c0 = 0;
+    c1 = __builtin_amdgcn_readfirstlane(pa_len(a, n));
+    unit = end;
+  }
+  const int qt0 = item % z.qtiles, h = item / z.qtiles, nh = n * c.H + h;
 
   // this lane's query rows: 16 QT of the (head of the group, query row) pairs
   uint4 q[QT][NC];
@@ -174,50 +284,41 @@ __global__ __launch_bounds__(64 * PA_NW, 2) void pa_kernel(PagedAttn a, PagedSpl
 #pragma unroll
     for (int e = 0; e < DE; ++e) o[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const float sc = a.scale * TA_LOG2E;
   const int32_t* table = c.table + n * c.table_sn;
   // 64 page ids of the table at a time, one per lane
   int pg0 = c0 >> c.shift, pg = pg0 + lane < c.max_pages ? table[pg0 + lane] : -1;
   const int64_t head = (int64_t)h << c.shift;
-  const uint32_t koff = lr * D * ES + lg * 16, voff = lg * 4 * D * ES + lr * DE * ES;
 
-  // loads the turn at `key`; bit s of the result: subtile s has rows in the pool
+  // Loads the turn at `key`; returns the live rows of its subtiles, 8 bits each. The rows past c1 and those of a page the
+  // pool does not have lie behind their buffer's end: the loads return 0 for them and touch no memory, so every turn issues
+  // the same loads (waits that count them need no branch) and a value nobody wrote meets no product.
   auto fetch = [&](Tile& t, int key) -> int {
     int live = 0;
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      const int k0 = key + 16 * s;
-      int i = (k0 >> c.shift) - pg0;
+      const int k0 = key + 16 * s, left = c1 - k0;
+      int i = left > 0 ? (k0 >> c.shift) - pg0 : 0;
       if (i >= 64) {
         pg0 += i;
         pg = pg0 + lane < c.max_pages ? table[pg0 + lane] : -1;
+        asm volatile("" : "+v"(pg));  // waited for here, not wherever the paths join (there: for every load in flight)
         i = 0;
       }
       const int page = __builtin_amdgcn_readlane(pg, i);
-      const bool ok = k0 < c1 && page >= 0 && page < c.pages;
-      live |= ok ? 1 << s : 0;
-      // rows nobody has: any page's, for the address alone
-      const int64_t off = ((ok ? page : 0) * c.page_sp + (head + (k0 & ((1 << c.shift) - 1))) * D) * ES;
-      const char* kp = (const char*)c.k + off;
-      const char* vp = (const char*)c.v + off;
+      const int have = page < 0 || page >= c.pages || left <= 0 ? 0 : left < 16 ? left : 16;
+      live |= have << (8 * s);
+      const int64_t off = ((have ? page : 0) * c.page_sp + (head + (k0 & ((1 << c.shift) - 1))) * D) * ES;
+      const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((char*)c.k + off, 0, have * D * ES, TA_BUF_WORD3);
+      const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((char*)c.v + off, 0, have * D * ES, TA_BUF_WORD3);
 #pragma unroll
-      for (int i2 = 0; i2 < NC; ++i2) t.k[s][i2] = ldg16(kp + koff + i2 * 64);
+      for (int i2 = 0; i2 < NC; ++i2)
+        t.k[s][i2] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, koff + i2 * 64, 0, 0));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) load_dwords<Tile::DW>(t.v[s][j], vp + voff + j * D * ES);
+      for (int j = 0; j < 4; ++j) load_dwords<Tile::DW>(t.v[s][j], vr, voff + j * D * ES);
     }
     return live;
   };
   auto compute = [&](Tile& t, int key, int live) {
-    const bool full = live == (1 << SUB) - 1 && key + KS <= c1;
-    if (!full) {
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (!(live >> s & 1) || key + 16 * s + lg * 4 + j >= c1)
-#pragma unroll
-            for (int w = 0; w < Tile::DW; ++w) t.v[s][j][w] = 0;
-    }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       float x[SUB][4];
@@ -228,12 +329,12 @@ __global__ __launch_bounds__(64 * PA_NW, 2) void pa_kernel(PagedAttn a, PagedSpl
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[s][i] = sv[i] * sc;
-          if (!full && (!(live >> s & 1) || key + 16 * s + lg * 4 + i >= c1)) x[s][i] = TA_NEG_INF;
+          x[s][i] = lg * 4 + i < (live >> (8 * s) & 255) ? x[s][i] : TA_NEG_INF;
           above |= x[s][i] - ref[qt] > PA_SLACK - PA_SHIFT;
         }
         if constexpr (W) {
           const int r = (qt0 * QT + qt) * 16 + lr;
-          if (r < rows)
+          if (r < rows && key < c1)
             *(f32x4*)(z.score + ((int64_t)nh * rows + r) * z.score_sn + key + 16 * s + lg * 4) =
                 f32x4{x[s][0], x[s][1], x[s][2], x[s][3]};
         }
@@ -258,32 +359,27 @@ __global__ __launch_bounds__(64 * PA_NW, 2) void pa_kernel(PagedAttn a, PagedSpl
 #pragma unroll
       for (int s = 0; s < SUB; ++s) l[qt] += (p[s][0] + p[s][1]) + (p[s][2] + p[s][3]);
       paged_values<D>(t, p, o[qt]);
+      if constexpr (QT > 1) __builtin_amdgcn_sched_barrier(0);  // one query tile's scores and probabilities live at a time
     }
   };
 
   int key = c0 + wave * KS;
   if (key < c1) {
     Tile ta, tb;
-    int la = fetch(ta, key), lb = 0;
-    for (;;) {
-      int next = key + PA_NW * KS;
-      if (next < c1) lb = fetch(tb, next);
+    int la = fetch(ta, key);
+    for (; key < c1; key += 2 * NW * KS) {  // two turns: the second may be past the end, then its weights are 0
+      const int lb = fetch(tb, key + NW * KS);
       compute(ta, key, la);
-      key = next;
-      if (key >= c1) break;
-      next = key + PA_NW * KS;
-      if (next < c1) la = fetch(ta, next);
-      compute(tb, key, lb);
-      key = next;
-      if (key >= c1) break;
+      la = fetch(ta, key + 2 * NW * KS);
+      compute(tb, key + NW * KS, lb);
     }
   }
 
-  // join the four waves: the upper half hands over to the lower half, twice
+  // join the waves: the upper half hands over to the lower half, until one has all
 #pragma unroll
   for (int t = 0; t < QT; ++t) l[t] = quad_sum(l[t]);
 #pragma unroll
-  for (int half = PA_NW / 2; half >= 1; half >>= 1) {
+  for (int half = NW / 2; half >= 1; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
@@ -310,66 +406,85 @@ __global__ __launch_bounds__(64 * PA_NW, 2) void pa_kernel(PagedAttn a, PagedSpl
     }
     __syncthreads();
   }
-  if (wave) return;
+  if (wave == 0) {
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = (qt0 * QT + t) * 16 + lr;
-    if (r >= rows) continue;
-    if (z.splits > 1) {
-      const int64_t at = ((int64_t)nh * z.splits + split) * rows + r;
-      float* po = z.part + at * D + lg * 4 * DE;
+    for (int t = 0; t < QT; ++t) {
+      const int r = (qt0 * QT + t) * 16 + lr;
+      if (r >= rows) continue;
+      if (slot >= 0) {
+        const int64_t at = (int64_t)slot * 16 * QT + t * 16 + lr;
+        float* po = z.part + at * D + lg * 4 * DE;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < DE; ++e) po[i * DE + e] = o[t][e][i];
-      if (lg == 0) z.ml[at] = make_float2(ref[t], l[t]);
-    } else {
-      const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
-      T* op = (T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lg * 4 * DE;
+          for (int e = 0; e < DE; ++e) po[i * DE + e] = o[t][e][i];
+        if (lg == 0) z.ml[at] = make_float2(ref[t], l[t]);
+      } else {
+        const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
+        T* op = (T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lg * 4 * DE;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < DE; ++e) op[i * DE + e] = (T)(o[t][e][i] * inv);
-      if (W && lg == 0) z.stat[(int64_t)nh * rows + r] = make_float2(ref[t], inv);
+          for (int e = 0; e < DE; ++e) op[i * DE + e] = (T)(o[t][e][i] * inv);
+        if (W && lg == 0) z.stat[(int64_t)nh * rows + r] = make_float2(ref[t], inv);
+      }
     }
+  }
   }
 }
 
-// Joins the splits of one query row per wave: 4 values of a partial output per lane, 256 / D partials at a time.
-template <typename T, int D, bool W>
+// Joins the partials of one query row per wave: 4 values of a partial output per lane, 256 / D partials at a time. Rows
+// that pa_kernel has written are left alone; rows without a key become 0.
+template <typename T, int D, int QT, bool W>
 __global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z) {
   constexpr int LPR = D / 4, GR = 64 / LPR;
-  const int lane = threadIdx.x & 63, rows = a.Hq / a.pool.H * a.Tq;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, G = a.Hq / a.pool.H, rows = G * a.Tq;
+  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= (int64_t)a.N * a.pool.H * rows) return;
-  const int r = (int)(row % rows), nh = (int)(row / rows), n = nh / a.pool.H, h = nh % a.pool.H, G = a.Hq / a.pool.H;
-  const int len = a.pool.pages > 0 ? pool_length(a.pool, n) : 0;
-  const int used = (int)(((int64_t)len + z.chunk - 1) / z.chunk);
-  const float2* ml = z.ml + (int64_t)nh * z.splits * rows + r;
-  float m = PA_REF0;
-  for (int s = lane; s < used; s += 64) m = fmaxf(m, ml[(int64_t)s * rows].x);
-  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-  float l = 0.f;
-  for (int s = lane; s < used; s += 64) {
-    const float2 v = ml[(int64_t)s * rows];
-    l += v.y * __builtin_amdgcn_exp2f(v.x - m);
+  const int r = (int)(row % rows), nh = (int)(row / rows), n = nh / a.pool.H, h = nh % a.pool.H;
+  const PagedUnits units(a, a.pool.H * z.qtiles, lane);
+  const PagedShares shares(z, units.total);
+  const int each = pa_units(__builtin_amdgcn_readfirstlane(pa_len(a, n)));
+  T* op = (T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lane * 4;
+  if (each == 0) {
+    if (lane < LPR)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) op[i] = (T)0.f;
+    return;
   }
-  for (int x = 32; x >= 1; x >>= 1) l += __shfl_xor(l, x, 64);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float* part = z.part + ((int64_t)nh * z.splits * rows + r) * D + lane % LPR * 4;
+  // the workgroups of the item's first and last unit
+  const int t0 = units.before(n) + (h * z.qtiles + r / (16 * QT)) * each;
+  const int w0 = shares.holder(t0), w1 = shares.holder(t0 + each - 1);
+  if (w0 == w1) return;
+  const int parts = w1 - w0 + 1, at = r % (16 * QT);
+  auto slot = [&](int i) { return (int64_t)(2 * (w0 + i) + (i == 0)) * (16 * QT) + at; };
+  // every group of lanes joins its share of the partials by itself (their loads wait for nothing but the lengths), then
+  // the groups are joined
+  float m = PA_REF0, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = lane / LPR; s < used; s += GR) {
-    const float f = __builtin_amdgcn_exp2f(ml[(int64_t)s * rows].x - m) * inv;
-    o += *(const f32x4*)(part + (int64_t)s * rows * D) * f;
-  }
-  for (int x = LPR; x < 64; x <<= 1)
+#pragma unroll 4
+  for (int i = lane / LPR; i < parts; i += GR) {
+    const float2 v = z.ml[slot(i)];
+    const f32x4 x = *(const f32x4*)(z.part + slot(i) * D + lane % LPR * 4);
+    const float to = fmaxf(m, v.x), f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(v.x - to);
+    m = to;
+    l = l * f0 + v.y * f1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
-  if (lane < LPR) {
-    T* op = (T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lane * 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) op[i] = (T)o[i];
+    for (int j = 0; j < 4; ++j) o[j] = o[j] * f0 + x[j] * f1;
   }
+#pragma unroll
+  for (int x = LPR; x < 64; x <<= 1) {
+    const float mo = __shfl_xor(m, x, 64), lo = __shfl_xor(l, x, 64);
+    const float to = fmaxf(m, mo), f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(mo - to);
+    m = to;
+    l = l * f0 + lo * f1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = o[j] * f0 + __shfl_xor(o[j], x, 64) * f1;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (lane < LPR)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) op[i] = (T)(o[i] * inv);
   if (W && lane == 0) z.stat[row] = make_float2(m, inv);
 }
 
@@ -377,7 +492,7 @@ __global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z
 // (each in steps of 16), joined in a fixed order.
 __global__ __launch_bounds__(256) void pa_weights_kernel(PagedAttn a, PagedSplit z) {
   __shared__ f32x4 sh[16][16];
-  const int n = blockIdx.y, len = a.pool.pages > 0 ? pool_length(a.pool, n) : 0, k0 = blockIdx.x * 64;
+  const int n = blockIdx.y, len = pa_len(a, n), k0 = blockIdx.x * 64;
   if (k0 >= len) return;
   const int all = a.Hq * a.Tq, kt = threadIdx.x & 15, rt = threadIdx.x >> 4;
   const int64_t first = (int64_t)n * all;
@@ -621,11 +736,6 @@ int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 
 namespace {
 
-int paged_qt(int64_t rows, int64_t D, int dtype) {
-  const int most = D == 128 ? 1 : D == 64 && dtype ? 2 : 4;  // more queries do not fit the registers
-  return rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
-}
-
 int cu_count() {
   static int count[64];
   int dev = 0;
@@ -638,20 +748,15 @@ int cu_count() {
 }
 
 // The split of a call and the bytes of its workspace; `rows`: the most rows a sequence can have.
-int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows,
-                    bool weights, int dtype) {
-  const int64_t qrows = Hq / H * Tq, qt = paged_qt(qrows, D, dtype);
-  z->qtiles = (int)((qrows + 16 * qt - 1) / (16 * qt));
-  const int64_t items = N * H * z->qtiles;
-  const int64_t target = 8 * cu_count(), least = 256;
-  z->turn = (int)((9 - items % 8) % 8);
-  int64_t chunk = (rows * items + target - 1) / target;
-  chunk = (chunk + 127) / 128 * 128;
-  if (chunk < least) chunk = least;
-  const int64_t whole = rows > 0 ? (rows + 127) / 128 * 128 : 128;
-  if (chunk > whole) chunk = whole;
-  z->chunk = (int)chunk;
-  z->splits = (int)(rows > chunk ? (rows + chunk - 1) / chunk : 1);
+template <typename T, int D, int QT>
+int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights) {
+  const int64_t qrows = Hq / H * Tq;
+  z->qtiles = (int)((qrows + 16 * QT - 1) / (16 * QT));
+  // Two workgroups per CU keep enough loads in flight (three: 3% slower on long caches, 30% at 64 query rows). Up to
+  // PA_WHOLE rows an item goes to one workgroup of eight waves, without a merge: one row over 8 x 700 rows 10.9 us on the
+  // GPU against 11.2 and a launch less for the host; over 8 x 2,000 rows 16.7 against 15.2.
+  z->groups = rows <= PA_WHOLE ? 0 : 2 * cu_count();
+  z->least = 2;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     char* p = ws + at;
@@ -659,59 +764,71 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
     return p;
   };
   const int64_t all = N * H * qrows;
-  z->part = (float*)take(z->splits > 1 ? all * z->splits * D * 4 : 0);
-  z->ml = (float2*)take(z->splits > 1 ? all * z->splits * 8 : 0);
+  z->part = (float*)take((int64_t)z->groups * 2 * 16 * QT * D * 4);
+  z->ml = (float2*)take((int64_t)z->groups * 2 * 16 * QT * 8);
   z->score_sn = (rows + 63) / 64 * 64;
   z->stat = (float2*)take(weights ? all * 8 : 0);
   z->score = (float*)take(weights ? all * z->score_sn * 4 : 0);
   return at;
 }
 
-template <typename T, int D, int QT>
-void launch_pa(const PagedAttn& a, const PagedSplit& z, hipStream_t stream) {
-  const unsigned grid = (unsigned)((int64_t)a.N * a.pool.H * z.splits * z.qtiles);
-  const unsigned merge = (unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4);
-  if (a.weights) {
-    hipLaunchKernelGGL((pa_kernel<T, D, QT, true>), dim3(grid), dim3(64 * PA_NW), 0, stream, a, z);
-    if (z.splits > 1) hipLaunchKernelGGL((pa_merge_kernel<T, D, true>), dim3(merge), dim3(256), 0, stream, a, z);
-    const unsigned wx = (unsigned)(z.score_sn / 64);
-    if (wx) hipLaunchKernelGGL(pa_weights_kernel, dim3(wx, a.N), dim3(256), 0, stream, a, z);
+template <typename T, int D, int QT, bool W>
+void launch_pa_w(const PagedAttn& a, const PagedSplit& z, hipStream_t stream) {
+  if (z.groups == 0) {
+    hipLaunchKernelGGL((pa_kernel<T, D, QT, W, 8>), dim3((unsigned)(a.N * a.pool.H * z.qtiles)), dim3(512), 0, stream, a, z);
   } else {
-    hipLaunchKernelGGL((pa_kernel<T, D, QT, false>), dim3(grid), dim3(64 * PA_NW), 0, stream, a, z);
-    if (z.splits > 1) hipLaunchKernelGGL((pa_merge_kernel<T, D, false>), dim3(merge), dim3(256), 0, stream, a, z);
+    hipLaunchKernelGGL((pa_kernel<T, D, QT, W, 4>), dim3((unsigned)z.groups), dim3(256), 0, stream, a, z);
+    const unsigned merge = (unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4);
+    hipLaunchKernelGGL((pa_merge_kernel<T, D, QT, W>), dim3(merge), dim3(256), 0, stream, a, z);
   }
+  if (W && z.score_sn)
+    hipLaunchKernelGGL(pa_weights_kernel, dim3((unsigned)(z.score_sn / 64), a.N), dim3(256), 0, stream, a, z);
+}
+
+// Launches (a != null) or sizes the workspace.
+template <typename T, int D, int QT>
+int64_t run_pa(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights,
+               hipStream_t stream) {
+  PagedSplit z;
+  const int64_t bytes = paged_split<T, D, QT>(&z, (char*)ws, N, Hq, H, Tq, rows, weights);
+  if (a && weights) launch_pa_w<T, D, QT, true>(*a, z, stream);
+  else if (a) launch_pa_w<T, D, QT, false>(*a, z, stream);
+  return bytes;
 }
 
 template <typename T, int D>
-void launch_pa_d(const PagedAttn& a, const PagedSplit& z, int qt, hipStream_t stream) {
-  if (qt == 1) return launch_pa<T, D, 1>(a, z, stream);
-  if constexpr (D < 128)
-    if (qt == 2) return launch_pa<T, D, 2>(a, z, stream);
-  if constexpr (D * sizeof(T) <= 128) launch_pa<T, D, 4>(a, z, stream);
+int64_t run_pa_d(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights,
+                 hipStream_t stream) {
+  const int64_t qrows = Hq / H * Tq;
+  constexpr int most = D == 128 ? 1 : D * sizeof(T) > 128 ? 2 : 4;  // more queries do not fit the registers
+  if constexpr (most >= 4)
+    if (qrows > 32) return run_pa<T, D, 4>(a, ws, N, Hq, H, Tq, rows, weights, stream);
+  if constexpr (most >= 2)
+    if (qrows > 16) return run_pa<T, D, 2>(a, ws, N, Hq, H, Tq, rows, weights, stream);
+  return run_pa<T, D, 1>(a, ws, N, Hq, H, Tq, rows, weights, stream);
 }
 
-template <typename T>
-void launch_pa_t(const PagedAttn& a, const PagedSplit& z, int qt, hipStream_t stream) {
-  if (a.pool.D == 32) launch_pa_d<T, 32>(a, z, qt, stream);
-  else if (a.pool.D == 64) launch_pa_d<T, 64>(a, z, qt, stream);
-  else launch_pa_d<T, 128>(a, z, qt, stream);
+int64_t run_pa_any(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows,
+                   bool weights, int dtype, hipStream_t stream) {
+  if (dtype == 0)
+    return D == 32   ? run_pa_d<bf16, 32>(a, ws, N, Hq, H, Tq, rows, weights, stream)
+           : D == 64 ? run_pa_d<bf16, 64>(a, ws, N, Hq, H, Tq, rows, weights, stream)
+                     : run_pa_d<bf16, 128>(a, ws, N, Hq, H, Tq, rows, weights, stream);
+  return D == 32   ? run_pa_d<float, 32>(a, ws, N, Hq, H, Tq, rows, weights, stream)
+         : D == 64 ? run_pa_d<float, 64>(a, ws, N, Hq, H, Tq, rows, weights, stream)
+                   : run_pa_d<float, 128>(a, ws, N, Hq, H, Tq, rows, weights, stream);
 }
 
 }  // namespace
 
 int64_t tabicl_launch_paged_attn_ws_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows, int weights,
                                           int dtype) {
-  PagedSplit z;
-  return paged_split(&z, nullptr, N, Hq, H, Tq, D, rows, weights != 0, dtype);
+  return run_pa_any(nullptr, nullptr, N, Hq, H, Tq, D, rows, weights != 0, dtype, nullptr);
 }
 
 int tabicl_launch_paged_attn(const PagedAttn& a, int dtype, void* ws, hipStream_t stream) {
-  PagedSplit z;
-  paged_split(&z, (char*)ws, a.N, a.Hq, a.pool.H, a.Tq, a.pool.D, (int64_t)a.pool.max_pages << a.pool.shift,
-              a.weights != nullptr, dtype);
-  const int qt = paged_qt((int64_t)a.Hq / a.pool.H * a.Tq, a.pool.D, dtype);
-  if (dtype == 0) launch_pa_t<bf16>(a, z, qt, stream);
-  else launch_pa_t<float>(a, z, qt, stream);
+  run_pa_any(&a, ws, a.N, a.Hq, a.pool.H, a.Tq, a.pool.D, (int64_t)a.pool.max_pages << a.pool.shift, a.weights != nullptr,
+             dtype, stream);
   return (int)hipGetLastError();
 }
 
