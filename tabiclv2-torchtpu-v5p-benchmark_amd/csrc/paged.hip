@@ -55,8 +55,8 @@ struct PagedSplit {
   int qtiles;
   float* part;   // [2 G][16 QT][D] unnormalised outputs
   float2* ml;    // [2 G][16 QT] (ref, sum)
-  float2* stat;  // [N Hq Tq] (ref, 1 / sum), for the weights
-  float* score;  // [N Hq Tq][score_sn] scores in log2 units, for the weights
+  float2* stat;  // [N Hq Tq] (ref, 1 / sum) for the weights, or null
+  float* score;  // [N Hq Tq][score_sn] scores in log2 units for the weights, or null: from K once more
   int64_t score_sn;
 };
 
@@ -165,20 +165,26 @@ __device__ __forceinline__ void load_dwords(uint32_t* d, __amdgpu_buffer_rsrc_t 
   }
 }
 
-// The products of one tile with the 16 queries of a query tile.
-template <typename T, int D>
-__device__ __forceinline__ f32x4 paged_scores(const PagedTile<T, D>& t, int sub, const uint4* q) {
+// The scores of 16 keys (chunks k of their rows) for 16 queries: key 4 (l / 16) + i, query l % 16.
+template <typename T, int NC>
+__device__ __forceinline__ f32x4 tile_scores(const uint4* k, const uint4* q) {
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int c = 0; c < PagedTile<T, D>::NC; ++c) {
+  for (int c = 0; c < NC; ++c) {
     if constexpr (sizeof(T) == 2)
-      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[sub][c]), __builtin_bit_cast(bf16x8, q[c]), s,
-                                                  0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[c]), __builtin_bit_cast(bf16x8, q[c]), s, 0, 0, 0);
     else
-      s = mfma16x16x16(__builtin_bit_cast(f32x4, t.k[sub][c]), __builtin_bit_cast(f32x4, q[c]), s);
+      s = mfma16x16x16(__builtin_bit_cast(f32x4, k[c]), __builtin_bit_cast(f32x4, q[c]), s);
   }
   return s;
 }
+
+// Sum over the 16 lanes of a row, in the registers (row_ror).
+template <int N>
+__device__ __forceinline__ float row_add(float x) {
+  return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float row16_sum(float x) { return row_add<1>(row_add<2>(row_add<4>(row_add<8>(x)))); }
 
 template <int D>
 __device__ __forceinline__ void paged_values(const PagedTile<bf16, D>& t, const float (*p)[4], f32x4* o) {
@@ -325,7 +331,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pa_kernel(PagedAttn a, PagedSplit 
       bool above = false;
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
-        const f32x4 sv = paged_scores<T, D>(t, s, q[qt]);
+        const f32x4 sv = tile_scores<T, NC>(t.k[s], q[qt]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[s][i] = sv[i] * sc;
@@ -426,7 +432,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pa_kernel(PagedAttn a, PagedSplit 
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int e = 0; e < DE; ++e) op[i * DE + e] = (T)(o[t][e][i] * inv);
-        if (W && lg == 0) z.stat[(int64_t)nh * rows + r] = make_float2(ref[t], inv);
+        if (z.stat && lg == 0) z.stat[(int64_t)nh * rows + r] = make_float2(ref[t], inv);
       }
     }
   }
@@ -435,7 +441,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pa_kernel(PagedAttn a, PagedSplit 
 
 // Joins the partials of one query row per wave: 4 values of a partial output per lane, 256 / D partials at a time. Rows
 // that pa_kernel has written are left alone; rows without a key become 0.
-template <typename T, int D, int QT, bool W>
+template <typename T, int D, int QT>
 __global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z) {
   constexpr int LPR = D / 4, GR = 64 / LPR;
   const int lane = threadIdx.x & 63, G = a.Hq / a.pool.H, rows = G * a.Tq;
@@ -485,7 +491,7 @@ __global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z
   if (lane < LPR)
 #pragma unroll
     for (int i = 0; i < 4; ++i) op[i] = (T)(o[i] * inv);
-  if (W && lane == 0) z.stat[row] = make_float2(m, inv);
+  if (z.stat && lane == 0) z.stat[row] = make_float2(m, inv);
 }
 
 // weights[n, i] += sum over the query rows of p: 64 keys per workgroup, 4 per thread, the query rows over 16 threads
@@ -511,6 +517,88 @@ __global__ __launch_bounds__(256) void pa_weights_kernel(PagedAttn a, PagedSplit
     for (int r = 0; r < 16; ++r) t += sh[r][threadIdx.x >> 2][threadIdx.x & 3];
     if (key < len) a.weights[n * a.weights_sn + key] += t;
   }
+}
+
+// The same from K itself, for many query rows per K/V head: the scores of 64 keys per wave once more, head after head (a
+// head's K rows are loaded while the one before is multiplied), normalised and summed in the registers, then over the 16
+// queries of a tile. Reads D values of a key per head where the scores are 8 bytes per query row, written and read.
+template <int D>
+__global__ __launch_bounds__(256) void pa_weights_keys_kernel(PagedAttn a, PagedSplit z) {
+  typedef bf16 T;
+  constexpr int ES = 2, NC = D * ES / 64, SUB = 4, KEYS = 16 * SUB;
+  struct Tile {
+    uint4 k[SUB][NC];
+  };
+  const PagedPool& c = a.pool;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
+  const int n = blockIdx.y, len = __builtin_amdgcn_readfirstlane(pa_len(a, n)), key0 = (blockIdx.x * 4 + wave) * KEYS;
+  if (key0 >= len) return;
+  const int G = a.Hq / c.H, rows = G * a.Tq, tiles = (rows + 15) / 16, at = (key0 + 16 * lane) >> c.shift;
+  const int pg = lane < SUB && at < c.max_pages ? c.table[n * c.table_sn + at] : -1;
+  const float sc = a.scale * TA_LOG2E;
+  const uint32_t koff = lr * D * ES + lg * 16;
+  int64_t off[SUB];
+  int have[SUB];
+#pragma unroll
+  for (int s = 0; s < SUB; ++s) {
+    const int page = __builtin_amdgcn_readlane(pg, s), left = len - key0 - 16 * s;
+    have[s] = page < 0 || page >= c.pages || left <= 0 ? 0 : left < 16 ? left : 16;
+    off[s] = ((have[s] ? page : 0) * c.page_sp + ((key0 + 16 * s) & ((1 << c.shift) - 1)) * D) * ES;
+  }
+  auto fetch = [&](Tile& t, int h) {  // past the last head: nothing
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+          (char*)c.k + off[s] + ((int64_t)(h < c.H ? h : 0) << c.shift) * D * ES, 0, h < c.H ? have[s] * D * ES : 0, TA_BUF_WORD3);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        t.k[s][i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, koff + i * 64, 0, 0));
+    }
+  };
+  float w[SUB][4];
+#pragma unroll
+  for (int s = 0; s < SUB; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[s][i] = 0.f;
+  auto compute = [&](Tile& t, int h) {
+    if (h >= c.H) return;
+    for (int qt = 0; qt < tiles; ++qt) {
+      const int r = qt * 16 + lr;
+      uint4 q[NC];
+      float2 st = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) q[i] = uint4{0, 0, 0, 0};
+      if (r < rows) {
+        const char* qp = (const char*)a.q + (n * a.q_sn + (h * G + r / a.Tq) * a.q_sh + (r % a.Tq) * a.q_st) * ES + lg * 16;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) q[i] = ldg16(qp + i * 64);
+        st = z.stat[((int64_t)n * c.H + h) * rows + r];
+      }
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        const f32x4 sv = tile_scores<T, NC>(t.k[s], q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[s][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(sv[i] * sc - st.x), st.y, w[s][i]);
+      }
+    }
+  };
+  Tile ta, tb;
+  fetch(ta, 0);
+  for (int h = 0; h < c.H; h += 2) {
+    fetch(tb, h + 1);
+    compute(ta, h);
+    fetch(ta, h + 2);
+    compute(tb, h + 1);
+  }
+  float* out = a.weights + n * a.weights_sn + key0 + lg * 4;
+#pragma unroll
+  for (int s = 0; s < SUB; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float sum = row16_sum(w[s][i]);
+      if (lr == 0 && lg * 4 + i < have[s]) out[16 * s + i] += sum;
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -557,184 +645,188 @@ __device__ __forceinline__ EvictSizes evict_sizes(const PagedEvict& a, int n) {
   return z;
 }
 
-// Selection, one workgroup per sequence: the threshold code by three digits (11, 11 and 10 bits) of a histogram in LDS,
-// then ranks. Wave w holds the rows [w seg, (w + 1) seg), lane l of step i row w seg + 64 i + l, so that a rank is the
-// count of earlier flags of the wave (ballots) and of the waves before it: two barriers per rank, none per step. Up to
-// PE_HELD steps the codes stay in registers from the first pass on; longer sequences read their weights again (from L2)
-// in each of the six passes.
-constexpr int PE_NW = PE_NT / 64, PE_HELD = 16, PE_BINS = 2048;
+// Three launches: the threshold (one workgroup per sequence), the ranks (a workgroup per 1,024 rows), the moves; the first two
+// are one where no sequence has more than 1,024 rows.
+//
+// A row competes if it is none of the recent ones; it stays if its code is above the threshold, or equal to it and among the
+// first `even` such rows. With before(r) the rows that stay below row r, the i-th place to fill is the row r < cut that goes
+// with r - before(r) = i, and the i-th last row to move is the row r >= cut that stays with cut - 1 - before(r) = i: each
+// row knows its rank by a count of the rows before it alone.
+struct EvictCut {
+  uint32_t threshold;
+  int even;
+};
+constexpr int PE_NW = PE_NT / 64, PE_BINS = 2048;
 
-// The exclusive sums over the waves of three counts each, in sh; returns this wave's, total in *all.
-__device__ __forceinline__ int wave_scan(int count, int* sh, int* all) {
+__device__ __forceinline__ int lanes_before(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+// f(row, code) for this thread's share of rows [0, end); load(row) gives the code, eight at a time in flight.
+template <typename L, typename F>
+__device__ __forceinline__ void each_code(int end, L load, F f) {
+  int base = 0;
+  for (; base + 8 * PE_NT <= end; base += 8 * PE_NT) {
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = load(base + j * PE_NT + (int)threadIdx.x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f(base + j * PE_NT + (int)threadIdx.x, c[j]);
+  }
+  for (int r = base + threadIdx.x; r < end; r += PE_NT) f(r, load(r));
+}
+
+// The sum of `count` (uniform) over the waves before this one, and over all.
+__device__ __forceinline__ int wave_offset(int count, int* sh, int* all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __syncthreads();
   if (lane == 0) sh[wave] = count;
   __syncthreads();
-  int before = 0, sum = 0;
-#pragma unroll
-  for (int w = 0; w < PE_NW; ++w) {
-    const int x = sh[w];
-    before += w < wave ? x : 0;
-    sum += x;
-  }
-  *all = sum;
-  return before;
+  const int upto = wave_sum_scan(lane < PE_NW ? sh[lane] : 0);
+  *all = __builtin_amdgcn_readlane(upto, PE_NW - 1);
+  return __builtin_amdgcn_readlane(upto, __builtin_amdgcn_readfirstlane(wave)) - count;
 }
 
-template <bool HELD>
-__device__ __forceinline__ void evict_select(const PagedEvict& a, int n, const EvictSizes z, int64_t* pairs, int32_t* npairs,
-                                             int* hist, int* sh) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// The threshold by three digits (11, 11 and 10 bits) of a histogram in LDS. One CU does it, bound by the latency and issue
+// of three passes over the weights (from L2), so it does nothing else and keeps eight loads a thread in flight: 16,384
+// rows take 12 us, 45,000 rows 22 us (four loads in flight: 42; with the ranks in it too, 16,384 rows took 29).
+__device__ __forceinline__ EvictCut evict_threshold(const PagedEvict& a, int n, const EvictSizes z) {
+  __shared__ int hist[PE_BINS], sh[PE_NW], pick[2];
+  const int tid = threadIdx.x, free_rows = z.len - z.recent;
   const float* w = a.weights + n * a.weights_sn;
-  const int64_t cap = (int64_t)a.pool.max_pages << a.pool.shift;
-  const int free_rows = z.len - z.recent;  // the rows that compete
-  const int steps = ((z.len + PE_NT - 1) / PE_NT), base = wave * steps * 64 + lane;
-  uint32_t held[HELD ? PE_HELD : 1];
-  if constexpr (HELD) {
-#pragma unroll
-    for (int i = 0; i < PE_HELD; ++i) {
-      const int r = base + i * 64;
-      held[i] = i < steps && r < free_rows ? weight_code(w[r]) : 0;
-    }
-  }
-  // f(step, row, code) over this lane's rows in order
-  auto each = [&](auto f) {
-    if constexpr (HELD) {
-#pragma unroll
-      for (int i = 0; i < PE_HELD; ++i)
-        if (i < steps) f(base + i * 64, held[i]);
-    } else {
-      for (int i = 0; i < steps; i += 8) {
-        uint32_t c[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = base + (i + j) * 64;
-          c[j] = i + j < steps && r < free_rows ? weight_code(w[r]) : 0;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (i + j < steps) f(base + (i + j) * 64, c[j]);
-      }
-    }
-  };
-  int want = z.kept - z.recent;  // of the rows [0, free_rows); in the end, of those of the threshold's weight
-  const bool any = want > 0;
-  uint32_t prefix = 0;
-  if (any) {
-#pragma unroll
-    for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
-      for (int i = tid; i < PE_BINS; i += PE_NT) hist[i] = 0;
-      __syncthreads();
-      each([&](int r, uint32_t c) {
-        const bool in = r < free_rows && (digit == 0 || (c >> (shift + bits)) == (prefix >> (shift + bits)));
-        if (in) atomicAdd(&hist[(c >> shift) & ((1u << bits) - 1)], 1);
+  int want = z.kept - z.recent;  // of the rows that compete; in the end, of those of the threshold's code
+  if (want == 0 || want == free_rows) return EvictCut{want == 0 ? 0xffffffffu : 0u, 0};  // no code is 0 or 2^32 - 1
+  for (int i = tid; i < PE_BINS; i += PE_NT) hist[i] = 0;
+  __syncthreads();
+  auto weight = [&](int r) { return weight_code(w[r]); };
+  uint32_t threshold = 0;
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, above = digit == 1 ? 21 : 10;
+    if (digit == 0)
+      each_code(free_rows, weight, [&](int, uint32_t c) { atomicAdd(&hist[c >> 21], 1); });
+    else
+      each_code(free_rows, weight, [&](int, uint32_t c) {
+        if ((c ^ threshold) >> above == 0) atomicAdd(&hist[c >> shift & ((1u << (above - shift)) - 1)], 1);
       });
-      __syncthreads();
-      // thread t sums the bins 2 t' and 2 t' + 1 with t' counted from the top: the first digit whose count from above
-      // reaches `want`
-      const int top = PE_BINS - 2 * tid - 1;
-      const int h1 = hist[top], h0 = hist[top - 1];
-      int incl = h0 + h1;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += y;
-      }
-      int all;
-      const int before = wave_scan(__shfl(incl, 63, 64), sh, &all) + incl - h0 - h1;
-      __syncthreads();
-      if (before < want && before + h0 + h1 >= want) {  // one thread
-        const bool first = before + h1 >= want;
-        sh[0] = first ? top : top - 1;
-        sh[1] = want - before - (first ? 0 : h1);
-      }
-      __syncthreads();
-      prefix |= (uint32_t)sh[0] << shift;
-      want = sh[1];
-      __syncthreads();
+    __syncthreads();
+    // thread t takes two bins, counted from the top: the first digit whose count from above reaches `want`
+    const int top = PE_BINS - 2 * tid - 1;
+    const int h1 = hist[top], h0 = hist[top - 1], upto = wave_sum_scan(h0 + h1);
+    hist[top] = hist[top - 1] = 0;
+    int all;
+    const int before = wave_offset(__builtin_amdgcn_readlane(upto, 63), sh, &all) + upto - h0 - h1;
+    if (before < want && before + h0 + h1 >= want) {  // one thread
+      const bool one = before + h1 >= want;
+      pick[0] = one ? top : top - 1;
+      pick[1] = want - before - (one ? 0 : h1);
     }
+    __syncthreads();
+    threshold |= (uint32_t)pick[0] << shift;
+    want = pick[1];
   }
-  const uint64_t below = (1ull << lane) - 1;
-  int ties = 0, all;
-  each([&](int r, uint32_t c) { ties += __popcll(__ballot(any && r < free_rows && c == prefix)); });
-  const int tie0 = wave_scan(ties, sh, &all);
-  auto kept = [&](int r, uint32_t c, int& at) {
-    const bool tie = any && r < free_rows && c == prefix;
-    const uint64_t b = __ballot(tie);
-    const bool k = r < z.len && (r >= free_rows || (any && c > prefix) || (tie && at + __popcll(b & below) < want));
-    at += __popcll(b);
-    return k;
-  };
-  int holes = 0, tails = 0, at = tie0;
-  each([&](int r, uint32_t c) {
-    const bool k = kept(r, c, at);
-    holes += __popcll(__ballot(r < z.kept && !k));
-    tails += __popcll(__ballot(r >= z.kept && k));
-  });
-  int hole = wave_scan(holes, sh, &all), tail = wave_scan(tails, sh, &all);
-  const int moves = all;
-  int32_t* pr = (int32_t*)(pairs + (int64_t)n * a.K);
+  return EvictCut{threshold, want};
+}
+
+__global__ __launch_bounds__(PE_NT) void paged_threshold_kernel(PagedEvict a, EvictCut* cuts) {
+  const EvictCut e = evict_threshold(a, blockIdx.x, evict_sizes(a, blockIdx.x));
+  if (threadIdx.x == 0) cuts[blockIdx.x] = e;
+}
+
+// Rows [1024 b, 1024 b + 1024) of sequence n, one per thread: what stays in place, the places to fill (holes [N, K], in
+// order) and the rows to move (tails [N, K], from the last one back), their number in moves[n]. ONE: the only block of its
+// sequence, which finds the threshold itself.
+template <bool ONE>
+__global__ __launch_bounds__(PE_NT) void paged_ranks_kernel(PagedEvict a, const EvictCut* cuts, int32_t* holes, int32_t* tails,
+                                                            int32_t* moves) {
+  __shared__ int sh[PE_NW];
+  const int n = blockIdx.y, tid = threadIdx.x, first = blockIdx.x * PE_NT, r = first + tid;
+  const EvictSizes z = evict_sizes(a, n);
+  const int64_t cap = (int64_t)a.pool.max_pages << a.pool.shift;
+  const int free_rows = z.len - z.recent, cut = z.kept;
+  EvictCut e;
+  if constexpr (ONE) e = evict_threshold(a, n, z);
+  else e = cuts[n];
+  const float* w = a.weights + n * a.weights_sn;
   int32_t* index = a.index + (int64_t)n * a.K;
   float* kw = a.kept_weights + n * cap;
-  at = tie0;
-  each([&](int r, uint32_t c) {
-    const bool k = kept(r, c, at), is_hole = r < z.kept && !k, is_tail = r >= z.kept && k;
-    const uint64_t bh = __ballot(is_hole), bt = __ballot(is_tail);
-    if (is_hole) pr[2 * (hole + __popcll(bh & below))] = r;
-    if (is_tail) pr[2 * (tail + __popcll(bt & below)) + 1] = r;
-    hole += __popcll(bh);
-    tail += __popcll(bt);
-    if (k && r < z.kept) {
+  if (blockIdx.x == 0 && tid == 0) {
+    a.kept_lengths[n] = cut;
+    if (cut == z.len) moves[n] = 0;
+  }
+  if (r >= cut && r < a.K) index[r] = -1;
+  if (r >= cut && r < cap) kw[r] = 0.f;
+  if (first >= z.len) return;
+  // the rows before the block: those above the threshold, and those equal to it
+  int more = 0, even = 0;
+  each_code(
+      first < free_rows ? first : free_rows, [&](int i) { return weight_code(w[i]); },
+      [&](int, uint32_t c) {
+        more += c > e.threshold;
+        even += c == e.threshold;
+      });
+  int more_before, even_before;
+  wave_offset(__builtin_amdgcn_readlane(wave_sum_scan(more), 63), sh, &more_before);
+  wave_offset(__builtin_amdgcn_readlane(wave_sum_scan(even), 63), sh, &even_before);
+  const float x = r < z.len ? w[r] : 0.f;
+  const uint32_t c = r < free_rows ? weight_code(x) : 0;
+  int all;
+  const uint64_t evens = __ballot(r < free_rows && c == e.threshold);
+  const int even_rank = even_before + wave_offset(__popcll(evens), sh, &all) + lanes_before(evens);
+  const bool keep = r < z.len && (r >= free_rows || c > e.threshold || (c == e.threshold && even_rank < e.even));
+  const uint64_t keeps = __ballot(keep);
+  const int before = more_before + (even_before < e.even ? even_before : e.even) + (first > free_rows ? first - free_rows : 0) +
+                     wave_offset(__popcll(keeps), sh, &all) + lanes_before(keeps);
+  if (r >= z.len) return;
+  if (r < cut) {
+    if (keep) {
       index[r] = r;
-      kw[r] = w[r];
+      kw[r] = x;
+    } else {
+      holes[(int64_t)n * a.K + r - before] = r;
     }
-  });
-  __syncthreads();
-  for (int i = tid; i < moves; i += PE_NT) {
-    const int to = pr[2 * i], from = pr[2 * i + 1];
-    index[to] = from;
-    kw[to] = w[from];
-  }
-  for (int r = z.kept + tid; r < a.K; r += PE_NT) index[r] = -1;
-  for (int64_t r = z.kept + tid; r < cap; r += PE_NT) kw[r] = 0.f;
-  if (tid == 0) {
-    npairs[n] = moves;
-    a.kept_lengths[n] = z.kept;
+  } else {
+    if (r == cut) moves[n] = cut - before;
+    if (keep) tails[(int64_t)n * a.K + cut - 1 - before] = r;
   }
 }
 
-// pairs [N, K]: (place, source row) of the rows that move, their count in npairs[n].
-__global__ __launch_bounds__(PE_NT) void paged_select_kernel(PagedEvict a, int64_t* pairs, int32_t* npairs) {
-  __shared__ int hist[PE_BINS], sh[PE_NW];
-  const int n = blockIdx.x;
-  const EvictSizes z = evict_sizes(a, n);
-  if (z.len <= PE_HELD * PE_NT)
-    evict_select<true>(a, n, z, pairs, npairs, hist, sh);
-  else
-    evict_select<false>(a, n, z, pairs, npairs, hist, sh);
-}
+// Moves: 16 bytes of K and of V per thread and block, PM_BLOCKS blocks at a time behind one look at the pair and the table.
+constexpr int PM_BLOCKS = 4;
 
-__global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a, const int64_t* pairs, const int32_t* npairs, int es) {
-  const int n = blockIdx.z, chunks = a.pool.D * es / 16;
-  const int64_t total = (int64_t)npairs[n] * a.pool.H * chunks;
-  char* kb = (char*)a.pool.k + blockIdx.y * a.block_sp * es;
-  char* vb = (char*)a.pool.v + blockIdx.y * a.block_sp * es;
+__global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a, const int32_t* holes, const int32_t* tails,
+                                                         const int32_t* moves, int es) {
+  const int n = blockIdx.z, chunks = a.pool.D * es / 16, b0 = blockIdx.y * PM_BLOCKS, count = moves[n];
+  const int64_t total = (int64_t)count * a.pool.H * chunks, cap = (int64_t)a.pool.max_pages << a.pool.shift;
+  char* kb = (char*)a.pool.k + b0 * a.block_sp * es;
+  char* vb = (char*)a.pool.v + b0 * a.block_sp * es;
+  const int64_t step = a.block_sp * es;
+  const int blocks = a.blocks - b0 < PM_BLOCKS ? (int)(a.blocks - b0) : PM_BLOCKS;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int c = (int)(i % chunks), h = (int)(i / chunks % a.pool.H);
-    const int32_t* p = (const int32_t*)(pairs + (int64_t)n * a.K + i / chunks / a.pool.H);
-    const int64_t to = pool_row(a.pool, n, h, p[0]), from = pool_row(a.pool, n, h, p[1]);
+    const int c = (int)(i % chunks), h = (int)(i / chunks % a.pool.H), pair = (int)(i / chunks / a.pool.H);
+    const int to_row = holes[(int64_t)n * a.K + pair], from_row = tails[(int64_t)n * a.K + count - 1 - pair];
+    if (b0 == 0 && h == 0 && c == 0) {
+      a.index[(int64_t)n * a.K + to_row] = from_row;
+      a.kept_weights[n * cap + to_row] = a.weights[n * a.weights_sn + from_row];
+    }
+    const int64_t to = pool_row(a.pool, n, h, to_row), from = pool_row(a.pool, n, h, from_row);
     if (to < 0 || from < 0) continue;
-    *(uint4*)(kb + to * es + c * 16) = ldg16(kb + from * es + c * 16);
-    *(uint4*)(vb + to * es + c * 16) = ldg16(vb + from * es + c * 16);
+    const int64_t fo = from * es + c * 16, so = to * es + c * 16;
+    uint4 k[PM_BLOCKS], v[PM_BLOCKS];
+#pragma unroll
+    for (int b = 0; b < PM_BLOCKS; ++b)
+      if (b < blocks) {
+        k[b] = ldg16(kb + b * step + fo);
+        v[b] = ldg16(vb + b * step + fo);
+      }
+#pragma unroll
+    for (int b = 0; b < PM_BLOCKS; ++b)
+      if (b < blocks) {
+        *(uint4*)(kb + b * step + so) = k[b];
+        *(uint4*)(vb + b * step + so) = v[b];
+      }
   }
 }
 
 int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
-
-}  // namespace
-
-namespace {
 
 int cu_count() {
   static int count[64];
@@ -767,8 +859,16 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
   z->part = (float*)take((int64_t)z->groups * 2 * 16 * QT * D * 4);
   z->ml = (float2*)take((int64_t)z->groups * 2 * 16 * QT * 8);
   z->score_sn = (rows + 63) / 64 * 64;
-  z->stat = (float2*)take(weights ? all * 8 : 0);
-  z->score = (float*)take(weights ? all * z->score_sn * 4 : 0);
+  z->stat = nullptr;
+  z->score = nullptr;
+  if (weights) {
+    z->stat = (float2*)take(all * 8);
+    // The scores kept for the weights, or K again (pa_weights_keys_kernel). 8 x 45,000 rows in bf16, D = 64, us kept / K
+    // again: 8 query rows a head 195 / 213, 16: 231 / 214, 64 (8 x 12,000): 133 / 103. Of few cached rows too few waves
+    // share the heads (8 x 2,000, 16 and 64 query rows: 23 / 32, 43 / 52), and in fp32 the products bound it (8 x 12,000, 64:
+    // 207 / 231).
+    if (sizeof(T) == 4 || 16 * qrows <= 3 * D || N * rows < 65536) z->score = (float*)take(all * z->score_sn * 4);
+  }
   return at;
 }
 
@@ -779,10 +879,12 @@ void launch_pa_w(const PagedAttn& a, const PagedSplit& z, hipStream_t stream) {
   } else {
     hipLaunchKernelGGL((pa_kernel<T, D, QT, W, 4>), dim3((unsigned)z.groups), dim3(256), 0, stream, a, z);
     const unsigned merge = (unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4);
-    hipLaunchKernelGGL((pa_merge_kernel<T, D, QT, W>), dim3(merge), dim3(256), 0, stream, a, z);
+    hipLaunchKernelGGL((pa_merge_kernel<T, D, QT>), dim3(merge), dim3(256), 0, stream, a, z);
   }
-  if (W && z.score_sn)
+  if (W)
     hipLaunchKernelGGL(pa_weights_kernel, dim3((unsigned)(z.score_sn / 64), a.N), dim3(256), 0, stream, a, z);
+  else if (sizeof(T) == 2 && z.stat)
+    hipLaunchKernelGGL(pa_weights_keys_kernel<D>, dim3((unsigned)((z.score_sn + 255) / 256), a.N), dim3(256), 0, stream, a, z);
 }
 
 // Launches (a != null) or sizes the workspace.
@@ -790,8 +892,8 @@ template <typename T, int D, int QT>
 int64_t run_pa(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights,
                hipStream_t stream) {
   PagedSplit z;
-  const int64_t bytes = paged_split<T, D, QT>(&z, (char*)ws, N, Hq, H, Tq, rows, weights);
-  if (a && weights) launch_pa_w<T, D, QT, true>(*a, z, stream);
+  const int64_t bytes = paged_split<T, D, QT>(&z, (char*)ws, N, Hq, H, Tq, rows, weights && rows > 0);
+  if (a && z.score) launch_pa_w<T, D, QT, true>(*a, z, stream);
   else if (a) launch_pa_w<T, D, QT, false>(*a, z, stream);
   return bytes;
 }
@@ -841,19 +943,34 @@ int tabicl_launch_paged_append(const PagedAppend& a, int dtype, hipStream_t stre
   return (int)hipGetLastError();
 }
 
-int64_t tabicl_launch_paged_evict_ws_bytes(int64_t N, int64_t K) { return align256(N * 4) + N * K * 8; }
+int64_t tabicl_launch_paged_evict_ws_bytes(int64_t N, int64_t K) {
+  return align256(N * sizeof(EvictCut)) + align256(N * 4) + 2 * align256(N * K * 4);
+}
 
 int tabicl_launch_paged_evict(const PagedEvict& a, int dtype, void* ws, hipStream_t stream) {
   const int es = dtype == 0 ? 2 : 4;
-  int32_t* npairs = (int32_t*)ws;
-  int64_t* pairs = (int64_t*)((char*)ws + align256((int64_t)a.N * 4));
-  hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)a.N), dim3(PE_NT), 0, stream, a, pairs, npairs);
-  if (a.K > 0 && a.blocks > 0) {
+  char* at = (char*)ws;
+  EvictCut* cuts = (EvictCut*)at;
+  at += align256((int64_t)a.N * sizeof(EvictCut));
+  int32_t* moves = (int32_t*)at;
+  at += align256((int64_t)a.N * 4);
+  int32_t* holes = (int32_t*)at;
+  int32_t* tails = (int32_t*)(at + align256((int64_t)a.N * a.K * 4));
+  const int64_t rows = (int64_t)a.pool.max_pages << a.pool.shift;
+  const dim3 blocks((unsigned)((rows + PE_NT - 1) / PE_NT), (unsigned)a.N), nt(PE_NT);
+  if (rows <= PE_NT) {
+    hipLaunchKernelGGL(paged_ranks_kernel<true>, dim3(1, (unsigned)a.N), nt, 0, stream, a, cuts, holes, tails, moves);
+  } else {
+    hipLaunchKernelGGL(paged_threshold_kernel, dim3((unsigned)a.N), nt, 0, stream, a, cuts);
+    hipLaunchKernelGGL(paged_ranks_kernel<false>, blocks, nt, 0, stream, a, cuts, holes, tails, moves);
+  }
+  if (a.K > 0) {
     const int64_t per = (int64_t)a.K * a.pool.H * (a.pool.D * es / 16);
     int64_t gx = (per + 255) / 256;
     if (gx > 1024) gx = 1024;
-    hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)gx, (unsigned)a.blocks, (unsigned)a.N), dim3(256), 0, stream, a,
-                       pairs, npairs, es);
+    const unsigned gy = a.blocks > PM_BLOCKS ? (unsigned)((a.blocks + PM_BLOCKS - 1) / PM_BLOCKS) : 1;
+    hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)gx, gy, (unsigned)a.N), dim3(256), 0, stream, a, holes, tails, moves,
+                       es);
   }
   return (int)hipGetLastError();
 }
