@@ -55,6 +55,7 @@ struct PagedSplit {
   int qtiles;
   float* part;   // [2 G][16 QT][D] unnormalised outputs
   float2* ml;    // [2 G][16 QT] (ref, sum)
+  int2* ends;    // [N H qtiles] the workgroups that hold the first and the last unit of an item
   float2* stat;  // [N Hq Tq] (ref, 1 / sum) for the weights, or null
   float* score;  // [N Hq Tq][score_sn] scores in log2 units for the weights, or null: from K once more
   int64_t score_sn;
@@ -108,16 +109,6 @@ struct PagedUnits {
       s = wave_sum_scan(u) + before;
     }
   }
-  // the first unit of sequence n
-  __device__ __forceinline__ int before(int n) const {
-    int u = own, s = upto;
-    for (int base = 64; base <= n; base += 64) {
-      const int sum = __builtin_amdgcn_readlane(s, 63);
-      u = load(base);
-      s = wave_sum_scan(u) + sum;
-    }
-    return __builtin_amdgcn_readlane(s - u, n & 63);
-  }
 };
 
 // Equal shares: `groups` workgroups (fewer, if they would get less than `least` units) of `share` units, the first `more`
@@ -131,11 +122,6 @@ struct PagedShares {
     more = total - share * groups;
   }
   __device__ __forceinline__ int first(int w) const { return w * share + (w < more ? w : more); }
-  // the workgroup that holds unit t
-  __device__ __forceinline__ int holder(int t) const {
-    const int big = more * (share + 1);
-    return t < big ? t / (share + 1) : more + (t - big) / share;
-  }
 };
 
 template <typename T, int D>
@@ -227,8 +213,25 @@ __device__ __forceinline__ void paged_values(const PagedTile<float, D>& t, const
   }
 }
 
+// N values to p, 16 bytes at a time.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* p, const float* x) {
+  constexpr int C = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < N; j += C) {
+    if constexpr (C == 4) {
+      *(f32x4*)(p + j) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+    } else {
+      const bf16x4 lo = cvt_bf16x4(f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]});
+      const bf16x4 hi = cvt_bf16x4(f32x4{x[j + 4], x[j + 5], x[j + 6], x[j + 7]});
+      *(bf16x8*)(p + j) = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+}
+
+// Rows [c0, c1) of an item by the NW waves of a workgroup: the output, or (slot >= 0) a partial of it.
 template <typename T, int D, int QT, bool W, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void pa_kernel(PagedAttn a, PagedSplit z) {
+__device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit& z, int n, int item, int c0, int c1, int slot) {
   typedef PagedTile<T, D> Tile;
   constexpr int SUB = Tile::SUB, KS = Tile::KS, NC = Tile::NC, DE = Tile::DE, ES = Tile::ES;
   __shared__ float sh_o[NW / 2][16 * QT][D + 4];
@@ -238,34 +241,6 @@ __global__ __launch_bounds__(64 * NW, 2) void pa_kernel(PagedAttn a, PagedSplit 
   const int G = a.Hq / c.H, rows = G * a.Tq;
   const float sc = a.scale * TA_LOG2E;
   const uint32_t koff = lr * D * ES + lg * 16, voff = lg * 4 * D * ES + lr * DE * ES;
-  const int per = c.H * z.qtiles;
-  int unit = 0, end = 1, n = 0, first = 0;
-  const PagedUnits units(a, per, lane);
-  if (z.groups) {
-    const PagedShares shares(z, units.total);
-    if ((int)blockIdx.x >= shares.groups) return;
-    unit = shares.first(blockIdx.x);
-    end = shares.first(blockIdx.x + 1);
-  }
-  while (unit < end) {
-  // the segment: rows [c0, c1) of an item
-  int item, c0, c1, slot = -1;
-  if (z.groups) {
-    n = units.find(unit, &first);
-    const int len = __builtin_amdgcn_readfirstlane(pa_len(a, n)), each = pa_units(len);
-    item = (unit - first) / each;
-    const int u0 = unit - first - item * each, u1 = u0 + end - unit < each ? u0 + end - unit : each;
-    c0 = u0 * PA_UNIT;
-    c1 = u1 * PA_UNIT < len ? u1 * PA_UNIT : len;
-    if (u1 - u0 < each) slot = 2 * blockIdx.x + (u0 == 0);
-    unit += u1 - u0;
-  } else {
-    n = blockIdx.x / per;
-    item = blockIdx.x % per;
-    c0 = 0;
-    c1 = __builtin_amdgcn_readfirstlane(pa_len(a, n));
-    unit = end;
-  }
   const int qt0 = item % z.qtiles, h = item / z.qtiles, nh = n * c.H + h;
 
   // this lane's query rows: 16 QT of the (head of the group, query row) pairs
@@ -417,27 +392,56 @@ __global__ __launch_bounds__(64 * NW, 2) void pa_kernel(PagedAttn a, PagedSplit 
     for (int t = 0; t < QT; ++t) {
       const int r = (qt0 * QT + t) * 16 + lr;
       if (r >= rows) continue;
+      const float inv = slot >= 0 ? 1.f : l[t] == 0.f ? 0.f : 1.f / l[t];
+      float x[4 * DE];  // columns 4 DE lg + j of the row
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < DE; ++e) x[i * DE + e] = o[t][e][i] * inv;
       if (slot >= 0) {
         const int64_t at = (int64_t)slot * 16 * QT + t * 16 + lr;
-        float* po = z.part + at * D + lg * 4 * DE;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < DE; ++e) po[i * DE + e] = o[t][e][i];
+        store_row<float, 4 * DE>(z.part + at * D + lg * 4 * DE, x);
         if (lg == 0) z.ml[at] = make_float2(ref[t], l[t]);
       } else {
-        const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
-        T* op = (T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lg * 4 * DE;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < DE; ++e) op[i * DE + e] = (T)(o[t][e][i] * inv);
+        store_row<T, 4 * DE>((T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lg * 4 * DE, x);
         if (z.stat && lg == 0) z.stat[(int64_t)nh * rows + r] = make_float2(ref[t], inv);
       }
     }
   }
+}
+
+// Equal shares of all items' units.
+template <typename T, int D, int QT, bool W>
+__global__ __launch_bounds__(256, 2) void pa_kernel(PagedAttn a, PagedSplit z) {
+  const int per = a.pool.H * z.qtiles;
+  const PagedUnits units(a, per, threadIdx.x & 63);
+  const PagedShares shares(z, units.total);
+  if ((int)blockIdx.x >= shares.groups) return;
+  int unit = shares.first(blockIdx.x);
+  const int end = shares.first(blockIdx.x + 1);
+  while (unit < end) {
+    int first;
+    const int n = units.find(unit, &first);
+    const int len = __builtin_amdgcn_readfirstlane(pa_len(a, n)), each = pa_units(len);
+    const int item = (unit - first) / each, u0 = unit - first - item * each;
+    const int u1 = u0 + end - unit < each ? u0 + end - unit : each;
+    if (threadIdx.x == 0 && u0 == 0) z.ends[n * per + item].x = blockIdx.x;
+    if (threadIdx.x == 0 && u1 == each) z.ends[n * per + item].y = blockIdx.x;
+    pa_segment<T, D, QT, W, 4>(a, z, n, item, u0 * PA_UNIT, u1 * PA_UNIT < len ? u1 * PA_UNIT : len,
+                               u1 - u0 < each ? 2 * blockIdx.x + (u0 == 0) : -1);
+    unit += u1 - u0;
   }
 }
+
+// A workgroup of eight waves for each item, where no sequence is long.
+template <typename T, int D, int QT, bool W>
+__global__ __launch_bounds__(512, 2) void pa_whole_kernel(PagedAttn a, PagedSplit z) {
+  const int per = a.pool.H * z.qtiles, n = blockIdx.x / per;
+  pa_segment<T, D, QT, W, 8>(a, z, n, blockIdx.x % per, 0, __builtin_amdgcn_readfirstlane(pa_len(a, n)), -1);
+}
+
+__device__ __forceinline__ void store4(float* p, f32x4 x) { *(f32x4*)p = x; }
+__device__ __forceinline__ void store4(bf16* p, f32x4 x) { *(bf16x4*)p = cvt_bf16x4(x); }
 
 // Joins the partials of one query row per wave: 4 values of a partial output per lane, 256 / D partials at a time. Rows
 // that pa_kernel has written are left alone; rows without a key become 0.
@@ -448,19 +452,14 @@ __global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z
   const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= (int64_t)a.N * a.pool.H * rows) return;
   const int r = (int)(row % rows), nh = (int)(row / rows), n = nh / a.pool.H, h = nh % a.pool.H;
-  const PagedUnits units(a, a.pool.H * z.qtiles, lane);
-  const PagedShares shares(z, units.total);
-  const int each = pa_units(__builtin_amdgcn_readfirstlane(pa_len(a, n)));
+  const int2 w = z.ends[nh * z.qtiles + r / (16 * QT)];
+  const int len = pa_len(a, n);
   T* op = (T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lane * 4;
-  if (each == 0) {
-    if (lane < LPR)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) op[i] = (T)0.f;
+  if (len == 0) {
+    if (lane < LPR) store4(op, f32x4{0.f, 0.f, 0.f, 0.f});
     return;
   }
-  // the workgroups of the item's first and last unit
-  const int t0 = units.before(n) + (h * z.qtiles + r / (16 * QT)) * each;
-  const int w0 = shares.holder(t0), w1 = shares.holder(t0 + each - 1);
+  const int w0 = __builtin_amdgcn_readfirstlane(w.x), w1 = __builtin_amdgcn_readfirstlane(w.y);
   if (w0 == w1) return;
   const int parts = w1 - w0 + 1, at = r % (16 * QT);
   auto slot = [&](int i) { return (int64_t)(2 * (w0 + i) + (i == 0)) * (16 * QT) + at; };
@@ -488,9 +487,7 @@ __global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z
     for (int j = 0; j < 4; ++j) o[j] = o[j] * f0 + __shfl_xor(o[j], x, 64) * f1;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane < LPR)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) op[i] = (T)(o[i] * inv);
+  if (lane < LPR) store4(op, o * inv);
   if (z.stat && lane == 0) z.stat[row] = make_float2(m, inv);
 }
 
@@ -688,7 +685,7 @@ __device__ __forceinline__ int wave_offset(int count, int* sh, int* all) {
 
 // The threshold by three digits (11, 11 and 10 bits) of a histogram in LDS. One CU does it, bound by the latency and issue
 // of three passes over the weights (from L2), so it does nothing else and keeps eight loads a thread in flight: 16,384
-// rows take 12 us, 45,000 rows 22 us (four loads in flight: 42; with the ranks in it too, 16,384 rows took 29).
+// rows take 14 us, 45,000 rows 21 us (four loads in flight: 42; with the ranks in it too, 16,384 rows took 29).
 __device__ __forceinline__ EvictCut evict_threshold(const PagedEvict& a, int n, const EvictSizes z) {
   __shared__ int hist[PE_BINS], sh[PE_NW], pick[2];
   const int tid = threadIdx.x, free_rows = z.len - z.recent;
@@ -858,6 +855,7 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
   const int64_t all = N * H * qrows;
   z->part = (float*)take((int64_t)z->groups * 2 * 16 * QT * D * 4);
   z->ml = (float2*)take((int64_t)z->groups * 2 * 16 * QT * 8);
+  z->ends = (int2*)take(z->groups ? N * H * z->qtiles * 8 : 0);
   z->score_sn = (rows + 63) / 64 * 64;
   z->stat = nullptr;
   z->score = nullptr;
@@ -875,9 +873,9 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
 template <typename T, int D, int QT, bool W>
 void launch_pa_w(const PagedAttn& a, const PagedSplit& z, hipStream_t stream) {
   if (z.groups == 0) {
-    hipLaunchKernelGGL((pa_kernel<T, D, QT, W, 8>), dim3((unsigned)(a.N * a.pool.H * z.qtiles)), dim3(512), 0, stream, a, z);
+    hipLaunchKernelGGL((pa_whole_kernel<T, D, QT, W>), dim3((unsigned)(a.N * a.pool.H * z.qtiles)), dim3(512), 0, stream, a, z);
   } else {
-    hipLaunchKernelGGL((pa_kernel<T, D, QT, W, 4>), dim3((unsigned)z.groups), dim3(256), 0, stream, a, z);
+    hipLaunchKernelGGL((pa_kernel<T, D, QT, W>), dim3((unsigned)z.groups), dim3(256), 0, stream, a, z);
     const unsigned merge = (unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4);
     hipLaunchKernelGGL((pa_merge_kernel<T, D, QT>), dim3(merge), dim3(256), 0, stream, a, z);
   }

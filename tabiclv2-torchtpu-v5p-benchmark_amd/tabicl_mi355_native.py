@@ -193,7 +193,7 @@ def direct(*ts: torch.Tensor | None) -> bool:
         return False
     grad = torch.is_grad_enabled()
     for t in ts:
-        if t is not None and (type(t) not in _PLAIN_TYPES or t.device.type != "cuda" or (grad and t.requires_grad)):
+        if t is not None and (type(t) not in _PLAIN_TYPES or not t.is_cuda or (grad and t.requires_grad)):
             return False
     return True
 
