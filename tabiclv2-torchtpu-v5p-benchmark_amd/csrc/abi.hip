@@ -747,6 +747,9 @@ int paged_attn_sizes(const char* op, int64_t N, int64_t Hq, int64_t H, int64_t T
     return fail(1, "%s: bad sizes N=%lld Hq=%lld H=%lld Tq=%lld D=%lld rows=%lld (Hq must be a multiple of H)", op,
                 (long long)N, (long long)Hq, (long long)H, (long long)Tq, (long long)D, (long long)rows);
   if (Tq > (1LL << 22) || N * Hq * Tq > (1LL << 22)) return fail(1, "%s: more than 2^22 query rows", op);
+  // units of 128 rows of every sequence, head and tile of 16 query rows are counted in 32 bits
+  if (N * H * ((Hq / H * Tq + 15) / 16) * (rows / 128 + 1) > (1LL << 30))
+    return fail(1, "%s: more than 2^37 cached rows over all sequences, heads and tiles of query rows", op);
   return 0;
 }
 
@@ -843,12 +846,14 @@ int tabicl_paged_evict(void* k_pages, void* v_pages, int64_t blocks, int64_t blo
                        int32_t* kept_lengths, int64_t N, int64_t H, int64_t D, int32_t dtype, void* ws, int64_t ws_bytes,
                        void* stream) {
   PagedEvict a = {};
-  int st = paged_pool("paged_evict", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+  int st = paged_pool("paged_evict", &a.pool, k_pages, v_pages, blocks > 0 ? pages : 0, page_sp, page_rows, table, table_sn, max_pages,
                       lengths, N, H, D, dtype);
   if (st) return st;
   const int64_t cap = max_pages * page_rows;
   if (blocks < 0 || blocks > 65535 || block_sp < 0 || !stride_ok(block_sp, dtype))
     return fail(1, "paged_evict: bad block count or stride");
+  if (N * (cap + 1024) > (1LL << 31) || N * ((blocks + 3) / 4 + 1) > PAGED_MAX_GRID)
+    return fail(1, "paged_evict: more than 2^31 rows over all sequences, or 2^25 blocks");
   if (recent < 0 || keep_all < 0 || K < 0 || K > cap) return fail(1, "paged_evict: needs recent, keep >= 0 and 0 <= K <= the capacity %lld", (long long)cap);
   if (N == 0) return 0;
   if (!kept_lengths || (K > 0 && !index) || (cap > 0 && (!weights || !kept_weights)) || weights_sn < cap)

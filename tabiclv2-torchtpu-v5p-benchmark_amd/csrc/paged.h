@@ -51,6 +51,10 @@ struct PagedEvict {
   int N;
 };
 
+// Workgroups of a launch (256 threads, or 1,024 for a quarter of them): below the 2^32 threads beyond which a launch leaves
+// workgroups out without an error.
+#define PAGED_MAX_GRID (1ll << 23)
+
 // dtype codes 0 bf16, 1 fp32. Return value: hipGetLastError() after the launches.
 int tabicl_launch_paged_attn(const PagedAttn& a, int dtype, void* ws, hipStream_t stream);
 int64_t tabicl_launch_paged_attn_ws_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows, int weights,

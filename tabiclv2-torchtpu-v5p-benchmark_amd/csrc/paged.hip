@@ -936,6 +936,7 @@ int tabicl_launch_paged_append(const PagedAppend& a, int dtype, hipStream_t stre
   const int es = dtype == 0 ? 2 : 4;
   const int64_t per_n = (int64_t)a.T * a.pool.H * (a.pool.D * es / 16);
   int64_t gx = (per_n + 255) / 256;
+  if (gx > PAGED_MAX_GRID / a.N) gx = PAGED_MAX_GRID / a.N;
   if (gx > 4096) gx = 4096;
   hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)gx, (unsigned)a.N), dim3(256), 0, stream, a, es);
   return (int)hipGetLastError();
@@ -964,9 +965,10 @@ int tabicl_launch_paged_evict(const PagedEvict& a, int dtype, void* ws, hipStrea
   }
   if (a.K > 0) {
     const int64_t per = (int64_t)a.K * a.pool.H * (a.pool.D * es / 16);
-    int64_t gx = (per + 255) / 256;
-    if (gx > 1024) gx = 1024;
     const unsigned gy = a.blocks > PM_BLOCKS ? (unsigned)((a.blocks + PM_BLOCKS - 1) / PM_BLOCKS) : 1;
+    int64_t gx = (per + 255) / 256;
+    if (gx > PAGED_MAX_GRID / ((int64_t)gy * a.N)) gx = PAGED_MAX_GRID / ((int64_t)gy * a.N);
+    if (gx > 1024) gx = 1024;
     hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)gx, gy, (unsigned)a.N), dim3(256), 0, stream, a, holes, tails, moves,
                        es);
   }

@@ -3,10 +3,11 @@ attend over the cached train rows of their table, and a cache over its budget ke
 
 IclKVCache (tabicl_mi355_icl.py) gives every estimator of a cache the same capacity; a service that holds many tables at
 once, that gets its train rows over time or answers one test row at a time keeps them here instead:
-  * paged_attention(q, k_pages, v_pages, table, lengths, weights) (op tabicl::paged_attn): attention of few query rows
-    over the cached rows, optionally adding up the attention weight that each cached row drew;
+  * paged_attention(q, k_pages, v_pages, table, lengths, weights) (ops tabicl::paged_attn, paged_attn_out,
+    paged_attn_weights_out): attention of few query rows over the cached rows, optionally adding up the attention weight
+    that each cached row drew;
   * paged_append (op tabicl::paged_append): new rows into the pages;
-  * paged_evict (op tabicl::paged_evict): cuts sequences to their rows of largest weight, in place;
+  * paged_evict (op tabicl::paged_evict_out): cuts sequences to their rows of largest weight, in place;
   * PagedIclKVCache: the pool, the page table and the lengths, with the surface of IclKVCache (append, query,
     attention_layer, query_blocks, usable as cached_query's icl_cache), and evict.
 
@@ -113,8 +114,8 @@ def _attn_launch(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     _, Hq, Tq, _ = shape
     q, qn, qh, qr = _rows16(q, q.element_size())
     on, oh, orow, od = out.stride()
-    if od != 1:
-        raise ValueError("out needs a contiguous last dim")
+    if od != 1 or (N > 1 and on == 0) or (Hq > 1 and oh == 0) or (Tq > 1 and orow == 0):
+        raise ValueError("out needs a contiguous last dim and a place of its own for each row")
     on, oh, orow = on if N > 1 else 0, oh if Hq > 1 else 0, orow if Tq > 1 else 0
     key = (N, Hq, H, Tq, D, rows, w_ptr != 0, code, dev)
     nbytes = _WS_BYTES.get(key)
@@ -126,29 +127,41 @@ def _attn_launch(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
               None if ws is None else ws.data_ptr(), nbytes, _nat.stream_of(q))
 
 
-@torch.library.custom_op("tabicl::paged_attn", mutates_args=("weights",))
-def _paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Optional[Tensor],
-                scale: float) -> Tensor:
-    """See paged_attention; weights is added to in place."""
+# Three ops, since torch.compile refuses an op that returns a tensor and may or may not change another.
+@torch.library.custom_op("tabicl::paged_attn", mutates_args=())
+def _paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float) -> Tensor:
+    """See paged_attention."""
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, out)
+    _attn_launch(q, k_pages, v_pages, table, lengths, None, scale, out)
     return out
 
 
 @_paged_attn.register_fake
-def _(q, k_pages, v_pages, table, lengths, weights, scale):  # noqa: ANN001
+def _(q, k_pages, v_pages, table, lengths, scale):  # noqa: ANN001
     return q.new_empty(q.shape)
 
 
-@torch.library.custom_op("tabicl::paged_attn_out", mutates_args=("out", "weights"))
-def _paged_attn_out(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Optional[Tensor],
-                    scale: float, out: Tensor) -> None:
+@torch.library.custom_op("tabicl::paged_attn_out", mutates_args=("out",))
+def _paged_attn_out(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float,
+                    out: Tensor) -> None:
     """tabicl::paged_attn written into `out`, any [N, Hq, Tq, D] view with a contiguous last dim."""
-    _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, out)
+    _attn_launch(q, k_pages, v_pages, table, lengths, None, scale, out)
 
 
 @_paged_attn_out.register_fake
-def _(q, k_pages, v_pages, table, lengths, weights, scale, out):  # noqa: ANN001
+def _(q, k_pages, v_pages, table, lengths, scale, out):  # noqa: ANN001
+    return None
+
+
+@torch.library.custom_op("tabicl::paged_attn_weights_out", mutates_args=("out", "weights"))
+def _paged_attn_weights_out(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float,
+                            out: Tensor, weights: Tensor) -> None:
+    """tabicl::paged_attn_out that adds the attention weights to `weights` in place."""
+    _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, out)
+
+
+@_paged_attn_weights_out.register_fake
+def _(q, k_pages, v_pages, table, lengths, scale, out, weights):  # noqa: ANN001
     return None
 
 
@@ -181,9 +194,13 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
             torch.autograd.graph.increment_version(weights)
         return o
     _no_grad("paged_attention", q, k_pages, v_pages, weights, out)
-    if out is None:
-        return torch.ops.tabicl.paged_attn(q, k_pages, v_pages, table, lengths, weights, scale)
-    torch.ops.tabicl.paged_attn_out(q, k_pages, v_pages, table, lengths, weights, scale, out)
+    if out is None and weights is None:
+        return torch.ops.tabicl.paged_attn(q, k_pages, v_pages, table, lengths, scale)
+    out = q.new_empty(q.shape) if out is None else out
+    if weights is None:
+        torch.ops.tabicl.paged_attn_out(q, k_pages, v_pages, table, lengths, scale, out)
+    else:
+        torch.ops.tabicl.paged_attn_weights_out(q, k_pages, v_pages, table, lengths, scale, out, weights)
     return out
 
 
@@ -239,7 +256,7 @@ def paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tenso
 
 
 def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int,
-                  recent: int, keep_n: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+                  recent: int, keep_n: Optional[Tensor], index: Tensor, kept_weights: Tensor, kept: Tensor) -> None:
     pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths, 1)
     w_sn = _check_weights(weights, N, pool[2] * pool[5], dev)
     if keep < 0 or recent < 0:
@@ -250,12 +267,12 @@ def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tens
     if dev != torch.cuda.current_device() if dev >= 0 else True:
         _nat.require_device(table)
         with torch.cuda.device(dev):
-            return _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n)
+            return _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights, kept)
     B, cap = k_pages.shape[0], pool[2] * pool[5]
     K = min(keep, cap)
-    index = table.new_empty(N, K)
-    kept_weights = weights.new_empty(N, cap)
-    kept = table.new_empty(N)
+    for t, shape, dtype in ((index, (N, K), torch.int32), (kept_weights, (N, cap), torch.float32), (kept, (N,), torch.int32)):
+        if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != dev:
+            raise ValueError(f"eviction writes to contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
     key = (N, K)
     nbytes = _WS_BYTES.get(key)
     if nbytes is None:
@@ -268,20 +285,18 @@ def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tens
               lengths.data_ptr(), weights.data_ptr(), w_sn, None if keep_n is None else keep_n.data_ptr(), keep, recent,
               index.data_ptr(), K, kept_weights.data_ptr(), kept.data_ptr(), N, H, D, code, ws.data_ptr(), nbytes,
               _nat.stream_of(table))
-    return index, kept_weights, kept
 
 
-@torch.library.custom_op("tabicl::paged_evict", mutates_args=("k_pages", "v_pages"))
-def _paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int, recent: int,
-                 keep_n: Optional[Tensor] = None) -> tuple[Tensor, Tensor, Tensor]:
+@torch.library.custom_op("tabicl::paged_evict_out", mutates_args=("k_pages", "v_pages", "index", "kept_weights", "kept"))
+def _paged_evict_out(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int,
+                     recent: int, keep_n: Optional[Tensor], index: Tensor, kept_weights: Tensor, kept: Tensor) -> None:
     """See paged_evict; keep_n is its tensor keep (keep then bounds it)."""
-    return _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n)
+    _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights, kept)
 
 
-@_paged_evict.register_fake
-def _(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n=None):  # noqa: ANN001
-    N, cap = table.shape[0], table.shape[1] * k_pages.shape[3]
-    return (table.new_empty(N, min(keep, cap)), weights.new_empty(N, cap), table.new_empty(N))
+@_paged_evict_out.register_fake
+def _(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights, kept):  # noqa: ANN001
+    return None
 
 
 def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor,
@@ -297,14 +312,21 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
     if k_pages.dim() == 4 and v_pages.dim() == 4:
         k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
     keep_n = None
+    N, cap = table.shape[0], table.shape[1] * k_pages.shape[3] if k_pages.dim() == 5 else 0
     if isinstance(keep, Tensor):
-        keep, keep_n = table.shape[1] * k_pages.shape[3], keep
+        keep, keep_n = cap, keep
+    keep, recent = int(keep), int(recent)
+    index = table.new_empty(N, max(0, min(keep, cap)))
+    kept_weights = weights.new_empty(N, cap)
+    kept = table.new_empty(N)
     if _nat.direct(k_pages, v_pages, table, lengths, weights, keep_n):
-        r = _evict_launch(k_pages, v_pages, table, lengths, weights, int(keep), int(recent), keep_n)
+        _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights, kept)
         torch.autograd.graph.increment_version((k_pages, v_pages))
-        return r
-    _no_grad("paged_evict", k_pages, v_pages, weights)
-    return torch.ops.tabicl.paged_evict(k_pages, v_pages, table, lengths, weights, int(keep), int(recent), keep_n)
+    else:
+        _no_grad("paged_evict", k_pages, v_pages, weights)
+        torch.ops.tabicl.paged_evict_out(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights,
+                                         kept)
+    return index, kept_weights, kept
 
 
 class PagedIclKVCache(_icl.IclKVCache):

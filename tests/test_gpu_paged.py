@@ -140,8 +140,10 @@ def test_strided_views(dev, dtype):
     got = paged.paged_attention(q, big[0, :, 1], big[1, :, 2], wide_t[:, :table.shape[1]], n, w)
     assert torch.equal(got, want) and (w[:, table.shape[1] * R:] == 0).all()
     assert abs(float(w.sum()) - N * H * T) < 1e-2
-    with pytest.raises(ValueError):
-        paged.paged_attention(q, kp, vp, table, n, None, None, torch.zeros_like(wide)[..., ::1][..., :D][..., ::2])
+    for bad in (torch.zeros(N, H, T, 2 * D, dtype=dtype, device=dev)[..., ::2],
+                torch.zeros(N, 1, T, D, dtype=dtype, device=dev).expand(N, H, T, D)):
+        with pytest.raises(ValueError, match="out needs"):
+            paged.paged_attention(q, kp, vp, table, n, None, None, bad)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
@@ -453,18 +455,65 @@ def test_ops_equal_direct_calls(dev):
         def step():
             paged.paged_append(kp[1], vp[1], table, n - 3, q, q)
             out = paged.paged_attention(q, kp[1], vp[1], table, n, w)
+            out1 = paged.paged_attention(q, kp[1], vp[1], table, n)
             paged.paged_attention(q, kp[0], vp[0], table, n, None, None, out2)
-            return (out, out2, w, *paged.paged_evict(kp, vp, table, n, w, 60, 3), kp, vp)
+            return (out, out1, out2, w, *paged.paged_evict(kp, vp, table, n, w, 60, 3), kp, vp)
 
         if mode is None:
             results.append(step())
         else:
             with mode:
                 results.append(step())
-    for name in ("paged_append", "paged_attn.", "paged_attn_out", "paged_evict"):
+    for name in ("paged_append", "paged_attn.", "paged_attn_out", "paged_attn_weights_out", "paged_evict_out"):
         assert any(name in s for s in Seen.names), (name, Seen.names)
     for a, b in zip(*results):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_compile(dev):
+    # torch.compile takes the wrappers as ops, whole graph, with their in-place results
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, 77, [300, 20], blocks=2)
+    w = torch.rand(2, table.shape[1] * 64, generator=g, device=dev)
+    start = [t.clone() for t in (kp, vp, w)]
+
+    def step(q, kp, vp, table, n, w):
+        paged.paged_append(kp[0], vp[0], table, n - 2, q, q)
+        out = torch.zeros_like(q)
+        paged.paged_attention(q * 2, kp[0], vp[0], table, n, w, None, out)
+        index, kw, kept = paged.paged_evict(kp, vp, table, n, w, 50, 4)
+        return out + 1, paged.paged_attention(q, kp[1], vp[1], table, kept), index, kw, kept
+
+    want = [t.clone() for t in (*step(q, kp, vp, table, n, w), kp, vp, w)]
+    for t, s in zip((kp, vp, w), start):
+        t.copy_(s)
+    got = (*torch.compile(step, fullgraph=True)(q, kp, vp, table, n, w), kp, vp, w)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_nothing_to_do(dev):
+    # no sequences, no query rows, no pages in the table, an empty pool, nothing to keep
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, 79, [40, 5], H=2, R=16, T=2)
+    assert paged.paged_attention(q[:0], kp, vp, table[:0], n[:0]).shape == (0, 2, 2, 64)
+    assert paged.paged_attention(q[:, :, :0], kp, vp, table, n).shape == (2, 2, 0, 64)
+    w = torch.rand(2, 48, generator=g, device=dev)
+    before = w.clone()
+    for pool, t in (((kp, vp), table[:, :0]), ((kp[:0], vp[:0]), table)):
+        assert (paged.paged_attention(q, *pool, t, n, w) == 0).all()
+        paged.paged_append(*pool, t, n, q, q)
+    assert torch.equal(w, before)
+    assert paged.paged_attention(q, kp, vp, table, n, w[:, :48], 0.1).shape == q.shape
+    index, kw, kept = paged.paged_evict(kp, vp, table, n, w, 0)
+    assert index.shape == (2, 0) and (kw == 0).all() and (kept == 0).all()
+    index, kw, kept = paged.paged_evict(kp[None, :0].expand(3, -1, -1, -1, -1).contiguous(), vp[None, :0].expand(3, -1, -1, -1, -1).contiguous(),
+                                        table, n, w, 7)
+    assert kept.tolist() == [7, 5]
+    index, kw, kept = paged.paged_evict(kp[None][:0], vp[None][:0], table, n, w, 7)
+    assert kept.tolist() == [7, 5] and set(index[0].tolist()) == set(w[0, :40].topk(7).indices.tolist())
+    torch.cuda.synchronize()
 
 
 def test_gradient_refused(dev):

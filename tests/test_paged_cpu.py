@@ -105,7 +105,8 @@ def test_abi_refuses_before_launch():
                      (dict(scale=float("nan")), "scale"), (dict(table=None), "table"), (dict(M=1 << 30), "page counts"),
                      (dict(w=a, wsn=255), "weights"), (dict(qs=(512, 63, 512)), "strides"), (dict(N=70000), "65535"),
                      (dict(Tq=1 << 23), "query rows"), (dict(w=a, wsn=256, wsb=8), "workspace"),
-                     (dict(pages=-1), "page counts")):
+                     (dict(pages=-1), "page counts"), (dict(w=a, wsn=1 << 30, M=1 << 20, N=9), "2^29"),
+                     (dict(M=1 << 22, N=500), "2^37")):
         assert attn(**kw) == 1 and word in nat.last_error(), (kw, nat.last_error())
     assert attn(N=0) == 0 and attn(Tq=0, q=None) == 0
     assert lib.tabicl_paged_attn_workspace_bytes(2, 8, 8, 1, 48, 1000, 0, 0) < 0
@@ -120,12 +121,13 @@ def test_abi_refuses_before_launch():
         assert append(**kw) == 1 and word in nat.last_error(), (kw, nat.last_error())
     assert append(T=0) == 0 and append(N=0) == 0
 
-    def evict(K=100, recent=0, ws=a, wsb=1 << 40, bsp=0, w=a, N=2):
-        return lib.tabicl_paged_evict(a, a, 1, bsp, 10, 8 * 64 * 64, 64, a, 4, 4, a, w, 256, None, 100, recent, a, K, a, a, N,
+    def evict(K=100, recent=0, ws=a, wsb=1 << 40, bsp=0, w=a, N=2, M=4):
+        return lib.tabicl_paged_evict(a, a, 1, bsp, 10, 8 * 64 * 64, 64, a, M, M, a, w, 64 * M, None, 100, recent, a, K, a, a, N,
                                       8, 64, 0, ws, wsb, None)
 
     for kw, word in ((dict(K=257), "capacity"), (dict(recent=-1), "recent"), (dict(ws=None), "workspace"),
-                     (dict(wsb=64), "workspace"), (dict(bsp=4), "block"), (dict(w=None), "weights")):
+                     (dict(wsb=64), "workspace"), (dict(bsp=4), "block"), (dict(w=None), "weights"),
+                     (dict(N=65000, M=1 << 10), "2^31")):
         assert evict(**kw) == 1 and word in nat.last_error(), (kw, nat.last_error())
     assert evict(N=0) == 0
 
