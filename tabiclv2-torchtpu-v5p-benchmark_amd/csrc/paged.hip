@@ -26,27 +26,27 @@ __device__ __forceinline__ int64_t pool_row(const PagedPool& c, int n, int h, in
 // ---------------------------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------------------------
-// Bound by the bytes of K and V, which are read once: a workgroup takes `chunk` rows of one (sequence, K/V head) and up
-// to 16 QT of its query rows (the heads of a group and the query rows together), its NW waves take turns of KS rows.
-// Nothing of K and V is shared between waves, so they go from memory straight into the registers of the matrix products,
-// a turn ahead of their use; LDS only joins the waves at the end.
+// Bound by the bytes of K and V, which are read once (one row over 8 x 45,000 cached rows of 8 heads: 124 us, 5.9 TB/s). A
+// workgroup takes a run of rows of one item: a sequence, a K/V head and up to 16 QT query rows (the heads of a group and
+// the query rows together); its NW waves take turns of KS rows. Nothing of K and V is shared between waves, so they go from
+// memory straight into the registers of the matrix products, a turn ahead of their use; LDS only joins the waves at the end.
 //   S^T = K Q^T  (16 keys x 16 queries): the A operand is 16 bytes of a K row per lane, the result holds query l % 16,
 //                keys 4 (l / 16) + i, which is the B operand of
 //   O^T = V^T P^T with the keys in that order: the A operand holds the values of column group l % 16 (D / 16 columns, one
 //                per product) of those keys; in bf16 the halves of pairs of rows are regrouped by v_perm_b32.
+// One query row leaves 15 of the 16 columns empty: the products stay far below the loads all the same.
 // bf16 probabilities enter as two bf16 terms (2^-16 of each left out), so that the output is off by its own rounding
 // alone; the second product costs nothing beside the loads. fp32 runs on the fp32 matrix unit.
-// Softmax: p = 2^(s - ref) with ref the running maximum + PA_SHIFT, moved only when a score passes it by more than 2^8
-// (one test per turn); the shift keeps sums of 2^30 products with values near the largest float finite.
+// Softmax: p = 2^(s - ref) with ref the running maximum + PA_SHIFT, moved only when a score passes the maximum by more than
+// 2^PA_SLACK (one test per turn); the shift keeps sums of products with values near the largest float finite.
 constexpr float PA_SHIFT = 24.f, PA_SLACK = 8.f;
 constexpr float PA_REF0 = -3.4028234663852886e38f;
 
-// The work is cut on the device, by the lengths as they are: a unit is PA_UNIT rows of one item (sequence, K/V head, query
-// tile), units are counted item after item, and workgroup w of G takes the units [w T / G, (w + 1) T / G) of all T: an equal
-// share whatever the lengths, with G two per CU. An item that one workgroup covers is
+// The work is cut on the device, by the lengths as they are: a unit is PA_UNIT rows of one item, units are counted item after
+// item, and G workgroups, two per CU, take equal runs of them, whatever the lengths. An item that one workgroup covers is
 // written at once; of the others each workgroup leaves a partial (at most two: one of an item begun before it, one of an
-// item it begins), which pa_merge_kernel joins. (A fixed number of rows per workgroup: 64 sequences of 500 to 10,000 rows
-// took 97 us at 8 workgroups per CU and 146 at 2, one sequence of 45,000 rows 39 and 27.)
+// item it begins), which pa_merge_kernel joins. (A fixed number of rows per workgroup instead: 64 sequences of 500 to
+// 10,000 rows took 97 us at 8 workgroups per CU and 146 at 2, one sequence of 45,000 rows 39 and 27; this way 84 and 26.)
 constexpr int PA_UNIT = 128, PA_WHOLE = 1024;
 
 struct PagedSplit {
@@ -300,19 +300,28 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
     return live;
   };
   auto compute = [&](Tile& t, int key, int live) {
+    const bool full = live == (SUB == 2 ? 16 << 8 | 16 : 16);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      float x[SUB][4];
-      bool above = false;
+      // scores in log2 units, rounded before the reference is taken off: the largest one's difference is then exact, however
+      // large it is (a fused product would leave the rounding of scores of 10^37 in the exponent)
+      float x[SUB][4], top = TA_NEG_INF;
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
         const f32x4 sv = tile_scores<T, NC>(t.k[s], q[qt]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[s][i] = sv[i] * sc;
-          x[s][i] = lg * 4 + i < (live >> (8 * s) & 255) ? x[s][i] : TA_NEG_INF;
-          above |= x[s][i] - ref[qt] > PA_SLACK - PA_SHIFT;
-        }
+        for (int i = 0; i < 4; ++i) x[s][i] = sv[i] * sc;
+      }
+      if (!full) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[s][i] = lg * 4 + i < (live >> (8 * s) & 255) ? x[s][i] : TA_NEG_INF;
+      }
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[s][i]);
         if constexpr (W) {
           const int r = (qt0 * QT + qt) * 16 + lr;
           if (r < rows && key < c1)
@@ -320,13 +329,8 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
                 f32x4{x[s][0], x[s][1], x[s][2], x[s][3]};
         }
       }
-      if (wave_any(above)) {
-        float m = x[0][0];
-#pragma unroll
-        for (int s = 0; s < SUB; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m = fmaxf(m, x[s][i]);
-        const float to = fmaxf(ref[qt], quad_max(m) + PA_SHIFT), f = __builtin_amdgcn_exp2f(ref[qt] - to);
+      if (wave_any(top - ref[qt] > PA_SLACK - PA_SHIFT)) {
+        const float to = fmaxf(ref[qt], quad_max(top) + PA_SHIFT), f = __builtin_amdgcn_exp2f(ref[qt] - to);
         ref[qt] = to;
         l[qt] *= f;
 #pragma unroll
@@ -348,11 +352,11 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
   if (key < c1) {
     Tile ta, tb;
     int la = fetch(ta, key);
-    for (; key < c1; key += 2 * NW * KS) {  // two turns: the second may be past the end, then its weights are 0
+    for (; key < c1; key += 2 * NW * KS) {
       const int lb = fetch(tb, key + NW * KS);
       compute(ta, key, la);
       la = fetch(ta, key + 2 * NW * KS);
-      compute(tb, key + NW * KS, lb);
+      if (key + NW * KS < c1) compute(tb, key + NW * KS, lb);
     }
   }
 
@@ -576,7 +580,8 @@ __global__ __launch_bounds__(256) void pa_weights_keys_kernel(PagedAttn a, Paged
         const f32x4 sv = tile_scores<T, NC>(t.k[s], q);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          w[s][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(sv[i] * sc - st.x), st.y, w[s][i]);
+          // a padded query row adds nothing, its product with an infinite key (0 times infinity) neither
+          w[s][i] = r < rows ? __builtin_fmaf(__builtin_amdgcn_exp2f(sv[i] * sc - st.x), st.y, w[s][i]) : w[s][i];
       }
     }
   };
@@ -842,8 +847,9 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
   const int64_t qrows = Hq / H * Tq;
   z->qtiles = (int)((qrows + 16 * QT - 1) / (16 * QT));
   // Two workgroups per CU keep enough loads in flight (three: 3% slower on long caches, 30% at 64 query rows). Up to
-  // PA_WHOLE rows an item goes to one workgroup of eight waves, without a merge: one row over 8 x 700 rows 10.9 us on the
-  // GPU against 11.2 and a launch less for the host; over 8 x 2,000 rows 16.7 against 15.2.
+  // PA_WHOLE rows an item goes to one workgroup of eight waves, without a merge: much the same on the GPU (split / whole:
+  // one row over 8 x 700 rows 10.4 / 10.4 us, over 1 x 1,000 9.1 / 10.4, over 64 x 1,000 30.6 / 27.8), but a launch and a
+  // workspace less, and such calls wait for the host (16.5 / 12.7 us).
   z->groups = rows <= PA_WHOLE ? 0 : 2 * cu_count();
   z->least = 2;
   int64_t at = 0;

@@ -88,6 +88,26 @@ def test_long_and_ragged(dev, dtype, lengths, T):
         assert abs(float(total[i]) - (8 * T if length else 0)) < 1e-3 * 8 * T
 
 
+@pytest.mark.parametrize("D,T,G,R", [(32, 7, 1, 64), (64, 13, 1, 16), (64, 20, 2, 256), (128, 25, 1, 32), (64, 70, 1, 64)])
+def test_weights_of_many_query_rows(dev, D, T, G, R):
+    # long caches and many query rows a head: the weights come from the keys once more; a page without rows, an infinite
+    # key (which the padding of the query rows meets too), a NaN one, an empty sequence
+    q, kp, vp, table, n, g = _case(dev, T, [33000, 1, 0, 20001], H=3, G=G, D=D, R=R, T=T, sharp=1.5)
+    q = q.abs() + 0.1
+    table[0, 5] = -1
+    at = lambda s, r: (table[s, r // R].long(), slice(None), r % R)  # noqa: E731
+    kp[at(0, 32000)] = float("-inf")
+    w = torch.rand(4, table.shape[1] * R, generator=g, device=dev) * 0.01
+    _attend(q, kp, vp, table, n, w, what="from the keys")
+    assert torch.isfinite(w).all()
+    kp[at(3, 7)] = float("nan")
+    before = w.clone()
+    import tabicl_mi355_paged as paged
+    paged.paged_attention(q, kp, vp, table, n, w)
+    assert torch.isnan(w[3, :20001]).all() and torch.equal(w[3, 20001:], before[3, 20001:])
+    assert torch.isfinite(w[:3]).all()
+
+
 def test_one_sequence_per_many(dev):
     # 300 sequences of a few rows
     q, kp, vp, table, n, g = _case(dev, 5, [(i * 7) % 40 for i in range(300)], H=1, R=16, T=2)
