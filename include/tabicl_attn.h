@@ -381,7 +381,7 @@ int tabicl_icl_cache_append(void* k_cache, void* v_cache, int64_t dst_sn, int64_
 
 /*
  * Attention of q [N, Hq, Tq, D] over the first lengths[n] rows of each sequence, query head h over K/V head
- * h / (Hq / H): softmax(scale q k^T) v in fp32 (bf16 probabilities are not rounded to bf16), written to out (element
+ * h / (Hq / H): softmax(scale q k^T) v in fp32 (bf16 probabilities enter as two bf16 terms each), written to out (element
  * strides, contiguous last dim). Rows without a key, or whose every score is -inf, are 0. weights (or NULL): fp32
  * [N, max_pages * page_rows] (row stride weights_sn), the probabilities summed over the query heads and rows are added
  * to the first lengths[n] entries; the sums' order is fixed. For one query row to a few hundred.
@@ -405,6 +405,14 @@ int tabicl_paged_append(void* k_pages, void* v_pages, int64_t pages, int64_t pag
                         const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const void* k,
                         const void* v, const int32_t* count, int64_t N, int64_t H, int64_t T, int64_t D, int64_t k_sn,
                         int64_t k_sh, int64_t k_st, int64_t v_sn, int64_t v_sh, int64_t v_st, int32_t dtype, void* stream);
+
+/*
+ * The way back, for callers that need a sequence's rows side by side: rows t < min(lengths[n], T) of k, v [N, H, T, D]
+ * (contiguous, 16-byte aligned) from the pages, 0 where a row has no page; rows past the length are not written.
+ */
+int tabicl_paged_gather(const void* k_pages, const void* v_pages, int64_t pages, int64_t page_sp, int64_t page_rows,
+                        const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, void* k, void* v,
+                        int64_t N, int64_t H, int64_t T, int64_t D, int32_t dtype, void* stream);
 
 /*
  * Cuts each sequence to kept = min(lengths[n], keep) rows, keep = keep_n[n] (device, or NULL: keep_all), clamped to

@@ -834,6 +834,23 @@ int tabicl_paged_append(void* k_pages, void* v_pages, int64_t pages, int64_t pag
   return launch_status(tabicl_launch_paged_append(a, dtype, (hipStream_t)stream), "paged_append");
 }
 
+int tabicl_paged_gather(const void* k_pages, const void* v_pages, int64_t pages, int64_t page_sp, int64_t page_rows,
+                        const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, void* k, void* v,
+                        int64_t N, int64_t H, int64_t T, int64_t D, int32_t dtype, void* stream) {
+  PagedGather a = {};
+  int st = paged_pool("paged_gather", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+                      lengths, N, H, D, dtype);
+  if (st) return st;
+  if (T < 0 || T > PAGED_MAX_ROWS) return fail(1, "paged_gather: bad row count %lld", (long long)T);
+  if (N == 0 || T == 0) return 0;
+  if (!k || !v || !aligned16(k) || !aligned16(v)) return fail(1, "paged_gather: k and v must be 16-byte aligned");
+  a.k = k;
+  a.v = v;
+  a.N = (int)N;
+  a.T = (int)T;
+  return launch_status(tabicl_launch_paged_gather(a, dtype, (hipStream_t)stream), "paged_gather");
+}
+
 int64_t tabicl_paged_evict_workspace_bytes(int64_t N, int64_t K) {
   if (N < 0 || N > 65535 || K < 0 || K > PAGED_MAX_ROWS) return -fail(1, "paged_evict_workspace_bytes: bad sizes");
   return tabicl_launch_paged_evict_ws_bytes(N, K);

@@ -37,6 +37,12 @@ struct PagedAppend {
   int N, T;
 };
 
+struct PagedGather {
+  PagedPool pool;
+  void *k, *v;  // [N, H, T, D] contiguous
+  int N, T;
+};
+
 struct PagedEvict {
   PagedPool pool;  // k, v: block 0
   int64_t blocks, block_sp;
@@ -60,5 +66,6 @@ int tabicl_launch_paged_attn(const PagedAttn& a, int dtype, void* ws, hipStream_
 int64_t tabicl_launch_paged_attn_ws_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows, int weights,
                                           int dtype);
 int tabicl_launch_paged_append(const PagedAppend& a, int dtype, hipStream_t stream);
+int tabicl_launch_paged_gather(const PagedGather& a, int dtype, hipStream_t stream);
 int tabicl_launch_paged_evict(const PagedEvict& a, int dtype, void* ws, hipStream_t stream);
 int64_t tabicl_launch_paged_evict_ws_bytes(int64_t N, int64_t rows);

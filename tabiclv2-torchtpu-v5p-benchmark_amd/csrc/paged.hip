@@ -622,6 +622,18 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a, int es
   }
 }
 
+// gather: k, v [N, H, T, D] <- the first min(lengths[n], T) rows of the pages (0 where there is no page), the same way back
+__global__ __launch_bounds__(256) void paged_gather_kernel(PagedGather a, int es) {
+  const int n = blockIdx.y, chunks = a.pool.D * es / 16, len = pool_length(a.pool, n), rows = len < a.T ? len : a.T;
+  const int64_t total = (int64_t)rows * a.pool.H * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int c = (int)(i % chunks), row = (int)(i / chunks % rows), h = (int)(i / chunks / rows);
+    const int64_t from = pool_row(a.pool, n, h, row), to = (((int64_t)n * a.pool.H + h) * a.T + row) * a.pool.D * es + c * 16;
+    *(uint4*)((char*)a.k + to) = from < 0 ? uint4{0, 0, 0, 0} : ldg16((const char*)a.pool.k + from * es + c * 16);
+    *(uint4*)((char*)a.v + to) = from < 0 ? uint4{0, 0, 0, 0} : ldg16((const char*)a.pool.v + from * es + c * 16);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // eviction: one workgroup per sequence selects, a second kernel moves
 // ---------------------------------------------------------------------------------------------
@@ -945,6 +957,15 @@ int tabicl_launch_paged_append(const PagedAppend& a, int dtype, hipStream_t stre
   if (gx > PAGED_MAX_GRID / a.N) gx = PAGED_MAX_GRID / a.N;
   if (gx > 4096) gx = 4096;
   hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)gx, (unsigned)a.N), dim3(256), 0, stream, a, es);
+  return (int)hipGetLastError();
+}
+
+int tabicl_launch_paged_gather(const PagedGather& a, int dtype, hipStream_t stream) {
+  const int es = dtype == 0 ? 2 : 4;
+  int64_t gx = ((int64_t)a.T * a.pool.H * (a.pool.D * es / 16) + 255) / 256;
+  if (gx > PAGED_MAX_GRID / a.N) gx = PAGED_MAX_GRID / a.N;
+  if (gx > 4096) gx = 4096;
+  hipLaunchKernelGGL(paged_gather_kernel, dim3((unsigned)gx, (unsigned)a.N), dim3(256), 0, stream, a, es);
   return (int)hipGetLastError();
 }
 

@@ -597,6 +597,10 @@ class IclKVCache:
         # promote_types(q, cache) as in the reference's cached branch (results/tpu_patch.diff:314-317)
         attn_dtype = torch.promote_types(q.dtype, k.dtype)
         q, k, v = q.to(attn_dtype), k.to(attn_dtype), v.to(attn_dtype)
+        return self._dense(q, k, v, valid_kv_len, out)
+
+    @staticmethod
+    def _dense(q: Tensor, k: Tensor, v: Tensor, valid_kv_len: Optional[Union[int, Tensor]], out: Optional[Tensor]) -> Tensor:
         if out is None:
             return icl_sdpa(q, k, v, valid_kv_len)
         if q.stride(-1) != 1:

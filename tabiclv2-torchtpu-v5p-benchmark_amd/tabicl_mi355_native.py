@@ -80,6 +80,7 @@ SIGNATURES = {
     "tabicl_paged_attn_workspace_bytes": [_i64] * 6 + [_i32] * 2,
     "tabicl_paged_append": [_c_p] * 2 + [_i64] * 3 + [_c_p, _i64, _i64, _c_p, _c_p, _c_p, _c_p] + [_i64] * 10
                            + [_i32, _c_p],
+    "tabicl_paged_gather": [_c_p] * 2 + [_i64] * 3 + [_c_p, _i64, _i64, _c_p, _c_p, _c_p] + [_i64] * 4 + [_i32, _c_p],
     "tabicl_paged_evict": [_c_p] * 2 + [_i64] * 5 + [_c_p, _i64, _i64, _c_p, _c_p, _i64, _c_p, _i64, _i64, _c_p, _i64,
                                                      _c_p, _c_p, _i64, _i64, _i64, _i32, _c_p, _i64, _c_p],
     "tabicl_paged_evict_workspace_bytes": [_i64] * 2,

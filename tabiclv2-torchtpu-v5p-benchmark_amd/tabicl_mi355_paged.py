@@ -6,7 +6,7 @@ once, that gets its train rows over time or answers one test row at a time keeps
   * paged_attention(q, k_pages, v_pages, table, lengths, weights) (ops tabicl::paged_attn, paged_attn_out,
     paged_attn_weights_out): attention of few query rows over the cached rows, optionally adding up the attention weight
     that each cached row drew;
-  * paged_append (op tabicl::paged_append): new rows into the pages;
+  * paged_append, paged_gather (ops of these names): new rows into the pages, rows out of them;
   * paged_evict (op tabicl::paged_evict_out): cuts sequences to their rows of largest weight, in place;
   * PagedIclKVCache: the pool, the page table and the lengths, with the surface of IclKVCache (append, query,
     attention_layer, query_blocks, usable as cached_query's icl_cache), and evict.
@@ -28,8 +28,8 @@ import tabicl_mi355_icl as _icl
 import tabicl_mi355_native as _nat
 
 
-# A call of few rows is over in 10 us on the GPU; the checks below cost 4 us on a CPU core of the box (12 as one test and
-# one generator expression per property).
+# A call of few rows is over in 10 us on the GPU; the checks below take 4 us of a host core (12 with a test and a generator
+# expression per property).
 def _rows16(t: Tensor, es: int):
     """(t, its (n, h, row) element strides) of [N, H, T, D] when its last dim is contiguous and it starts, and its other
     dims step, in multiples of 16 bytes (what the kernels' loads need), else of a contiguous copy. A dim of one entry,
@@ -255,6 +255,47 @@ def paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tenso
         torch.ops.tabicl.paged_append(k_pages, v_pages, table, lengths, k, v, count)
 
 
+def _gather_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: Tensor, v: Tensor) -> None:
+    pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths)
+    if dev != torch.cuda.current_device() if dev >= 0 else True:
+        _nat.require_device(k_pages)
+        with torch.cuda.device(dev):
+            return _gather_launch(k_pages, v_pages, table, lengths, k, v)
+    _nat.call("tabicl_paged_gather", k_pages.data_ptr(), v_pages.data_ptr(), *pool, lengths.data_ptr(), k.data_ptr(),
+              v.data_ptr(), N, H, k.shape[2], D, code, _nat.stream_of(k))
+
+
+def _gather(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tensor, Tensor]:
+    shape = (table.shape[0], k_pages.shape[1], rows, k_pages.shape[3])
+    k, v = k_pages.new_empty(shape), v_pages.new_empty(shape)
+    _gather_launch(k_pages, v_pages, table, lengths, k, v)
+    return k, v
+
+
+@torch.library.custom_op("tabicl::paged_gather", mutates_args=())
+def _paged_gather(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tensor, Tensor]:
+    """See paged_gather."""
+    return _gather(k_pages, v_pages, table, lengths, rows)
+
+
+@_paged_gather.register_fake
+def _(k_pages, v_pages, table, lengths, rows):  # noqa: ANN001
+    shape = (table.shape[0], k_pages.shape[1], rows, k_pages.shape[3])
+    return k_pages.new_empty(shape), v_pages.new_empty(shape)
+
+
+def paged_gather(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tensor, Tensor]:
+    """k, v [N, H, rows, D] with the first min(lengths[n], rows) rows of each sequence side by side, 0 where a row has no
+    page; what lies past a sequence's length is not written. For calls that the dense kernels answer faster (many query
+    rows), or to copy a cache out of its pool."""
+    _no_grad("paged_gather", k_pages, v_pages)
+    if k_pages.dim() != 4 or rows < 0:
+        raise ValueError(f"paged_gather needs pools [pages, H, page_rows, D] and rows >= 0, got {tuple(k_pages.shape)}, {rows}")
+    if _nat.direct(k_pages, v_pages, table, lengths):
+        return _gather(k_pages, v_pages, table, lengths, int(rows))
+    return torch.ops.tabicl.paged_gather(k_pages, v_pages, table, lengths, int(rows))
+
+
 def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int,
                   recent: int, keep_n: Optional[Tensor], index: Tensor, kept_weights: Tensor, kept: Tensor) -> None:
     pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths, 1)
@@ -270,9 +311,6 @@ def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tens
             return _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights, kept)
     B, cap = k_pages.shape[0], pool[2] * pool[5]
     K = min(keep, cap)
-    for t, shape, dtype in ((index, (N, K), torch.int32), (kept_weights, (N, cap), torch.float32), (kept, (N,), torch.int32)):
-        if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != dev:
-            raise ValueError(f"eviction writes to contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
     key = (N, K)
     nbytes = _WS_BYTES.get(key)
     if nbytes is None:
@@ -291,6 +329,11 @@ def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tens
 def _paged_evict_out(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int,
                      recent: int, keep_n: Optional[Tensor], index: Tensor, kept_weights: Tensor, kept: Tensor) -> None:
     """See paged_evict; keep_n is its tensor keep (keep then bounds it)."""
+    N, cap = table.shape[0], table.shape[1] * k_pages.shape[-2]
+    for t, shape, dtype in ((index, (N, max(0, min(keep, cap))), torch.int32), (kept_weights, (N, cap), torch.float32),
+                            (kept, (N,), torch.int32)):
+        if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.device != table.device:
+            raise ValueError(f"eviction writes to contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
     _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights, kept)
 
 
@@ -327,6 +370,13 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
         torch.ops.tabicl.paged_evict_out(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights,
                                          kept)
     return index, kept_weights, kept
+
+
+# PagedIclKVCache.query gathers a block's rows for the dense kernel, which shares each tile of K and V among 256 query rows,
+# from so many query rows and so many products of query rows and cached rows (per head) on. us in the pages / gathered, for
+# query rows T: 8 x 45,000 cached rows T 128 241 / 449, 256 438 / 462, 384 648 / 568, 5000 9164 / 3440; 8 x 5,000 rows 256
+# 72 / 69, 512 120 / 87; 1 x 20,000 rows 512 65 / 98, 1000 101 / 102; 8 x 700 rows 512 39 / 56, 5000 285 / 88.
+_DENSE_QUERY_ROWS, _DENSE_SCORES = 256, 1 << 24
 
 
 class PagedIclKVCache(_icl.IclKVCache):
@@ -448,6 +498,10 @@ class PagedIclKVCache(_icl.IclKVCache):
         if torch.promote_types(q.dtype, dt) != dt:
             raise ValueError(f"q is {q.dtype}, wider than the {dt} cache: cast it")
         w = max(1, -(-longest // self.page_rows))
+        if q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and q.shape[3] == 64 \
+                and dt == torch.bfloat16 and self.weights is None:
+            k, v = paged_gather(self.keys[block], self.values[block], self.table[:, :w], lengths, longest)
+            return self._dense(q.to(dt), k, v, lengths, out)
         weights = None if self.weights is None else self.weights[:, :w * self.page_rows]
         return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out)
 

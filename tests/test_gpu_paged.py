@@ -317,6 +317,29 @@ def test_append_layouts(dev):
         assert torch.equal(kp.cpu(), want[0]) and torch.equal(vp.cpu(), want[1]) and (pool[:, 1] == 9).all()
 
 
+@pytest.mark.parametrize("dtype,D,R", [(BF, 64, 64), (F32, 32, 16), (BF, 128, 256), (F32, 128, 32)])
+def test_gather(dev, dtype, D, R):
+    # rows side by side; past the length (and past `rows`) nothing is written, a row without a page is 0
+    import tabicl_mi355_paged as paged
+    lengths = [0, 1, 100, 513, 300]
+    q, kp, vp, table, n, g = _case(dev, D, lengths, H=3, R=R, D=D, dtype=dtype)
+    table[3, 1] = -1
+    for rows in (513, 200, 700, 0):
+        k, v = paged.paged_gather(kp, vp, table, n, rows)
+        marked = torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+        paged._gather_launch(kp, vp, table, n, *marked)
+        torch.cuda.synchronize()
+        assert k.shape == v.shape == (5, 3, rows, D)
+        for s, length in enumerate(lengths):
+            have = min(length, rows)
+            at, page, row = ref.rows_of(table[s], have, R, kp.shape[0])
+            for t, m, pages in ((k, marked[0], kp), (v, marked[1], vp)):
+                want = torch.zeros(have, 3, D, dtype=dtype, device=dev)
+                want[at] = pages[page, :, row]
+                assert torch.equal(t[s, :, :have], want.transpose(0, 1)) and torch.equal(m[s, :, :have], want.transpose(0, 1))
+                assert (m[s, :, have:] == 7).all()
+
+
 # ---------------------------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------------------------
@@ -598,6 +621,40 @@ def test_cache_together(dev, dtype):
     c.evict([300, 256, 1])
     c.release(1)
     assert [c.length(1, s) for s in range(S)] == [300, 0, 1]
+
+
+@pytest.mark.parametrize("valid", [None, 150])
+def test_cache_many_query_rows(dev, valid, monkeypatch):
+    # query rows by the hundred: gathered for the dense kernel, the same attention (to the bf16 bars: its probabilities are
+    # bf16); an output view, an empty sequence, a valid length as a tensor; fewer rows and a tracked cache stay on the pages
+    import tabicl_mi355_paged as paged
+    from parity import check
+    monkeypatch.setattr(paged, "_DENSE_SCORES", 1)
+    gathers = []
+    gather = paged.paged_gather
+    monkeypatch.setattr(paged, "paged_gather", lambda *a: gathers.append(a[-1]) or gather(*a))
+    g = torch.Generator(device=dev).manual_seed(83)
+    for rows, track in (([700, 300, 65], False), ([700, 0, 65], False), ([700, 300, 65], True)):
+        c = paged.PagedIclKVCache(3, 1, 8, 64, 800, 40, 64, BF, dev, track=track)
+        k, v = (torch.randn(3, 8, 700, 64, generator=g, device=dev).to(BF) for _ in range(2))
+        c.append(0, k, v, rows)
+        q = torch.randn(3, 600, 8, 64, generator=g, device=dev).to(BF).transpose(1, 2)
+        out = torch.zeros(3, 600, 8, 64, dtype=BF, device=dev)
+        got = c.query(0, q, valid)
+        c.query(0, q, valid, out.transpose(1, 2))
+        torch.cuda.synchronize()
+        assert torch.equal(out.transpose(1, 2), got)
+        if valid is not None:
+            assert torch.equal(c.query(0, q, torch.tensor([valid], device=dev)), got)
+        for s, r in enumerate(rows):
+            r = r if valid is None else min(r, valid)
+            if r == 0:
+                assert (got[s] == 0).all()
+                continue
+            p = torch.softmax(q[s].double() @ k[s, :, :r].double().transpose(1, 2) / 8, -1)
+            check(got[s], p @ v[s, :, :r].double(), BF, f"sequence {s} of {rows}")
+        c.query(0, q[:, :, :255], valid)
+    assert gathers == ([700] * 4 if valid is None else [150, 150, 700] * 2)  # the untracked caches' calls
 
 
 def test_cached_query_on_pages(dev):

@@ -26,6 +26,11 @@ def test_no_cpu_path():
         paged.paged_append(k, v, t, n, q, q)
     with pytest.raises(nat.NativeLibraryError):
         paged.paged_evict(k, v, t, n, torch.zeros(2, 48), 4)
+    with pytest.raises(nat.NativeLibraryError):
+        paged.paged_gather(k, v, t, n, 9)
+    for bad in ((k[0], v[0], t, n, 9), (k, v, t, n, -1), (k, v[:2], t, n, 9), (k, v, t.long(), n, 9)):
+        with pytest.raises(ValueError):
+            paged.paged_gather(*bad)
 
 
 @pytest.mark.parametrize("change,word", [
@@ -120,6 +125,13 @@ def test_abi_refuses_before_launch():
     for kw, word in ((dict(T=-1), "row count"), (dict(k=a + 8), "aligned"), (dict(ks=(64, 64, 4)), "strides")):
         assert append(**kw) == 1 and word in nat.last_error(), (kw, nat.last_error())
     assert append(T=0) == 0 and append(N=0) == 0
+
+    def gather(T=3, k=a, N=2, D=64):
+        return lib.tabicl_paged_gather(a, a, 10, 8 * 64 * D, 64, a, 4, 4, a, k, a, N, 8, T, D, 0, None)
+
+    for kw, word in ((dict(T=-1), "row count"), (dict(k=a + 4), "aligned"), (dict(k=None), "aligned"), (dict(D=48), "head dim")):
+        assert gather(**kw) == 1 and word in nat.last_error(), (kw, nat.last_error())
+    assert gather(T=0) == 0 and gather(N=0) == 0
 
     def evict(K=100, recent=0, ws=a, wsb=1 << 40, bsp=0, w=a, N=2, M=4):
         return lib.tabicl_paged_evict(a, a, 1, bsp, 10, 8 * 64 * 64, 64, a, M, M, a, w, 64 * M, None, 100, recent, a, K, a, a, N,
