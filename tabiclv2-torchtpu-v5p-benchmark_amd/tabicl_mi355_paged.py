@@ -390,7 +390,8 @@ class PagedIclKVCache(_icl.IclKVCache):
     [sequences, capacity]); evict(keep) cuts the sequences to their heaviest rows and returns the emptied pages.
 
     Pages are given out on the host; the page table and the lengths live on the GPU, so a query costs no host sync. Calls
-    follow each other on one stream. Only queries can be captured in a graph (the others keep books on the host)."""
+    follow each other on one stream. Only queries without a number for valid_kv_len can be captured in a graph and replayed as
+    the cache grows (the other calls keep books on the host)."""
 
     def __init__(self, sequences: int, blocks: int, heads: int, head_dim: int, max_rows: int, pages: int,
                  page_rows: int = 64, dtype: torch.dtype = torch.bfloat16, device: Union[str, torch.device] = "cuda",
@@ -409,7 +410,7 @@ class PagedIclKVCache(_icl.IclKVCache):
         self._held = [0] * sequences  # pages a sequence holds
         self._rows = [[0] * sequences for _ in range(blocks)]  # the lengths' host copy
         self._free = list(range(pages - 1, -1, -1))
-        self._owner = True
+        self._root, self._first = self, 0  # of a view: the cache it shows, and its first sequence there
 
     @property
     def shape(self):
@@ -421,17 +422,21 @@ class PagedIclKVCache(_icl.IclKVCache):
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _lengths_of(self, block: int) -> list:
+        """The block's lengths on the host (of a view: as the cache it shows has them now)."""
+        return self._root._rows[block][self._first:self._first + self.table.shape[0]]
+
     def length(self, block: int, sequence: int = 0) -> int:
-        return self._rows[block][sequence]
+        return self._lengths_of(block)[sequence]
 
     def default_valid(self, block: int) -> Tensor:
         """The block's filled lengths as the int32 device tensor the kernels take."""
-        if not any(self._rows[block]):
+        if not any(self._lengths_of(block)):
             raise ValueError(f"block {block} of the cache has no rows: append before querying")
         return self.lengths[block]
 
     def _own(self, what: str) -> None:
-        if not self._owner:
+        if self._root is not self:
             raise ValueError(f"{what}: a view of some of a cache's estimators answers queries only")
 
     def reserve(self, rows: Union[int, Sequence[int]]) -> None:
@@ -487,7 +492,7 @@ class PagedIclKVCache(_icl.IclKVCache):
         """Attention of q [sequences, H, Tq, d] over `block` of the cache: each sequence's own rows, of those the ones
         below valid_kv_len if given (a number, or one per sequence). q in the cache's dtype or one that widens to it."""
         lengths = self.default_valid(block)
-        longest = max(self._rows[block])
+        longest = max(self._lengths_of(block))
         if isinstance(valid_kv_len, Tensor):
             lengths = torch.minimum(valid_kv_len.to(device=lengths.device, dtype=torch.int32).reshape(-1).expand_as(lengths),
                                     lengths)
@@ -498,7 +503,9 @@ class PagedIclKVCache(_icl.IclKVCache):
         if torch.promote_types(q.dtype, dt) != dt:
             raise ValueError(f"q is {q.dtype}, wider than the {dt} cache: cast it")
         w = max(1, -(-longest // self.page_rows))
-        if q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and q.shape[3] == 64 \
+        if self.keys.is_cuda and torch.cuda.is_current_stream_capturing():
+            w = self.table.shape[1]  # a replay meets the lengths of its time, not today's
+        elif q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and q.shape[3] == 64 \
                 and dt == torch.bfloat16 and self.weights is None:
             k, v = paged_gather(self.keys[block], self.values[block], self.table[:, :w], lengths, longest)
             return self._dense(q.to(dt), k, v, lengths, out)
@@ -565,8 +572,7 @@ class PagedIclKVCache(_icl.IclKVCache):
         view.table = self.table[start:stop]
         view.lengths = self.lengths[:, start:stop]
         view.weights = None if self.weights is None else self.weights[start:stop]
-        view._rows = [r[start:stop] for r in self._rows]
-        view._owner = False
+        view._first = self._first + start
         return view
 
     def block_kv(self, block: int):

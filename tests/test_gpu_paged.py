@@ -623,6 +623,38 @@ def test_cache_together(dev, dtype):
     assert [c.length(1, s) for s in range(S)] == [300, 0, 1]
 
 
+@pytest.mark.parametrize("T", [2, 300])
+def test_cache_query_in_a_graph(dev, T, monkeypatch):
+    # a query captured once answers over the rows of the replay's time: more pages, fewer rows after an eviction
+    import tabicl_mi355_paged as paged
+    monkeypatch.setattr(paged, "_DENSE_SCORES", 1)
+    g = torch.Generator(device=dev).manual_seed(85)
+    c = paged.PagedIclKVCache(2, 1, 8, 64, 2000, 80, 64, BF, dev, track=T == 2)
+    rows = lambda n: torch.randn(2, 8, n, 64, generator=g, device=dev).to(BF)  # noqa: E731
+    c.append(0, rows(90), rows(90))
+    q = rows(T)
+    c.query(0, q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.query(0, q)
+    for step in range(3):
+        if step < 2:
+            c.append(0, rows(700), rows(700), [700, 300 * step])
+        elif T == 2:
+            c.evict(400)
+        q.copy_(rows(T))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        k, v = paged.paged_gather(c.keys[0], c.values[0], c.table, c.lengths[0], c.capacity)
+        for s in range(2):
+            n = c.length(0, s)
+            p = torch.softmax(q[s].double() @ k[s, :, :n].double().transpose(1, 2) / 8, -1)
+            want = p @ v[s, :, :n].double()
+            assert (out[s].double() - want).abs().max() <= 2.0 ** -8 * want.abs().max() + 1e-4, (step, s)
+
+
 @pytest.mark.parametrize("valid", [None, 150])
 def test_cache_many_query_rows(dev, valid, monkeypatch):
     # query rows by the hundred: gathered for the dense kernel, the same attention (to the bf16 bars: its probabilities are

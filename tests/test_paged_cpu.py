@@ -227,6 +227,10 @@ def test_cache_appends_and_queries(plain):
             assert torch.allclose(o[s], torch.einsum("htr,rhd->thd", p, v), atol=1e-5)
     view = c.estimators(1, 3)
     assert torch.allclose(view.query(1, q[1:]), out[1:], atol=1e-6)
+    for b in range(2):  # the view shows what the cache gets later
+        c.append(b, k[None].expand(3, -1, -1, -1).transpose(1, 2)[:, :, :5], v[None].expand(3, -1, -1, -1).transpose(1, 2)[:, :, :5])
+    assert view.length(1, 0) == 47 and view.length(1, 1) == 22
+    assert torch.allclose(view.estimators(1, 2).query(1, q[2:]), c.query(1, q)[2:], atol=1e-6)
     with pytest.raises(ValueError, match="queries only"):
         view.append(0, torch.zeros(2, 2, 1, 32), torch.zeros(2, 2, 1, 32))
 
