@@ -43,8 +43,8 @@ constexpr float PA_SHIFT = 24.f, PA_SLACK = 8.f;
 constexpr float PA_REF0 = -3.4028234663852886e38f;
 
 // The work is cut on the device, by the lengths as they are: a unit is PA_UNIT rows of one item, units are counted item after
-// item, and G workgroups, two per CU, take equal runs of them, whatever the lengths. An item that one workgroup covers is
-// written at once; of the others each workgroup leaves a partial (at most two: one of an item begun before it, one of an
+// item, and G workgroups (pa_waves per CU) take equal runs of them, whatever the lengths. An item that one workgroup covers
+// is written at once; of the others each workgroup leaves a partial (at most two: one of an item begun before it, one of an
 // item it begins), which pa_merge_kernel joins. (A fixed number of rows per workgroup instead: 64 sequences of 500 to
 // 10,000 rows took 97 us at 8 workgroups per CU and 146 at 2, one sequence of 45,000 rows 39 and 27; this way 84 and 26.)
 constexpr int PA_UNIT = 128, PA_WHOLE = 1024;
@@ -414,9 +414,14 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
   }
 }
 
+// Waves per SIMD that the registers of a kernel allow: one for tiles of 32 and 64 query rows of 128 dims. In tiles of 16 with
+// two waves every tile reads K and V again (tiles of 16 / larger: bf16, 32 query rows a head over 8 x 5,000 rows 57 / 42 us,
+// 64 rows 104 / 48; fp32, 17 rows 102 / 70, 34 rows over 49 x 5,311 372 / 304).
+constexpr int pa_waves(int D, int QT) { return D == 128 && QT > 1 ? 1 : 2; }
+
 // Equal shares of all items' units.
 template <typename T, int D, int QT, bool W>
-__global__ __launch_bounds__(256, 2) void pa_kernel(PagedAttn a, PagedSplit z) {
+__global__ __launch_bounds__(256, pa_waves(D, QT)) void pa_kernel(PagedAttn a, PagedSplit z) {
   const int per = a.pool.H * z.qtiles;
   const PagedUnits units(a, per, threadIdx.x & 63);
   const PagedShares shares(z, units.total);
@@ -439,7 +444,7 @@ __global__ __launch_bounds__(256, 2) void pa_kernel(PagedAttn a, PagedSplit z) {
 
 // A workgroup of eight waves for each item, where no sequence is long.
 template <typename T, int D, int QT, bool W>
-__global__ __launch_bounds__(512, 2) void pa_whole_kernel(PagedAttn a, PagedSplit z) {
+__global__ __launch_bounds__(512) void pa_whole_kernel(PagedAttn a, PagedSplit z) {
   const int per = a.pool.H * z.qtiles, n = blockIdx.x / per;
   pa_segment<T, D, QT, W, 8>(a, z, n, blockIdx.x % per, 0, __builtin_amdgcn_readfirstlane(pa_len(a, n)), -1);
 }
@@ -504,6 +509,9 @@ __global__ __launch_bounds__(256) void pa_weights_kernel(PagedAttn a, PagedSplit
   const int all = a.Hq * a.Tq, kt = threadIdx.x & 15, rt = threadIdx.x >> 4;
   const int64_t first = (int64_t)n * all;
   f32x4 w = {0.f, 0.f, 0.f, 0.f};
+  // Eight loads in flight: of few cached rows their latency is all there is (61 query rows in two heads a group over 22 x 9
+  // rows: the whole call 71 -> 45 us; 59 over 5 x 1,700 39 -> 33).
+#pragma unroll 8
   for (int r = rt; r < all; r += 16) {
     const float2 st = z.stat[first + r];
     const f32x4 s = *(const f32x4*)(z.score + (first + r) * z.score_sn + k0 + kt * 4);
@@ -865,7 +873,7 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
   // PA_WHOLE rows an item goes to one workgroup of eight waves, without a merge: much the same on the GPU (split / whole:
   // one row over 8 x 700 rows 10.4 / 10.4 us, over 1 x 1,000 9.1 / 10.4, over 64 x 1,000 30.6 / 27.8), but a launch and a
   // workspace less, and such calls wait for the host (16.5 / 12.7 us).
-  z->groups = rows <= PA_WHOLE ? 0 : 2 * cu_count();
+  z->groups = rows <= PA_WHOLE ? 0 : pa_waves(D, QT) * cu_count();
   z->least = 2;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -894,7 +902,8 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
 template <typename T, int D, int QT, bool W>
 void launch_pa_w(const PagedAttn& a, const PagedSplit& z, hipStream_t stream) {
   if (z.groups == 0) {
-    hipLaunchKernelGGL((pa_whole_kernel<T, D, QT, W>), dim3((unsigned)(a.N * a.pool.H * z.qtiles)), dim3(512), 0, stream, a, z);
+    if constexpr (pa_waves(D, QT) == 2)
+      hipLaunchKernelGGL((pa_whole_kernel<T, D, QT, W>), dim3((unsigned)(a.N * a.pool.H * z.qtiles)), dim3(512), 0, stream, a, z);
   } else {
     hipLaunchKernelGGL((pa_kernel<T, D, QT, W>), dim3((unsigned)z.groups), dim3(256), 0, stream, a, z);
     const unsigned merge = (unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4);
@@ -921,11 +930,13 @@ template <typename T, int D>
 int64_t run_pa_d(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights,
                  hipStream_t stream) {
   const int64_t qrows = Hq / H * Tq;
-  constexpr int most = D == 128 ? 1 : D * sizeof(T) > 128 ? 2 : 4;  // more queries do not fit the registers
-  if constexpr (most >= 4)
-    if (qrows > 32) return run_pa<T, D, 4>(a, ws, N, Hq, H, Tq, rows, weights, stream);
-  if constexpr (most >= 2)
-    if (qrows > 16) return run_pa<T, D, 2>(a, ws, N, Hq, H, Tq, rows, weights, stream);
+  // Query rows of a tile: 16 to 64. fp32 of 64 dims keeps to 32 (64 would be one wave per SIMD; 64 query rows over 8 x 5,000
+  // rows 62 / 66 us), and of 128 dims the kernel of whole items to 16: short caches are read from L2 anyhow, and two waves
+  // hide more of it (8 x 900 rows, tiles of 16 / larger: bf16, 64 query rows 23.5 / 24.9 us, fp32, 32 rows 27 / 40).
+  const int most = D == 128 ? (rows <= PA_WHOLE ? 16 : 64) : D * sizeof(T) > 128 ? 32 : 64;
+  if constexpr (D == 128 || D * sizeof(T) <= 128)
+    if (qrows > 32 && most == 64) return run_pa<T, D, 4>(a, ws, N, Hq, H, Tq, rows, weights, stream);
+  if (qrows > 16 && most >= 32) return run_pa<T, D, 2>(a, ws, N, Hq, H, Tq, rows, weights, stream);
   return run_pa<T, D, 1>(a, ws, N, Hq, H, Tq, rows, weights, stream);
 }
 
