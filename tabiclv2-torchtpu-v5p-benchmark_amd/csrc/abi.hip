@@ -719,8 +719,7 @@ int paged_pool(const char* op, PagedPool* c, const void* k_pages, const void* v_
   if (page_rows < 16 || page_rows > (1 << 20) || (page_rows & (page_rows - 1)))
     return fail(1, "%s: page_rows must be a power of two from 16 to 2^20, got %lld", op, (long long)page_rows);
   if (N < 0 || N > 65535 || H < 1 || H > 1024) return fail(1, "%s: needs 0 <= N <= 65535 and 1 <= H <= 1024", op);
-  if (pages < 0 || pages > 0x7fffffffLL || max_pages < 0 || max_pages * page_rows > PAGED_MAX_ROWS || table_sn < 0 ||
-      max_pages > PAGED_MAX_ROWS)
+  if (pages < 0 || pages > 0x7fffffffLL || max_pages < 0 || max_pages > PAGED_MAX_ROWS / page_rows || table_sn < 0)
     return fail(1, "%s: bad page counts (pages %lld, max_pages %lld)", op, (long long)pages, (long long)max_pages);
   if (page_sp < H * page_rows * D || !stride_ok(page_sp, dtype) || (pages && page_sp > (1LL << 60) / pages))
     return fail(1, "%s: the page stride must be a multiple of 16 bytes and at least H * page_rows * D", op);
@@ -863,19 +862,20 @@ int tabicl_paged_evict(void* k_pages, void* v_pages, int64_t blocks, int64_t blo
                        int32_t* kept_lengths, int64_t N, int64_t H, int64_t D, int32_t dtype, void* ws, int64_t ws_bytes,
                        void* stream) {
   PagedEvict a = {};
-  int st = paged_pool("paged_evict", &a.pool, k_pages, v_pages, blocks > 0 ? pages : 0, page_sp, page_rows, table, table_sn, max_pages,
-                      lengths, N, H, D, dtype);
+  int st = paged_pool("paged_evict", &a.pool, k_pages, v_pages, blocks > 0 ? pages : 0, page_sp, page_rows, table, table_sn,
+                      max_pages, lengths, N, H, D, dtype);
   if (st) return st;
   const int64_t cap = max_pages * page_rows;
   if (blocks < 0 || blocks > 65535 || block_sp < 0 || !stride_ok(block_sp, dtype))
     return fail(1, "paged_evict: bad block count or stride");
   if (N * (cap + 1024) > (1LL << 31) || N * ((blocks + 3) / 4 + 1) > PAGED_MAX_GRID)
     return fail(1, "paged_evict: more than 2^31 rows over all sequences, or 2^25 blocks");
-  if (recent < 0 || keep_all < 0 || K < 0 || K > cap) return fail(1, "paged_evict: needs recent, keep >= 0 and 0 <= K <= the capacity %lld", (long long)cap);
+  if (recent < 0 || keep_all < 0 || K < 0 || K > cap)
+    return fail(1, "paged_evict: needs recent, keep >= 0 and 0 <= K <= the capacity %lld", (long long)cap);
   if (N == 0) return 0;
   if (!kept_lengths || (K > 0 && !index) || (cap > 0 && (!weights || !kept_weights)) || weights_sn < cap)
     return fail(1, "paged_evict: weights and kept_weights need rows of max_pages * page_rows values");
-  if (N * K > 0 && (!ws || !aligned16(ws) || ws_bytes < tabicl_launch_paged_evict_ws_bytes(N, K)))
+  if ((!ws || !aligned16(ws) || ws_bytes < tabicl_launch_paged_evict_ws_bytes(N, K)))
     return fail(1, "paged_evict: workspace of %lld bytes (16-byte aligned) required",
                 (long long)tabicl_launch_paged_evict_ws_bytes(N, K));
   a.blocks = blocks;

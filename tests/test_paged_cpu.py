@@ -144,6 +144,17 @@ def test_abi_refuses_before_launch():
     assert evict(N=0) == 0
 
 
+def test_abi_evict_of_everything_needs_its_workspace():
+    # K = 0 keeps nothing, but the number of moves still goes through the workspace
+    import tabicl_mi355_native as nat
+    a, need = 0x1000, nat.load().tabicl_paged_evict_workspace_bytes(2, 0)
+    assert need > 0
+    for ws, size in ((None, 1 << 40), (a, need - 1), (a + 8, need)):
+        st = nat.load().tabicl_paged_evict(a, a, 1, 0, 10, 8 * 64 * 64, 64, a, 4, 4, a, a, 256, None, 0, 0, None, 0, a, a, 2, 8,
+                                           64, 0, ws, size, None)
+        assert st == 1 and "workspace" in nat.last_error()
+
+
 # ---------------------------------------------------------------------------------------------
 # PagedIclKVCache
 # ---------------------------------------------------------------------------------------------
