@@ -127,6 +127,12 @@ def _attn_launch(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
               None if ws is None else ws.data_ptr(), nbytes, _nat.stream_of(q))
 
 
+def _apart(q: Tensor, out: Tensor) -> Tensor:
+    """q, or a copy of it where `out` may overlap it: the kernels read q again after parts of the output are written (the
+    weights, and the tiles of one item in several workgroups)."""
+    return q.clone() if q.untyped_storage().data_ptr() == out.untyped_storage().data_ptr() else q
+
+
 # Three ops, since torch.compile refuses an op that returns a tensor and may or may not change another.
 @torch.library.custom_op("tabicl::paged_attn", mutates_args=())
 def _paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float) -> Tensor:
@@ -145,7 +151,7 @@ def _(q, k_pages, v_pages, table, lengths, scale):  # noqa: ANN001
 def _paged_attn_out(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float,
                     out: Tensor) -> None:
     """tabicl::paged_attn written into `out`, any [N, Hq, Tq, D] view with a contiguous last dim."""
-    _attn_launch(q, k_pages, v_pages, table, lengths, None, scale, out)
+    _attn_launch(_apart(q, out), k_pages, v_pages, table, lengths, None, scale, out)
 
 
 @_paged_attn_out.register_fake
@@ -157,7 +163,7 @@ def _(q, k_pages, v_pages, table, lengths, scale, out):  # noqa: ANN001
 def _paged_attn_weights_out(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float,
                             out: Tensor, weights: Tensor) -> None:
     """tabicl::paged_attn_out that adds the attention weights to `weights` in place."""
-    _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, out)
+    _attn_launch(_apart(q, out), k_pages, v_pages, table, lengths, weights, scale, out)
 
 
 @_paged_attn_weights_out.register_fake
@@ -179,7 +185,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     sums. weights: an optional fp32 [N, >= max_pages page_rows] tensor; the probabilities of each cached row, summed over
     query heads and rows, are added to it in place (entries past the length are left as they are), always in the same
     order of sums. out: written in place of a new tensor, any [N, Hq, Tq, D] view whose last dim is contiguous and whose
-    rows start on 16 bytes.
+    rows start on 16 bytes (q itself, too).
 
     The work is split over the cached rows, so one test row over one long table fills the GPU; a table slice
     table[:, :w] that covers the longest sequence spares the workgroups of pages nobody holds. For up to a few hundred
@@ -187,7 +193,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, table, lengths, weights, out):
         o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-        _attn_launch(q, k_pages, v_pages, table, lengths, weights, scale, o)
+        _attn_launch(q if out is None else _apart(q, out), k_pages, v_pages, table, lengths, weights, scale, o)
         if out is not None:
             torch.autograd.graph.increment_version(out)
         if weights is not None:
@@ -441,7 +447,7 @@ class PagedIclKVCache(_icl.IclKVCache):
 
     def reserve(self, rows: Union[int, Sequence[int]]) -> None:
         """Pages for sequences of up to `rows` rows (a number, or one per sequence), given out now rather than by the
-        appends that fill them."""
+        appends that fill them. They stay a sequence's own until it is released or the cache evicts."""
         self._own("reserve")
         S, R = self.table.shape[0], self.page_rows
         rows = [int(rows)] * S if isinstance(rows, int) else [int(r) for r in rows]
@@ -490,7 +496,9 @@ class PagedIclKVCache(_icl.IclKVCache):
     def query(self, block: int, q: Tensor, valid_kv_len: Optional[Union[int, Tensor]] = None,
               out: Optional[Tensor] = None) -> Tensor:
         """Attention of q [sequences, H, Tq, d] over `block` of the cache: each sequence's own rows, of those the ones
-        below valid_kv_len if given (a number, or one per sequence). q in the cache's dtype or one that widens to it."""
+        below valid_kv_len if given (a number, or one per sequence). q in the cache's dtype or one that widens to it. No
+        gradient, however many query rows there are."""
+        _no_grad("PagedIclKVCache.query", q, out)
         lengths = self.default_valid(block)
         longest = max(self._lengths_of(block))
         if isinstance(valid_kv_len, Tensor):
@@ -508,14 +516,14 @@ class PagedIclKVCache(_icl.IclKVCache):
         elif q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and q.shape[3] == 64 \
                 and dt == torch.bfloat16 and self.weights is None:
             k, v = paged_gather(self.keys[block], self.values[block], self.table[:, :w], lengths, longest)
-            return self._dense(q.to(dt), k, v, lengths, out)
+            return self._dense(q.to(dt) if out is None else _apart(q.to(dt), out), k, v, lengths, out)
         weights = None if self.weights is None else self.weights[:, :w * self.page_rows]
         return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out)
 
     def evict(self, keep: Union[int, Sequence[int]], recent: int = 0) -> Tensor:
         """Cuts each sequence to at most keep rows (a number, or one per sequence), in every block alike: its `recent`
-        last rows and the heaviest of the others (paged_evict by the tracked weights, which follow their rows). Emptied
-        pages go back to the pool. Returns index [sequences, K] int32: slot j now holds the old row index[s, j]."""
+        last rows and the heaviest of the others (paged_evict by the tracked weights, which follow their rows). Pages
+        behind the kept rows, reserved ones too, go back to the pool. Returns index [sequences, K] int32: slot j now holds the old row index[s, j]."""
         self._own("evict")
         if self.weights is None:
             raise ValueError("evict needs a cache built with track=True")
@@ -541,12 +549,13 @@ class PagedIclKVCache(_icl.IclKVCache):
     def release(self, sequence: int) -> None:
         """Forgets a sequence: its pages go back to the pool, its place can be filled anew."""
         self._own("release")
+        sequence = range(len(self._held))[sequence]
         for rows in self._rows:
             rows[sequence] = 0
         self.lengths[:, sequence] = 0
         if self.weights is not None:
             self.weights[sequence] = 0.0
-        self._give_back([max(r[s] for r in self._rows) if s != sequence else 0 for s in range(len(self._held))])
+        self._give_back([0 if s == sequence else held * self.page_rows for s, held in enumerate(self._held)])
 
     def _give_back(self, rows) -> None:  # noqa: ANN001
         """Pages past each sequence's first `rows` rows back to the pool."""

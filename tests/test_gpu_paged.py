@@ -724,3 +724,40 @@ def test_cached_query_on_pages(dev):
         a = pages.query_blocks(x, wd.icl_blocks)
         parts = pages.query_chunked(x, wd.icl_blocks, [(0, 1), (1, 2)])
     check(parts, a, BF, "chunked", abs_tol=2e-2 * max(1.0, float(a.abs().max())))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T,G", [(17, 1), (32, 1), (33, 1), (13, 5), (130, 1)])
+def test_query_tiles_of_128_dims_on_long_caches(dev, dtype, T, G):
+    # beyond 1,024 rows the query rows of a head go by 32 and 64 to a tile
+    q, kp, vp, table, n, g = _case(dev, T, [1500, 0, 2777], H=2, G=G, D=128, R=64, T=T, dtype=dtype, slack=1, sharp=1.5)
+    table[2, 3] = -1
+    w = torch.rand(3, table.shape[1] * 64, generator=g, device=dev)
+    _attend(q, kp, vp, table, n, None, what="tiles")
+    _attend(q, kp, vp, table, n, w, what="tiles, weights")
+
+
+@pytest.mark.parametrize("T,lengths", [(3, [300, 40]), (40, [9000, 17]), (70, [40000, 25001])])
+def test_output_over_the_queries(dev, T, lengths):
+    # in place, and shifted within one buffer; with the weights from the scores and from K again
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, T, lengths, H=4, T=T)
+    w = [torch.zeros(2, table.shape[1] * 64, device=dev) for _ in range(3)]
+    want = paged.paged_attention(q, kp, vp, table, n, w[0])
+    for weights in (None, w[1]):
+        buf = torch.zeros(2, 4, T + 1, 64, dtype=BF, device=dev)
+        buf[:, :, 1:] = q
+        for out in (buf[:, :, 1:], buf[:, :, :T]):
+            buf[:, :, 1:] = q
+            if weights is not None:
+                weights.zero_()
+            print(f"[paged] in place {T} {lengths} {weights is not None}", flush=True)
+            assert paged.paged_attention(buf[:, :, 1:], kp, vp, table, n, weights, None, out) is out
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            if weights is not None:
+                assert torch.equal(weights, w[0])
+    buf = q.clone()
+    torch.ops.tabicl.paged_attn_weights_out(buf, kp, vp, table, n, 0.125, buf, w[2])
+    torch.cuda.synchronize()
+    assert torch.equal(buf, want) and torch.equal(w[2], w[0])

@@ -308,3 +308,33 @@ def test_cache_refuses(plain):
         t.evict([1, 2])
     with pytest.raises(ValueError, match="keep"):
         t.evict(-1)
+
+
+def test_release_keeps_what_others_reserved(plain):
+    c = _cache(plain)
+    c.reserve([30, 50, 0])
+    z = torch.zeros(3, 2, 10, 32)
+    for b in range(2):
+        c.append(b, z, z, [10, 3, 0])
+    table = c.table.clone()
+    assert c.free_pages == 12 - 2 - 4
+    c.release(-3)
+    assert c.free_pages == 12 - 4 and (c.table[0] == -1).all() and torch.equal(c.table[1], table[1])
+    assert c.length(1, 1) == 3
+    with pytest.raises(IndexError):
+        c.release(3)
+    c.release(1)
+    assert c.free_pages == 12
+
+
+@pytest.mark.parametrize("rows", [1, 2000])
+def test_query_refuses_gradients(plain, rows):
+    # at every number of query rows, also where the dense kernel would answer
+    c = plain.PagedIclKVCache(1, 1, 1, 64, 64, 4, device="cpu")
+    z = torch.zeros(1, 1, 8, 64, dtype=torch.bfloat16)
+    c.append(0, z, z)
+    q = torch.zeros(1, 1, rows, 64, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        c.query(0, q)
+    with torch.no_grad():
+        assert c.query(0, q).shape == q.shape
