@@ -452,34 +452,46 @@ __global__ __launch_bounds__(512) void pa_whole_kernel(PagedAttn a, PagedSplit z
 __device__ __forceinline__ void store4(float* p, f32x4 x) { *(f32x4*)p = x; }
 __device__ __forceinline__ void store4(bf16* p, f32x4 x) { *(bf16x4*)p = cvt_bf16x4(x); }
 
-// Joins the partials of one query row per wave: 4 values of a partial output per lane, 256 / D partials at a time. Rows
-// that pa_kernel has written are left alone; rows without a key become 0.
+// Where the partials of query row r (of all rows of K/V head h of sequence n) are: `parts` of them, from workgroup w0 on;
+// one: pa_kernel has written the row.
+template <int QT>
+struct PagedParts {
+  int w0, parts, at;
+  __device__ __forceinline__ PagedParts(const PagedSplit& z, int nh, int r) {
+    const int2 w = z.ends[nh * z.qtiles + r / (16 * QT)];
+    w0 = w.x;
+    parts = w.y - w0 + 1;
+    at = r % (16 * QT);
+  }
+  __device__ __forceinline__ int64_t slot(int i) const { return (int64_t)(2 * (w0 + i) + (i == 0)) * (16 * QT) + at; }
+};
+
+// Joins the partials of a query row in a wave: 4 values of a partial output per lane, 256 / D partials at a time. Rows that
+// pa_kernel has written are left alone; rows without a key become 0.
 template <typename T, int D, int QT>
-__global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z) {
+__device__ __forceinline__ void pa_merge_row(const PagedAttn& a, const PagedSplit& z, int64_t row) {
   constexpr int LPR = D / 4, GR = 64 / LPR;
   const int lane = threadIdx.x & 63, G = a.Hq / a.pool.H, rows = G * a.Tq;
-  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= (int64_t)a.N * a.pool.H * rows) return;
   const int r = (int)(row % rows), nh = (int)(row / rows), n = nh / a.pool.H, h = nh % a.pool.H;
-  const int2 w = z.ends[nh * z.qtiles + r / (16 * QT)];
+  PagedParts<QT> p(z, nh, r);
+  p.w0 = __builtin_amdgcn_readfirstlane(p.w0);
+  p.parts = __builtin_amdgcn_readfirstlane(p.parts);
   const int len = pa_len(a, n);
   T* op = (T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lane * 4;
   if (len == 0) {
     if (lane < LPR) store4(op, f32x4{0.f, 0.f, 0.f, 0.f});
     return;
   }
-  const int w0 = __builtin_amdgcn_readfirstlane(w.x), w1 = __builtin_amdgcn_readfirstlane(w.y);
-  if (w0 == w1) return;
-  const int parts = w1 - w0 + 1, at = r % (16 * QT);
-  auto slot = [&](int i) { return (int64_t)(2 * (w0 + i) + (i == 0)) * (16 * QT) + at; };
+  if (p.parts == 1) return;
   // every group of lanes joins its share of the partials by itself (their loads wait for nothing but the lengths), then
   // the groups are joined
   float m = PA_REF0, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = lane / LPR; i < parts; i += GR) {
-    const float2 v = z.ml[slot(i)];
-    const f32x4 x = *(const f32x4*)(z.part + slot(i) * D + lane % LPR * 4);
+  for (int i = lane / LPR; i < p.parts; i += GR) {
+    const float2 v = z.ml[p.slot(i)];
+    const f32x4 x = *(const f32x4*)(z.part + p.slot(i) * D + lane % LPR * 4);
     const float to = fmaxf(m, v.x), f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(v.x - to);
     m = to;
     l = l * f0 + v.y * f1;
@@ -500,12 +512,16 @@ __global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z
   if (z.stat && lane == 0) z.stat[row] = make_float2(m, inv);
 }
 
-// weights[n, i] += sum over the query rows of p: 64 keys per workgroup, 4 per thread, the query rows over 16 threads
-// (each in steps of 16), joined in a fixed order.
-__global__ __launch_bounds__(256) void pa_weights_kernel(PagedAttn a, PagedSplit z) {
+template <typename T, int D, int QT>
+__global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z) {
+  pa_merge_row<T, D, QT>(a, z, (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+}
+
+// weights[n, i] += sum over the query rows of p (stat: their references and sums): the 64 keys from k0 on, 4 per thread, the
+// query rows over 16 threads (each in steps of 16), joined in a fixed order.
+__device__ __forceinline__ void pa_weights_keys64(const PagedAttn& a, const PagedSplit& z, int n, int len, int k0,
+                                                  const float2* stat) {
   __shared__ f32x4 sh[16][16];
-  const int n = blockIdx.y, len = pa_len(a, n), k0 = blockIdx.x * 64;
-  if (k0 >= len) return;
   const int all = a.Hq * a.Tq, kt = threadIdx.x & 15, rt = threadIdx.x >> 4;
   const int64_t first = (int64_t)n * all;
   f32x4 w = {0.f, 0.f, 0.f, 0.f};
@@ -513,7 +529,7 @@ __global__ __launch_bounds__(256) void pa_weights_kernel(PagedAttn a, PagedSplit
   // rows: the whole call 71 -> 45 us; 59 over 5 x 1,700 39 -> 33).
 #pragma unroll 8
   for (int r = rt; r < all; r += 16) {
-    const float2 st = z.stat[first + r];
+    const float2 st = stat[r];
     const f32x4 s = *(const f32x4*)(z.score + (first + r) * z.score_sn + k0 + kt * 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[i] - st.x), st.y, w[i]);
@@ -526,6 +542,46 @@ __global__ __launch_bounds__(256) void pa_weights_kernel(PagedAttn a, PagedSplit
     for (int r = 0; r < 16; ++r) t += sh[r][threadIdx.x >> 2][threadIdx.x & 3];
     if (key < len) a.weights[n * a.weights_sn + key] += t;
   }
+}
+
+__global__ __launch_bounds__(256) void pa_weights_kernel(PagedAttn a, PagedSplit z) {
+  const int n = blockIdx.y, len = pa_len(a, n), k0 = blockIdx.x * 64;
+  if (k0 < len) pa_weights_keys64(a, z, n, len, k0, z.stat + (int64_t)n * a.Hq * a.Tq);
+}
+
+// Both in one launch for up to PA_JOIN query rows of a sequence: the first workgroups merge, the others join the references
+// and sums of their sequence's rows for themselves and add the weights up.
+constexpr int PA_JOIN = 32;
+
+template <typename T, int D, int QT>
+__global__ __launch_bounds__(256) void pa_merge_weights_kernel(PagedAttn a, PagedSplit z, int merges) {
+  __shared__ float2 stat[PA_JOIN];
+  if ((int)blockIdx.x < merges)
+    return pa_merge_row<T, D, QT>(a, z, (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  const int at = blockIdx.x - merges, blocks = (int)(z.score_sn / 64), n = at / blocks, k0 = at % blocks * 64;
+  const int len = pa_len(a, n), rows = a.Hq / a.pool.H * a.Tq, all = a.Hq * a.Tq;
+  if (k0 >= len) return;
+#pragma unroll 2
+  for (int i = threadIdx.x / 16; i < all; i += 16) {  // 16 lanes a row
+    const PagedParts<QT> p(z, n * a.pool.H + i / rows, i % rows);
+    float m = PA_REF0, l = 0.f;
+    for (int j = threadIdx.x % 16; j < p.parts; j += 16) {
+      const float2 v = z.ml[p.slot(j)];
+      const float to = fmaxf(m, v.x);
+      l = l * __builtin_amdgcn_exp2f(m - to) + v.y * __builtin_amdgcn_exp2f(v.x - to);
+      m = to;
+    }
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) {
+      const float mo = __shfl_xor(m, x, 64), lo = __shfl_xor(l, x, 64), to = fmaxf(m, mo);
+      l = l * __builtin_amdgcn_exp2f(m - to) + lo * __builtin_amdgcn_exp2f(mo - to);
+      m = to;
+    }
+    if (threadIdx.x % 16 == 0)  // one part: pa_kernel has left the pair, and nothing in ml
+      stat[i] = p.parts == 1 ? z.stat[(int64_t)n * all + i] : make_float2(m, l == 0.f ? 0.f : 1.f / l);
+  }
+  __syncthreads();
+  pa_weights_keys64(a, z, n, len, k0, stat);
 }
 
 // The same from K itself, for many query rows per K/V head: the scores of 64 keys per wave once more, head after head (a
@@ -907,6 +963,15 @@ void launch_pa_w(const PagedAttn& a, const PagedSplit& z, hipStream_t stream) {
   } else {
     hipLaunchKernelGGL((pa_kernel<T, D, QT, W>), dim3((unsigned)z.groups), dim3(256), 0, stream, a, z);
     const unsigned merge = (unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4);
+    // In one launch where the workgroups of the weights all fit on the GPU at once and each has few rows to join (us of the
+    // whole call, apart / in one, 8 heads: one query row over 8 x 2,000 rows 17.5 / 14.5, over 8 x 15,000 60.6 / 58.1, over
+    // 64 x 4,000 111.2 / 112.1; 4 rows 18.2 / 16.1, 67.1 / 65.4, 125.9 / 130.0; 8 rows over 1 x 45,000 32.4 / 34.3).
+    if constexpr (W && QT <= 2)  // more query rows a tile, more than PA_JOIN a sequence
+      if (a.Hq * a.Tq <= PA_JOIN && a.N * z.score_sn <= 64 * 8 * (int64_t)cu_count()) {
+        const unsigned blocks = (unsigned)(z.score_sn / 64 * a.N);
+        hipLaunchKernelGGL((pa_merge_weights_kernel<T, D, QT>), dim3(merge + blocks), dim3(256), 0, stream, a, z, (int)merge);
+        return;
+      }
     hipLaunchKernelGGL((pa_merge_kernel<T, D, QT>), dim3(merge), dim3(256), 0, stream, a, z);
   }
   if (W)

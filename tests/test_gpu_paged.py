@@ -761,3 +761,20 @@ def test_output_over_the_queries(dev, T, lengths):
     torch.ops.tabicl.paged_attn_weights_out(buf, kp, vp, table, n, 0.125, buf, w[2])
     torch.cuda.synchronize()
     assert torch.equal(buf, want) and torch.equal(w[2], w[0])
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (F32, 64), (BF, 128), (F32, 32)])
+@pytest.mark.parametrize("H,G,T,lengths", [
+    (8, 1, 1, [1999, 0, 5, 1030]), (1, 1, 32, [20000]), (1, 1, 33, [9000, 1]), (2, 8, 2, [1100, 4096]), (4, 1, 8, [128, 2048]),
+    (1, 3, 1, [45000]), (2, 1, 1, [1500] * 70)])
+def test_weights_of_few_rows(dev, dtype, D, H, G, T, lengths):
+    # the references and sums joined where the weights are added up: items of one and of many parts, rows without a key,
+    # up to 32 query rows a sequence and beyond
+    q, kp, vp, table, n, g = _case(dev, T + H, lengths, H=H, G=G, D=D, T=T, dtype=dtype, sharp=2.0)
+    w = torch.rand(len(lengths), table.shape[1] * 64 + 3, generator=g, device=dev)
+    out = _attend(q, kp, vp, table, n, w, what="joined")
+    again = torch.zeros_like(w), torch.zeros_like(w)
+    import tabicl_mi355_paged as paged
+    for x in again:
+        assert torch.equal(paged.paged_attention(q, kp, vp, table, n, x), out)
+    assert torch.equal(*again)
