@@ -385,7 +385,7 @@ int tabicl_icl_cache_append(void* k_cache, void* v_cache, int64_t dst_sn, int64_
  * strides, contiguous last dim). Rows without a key, or whose every score is -inf, are 0. weights (or NULL): fp32
  * [N, max_pages * page_rows] (row stride weights_sn), the probabilities summed over the query heads and rows are added
  * to the first lengths[n] entries; the sums' order is fixed. For one query row to a few hundred.
- * ws: tabicl_paged_attn_workspace_bytes(...) bytes, 16-byte aligned.
+ * out must not overlap q (the weights read q again). ws: tabicl_paged_attn_workspace_bytes(...) bytes, 16-byte aligned.
  */
 int tabicl_paged_attn(const void* q, const void* k_pages, const void* v_pages, int64_t pages, int64_t page_sp,
                       int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths,
@@ -399,7 +399,7 @@ int64_t tabicl_paged_attn_workspace_bytes(int64_t N, int64_t Hq, int64_t H, int6
 /*
  * Writes rows t < count[n] (NULL: all T) of k, v [N, H, T, D] (element strides, contiguous last dim) to rows
  * lengths[n] + t of each sequence; rows at or past max_pages * page_rows are dropped. lengths stays as it is (the
- * other blocks append at the same rows). Two sequences must not share a page that is written.
+ * other blocks append at the same rows). A page that is written must stand in the table once.
  */
 int tabicl_paged_append(void* k_pages, void* v_pages, int64_t pages, int64_t page_sp, int64_t page_rows,
                         const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const void* k,
@@ -421,7 +421,8 @@ int tabicl_paged_gather(const void* k_pages, const void* v_pages, int64_t pages,
  * rows are not kept, in order; no other row moves. All blocks (element stride block_sp) move alike. Written:
  * index [N, K] (slot j holds the old row index[n, j]; -1 from kept on), kept_weights [N, max_pages * page_rows]
  * (weights of the kept rows in their slots, 0 after), kept_lengths [N]. weights, table and lengths stay as they are.
- * No two sequences may share a page. ws: tabicl_paged_evict_workspace_bytes(N, K) bytes, 16-byte aligned.
+ * No page may stand in the table twice; kept_weights must not overlap weights. ws: tabicl_paged_evict_workspace_bytes(N, K)
+ * bytes, 16-byte aligned (of K = 0 too).
  */
 int tabicl_paged_evict(void* k_pages, void* v_pages, int64_t blocks, int64_t block_sp, int64_t pages, int64_t page_sp,
                        int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages,

@@ -251,8 +251,8 @@ def paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tenso
                  count: Optional[Tensor] = None) -> None:
     """Rows t < count[n] (int32 [N]; default all) of k, v [N, H, T, D] into rows lengths[n] + t of each sequence of the
     pool (any strides with a contiguous last dim, e.g. the heads of a K|V projection). lengths is read, not changed: the
-    other blocks of a model append at the same rows. Rows that the table has no page for are dropped. Two sequences
-    must not share a page that is written."""
+    other blocks of a model append at the same rows. Rows that the table has no page for are dropped. A page that
+    is written must stand in the table once."""
     if _nat.direct(k_pages, v_pages, table, lengths, k, v, count):
         _append_launch(k_pages, v_pages, table, lengths, k, v, count)
         torch.autograd.graph.increment_version((k_pages, v_pages))
@@ -356,8 +356,8 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
     ties: the lower row; NaN counts as -inf). Kept rows past the cut move, in order, to the places of the evicted ones
     below it; nothing else moves. Returns index [N, K] int32 (slot j holds the old row index[n, j], -1 from kept on; K =
     keep, or the capacity for a tensor), the weights in their new slots [N, max_pages page_rows] (0 past the cut) and
-    kept [N] int32. weights, table and lengths are not changed: take over the new ones. No two sequences may share a
-    page."""
+    kept [N] int32. weights, table and lengths are not changed: take over the new ones. No page may stand in the table
+    twice."""
     if k_pages.dim() == 4 and v_pages.dim() == 4:
         k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
     keep_n = None

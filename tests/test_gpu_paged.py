@@ -778,3 +778,92 @@ def test_weights_of_few_rows(dev, dtype, D, H, G, T, lengths):
     for x in again:
         assert torch.equal(paged.paged_attention(q, kp, vp, table, n, x), out)
     assert torch.equal(*again)
+
+
+@pytest.mark.parametrize("seed,D,dtype,tracked", [(0, 64, BF, True), (1, 128, BF, True), (2, 32, F32, True), (3, 64, BF, False)])
+def test_cache_through_random_calls(dev, seed, D, dtype, tracked):
+    # appends, reservations, queries of many widths, evictions and releases in any order against lists of rows
+    import random
+    import tabicl_mi355_paged as paged
+    S, B, H, R, cap = 4, 2, 2, 32, 2400
+    rng, g = random.Random(seed), torch.Generator(device=dev).manual_seed(seed)
+    c = paged.PagedIclKVCache(S, B, H, D, cap, 240, R, dtype, dev, track=tracked)
+    for t in (c.keys, c.values):
+        t.fill_(float("nan"))
+    rows = [[(torch.empty(H, 0, D, dtype=dtype, device=dev),) * 2 for _ in range(S)] for _ in range(B)]
+    for step in range(60):
+        have = [rows[0][s][0].shape[1] for s in range(S)]
+        what = rng.choice(["append", "append", "query", "query", "query", "evict", "release", "reserve", "captured"])
+        print(f"[paged] step {step} {what} {have} free {c.free_pages}", flush=True)
+        if what == "append":
+            T = rng.choice([1, 7, 33, 400, 1500])
+            new = [rng.choice([0, T, rng.randint(0, T)]) for _ in range(S)]
+            new = [min(n, cap - h) for n, h in zip(new, have)]
+            if sum(max(c._held[s], -(-(h + n) // R)) - c._held[s] for s, (h, n) in enumerate(zip(have, new))) > c.free_pages:
+                with pytest.raises(ValueError, match="pages wanted"):
+                    c.append(0, *(torch.zeros(S, H, T, D, dtype=dtype, device=dev),) * 2, new)
+                continue
+            for b in range(B):
+                k, v = (torch.randn(S, T, H, D, generator=g, device=dev).to(dtype).transpose(1, 2) for _ in range(2))
+                c.append(b, k, v, new)
+                for s in range(S):
+                    rows[b][s] = tuple(torch.cat([o, x[s, :, :new[s]]], 1) for o, x in zip(rows[b][s], (k, v)))
+        elif what in ("query", "captured") and max(have):
+            b, T = rng.randrange(B), rng.choice([1, 3, 20, 70])
+            q = torch.randn(S, H, T, D, generator=g, device=dev).to(dtype)
+            before = None if c.weights is None else c.weights.clone()
+            want, w, tol, wtol = ref.attention(q, c.keys[b], c.values[b], c.table, c.lengths[b], D ** -0.5, before)
+            if what == "query":
+                out = c.query(b, q, None, rng.choice([None, torch.empty_like(q), q]))
+            else:
+                c.query(b, q)
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    out = c.query(b, q)
+                for _ in range(2):
+                    if before is not None:
+                        c.weights.copy_(before)
+                    graph.replay()
+            torch.cuda.synchronize()
+            ref.near(out, want, tol, "out")
+            if before is not None:
+                ref.near(c.weights, w, wtol, "weights")
+        if what == "evict" and tracked:
+            keep = rng.choice([rng.randint(0, 2000), [rng.randint(0, 2000) for _ in range(S)]])
+            recent = rng.choice([0, 5, 3000])
+            before = c.weights.clone()
+            index = c.evict(keep, recent).long()
+            for s in range(S):
+                n = min(have[s], keep if isinstance(keep, int) else keep[s])
+                idx, last = index[s, :n], min(recent, n)
+                assert (index[s, n:] == -1).all() and len(set(idx.tolist())) == n
+                assert set(range(have[s] - last, have[s])) <= set(idx.tolist())
+                assert torch.equal(c.weights[s, :n], before[s, idx]) and (c.weights[s, n:] == 0).all()
+                gone = torch.ones(have[s] - last, dtype=torch.bool, device=dev)  # of the rows that compete
+                gone[idx[idx < have[s] - last]] = False
+                older = before[s, :have[s] - last]
+                assert not gone.any() or gone.all() or older[gone].max() <= older[~gone].min()
+                for b in range(B):
+                    rows[b][s] = tuple(x[:, idx] for x in rows[b][s])
+        elif what == "release":
+            s = rng.randrange(S)
+            c.release(s)
+            for b in range(B):
+                rows[b][s] = tuple(x[:, :0] for x in rows[b][s])
+        elif what == "reserve":
+            want = [rng.randint(0, 600) for _ in range(S)]
+            if sum(max(0, -(-n // R) - held) for n, held in zip(want, c._held)) <= c.free_pages:
+                c.reserve(want)
+        # the books, and what the pages hold
+        assert c.free_pages + sum(c._held) == 240
+        table = c.table.tolist()
+        owned = [p for t in table for p in t if p >= 0]
+        assert len(set(owned)) == len(owned) == sum(c._held)
+        for b in range(B):
+            assert c.lengths[b].tolist() == [rows[b][s][0].shape[1] for s in range(S)]
+            for s in range(S):
+                n = c.length(b, s)
+                _, page, row = ref.rows_of(c.table[s], n, R, 240)
+                for pool, want in zip((c.keys, c.values), rows[b][s]):
+                    assert torch.equal(pool[b][page, :, row].transpose(0, 1), want)
