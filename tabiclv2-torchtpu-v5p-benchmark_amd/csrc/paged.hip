@@ -52,6 +52,7 @@ constexpr int PA_UNIT = 128, PA_WHOLE = 1024;
 struct PagedSplit {
   int groups;    // G, or 0: a workgroup of eight waves for each item
   int least;     // units a workgroup takes at least
+  int few;       // below so many units, half of the workgroups share them
   int qtiles;
   float* part;   // [2 G][16 QT][D] unnormalised outputs
   float2* ml;    // [2 G][16 QT] (ref, sum)
@@ -111,13 +112,14 @@ struct PagedUnits {
   }
 };
 
-// Equal shares: `groups` workgroups (fewer, if they would get less than `least` units) of `share` units, the first `more`
-// of them one more.
+// Equal shares: `groups` workgroups (half of them below `few` units, and fewer if they would get less than `least` units) of
+// `share` units, the first `more` of them one more.
 struct PagedShares {
   int groups, share, more;
   __device__ __forceinline__ PagedShares(const PagedSplit& z, int total) {
     groups = total / z.least;
-    groups = groups < 1 ? 1 : groups < z.groups ? groups : z.groups;
+    const int most = total < z.few ? z.groups / 2 : z.groups;
+    groups = groups < 1 ? 1 : groups < most ? groups : most;
     share = total / groups;
     more = total - share * groups;
   }
@@ -344,7 +346,9 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
 #pragma unroll
       for (int s = 0; s < SUB; ++s) l[qt] += (p[s][0] + p[s][1]) + (p[s][2] + p[s][3]);
       paged_values<D>(t, p, o[qt]);
-      if constexpr (QT > 1) __builtin_amdgcn_sched_barrier(0);  // one query tile's scores and probabilities live at a time
+      // one query tile's scores and probabilities live at a time, where stored scores take the registers too (12 dwords a
+      // lane spilled without it; elsewhere the tiles overlap: 64 query rows of 64 dims over 8 x 12,000 rows 57.5 -> 56 us)
+      if constexpr (QT > 1 && W) __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -931,6 +935,12 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
   // workspace less, and such calls wait for the host (16.5 / 12.7 us).
   z->groups = rows <= PA_WHOLE ? 0 : pa_waves(D, QT) * cu_count();
   z->least = 2;
+  // Of few units one workgroup per CU: half the partials, half the waves to join, and the loads of four waves are enough for
+  // as long as the call then takes (us, two per CU / one: 64 query rows over 8 x 5,000 rows 30.3 / 28.9, over 1 x 45,000
+  // 36.5 / 31.5, one row over 1 x 45,000 26.0 / 23.4, over 8 x 5,000 21.6 / 20.2; fp32, 32 rows over 8 x 5,000 43.9 / 40.2.
+  // With the limit at 24 units a workgroup, one row over 64 x 2,000 51.4 / 52.9; rows of 32 dims, 64 query rows over
+  // 8 x 5,000 22.1 / 23.2).
+  z->few = D > 32 && pa_waves(D, QT) == 2 ? 12 * z->groups : 0;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     char* p = ws + at;
