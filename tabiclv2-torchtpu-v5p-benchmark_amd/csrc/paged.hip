@@ -167,6 +167,14 @@ __device__ __forceinline__ f32x4 tile_scores(const uint4* k, const uint4* q) {
   return s;
 }
 
+// A score in log2 units, rounded before the reference is taken off: the difference of the largest one is then exact, however
+// large it is, and the same wherever it is formed. (A fused product would leave the rounding of the product in the exponent:
+// at scores of 10^9 the probabilities of a row added up to 10^7.)
+__device__ __forceinline__ float log2_score(float s, float sc) {
+#pragma clang fp contract(off)
+  return s * sc;
+}
+
 // Sum over the 16 lanes of a row, in the registers (row_ror).
 template <int N>
 __device__ __forceinline__ float row_add(float x) {
@@ -305,14 +313,12 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
     const bool full = live == (SUB == 2 ? 16 << 8 | 16 : 16);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      // scores in log2 units, rounded before the reference is taken off: the largest one's difference is then exact, however
-      // large it is (a fused product would leave the rounding of scores of 10^37 in the exponent)
       float x[SUB][4], top = TA_NEG_INF;
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
         const f32x4 sv = tile_scores<T, NC>(t.k[s], q[qt]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[s][i] = sv[i] * sc;
+        for (int i = 0; i < 4; ++i) x[s][i] = log2_score(sv[i], sc);
       }
       if (!full) {
 #pragma unroll
@@ -649,7 +655,7 @@ __global__ __launch_bounds__(256) void pa_weights_keys_kernel(PagedAttn a, Paged
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           // a padded query row adds nothing, its product with an infinite key (0 times infinity) neither
-          w[s][i] = r < rows ? __builtin_fmaf(__builtin_amdgcn_exp2f(sv[i] * sc - st.x), st.y, w[s][i]) : w[s][i];
+          w[s][i] = r < rows ? __builtin_fmaf(__builtin_amdgcn_exp2f(log2_score(sv[i], sc) - st.x), st.y, w[s][i]) : w[s][i];
       }
     }
   };

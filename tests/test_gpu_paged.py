@@ -867,3 +867,29 @@ def test_cache_through_random_calls(dev, seed, D, dtype, tracked):
                 _, page, row = ref.rows_of(c.table[s], n, R, 240)
                 for pool, want in zip((c.keys, c.values), rows[b][s]):
                     assert torch.equal(pool[b][page, :, row].transpose(0, 1), want)
+
+
+@pytest.mark.parametrize("size", [1e6, 1e8, 1e10])
+@pytest.mark.parametrize("T,lengths", [(13, [40000, 25600]), (70, [65000, 700])])
+def test_weights_of_large_scores(dev, size, T, lengths):
+    # weights from the keys once more, products q.K of `size`: every query row's probabilities sum to one, and they are
+    # those of the same rows twelve at a time, which come from stored scores. Both take the same bf16 products; a
+    # probability's rounding errors are the exponential's, the sums' over the keys (n / 32 + 128 steps) and the
+    # normaliser's, the weights' those of one addition per query row.
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, T, lengths, H=2, T=T)
+    q = (q.float() * size ** 0.5).to(BF)
+    kp *= size ** 0.5
+    w, few = torch.zeros(2, table.shape[1] * 64, device=dev), torch.zeros(2, table.shape[1] * 64, device=dev)
+    assert w.numel() >= 65536
+    print(f"[paged] large scores {size} {T} {lengths}", flush=True)
+    out = paged.paged_attention(q, kp, vp, table, n, w)
+    for t in range(0, T, 12):
+        paged.paged_attention(q[:, :, t:t + 12], kp, vp, table, n, few)
+    torch.cuda.synchronize()
+    assert torch.isfinite(out).all() and torch.isfinite(w).all()
+    for s, length in enumerate(lengths):
+        e = (length / 32 + 128 + 2 * T + 16) * 2.0 ** -24
+        assert abs(float(w[s].double().sum()) / (2 * T) - 1) <= e
+        diff = (w[s].double() - few[s].double()).abs()
+        assert bool((diff <= 2 * e * few[s].double() + 2.0 ** -100).all()), float((diff / few[s].clamp(min=1e-30)).max())
