@@ -7,6 +7,8 @@
 #include "launch.h"
 #include "paged.h"
 
+#include <numeric>
+
 namespace {
 
 __device__ __forceinline__ int pool_length(const PagedPool& c, int n) {
@@ -930,6 +932,39 @@ int cu_count() {
   return count[dev];
 }
 
+// Scores kept for the weights take at most this many bytes, or those of 16 query rows of every K/V head where these are
+// more (an eighth of an fp32 cache of 64 dims): tracked queries by the hundred go in slices (pa_slice), which read the cache
+// as often as one launch does where they are whole tiles (bf16, 5,000 query rows over 1 x 45,000 rows: 4.4 ms with 6.9 GB, 4.8
+// in slices; fp32, 1,000 over 8 x 45,000: 11.1 ms with 11 GB, 12.1).
+constexpr int64_t PA_SCORE_BYTES = 1ll << 30;
+
+// Whether the weights of a call take scores kept by the first pass, or K again (pa_weights_keys_kernel). 8 x 45,000 rows in
+// bf16, D = 64, us kept / K again: 8 query rows a head 195 / 213, 16: 231 / 214, 64 (8 x 12,000): 133 / 103. Of few cached rows
+// too few waves share the heads (8 x 2,000, 16 and 64 query rows: 23 / 32, 43 / 52), and in fp32 the products bound it
+// (8 x 12,000, 64: 207 / 231).
+template <typename T, int D>
+bool pa_keeps_scores(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows) {
+  if (sizeof(T) == 4 || N * rows < 65536) return true;
+  return 16 * (Hq / H * Tq) <= 3 * D && N * Hq * Tq * ((rows + 63) / 64 * 64) * 4 <= PA_SCORE_BYTES;
+}
+
+// Query rows (of each head) that a launch takes: all, or as many as keep their scores within PA_SCORE_BYTES, in whole tiles
+// where that many are left.
+template <typename T, int D>
+int64_t pa_slice(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights) {
+  if (!weights || !pa_keeps_scores<T, D>(N, Hq, H, Tq, rows)) return Tq;
+  const int64_t each = N * Hq * ((rows + 63) / 64 * 64) * 4, G = Hq / H;
+  int64_t t = PA_SCORE_BYTES / each;
+  if (t < 16 / G) t = 16 / G;
+  if (t < 1) t = 1;
+  if (t >= Tq) return Tq;
+  for (int64_t tile = 64; tile >= 16; tile /= 2) {
+    const int64_t step = tile / std::gcd(tile, G);
+    if (t >= step) return t - t % step;
+  }
+  return t;
+}
+
 // The split of a call and the bytes of its workspace; `rows`: the most rows a sequence can have.
 template <typename T, int D, int QT>
 int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights) {
@@ -962,11 +997,7 @@ int64_t paged_split(PagedSplit* z, char* ws, int64_t N, int64_t Hq, int64_t H, i
   z->score = nullptr;
   if (weights) {
     z->stat = (float2*)take(all * 8);
-    // The scores kept for the weights, or K again (pa_weights_keys_kernel). 8 x 45,000 rows in bf16, D = 64, us kept / K
-    // again: 8 query rows a head 195 / 213, 16: 231 / 214, 64 (8 x 12,000): 133 / 103. Of few cached rows too few waves
-    // share the heads (8 x 2,000, 16 and 64 query rows: 23 / 32, 43 / 52), and in fp32 the products bound it (8 x 12,000, 64:
-    // 207 / 231).
-    if (sizeof(T) == 4 || 16 * qrows <= 3 * D || N * rows < 65536) z->score = (float*)take(all * z->score_sn * 4);
+    if (pa_keeps_scores<T, D>(N, Hq, H, Tq, rows)) z->score = (float*)take(all * z->score_sn * 4);
   }
   return at;
 }
@@ -1008,8 +1039,8 @@ int64_t run_pa(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, i
 }
 
 template <typename T, int D>
-int64_t run_pa_d(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights,
-                 hipStream_t stream) {
+int64_t run_pa_rows(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights,
+                    hipStream_t stream) {
   const int64_t qrows = Hq / H * Tq;
   // Query rows of a tile: 16 to 64. fp32 of 64 dims keeps to 32 (64 would be one wave per SIMD; 64 query rows over 8 x 5,000
   // rows 62 / 66 us), and of 128 dims the kernel of whole items to 16: short caches are read from L2 anyhow, and two waves
@@ -1019,6 +1050,29 @@ int64_t run_pa_d(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H,
     if (qrows > 32 && most == 64) return run_pa<T, D, 4>(a, ws, N, Hq, H, Tq, rows, weights, stream);
   if (qrows > 16 && most >= 32) return run_pa<T, D, 2>(a, ws, N, Hq, H, Tq, rows, weights, stream);
   return run_pa<T, D, 1>(a, ws, N, Hq, H, Tq, rows, weights, stream);
+}
+
+// The query rows in slices, one launch after the other on the stream (the weights add up in this order); they share a
+// workspace.
+template <typename T, int D>
+int64_t run_pa_d(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights,
+                 hipStream_t stream) {
+  const int64_t slice = pa_slice<T, D>(N, Hq, H, Tq, rows, weights && rows > 0);
+  int64_t bytes = 0;
+  for (int64_t t = 0; t < Tq; t += slice) {
+    const int64_t left = Tq - t < slice ? Tq - t : slice;
+    if (!a && t > 0 && left == slice) continue;  // the last one may be sized otherwise
+    PagedAttn part;
+    if (a) {
+      part = *a;
+      part.q = (const char*)a->q + t * a->q_st * sizeof(T);
+      part.out = (char*)a->out + t * a->o_st * sizeof(T);
+      part.Tq = (int)left;
+    }
+    const int64_t b = run_pa_rows<T, D>(a ? &part : nullptr, ws, N, Hq, H, left, rows, weights, stream);
+    bytes = b > bytes ? b : bytes;
+  }
+  return bytes;
 }
 
 int64_t run_pa_any(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows,

@@ -893,3 +893,27 @@ def test_weights_of_large_scores(dev, size, T, lengths):
         assert abs(float(w[s].double().sum()) / (2 * T) - 1) <= e
         diff = (w[s].double() - few[s].double()).abs()
         assert bool((diff <= 2 * e * few[s].double() + 2.0 ** -100).all()), float((diff / few[s].clamp(min=1e-30)).max())
+
+
+@pytest.mark.parametrize("H,G,D,T,lengths,dtype", [
+    (8, 1, 64, 12001, [3000], BF), (8, 1, 64, 2500, [7000, 33], F32), (2, 3, 128, 5000, [1000, 0, 5000], F32),
+    (1, 5, 32, 14000, [4000], F32)])
+def test_weights_of_query_rows_in_slices(dev, H, G, D, T, lengths, dtype):
+    # more scores than are kept at a time: slices of the query rows, the last one shorter; the rows of an output view
+    import tabicl_mi355_native as nat
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, T, lengths, H=H, G=G, D=D, T=T, dtype=dtype)
+    N, rows = len(lengths), table.shape[1] * 64
+    assert N * H * G * T * rows * 4 > 1 << 30
+    assert nat.load().tabicl_paged_attn_workspace_bytes(N, H * G, H, T, D, rows, 1, int(dtype is F32)) < 1152 << 20
+    w = torch.rand(N, rows, generator=g, device=dev)
+    w0, w1 = w.clone(), w.clone()
+    want = _attend(q, kp, vp, table, n, w, what="slices")
+    merged = torch.empty(N, T, H * G, D, dtype=dtype, device=dev)
+    proj = torch.empty(N, T, H * G, D, dtype=dtype, device=dev).copy_(q.transpose(1, 2))
+    paged.paged_attention(proj.transpose(1, 2), kp, vp, table, n, w0, None, merged.transpose(1, 2))
+    torch.cuda.synchronize()
+    assert torch.equal(merged.transpose(1, 2), want) and torch.equal(w0, w)
+    paged.paged_attention(q, kp, vp, table, n, w1, None, q)  # over the queries
+    torch.cuda.synchronize()
+    assert torch.equal(q, want) and torch.equal(w1, w)

@@ -338,3 +338,16 @@ def test_query_refuses_gradients(plain, rows):
         c.query(0, q)
     with torch.no_grad():
         assert c.query(0, q).shape == q.shape
+
+
+@pytest.mark.parametrize("N,H,G,D,rows,dtype", [
+    (1, 8, 1, 64, 50048, 0), (8, 8, 1, 64, 8128, 0), (8, 8, 1, 64, 45056, 0), (8, 8, 1, 64, 45056, 1), (64, 8, 1, 64, 45056, 0),
+    (64, 2, 12, 128, 1024, 1), (1, 8, 3, 32, 50048, 1), (3, 1, 64, 64, 21824, 0), (64, 8, 1, 64, 45056, 1)])
+def test_workspace_is_bounded_in_the_query_rows(N, H, G, D, rows, dtype):
+    # the scores kept for the weights: at most 1 GiB, or 16 query rows of every K/V head; 128 MiB cover the partials, the
+    # references and the sums of up to 2^22 query rows
+    import tabicl_mi355_native as nat
+    scores = max(1 << 30, N * H * max(16, G) * rows * 4)
+    sizes = [nat.load().tabicl_paged_attn_workspace_bytes(N, H * G, H, Tq, D, rows, 1, dtype)
+             for Tq in (1, 8, 13, 64, 100, 1000, 5000, 20000) if N * H * G * Tq <= 1 << 22]
+    assert all(0 < n <= scores + (128 << 20) for n in sizes), sizes
