@@ -384,8 +384,9 @@ int tabicl_icl_cache_append(void* k_cache, void* v_cache, int64_t dst_sn, int64_
  * h / (Hq / H): softmax(scale q k^T) v in fp32 (bf16 probabilities enter as two bf16 terms each), written to out (element
  * strides, contiguous last dim). Rows without a key, or whose every score is -inf, are 0. weights (or NULL): fp32
  * [N, max_pages * page_rows] (row stride weights_sn), the probabilities summed over the query heads and rows are added
- * to the first lengths[n] entries; the sums' order is fixed. For one query row to a few hundred; with weights more of them
- * go in slices, one after the other on the stream, where the workspace would pass 1 GiB.
+ * to the first lengths[n] entries; the sums' order is fixed. For one query row to a few hundred; more go in
+ * slices, one after the other on the stream, beyond 2^22 query rows over all sequences and heads (up to 2^26), and with
+ * weights where the workspace would pass 1 GiB.
  * out must not overlap q (the weights read q again). ws: tabicl_paged_attn_workspace_bytes(...) bytes, 16-byte aligned.
  */
 int tabicl_paged_attn(const void* q, const void* k_pages, const void* v_pages, int64_t pages, int64_t page_sp,

@@ -745,9 +745,9 @@ int paged_attn_sizes(const char* op, int64_t N, int64_t Hq, int64_t H, int64_t T
       rows > PAGED_MAX_ROWS || (D != 32 && D != 64 && D != 128))
     return fail(1, "%s: bad sizes N=%lld Hq=%lld H=%lld Tq=%lld D=%lld rows=%lld (Hq must be a multiple of H)", op,
                 (long long)N, (long long)Hq, (long long)H, (long long)Tq, (long long)D, (long long)rows);
-  if (Tq > (1LL << 22) || N * Hq * Tq > (1LL << 22)) return fail(1, "%s: more than 2^22 query rows", op);
-  // units of 128 rows of every sequence, head and tile of 16 query rows are counted in 32 bits
-  if (N * H * ((Hq / H * Tq + 15) / 16) * (rows / 128 + 1) > (1LL << 30))
+  if (Tq > PAGED_MAX_QUERIES || N * Hq > PAGED_MAX_QUERIES || N * Hq * Tq > 16 * PAGED_MAX_QUERIES)
+    return fail(1, "%s: more than 2^26 query rows, or 2^22 of one head, or 2^22 heads over all sequences", op);
+  if (Tq > 0 && N * H * ((Hq / H + 15) / 16) * (rows / 128 + 1) > PAGED_MAX_UNITS)
     return fail(1, "%s: more than 2^37 cached rows over all sequences, heads and tiles of query rows", op);
   return 0;
 }

@@ -61,6 +61,11 @@ struct PagedEvict {
 // workgroups out without an error.
 #define PAGED_MAX_GRID (1ll << 23)
 
+// Query rows over all sequences and heads that a launch of the attention takes, and units (128 rows of a sequence, K/V head
+// and tile of 16 query rows), which it counts in 32 bits. Calls of more query rows go in slices.
+#define PAGED_MAX_QUERIES (1ll << 22)
+#define PAGED_MAX_UNITS (1ll << 30)
+
 // dtype codes 0 bf16, 1 fp32. Return value: hipGetLastError() after the launches.
 int tabicl_launch_paged_attn(const PagedAttn& a, int dtype, void* ws, hipStream_t stream);
 int64_t tabicl_launch_paged_attn_ws_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows, int weights,

@@ -948,14 +948,19 @@ bool pa_keeps_scores(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows)
   return 16 * (Hq / H * Tq) <= 3 * D && N * Hq * Tq * ((rows + 63) / 64 * 64) * 4 <= PA_SCORE_BYTES;
 }
 
-// Query rows (of each head) that a launch takes: all, or as many as keep their scores within PA_SCORE_BYTES, in whole tiles
-// where that many are left.
+// Query rows (of each head) that a launch takes: all, or as many as its counters hold (PAGED_MAX_QUERIES, PAGED_MAX_UNITS) and
+// as keep their scores within PA_SCORE_BYTES, in whole tiles where that many are left.
 template <typename T, int D>
 int64_t pa_slice(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, bool weights) {
-  if (!weights || !pa_keeps_scores<T, D>(N, Hq, H, Tq, rows)) return Tq;
-  const int64_t each = N * Hq * ((rows + 63) / 64 * 64) * 4, G = Hq / H;
-  int64_t t = PA_SCORE_BYTES / each;
-  if (t < 16 / G) t = 16 / G;
+  const int64_t G = Hq / H, units = N * H * (rows / 128 + 1);
+  int64_t t = PAGED_MAX_QUERIES / (N * Hq);
+  const int64_t counted = PAGED_MAX_UNITS / units * 16 / G;
+  t = counted < t ? counted : t;
+  if (weights && pa_keeps_scores<T, D>(N, Hq, H, Tq, rows)) {
+    int64_t kept = PA_SCORE_BYTES / (N * Hq * ((rows + 63) / 64 * 64) * 4);
+    if (kept < 16 / G) kept = 16 / G;
+    t = kept < t ? kept : t;
+  }
   if (t < 1) t = 1;
   if (t >= Tq) return Tq;
   for (int64_t tile = 64; tile >= 16; tile /= 2) {

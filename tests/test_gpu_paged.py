@@ -917,3 +917,13 @@ def test_weights_of_query_rows_in_slices(dev, H, G, D, T, lengths, dtype):
     paged.paged_attention(q, kp, vp, table, n, w1, None, q)  # over the queries
     torch.cuda.synchronize()
     assert torch.equal(q, want) and torch.equal(w1, w)
+
+
+@pytest.mark.parametrize("lengths,weighted", [([200, 3, 0, 64, 17, 100, 1, 128], True), ([1100] + [5] * 7, False)])
+def test_query_rows_beyond_one_launch(dev, lengths, weighted):
+    # more than 2^22 query rows over all sequences and heads
+    T = 66000
+    q, kp, vp, table, n, g = _case(dev, 3, lengths, H=8, D=32, T=T)
+    assert 8 * 8 * T > 1 << 22
+    w = torch.zeros(8, table.shape[1] * 64, device=dev) if weighted else None
+    _attend(q, kp, vp, table, n, w, what="many rows")

@@ -351,3 +351,14 @@ def test_workspace_is_bounded_in_the_query_rows(N, H, G, D, rows, dtype):
     sizes = [nat.load().tabicl_paged_attn_workspace_bytes(N, H * G, H, Tq, D, rows, 1, dtype)
              for Tq in (1, 8, 13, 64, 100, 1000, 5000, 20000) if N * H * G * Tq <= 1 << 22]
     assert all(0 < n <= scores + (128 << 20) for n in sizes), sizes
+
+
+def test_query_rows_beyond_one_launch():
+    # the query of 70,000 test rows by 8 estimators of 8 heads, which IclKVCache takes: slices, whatever the cache
+    import tabicl_mi355_native as nat
+    size = nat.load().tabicl_paged_attn_workspace_bytes
+    for rows, weights, dtype in ((45056, 0, 0), (45056, 1, 0), (45056, 0, 1), (1024, 1, 0), (1 << 24, 0, 0)):
+        assert 0 <= size(8, 8, 8, 70000, 64, rows, weights, dtype) <= (1152 << 20), (rows, weights, dtype, nat.last_error())
+    assert size(8, 8, 8, 1 << 20, 64, 45056, 0, 0) > 0
+    for n in ((8, 8, 8, (1 << 20) + 1, 64, 45056, 0, 0), (1, 1, 1, (1 << 22) + 1, 64, 64, 0, 0), (65535, 128, 1, 1, 64, 64, 0, 0)):
+        assert size(*n) < 0 and "query rows" in nat.last_error()
