@@ -383,6 +383,10 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
 # query rows T: 8 x 45,000 cached rows T 128 241 / 449, 256 438 / 462, 384 648 / 568, 5000 9164 / 3440; 8 x 5,000 rows 256
 # 72 / 69, 512 120 / 87; 1 x 20,000 rows 512 65 / 98, 1000 101 / 102; 8 x 700 rows 512 39 / 56, 5000 285 / 88.
 _DENSE_QUERY_ROWS, _DENSE_SCORES = 256, 1 << 24
+# Bytes of K and V that a gather puts side by side (more only for a single sequence of more): the sequences go in runs, each
+# padded to its own longest one. us of all at once / in runs of 2 GiB / 1 GiB, T 384: 16 x 45,000 rows 1246 / 1243 / 1262, one
+# table of 50,000 rows beside 63 of 500 752 (6.3 GB) / 514 / 507, 40 of 100 to 20,000 763 / 713 / 829.
+_GATHER_BYTES = 2 << 30
 
 
 class PagedIclKVCache(_icl.IclKVCache):
@@ -515,10 +519,32 @@ class PagedIclKVCache(_icl.IclKVCache):
             w = self.table.shape[1]  # a replay meets the lengths of its time, not today's
         elif q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and q.shape[3] == 64 \
                 and dt == torch.bfloat16 and self.weights is None:
-            k, v = paged_gather(self.keys[block], self.values[block], self.table[:, :w], lengths, longest)
-            return self._dense(q.to(dt) if out is None else _apart(q.to(dt), out), k, v, lengths, out)
+            return self._gathered(block, q.to(dt), lengths, longest, out)
         weights = None if self.weights is None else self.weights[:, :w * self.page_rows]
         return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out)
+
+    def _gathered(self, block: int, q: Tensor, lengths: Tensor, longest: int, out: Optional[Tensor]) -> Tensor:
+        """query by the dense kernel, over the rows of one run of sequences after the other side by side."""
+        each = [min(n, longest) for n in self._lengths_of(block)]
+        most = _GATHER_BYTES // (2 * q.shape[1] * q.shape[3] * q.element_size())  # cached rows of a run
+        if out is not None:
+            q = _apart(q, out)
+        elif len(each) * longest > most:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        start, o = 0, None
+        while start < len(each):
+            stop, rows = start + 1, each[start]
+            while stop < len(each) and (stop + 1 - start) * max(rows, each[stop]) <= most:
+                rows = max(rows, each[stop])
+                stop += 1
+            rows = max(1, rows)
+            run = slice(start, stop)
+            k, v = paged_gather(self.keys[block], self.values[block], self.table[run, :-(-rows // self.page_rows)], lengths[run],
+                                rows)
+            o = self._dense(q[run], k, v, lengths[run], None if out is None else out[run])
+            del k, v  # before the next run's
+            start = stop
+        return o if out is None else out
 
     def evict(self, keep: Union[int, Sequence[int]], recent: int = 0) -> Tensor:
         """Cuts each sequence to at most keep rows (a number, or one per sequence), in every block alike: its `recent`

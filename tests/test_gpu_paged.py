@@ -927,3 +927,30 @@ def test_query_rows_beyond_one_launch(dev, lengths, weighted):
     assert 8 * 8 * T > 1 << 22
     w = torch.zeros(8, table.shape[1] * 64, device=dev) if weighted else None
     _attend(q, kp, vp, table, n, w, what="many rows")
+
+
+def test_cache_many_query_rows_of_ragged_tables(dev, monkeypatch):
+    # the gathered rows in runs of sequences: the same attention as all at once, whichever sequences share a run
+    import tabicl_mi355_paged as paged
+    from parity import check
+    monkeypatch.setattr(paged, "_DENSE_SCORES", 1)
+    lengths = [40, 3000, 0, 700, 1, 5000, 64, 129]
+    c = paged.PagedIclKVCache(8, 1, 8, 64, 5000, 150, 64, BF, dev)
+    g = torch.Generator(device=dev).manual_seed(87)
+    k, v = (torch.randn(8, 8, 5000, 64, generator=g, device=dev).to(BF) for _ in range(2))
+    c.append(0, k, v, lengths)
+    q = torch.randn(8, 300, 8, 64, generator=g, device=dev).to(BF).transpose(1, 2)
+    for rows in (1, 1500, 8000):
+        monkeypatch.setattr(paged, "_GATHER_BYTES", rows * 2 * 8 * 64 * 2)
+        got, out = c.query(0, q), torch.zeros(8, 300, 8, 64, dtype=BF, device=dev)
+        c.query(0, q, None, out.transpose(1, 2))
+        over = q.clone()
+        c.query(0, over, None, over)
+        torch.cuda.synchronize()
+        assert torch.equal(out.transpose(1, 2), got) and torch.equal(over, got)
+        for s, n in enumerate(lengths):
+            if n == 0:
+                assert (got[s] == 0).all()
+            else:
+                p = torch.softmax(q[s].double() @ k[s, :, :n].double().transpose(1, 2) / 8, -1)
+                check(got[s], p @ v[s, :, :n].double(), BF, f"sequence {s}, runs of {rows} rows")

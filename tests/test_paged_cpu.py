@@ -362,3 +362,48 @@ def test_query_rows_beyond_one_launch():
     assert size(8, 8, 8, 1 << 20, 64, 45056, 0, 0) > 0
     for n in ((8, 8, 8, (1 << 20) + 1, 64, 45056, 0, 0), (1, 1, 1, (1 << 22) + 1, 64, 64, 0, 0), (65535, 128, 1, 1, 64, 64, 0, 0)):
         assert size(*n) < 0 and "query rows" in nat.last_error()
+
+
+def test_gather_of_ragged_tables_is_bounded(plain, monkeypatch):
+    # one long table among short ones: K and V side by side never take more than the bound, except a single table's own
+    lengths = [3, 0, 900, 20, 1, 300, 300, 300, 7]
+    c = plain.PagedIclKVCache(9, 1, 2, 64, 1000, 150, 16, torch.bfloat16, "cpu")
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(9, 2, 900, 64, generator=g).bfloat16() for _ in range(2))
+    c.append(0, k, v, lengths)
+    row, taken = 2 * 2 * 64 * 2, []
+
+    def gather(kp, vp, table, n, rows):
+        taken.append((table.shape[0], table.shape[0] * rows * row))
+        out = [torch.full((table.shape[0], 2, rows, 64), float("nan"), dtype=torch.bfloat16) for _ in range(2)]
+        for s in range(table.shape[0]):
+            at, page, r = ref.rows_of(table[s], min(int(n[s]), rows), 16, kp.shape[0])
+            for o, pages in zip(out, (kp, vp)):
+                o[s][:, at] = pages[page, :, r].transpose(0, 1)
+        return out
+
+    def dense(q, kd, vd, n, out):
+        o = torch.zeros(q.shape, dtype=q.dtype)
+        for s in range(len(n)):
+            m = int(n[s])
+            if m:
+                p = torch.softmax(q[s].double() @ kd[s, :, :m].double().transpose(1, 2) / 8, -1)
+                o[s] = (p @ vd[s, :, :m].double()).to(q.dtype)
+        return o if out is None else out.copy_(o)
+
+    monkeypatch.setattr(plain, "paged_gather", gather)
+    monkeypatch.setattr(plain.PagedIclKVCache, "_dense", staticmethod(dense))
+    monkeypatch.setattr(plain, "_DENSE_SCORES", 1)
+    monkeypatch.setattr(plain, "_GATHER_BYTES", 700 * row, raising=False)
+    q = torch.randn(9, 300, 2, 64, generator=g).bfloat16().transpose(1, 2)
+    for valid in (None, 250, torch.tensor([900, 9, 700, 2, 2, 2, 300, 300, 300])):
+        taken.clear()
+        want = [min(n, 900 if valid is None else int(valid) if not torch.is_tensor(valid) else int(valid[s])) for s, n in
+                enumerate(lengths)]
+        buf = torch.zeros(9, 300, 2, 64, dtype=torch.bfloat16)
+        got = c.query(0, q, valid)
+        assert c.query(0, q, valid, buf.transpose(1, 2)).data_ptr() == buf.data_ptr()
+        assert torch.equal(got, buf.transpose(1, 2))
+        assert all(size <= 700 * row or n == 1 for n, size in taken), taken
+        for s, n in enumerate(want):
+            assert torch.equal(got[s], dense(q[s:s + 1], k[s:s + 1], v[s:s + 1], [n], None)[0]), (valid, s)
