@@ -500,9 +500,13 @@ class PagedIclKVCache(_icl.IclKVCache):
     def query(self, block: int, q: Tensor, valid_kv_len: Optional[Union[int, Tensor]] = None,
               out: Optional[Tensor] = None) -> Tensor:
         """Attention of q [sequences, H, Tq, d] over `block` of the cache: each sequence's own rows, of those the ones
-        below valid_kv_len if given (a number, or one per sequence). q in the cache's dtype or one that widens to it. No
+        below valid_kv_len if given (a number, or a tensor of one for all or one per sequence). q in the cache's dtype or one
+        that widens to it, its heads as many as the cache's or a multiple (head h reads head h // (Hq // H) of the cache). No
         gradient, however many query rows there are."""
         _no_grad("PagedIclKVCache.query", q, out)
+        S, (_, _, H, _, D) = self.table.shape[0], self.keys.shape
+        if q.dim() != 4 or q.shape[0] != S or q.shape[1] == 0 or q.shape[1] % H or q.shape[3] != D:
+            raise ValueError(f"query expects q [{S}, {H} heads or a multiple, Tq, {D}], got {tuple(q.shape)}")
         lengths = self.default_valid(block)
         longest = max(self._lengths_of(block))
         if isinstance(valid_kv_len, Tensor):
@@ -517,8 +521,8 @@ class PagedIclKVCache(_icl.IclKVCache):
         w = max(1, -(-longest // self.page_rows))
         if self.keys.is_cuda and torch.cuda.is_current_stream_capturing():
             w = self.table.shape[1]  # a replay meets the lengths of its time, not today's
-        elif q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and q.shape[3] == 64 \
-                and dt == torch.bfloat16 and self.weights is None:
+        elif q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and D == 64 \
+                and q.shape[1] == H and dt == torch.bfloat16 and self.weights is None:
             return self._gathered(block, q.to(dt), lengths, longest, out)
         weights = None if self.weights is None else self.weights[:, :w * self.page_rows]
         return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out)

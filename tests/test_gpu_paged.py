@@ -954,3 +954,16 @@ def test_cache_many_query_rows_of_ragged_tables(dev, monkeypatch):
             else:
                 p = torch.softmax(q[s].double() @ k[s, :, :n].double().transpose(1, 2) / 8, -1)
                 check(got[s], p @ v[s, :, :n].double(), BF, f"sequence {s}, runs of {rows} rows")
+
+
+def test_cache_many_query_rows_of_grouped_heads(dev, monkeypatch):
+    # groups of query heads stay on the pages at any number of rows
+    import tabicl_mi355_paged as paged
+    monkeypatch.setattr(paged, "_DENSE_SCORES", 1)
+    c = paged.PagedIclKVCache(2, 1, 2, 64, 2000, 40, 64, BF, dev)
+    g = torch.Generator(device=dev).manual_seed(89)
+    k, v = (torch.randn(2, 2, 1100, 64, generator=g, device=dev).to(BF) for _ in range(2))
+    c.append(0, k, v, [1100, 90])
+    q = torch.randn(2, 6, 400, 64, generator=g, device=dev).to(BF)
+    want, _, tol, _ = ref.attention(q, c.keys[0], c.values[0], c.table, c.lengths[0], 0.125)
+    ref.near(c.query(0, q), want, tol, "grouped heads")

@@ -407,3 +407,22 @@ def test_gather_of_ragged_tables_is_bounded(plain, monkeypatch):
         assert all(size <= 700 * row or n == 1 for n, size in taken), taken
         for s, n in enumerate(want):
             assert torch.equal(got[s], dense(q[s:s + 1], k[s:s + 1], v[s:s + 1], [n], None)[0]), (valid, s)
+
+
+@pytest.mark.parametrize("T", [1, 300])
+def test_query_shapes(plain, monkeypatch, T):
+    # the same heads at every number of query rows: groups of them too, and a refusal that names what is expected
+    monkeypatch.setattr(plain, "_DENSE_SCORES", 1)
+    c = plain.PagedIclKVCache(2, 1, 2, 64, 64, 8, 16, torch.bfloat16, "cpu")
+    g = torch.Generator().manual_seed(6)
+    k, v = (torch.randn(2, 2, 40, 64, generator=g).bfloat16() for _ in range(2))
+    c.append(0, k, v, [40, 7])
+    q = torch.randn(2, 6, T, 64, generator=g).bfloat16()
+    got = c.query(0, q)
+    for s, n in enumerate((40, 7)):
+        for h in range(6):
+            p = torch.softmax(q[s, h].double() @ k[s, h // 3, :n].double().t() / 8, -1)
+            assert torch.equal(got[s, h], (p @ v[s, h // 3, :n].double()).to(q.dtype))
+    for shape in ((3, 2, T, 64), (1, 2, T, 64), (2, 3, T, 64), (2, 0, T, 64), (2, 1, T, 64), (2, 2, T, 32), (2, 2, 64), (T, 64)):
+        with pytest.raises(ValueError, match="query expects"):
+            c.query(0, torch.zeros(shape, dtype=torch.bfloat16))
