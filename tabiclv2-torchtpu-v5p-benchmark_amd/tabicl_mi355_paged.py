@@ -440,8 +440,9 @@ class PagedIclKVCache(_icl.IclKVCache):
         return self._lengths_of(block)[sequence]
 
     def default_valid(self, block: int) -> Tensor:
-        """The block's filled lengths as the int32 device tensor the kernels take."""
-        if not any(self._lengths_of(block)):
+        """The block's filled lengths as the int32 device tensor the kernels take (of a view too: a table without rows
+        answers 0 as long as another one of the cache it shows has some)."""
+        if not any(self._root._rows[block]):
             raise ValueError(f"block {block} of the cache has no rows: append before querying")
         return self.lengths[block]
 

@@ -967,3 +967,27 @@ def test_cache_many_query_rows_of_grouped_heads(dev, monkeypatch):
     q = torch.randn(2, 6, 400, 64, generator=g, device=dev).to(BF)
     want, _, tol, _ = ref.attention(q, c.keys[0], c.values[0], c.table, c.lengths[0], 0.125)
     ref.near(c.query(0, q), want, tol, "grouped heads")
+
+
+@pytest.mark.parametrize("T", [3, 400])
+def test_cache_chunks_of_empty_tables(dev, T, monkeypatch):
+    # query_chunked over chunks with and without rows equals one query over all of them
+    import tabicl_mi355_icl as icl
+    import tabicl_mi355_paged as paged
+    monkeypatch.setattr(paged, "_DENSE_SCORES", 1)
+    g = torch.Generator(device=dev).manual_seed(91)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    blocks = [icl.IclBlockWeights(r(512), r(512), (r(1536, 512) / 22).to(BF), None, (r(512, 512) / 22).to(BF), None, r(512), r(512),
+                                  (r(1024, 512) / 22).to(BF), None, (r(512, 1024) / 32).to(BF), None) for _ in range(2)]
+    c = paged.PagedIclKVCache(4, 2, 8, 64, 300, 30, 64, BF, dev)
+    for b in range(2):
+        c.append(b, r(4, 8, 300, 64).to(BF), r(4, 8, 300, 64).to(BF), [300, 0, 50, 0])
+    c.release(2)
+    x = r(4, T, 512)
+    with torch.no_grad():
+        want = c.query_blocks(x, blocks)
+        for chunks in ([(0, 1), (1, 2), (2, 4)], [(0, 2), (2, 3), (3, 4)]):
+            got = c.query_chunked(x, blocks, chunks)
+            torch.cuda.synchronize()
+            assert torch.allclose(got, want, rtol=2.0 ** -6, atol=2.0 ** -6 * float(want.abs().max()))
+            assert torch.isfinite(got).all()

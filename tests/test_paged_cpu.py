@@ -426,3 +426,23 @@ def test_query_shapes(plain, monkeypatch, T):
     for shape in ((3, 2, T, 64), (1, 2, T, 64), (2, 3, T, 64), (2, 0, T, 64), (2, 1, T, 64), (2, 2, T, 32), (2, 2, 64), (T, 64)):
         with pytest.raises(ValueError, match="query expects"):
             c.query(0, torch.zeros(shape, dtype=torch.bfloat16))
+
+
+def test_chunks_of_empty_tables(plain):
+    # a chunk without a row answers as the whole query does: 0
+    c = _cache(plain)
+    g = torch.Generator().manual_seed(7)
+    k, v = (torch.randn(3, 2, 20, 32, generator=g) for _ in range(2))
+    for b in range(2):
+        c.append(b, k, v, [20, 0, 5])
+    c.release(2)
+    q = torch.randn(3, 2, 4, 32, generator=g)
+    want = c.query(1, q)
+    assert (want[1:] == 0).all() and (want[0] != 0).any()
+    for a, b in ((0, 1), (1, 2), (2, 3), (1, 3)):
+        assert torch.equal(c.estimators(a, b).query(1, q[a:b]), want[a:b])
+    views = [c.estimators(s, s + 1) for s in range(3)]
+    c.release(0)  # nothing left: refused, by the cache and by its views
+    for x, y in [(c, q)] + [(w, q[:1]) for w in views]:
+        with pytest.raises(ValueError, match="append before"):
+            x.query(1, y)
