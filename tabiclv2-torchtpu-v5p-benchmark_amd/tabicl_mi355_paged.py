@@ -400,8 +400,8 @@ class PagedIclKVCache(_icl.IclKVCache):
     [sequences, capacity]); evict(keep) cuts the sequences to their heaviest rows and returns the emptied pages.
 
     Pages are given out on the host; the page table and the lengths live on the GPU, so a query costs no host sync. Calls
-    follow each other on one stream. Only queries without a number for valid_kv_len can be captured in a graph and replayed as
-    the cache grows (the other calls keep books on the host)."""
+    follow each other on one stream. Only queries can be captured in a graph and replayed as the cache grows (the other calls
+    keep books on the host)."""
 
     def __init__(self, sequences: int, blocks: int, heads: int, head_dim: int, max_rows: int, pages: int,
                  page_rows: int = 64, dtype: torch.dtype = torch.bfloat16, device: Union[str, torch.device] = "cuda",
@@ -510,18 +510,19 @@ class PagedIclKVCache(_icl.IclKVCache):
             raise ValueError(f"query expects q [{S}, {H} heads or a multiple, Tq, {D}], got {tuple(q.shape)}")
         lengths = self.default_valid(block)
         longest = max(self._lengths_of(block))
+        captured = self.keys.is_cuda and torch.cuda.is_current_stream_capturing()  # a replay meets the lengths of its time
         if isinstance(valid_kv_len, Tensor):
             lengths = torch.minimum(valid_kv_len.to(device=lengths.device, dtype=torch.int32).reshape(-1).expand_as(lengths),
                                     lengths)
-        elif valid_kv_len is not None and int(valid_kv_len) < longest:
-            longest = max(0, int(valid_kv_len))
+        elif valid_kv_len is not None and (captured or int(valid_kv_len) < longest):
+            longest = max(0, min(int(valid_kv_len), self.capacity))
             lengths = lengths.clamp(max=longest)
         dt = self.keys.dtype
         if torch.promote_types(q.dtype, dt) != dt:
             raise ValueError(f"q is {q.dtype}, wider than the {dt} cache: cast it")
         w = max(1, -(-longest // self.page_rows))
-        if self.keys.is_cuda and torch.cuda.is_current_stream_capturing():
-            w = self.table.shape[1]  # a replay meets the lengths of its time, not today's
+        if captured:
+            w = self.table.shape[1]
         elif q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and D == 64 \
                 and q.shape[1] == H and dt == torch.bfloat16 and self.weights is None:
             return self._gathered(block, q.to(dt), lengths, longest, out)

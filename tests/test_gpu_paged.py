@@ -991,3 +991,33 @@ def test_cache_chunks_of_empty_tables(dev, T, monkeypatch):
             torch.cuda.synchronize()
             assert torch.allclose(got, want, rtol=2.0 ** -6, atol=2.0 ** -6 * float(want.abs().max()))
             assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("T", [2, 300])
+def test_cache_query_with_a_limit_in_a_graph(dev, T, monkeypatch):
+    # a number for valid_kv_len holds in every replay, also where the cache was shorter when the query was captured
+    import tabicl_mi355_paged as paged
+    monkeypatch.setattr(paged, "_DENSE_SCORES", 1)
+    g = torch.Generator(device=dev).manual_seed(93)
+    c = paged.PagedIclKVCache(2, 1, 8, 64, 1000, 40, 64, BF, dev, track=T == 2)
+    rows = lambda n: torch.randn(2, 8, n, 64, generator=g, device=dev).to(BF)  # noqa: E731
+    c.append(0, rows(90), rows(90), [90, 60])
+    q = rows(T)
+    for limit in (200, 250, 75, 10 ** 12, 0):
+        c.query(0, q, limit)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = c.query(0, q, limit)
+        c.append(0, rows(150), rows(150), [150, 20])
+        for _ in range(2):
+            q.copy_(rows(T))
+            before = None if c.weights is None else c.weights.clone()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            n = c.lengths[0].clamp(max=min(limit, 1000))
+            want, w, tol, wtol = ref.attention(q, c.keys[0], c.values[0], c.table, n, 0.125, before)
+            ref.near(out, want, tol, f"limit {limit}")
+            if before is not None:
+                ref.near(c.weights, w, wtol, f"limit {limit}, weights")
