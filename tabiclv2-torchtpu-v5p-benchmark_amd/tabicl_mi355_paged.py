@@ -446,9 +446,14 @@ class PagedIclKVCache(_icl.IclKVCache):
             raise ValueError(f"block {block} of the cache has no rows: append before querying")
         return self.lengths[block]
 
+    def _capturing(self) -> bool:
+        return self.keys.is_cuda and torch.cuda.is_current_stream_capturing()
+
     def _own(self, what: str) -> None:
         if self._root is not self:
             raise ValueError(f"{what}: a view of some of a cache's estimators answers queries only")
+        if self._capturing():  # a replay would repeat what it did on the GPU and not what it wrote down here
+            raise ValueError(f"{what} keeps books on the host: only queries can be captured in a graph")
 
     def reserve(self, rows: Union[int, Sequence[int]]) -> None:
         """Pages for sequences of up to `rows` rows (a number, or one per sequence), given out now rather than by the
@@ -510,7 +515,7 @@ class PagedIclKVCache(_icl.IclKVCache):
             raise ValueError(f"query expects q [{S}, {H} heads or a multiple, Tq, {D}], got {tuple(q.shape)}")
         lengths = self.default_valid(block)
         longest = max(self._lengths_of(block))
-        captured = self.keys.is_cuda and torch.cuda.is_current_stream_capturing()  # a replay meets the lengths of its time
+        captured = self._capturing()  # a replay meets the lengths of its time
         if isinstance(valid_kv_len, Tensor):
             lengths = torch.minimum(valid_kv_len.to(device=lengths.device, dtype=torch.int32).reshape(-1).expand_as(lengths),
                                     lengths)

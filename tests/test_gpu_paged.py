@@ -1021,3 +1021,29 @@ def test_cache_query_with_a_limit_in_a_graph(dev, T, monkeypatch):
             ref.near(out, want, tol, f"limit {limit}")
             if before is not None:
                 ref.near(c.weights, w, wtol, f"limit {limit}, weights")
+
+
+def test_cache_books_refuse_capture(dev):
+    # calls that keep books on the host are refused while a graph is captured, and change nothing
+    import tabicl_mi355_paged as paged
+    c = paged.PagedIclKVCache(2, 1, 8, 64, 500, 20, 64, BF, dev, track=True)
+    z = torch.zeros(2, 8, 10, 64, dtype=BF, device=dev)
+    c.append(0, z, z)
+    c.reserve(500)  # an append needs no page: nothing else would stop it
+    q = torch.ones(2, 8, 1, 64, dtype=BF, device=dev)
+    c.query(0, q)
+    before = [t.clone() for t in (c.table, c.lengths, c.weights)], c.free_pages
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.query(0, q)
+        for call in (lambda: c.append(0, z, z), lambda: c.append(0, z, z, [1, 0]), lambda: c.evict(4), lambda: c.release(0),
+                     lambda: c.reserve(20)):
+            with pytest.raises(ValueError, match="captured"):
+                call()
+    assert c.length(0, 0) == c.length(0, 1) == 10 and c.free_pages == before[1]
+    for t, b in zip((c.table, c.lengths, c.weights), before[0]):
+        assert torch.equal(t, b)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, c.query(0, q))
