@@ -517,8 +517,10 @@ class PagedIclKVCache(_icl.IclKVCache):
         longest = max(self._lengths_of(block))
         captured = self._capturing()  # a replay meets the lengths of its time
         if isinstance(valid_kv_len, Tensor):
-            lengths = torch.minimum(valid_kv_len.to(device=lengths.device, dtype=torch.int32).reshape(-1).expand_as(lengths),
-                                    lengths)
+            valid = valid_kv_len.to(lengths.device).reshape(-1).expand_as(lengths)
+            if valid.dtype is not torch.int32:  # compared in 64 bits: a cast first would wrap a number beyond 32 round
+                valid = valid.to(torch.int64).clamp(min=0)
+            lengths = torch.minimum(valid, lengths, out=torch.empty_like(lengths))
         elif valid_kv_len is not None and (captured or int(valid_kv_len) < longest):
             longest = max(0, min(int(valid_kv_len), self.capacity))
             lengths = lengths.clamp(max=longest)

@@ -446,3 +446,21 @@ def test_chunks_of_empty_tables(plain):
     for x, y in [(c, q)] + [(w, q[:1]) for w in views]:
         with pytest.raises(ValueError, match="append before"):
             x.query(1, y)
+
+
+def test_valid_lengths_of_other_types(plain):
+    # numbers beyond 32 bits mean no limit, as a tensor too
+    c = _cache(plain)
+    g = torch.Generator().manual_seed(8)
+    k, v = (torch.randn(3, 2, 20, 32, generator=g) for _ in range(2))
+    c.append(1, k, v, [20, 3, 5])
+    q = torch.randn(3, 2, 4, 32, generator=g)
+    free, cut = c.query(1, q), c.query(1, q, torch.tensor([4, 4, 4], dtype=torch.int32))
+    for big in (2 ** 63 - 1, 2 ** 31, 2 ** 32 + 4):
+        for valid in (big, torch.tensor(big), torch.tensor([big]), torch.tensor([big, 2 ** 40, 20])):
+            assert torch.equal(c.query(1, q, valid), free), valid
+    for valid in (4, torch.tensor([4]), torch.tensor([4, 4, 4]), torch.tensor([4, 2 ** 40, 4]).clamp(max=4),
+                  torch.tensor([4] * 3, dtype=torch.uint8), torch.tensor([4] * 3, dtype=torch.int16)):
+        assert torch.equal(c.query(1, q, valid), cut), valid
+    for none in (0, -1, torch.tensor(-2 ** 40), torch.tensor([0, -1, -2 ** 63])):
+        assert (c.query(1, q, none) == 0).all(), none
