@@ -22,6 +22,7 @@ from __future__ import annotations
 from typing import Optional, Sequence, Union
 
 import torch
+import torch.autograd.forward_ad as _fwd
 from torch import Tensor
 
 import tabicl_mi355_icl as _icl
@@ -174,6 +175,9 @@ def _(q, k_pages, v_pages, table, lengths, scale, out, weights):  # noqa: ANN001
 def _no_grad(what: str, *ts: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise ValueError(f"{what} has no gradient (a serving operator): detach its inputs or call it under no_grad")
+    # forward mode: an op without a formula would drop the tangent and say nothing
+    if getattr(_fwd, "_current_level", 0) >= 0 and any(t is not None and _fwd.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError(f"{what} has no gradient, nor one in forward mode (a serving operator): detach its inputs")
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor,

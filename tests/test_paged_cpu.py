@@ -464,3 +464,42 @@ def test_valid_lengths_of_other_types(plain):
         assert torch.equal(c.query(1, q, valid), cut), valid
     for none in (0, -1, torch.tensor(-2 ** 40), torch.tensor([0, -1, -2 ** 63])):
         assert (c.query(1, q, none) == 0).all(), none
+
+
+def test_forward_tangents_are_refused():
+    # as gradients in reverse mode are: none of the operators carries a tangent on
+    import torch.autograd.forward_ad as fw
+    import tabicl_mi355_native as nat
+    import tabicl_mi355_paged as paged
+    k, v = _pool()
+    t, n, q, w = _table(), torch.tensor([5, 9], dtype=torch.int32), torch.zeros(2, 2, 1, 64), torch.zeros(2, 48)
+    calls = {"q": lambda x: paged.paged_attention(x, k, v, t, n), "k_pages": lambda x: paged.paged_attention(q, x, v, t, n),
+             "v_pages": lambda x: paged.paged_attention(q, k, x, t, n), "weights": lambda x: paged.paged_attention(q, k, v, t, n, x),
+             "out": lambda x: paged.paged_attention(q, k, v, t, n, None, None, x), "k": lambda x: paged.paged_append(k, v, t, n, x, q),
+             "v": lambda x: paged.paged_append(k, v, t, n, q, x), "append": lambda x: paged.paged_append(x, v, t, n, q, q),
+             "gather": lambda x: paged.paged_gather(k, x, t, n, 3), "evict": lambda x: paged.paged_evict(x, v, t, n, w, 3),
+             "evict weights": lambda x: paged.paged_evict(k, v, t, n, x, 3)}
+    args = dict.fromkeys(("q", "out", "k", "v"), q) | dict.fromkeys(("weights", "evict weights"), w)
+    for name, call in calls.items():
+        x = args.get(name, k)
+        with fw.dual_level():
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="no gradient"):
+                    call(fw.make_dual(x.clone(), torch.ones_like(x)))
+            with pytest.raises(nat.NativeLibraryError):  # a level alone changes nothing
+                call(x)
+        with pytest.raises(ValueError, match="no gradient"):
+            torch.func.jvp(call, (x.clone(),), (torch.ones_like(x),))
+
+
+def test_query_refuses_forward_tangents(plain):
+    import torch.autograd.forward_ad as fw
+    c = plain.PagedIclKVCache(1, 1, 1, 64, 64, 4, 16, torch.float32, "cpu")
+    z = torch.zeros(1, 1, 8, 64)
+    c.append(0, z, z)
+    with fw.dual_level():
+        for T in (2, 2000):
+            q = torch.zeros(1, 1, T, 64)
+            with torch.no_grad(), pytest.raises(ValueError, match="no gradient"):
+                c.query(0, fw.make_dual(q, torch.ones_like(q)))
+            assert c.query(0, q).shape == q.shape
