@@ -19,10 +19,11 @@ position is not part of its key), which is what lets eviction fill the places of
 No counterpart in the reference, whose cache is one padded tensor per block (scripts/tabicl_tpu_bucketed.py:413-435)."""
 from __future__ import annotations
 
-from typing import Optional, Sequence, Union
+from typing import Callable, Optional, Sequence, Union
 
 import torch
 import torch.autograd.forward_ad as _fwd
+import torch.nn.functional as F
 from torch import Tensor
 
 import tabicl_mi355_icl as _icl
@@ -172,11 +173,15 @@ def _(q, k_pages, v_pages, table, lengths, scale, out, weights):  # noqa: ANN001
     return None
 
 
+def _fwd_level() -> int:
+    return getattr(_fwd, "_current_level", 0)
+
+
 def _no_grad(what: str, *ts: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise ValueError(f"{what} has no gradient (a serving operator): detach its inputs or call it under no_grad")
     # forward mode: an op without a formula would drop the tangent and say nothing
-    if getattr(_fwd, "_current_level", 0) >= 0 and any(t is not None and _fwd.unpack_dual(t).tangent is not None for t in ts):
+    if _fwd_level() >= 0 and any(t is not None and _fwd.unpack_dual(t).tangent is not None for t in ts):
         raise ValueError(f"{what} has no gradient, nor one in forward mode (a serving operator): detach its inputs")
 
 
@@ -562,6 +567,15 @@ class PagedIclKVCache(_icl.IclKVCache):
             del k, v  # before the next run's
             start = stop
         return o if out is None else out
+
+    def query_blocks(self, x: Tensor, blocks, valid_kv_len: Optional[Union[int, Tensor]] = None,  # noqa: ANN001
+                     q_transform: Optional[Callable[[Tensor], Tensor]] = None,
+                     activation: Callable[[Tensor], Tensor] = F.gelu) -> Tensor:
+        """IclKVCache.query_blocks over the pages. No gradient: the layers around the attention would pass on their own part
+        of it alone, so one of x or of any weight is refused here."""
+        if torch.is_grad_enabled() or _fwd_level() >= 0:
+            _no_grad("PagedIclKVCache.query_blocks", x, *(t for w in blocks for t in vars(w).values() if isinstance(t, Tensor)))
+        return super().query_blocks(x, blocks, valid_kv_len, q_transform, activation)
 
     def evict(self, keep: Union[int, Sequence[int]], recent: int = 0) -> Tensor:
         """Cuts each sequence to at most keep rows (a number, or one per sequence), in every block alike: its `recent`

@@ -1047,3 +1047,32 @@ def test_cache_books_refuse_capture(dev):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, c.query(0, q))
+
+
+def test_query_blocks_refuse_gradients(dev):
+    # of the rows and of any weight, in both modes: the layers between the attentions would drop them without a word
+    import torch.autograd.forward_ad as fw
+    import dataclasses
+    import tabicl_mi355_icl as icl
+    import tabicl_mi355_paged as paged
+    g = torch.Generator(device=dev).manual_seed(95)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    blocks = [icl.IclBlockWeights(r(512), r(512), (r(1536, 512) / 22).to(BF), None, (r(512, 512) / 22).to(BF), None, r(512), r(512),
+                                  (r(1024, 512) / 22).to(BF), None, (r(512, 1024) / 32).to(BF), None) for _ in range(2)]
+    c = paged.PagedIclKVCache(1, 2, 8, 64, 100, 4, 64, BF, dev)
+    for b in range(2):
+        c.append(b, r(1, 8, 100, 64).to(BF), r(1, 8, 100, 64).to(BF))
+    x = r(1, 5, 512)
+    want = c.query_blocks(x, blocks)
+    for name in (None, "ln1_w", "in_w", "out_w", "ln2_b", "ff2_w"):
+        other = blocks if name is None else [dataclasses.replace(blocks[0], **{name: getattr(blocks[0], name).clone().requires_grad_()}),
+                                             blocks[1]]
+        y = x.clone().requires_grad_() if name is None else x
+        with pytest.raises(ValueError, match="no gradient"):
+            c.query_blocks(y, other)
+        with pytest.raises(ValueError, match="no gradient"):
+            c.query_chunked(y, other, [(0, 1)])
+        with torch.no_grad():
+            assert torch.equal(c.query_blocks(y, other), want)
+    with fw.dual_level(), pytest.raises(ValueError, match="no gradient"):
+        c.query_blocks(fw.make_dual(x, torch.ones_like(x)), blocks)
