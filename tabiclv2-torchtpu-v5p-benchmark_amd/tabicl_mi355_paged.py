@@ -326,14 +326,10 @@ def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tens
             return _evict_launch(k_pages, v_pages, table, lengths, weights, keep, recent, keep_n, index, kept_weights, kept)
     B, cap = k_pages.shape[0], pool[2] * pool[5]
     K = min(keep, cap)
-    key = (N, K)
-    nbytes = _WS_BYTES.get(key)
-    if nbytes is None:
-        nbytes = int(_nat.load().tabicl_paged_evict_workspace_bytes(N, K))
-        if nbytes < 0:
-            raise _nat.UnsupportedShapeError(f"tabicl_paged_evict: {_nat.last_error()}")
-        _WS_BYTES[key] = nbytes = max(nbytes, 16)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=table.device)
+    nbytes = int(_nat.load().tabicl_paged_evict_workspace_bytes(N, K))  # not kept: K changes with the data
+    if nbytes < 0:
+        raise _nat.UnsupportedShapeError(f"tabicl_paged_evict: {_nat.last_error()}")
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=table.device)
     _nat.call("tabicl_paged_evict", k_pages.data_ptr(), v_pages.data_ptr(), B, k_pages.stride(0) if B > 1 else 0, *pool,
               lengths.data_ptr(), weights.data_ptr(), w_sn, None if keep_n is None else keep_n.data_ptr(), keep, recent,
               index.data_ptr(), K, kept_weights.data_ptr(), kept.data_ptr(), N, H, D, code, ws.data_ptr(), nbytes,

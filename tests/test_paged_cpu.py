@@ -503,3 +503,27 @@ def test_query_refuses_forward_tangents(plain):
             with torch.no_grad(), pytest.raises(ValueError, match="no gradient"):
                 c.query(0, fw.make_dual(q, torch.ones_like(q)))
             assert c.query(0, q).shape == q.shape
+
+
+def test_workspace_sizes_do_not_pile_up(monkeypatch):
+    # what is kept of workspace sizes has a bound, for evictions (whose sizes change with the data) as for queries
+    import tabicl_mi355_native as nat
+    import tabicl_mi355_paged as paged
+    monkeypatch.setattr(paged, "_WS_BYTES", {})
+    k, v = _pool()
+    t, n = _table(), torch.tensor([5, 9], dtype=torch.int32)
+    table = torch.zeros(2, 400, dtype=torch.int32)
+    monkeypatch.setattr(nat, "call", lambda *a: None)
+    monkeypatch.setattr(nat, "require_device", lambda *a: None)
+    monkeypatch.setattr(nat, "stream_of", lambda *a: 0)
+    monkeypatch.setattr(nat, "direct", lambda *a: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    w = torch.zeros(2, 6400)
+    for keep in range(5000):
+        paged.paged_evict(k, v, table, n, w, keep)
+        assert len(paged._WS_BYTES) <= 4096
+    for width in range(1, 400, 7):
+        for T in range(1, 90):
+            paged.paged_attention(torch.zeros(2, 2, T, 64), k, v, table[:, :width], n)
+        assert len(paged._WS_BYTES) <= 4096
