@@ -369,7 +369,7 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
     N, cap = table.shape[0], table.shape[1] * k_pages.shape[3] if k_pages.dim() == 5 else 0
     if isinstance(keep, Tensor):
         keep, keep_n = cap, keep
-    keep, recent = int(keep), int(recent)
+    keep, recent = min(int(keep), cap), min(int(recent), cap)  # the entry points take 64 bits
     index = table.new_empty(N, max(0, min(keep, cap)))
     kept_weights = weights.new_empty(N, cap)
     kept = table.new_empty(N)

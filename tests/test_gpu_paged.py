@@ -1076,3 +1076,11 @@ def test_query_blocks_refuse_gradients(dev):
             assert torch.equal(c.query_blocks(y, other), want)
     with fw.dual_level(), pytest.raises(ValueError, match="no gradient"):
         c.query_blocks(fw.make_dual(x, torch.ones_like(x)), blocks)
+
+
+@pytest.mark.parametrize("keep,recent", [(2 ** 64 + 5, 0), (10, 2 ** 64 + 1), (2 ** 63, 2 ** 63)])
+def test_evict_with_numbers_beyond_64_bits(dev, keep, recent):
+    # no limit, and all rows recent: not what is left of the number in 64 bits
+    q, kp, vp, table, n, g = _case(dev, 19, [40, 0, 64], H=2, R=16, D=32, blocks=2)
+    w = torch.rand(3, table.shape[1] * 16, generator=g, device=dev)
+    _evict(kp, vp, table, n, w, keep, recent, "huge numbers")
