@@ -735,8 +735,8 @@ __device__ __forceinline__ EvictSizes evict_sizes(const PagedEvict& a, int n) {
   return z;
 }
 
-// Three launches: the threshold (one workgroup per sequence), the ranks (a workgroup per 1,024 rows), the moves; the first two
-// are one where no sequence has more than 1,024 rows.
+// Three launches: the threshold (one workgroup per sequence), the ranks (a workgroup per 1,024 rows, or more rows where there
+// are many), the moves; the first two are one where no sequence has more than 1,024 rows.
 //
 // A row competes if it is none of the recent ones; it stays if its code is above the threshold, or equal to it and among the
 // first `even` such rows. With before(r) the rows that stay below row r, the i-th place to fill is the row r < cut that goes
@@ -824,16 +824,21 @@ __global__ __launch_bounds__(PE_NT) void paged_threshold_kernel(PagedEvict a, Ev
   if (threadIdx.x == 0) cuts[blockIdx.x] = e;
 }
 
-// Rows [1024 b, 1024 b + 1024) of sequence n, one per thread: what stays in place, the places to fill (holes [N, K], in
-// order) and the rows to move (tails [N, K], from the last one back), their number in moves[n]. ONE: the only block of its
-// sequence, which finds the threshold itself.
+// `span` blocks of 1,024 rows of sequence n, one row per thread at a time: what stays in place, the places to fill (holes
+// [N, K], in order) and the rows to move (tails [N, K], from the last one back), their number in moves[n]. ONE: the only block
+// of its sequence, which finds the threshold itself. Each workgroup counts the rows before its first one; the span keeps the
+// workgroups of a sequence to PE_GROUPS, and the time in proportion to the rows (2^22 rows 4.9 -> 2.0 ms, 2^24 61 -> 8.1,
+// against a span of one; 2^30, which the entry point takes, would run for minutes).
+constexpr int PE_GROUPS = 256;
+
 template <bool ONE>
 __global__ __launch_bounds__(PE_NT) void paged_ranks_kernel(PagedEvict a, const EvictCut* cuts, int32_t* holes, int32_t* tails,
-                                                            int32_t* moves) {
+                                                            int32_t* moves, int span) {
   __shared__ int sh[PE_NW];
-  const int n = blockIdx.y, tid = threadIdx.x, first = blockIdx.x * PE_NT, r = first + tid;
+  const int n = blockIdx.y, tid = threadIdx.x;
   const EvictSizes z = evict_sizes(a, n);
-  const int64_t cap = (int64_t)a.pool.max_pages << a.pool.shift;
+  const int64_t cap = (int64_t)a.pool.max_pages << a.pool.shift, start = (int64_t)blockIdx.x * span * PE_NT;
+  const int64_t stop = start + (int64_t)span * PE_NT;
   const int free_rows = z.len - z.recent, cut = z.kept;
   EvictCut e;
   if constexpr (ONE) e = evict_threshold(a, n, z);
@@ -845,13 +850,15 @@ __global__ __launch_bounds__(PE_NT) void paged_ranks_kernel(PagedEvict a, const 
     a.kept_lengths[n] = cut;
     if (cut == z.len) moves[n] = 0;
   }
-  if (r >= cut && r < a.K) index[r] = -1;
-  if (r >= cut && r < cap) kw[r] = 0.f;
-  if (first >= z.len) return;
-  // the rows before the block: those above the threshold, and those equal to it
+  for (int64_t r = start + tid; r < stop; r += PE_NT) {
+    if (r >= cut && r < a.K) index[r] = -1;
+    if (r >= cut && r < cap) kw[r] = 0.f;
+  }
+  if (start >= z.len) return;
+  // the rows before: those above the threshold, and those equal to it
   int more = 0, even = 0;
   each_code(
-      first < free_rows ? first : free_rows, [&](int i) { return weight_code(w[i]); },
+      start < free_rows ? (int)start : free_rows, [&](int i) { return weight_code(w[i]); },
       [&](int, uint32_t c) {
         more += c > e.threshold;
         even += c == e.threshold;
@@ -859,26 +866,36 @@ __global__ __launch_bounds__(PE_NT) void paged_ranks_kernel(PagedEvict a, const 
   int more_before, even_before;
   wave_offset(__builtin_amdgcn_readlane(wave_sum_scan(more), 63), sh, &more_before);
   wave_offset(__builtin_amdgcn_readlane(wave_sum_scan(even), 63), sh, &even_before);
-  const float x = r < z.len ? w[r] : 0.f;
-  const uint32_t c = r < free_rows ? weight_code(x) : 0;
-  int all;
-  const uint64_t evens = __ballot(r < free_rows && c == e.threshold);
-  const int even_rank = even_before + wave_offset(__popcll(evens), sh, &all) + lanes_before(evens);
-  const bool keep = r < z.len && (r >= free_rows || c > e.threshold || (c == e.threshold && even_rank < e.even));
-  const uint64_t keeps = __ballot(keep);
-  const int before = more_before + (even_before < e.even ? even_before : e.even) + (first > free_rows ? first - free_rows : 0) +
-                     wave_offset(__popcll(keeps), sh, &all) + lanes_before(keeps);
-  if (r >= z.len) return;
-  if (r < cut) {
-    if (keep) {
-      index[r] = r;
-      kw[r] = x;
-    } else {
-      holes[(int64_t)n * a.K + r - before] = r;
+  const int end = stop < z.len ? (int)stop : z.len;
+  for (int first = (int)start; first < end; first += PE_NT) {
+    const int r = first + tid;
+    const float x = r < z.len ? w[r] : 0.f;
+    const uint32_t c = r < free_rows ? weight_code(x) : 0;
+    int all, evens_here;
+    const uint64_t evens = __ballot(r < free_rows && c == e.threshold);
+    const int even_rank = even_before + wave_offset(__popcll(evens), sh, &evens_here) + lanes_before(evens);
+    const bool keep = r < z.len && (r >= free_rows || c > e.threshold || (c == e.threshold && even_rank < e.even));
+    const uint64_t keeps = __ballot(keep);
+    const int before = more_before + (even_before < e.even ? even_before : e.even) +
+                       (first > free_rows ? first - free_rows : 0) + wave_offset(__popcll(keeps), sh, &all) + lanes_before(keeps);
+    if (r < z.len) {
+      if (r < cut) {
+        if (keep) {
+          index[r] = r;
+          kw[r] = x;
+        } else {
+          holes[(int64_t)n * a.K + r - before] = r;
+        }
+      } else {
+        if (r == cut) moves[n] = cut - before;
+        if (keep) tails[(int64_t)n * a.K + cut - 1 - before] = r;
+      }
     }
-  } else {
-    if (r == cut) moves[n] = cut - before;
-    if (keep) tails[(int64_t)n * a.K + cut - 1 - before] = r;
+    if (first + PE_NT < end) {  // the next block's rows before
+      wave_offset(__popcll(__ballot(r < free_rows && c > e.threshold)), sh, &all);
+      more_before += all;
+      even_before += evens_here;
+    }
   }
 }
 
@@ -1137,12 +1154,14 @@ int tabicl_launch_paged_evict(const PagedEvict& a, int dtype, void* ws, hipStrea
   int32_t* holes = (int32_t*)at;
   int32_t* tails = (int32_t*)(at + align256((int64_t)a.N * a.K * 4));
   const int64_t rows = (int64_t)a.pool.max_pages << a.pool.shift;
-  const dim3 blocks((unsigned)((rows + PE_NT - 1) / PE_NT), (unsigned)a.N), nt(PE_NT);
+  const int64_t blocks = (rows + PE_NT - 1) / PE_NT, span = (blocks + PE_GROUPS - 1) / PE_GROUPS;
+  const dim3 nt(PE_NT);
   if (rows <= PE_NT) {
-    hipLaunchKernelGGL(paged_ranks_kernel<true>, dim3(1, (unsigned)a.N), nt, 0, stream, a, cuts, holes, tails, moves);
+    hipLaunchKernelGGL(paged_ranks_kernel<true>, dim3(1, (unsigned)a.N), nt, 0, stream, a, cuts, holes, tails, moves, 1);
   } else {
     hipLaunchKernelGGL(paged_threshold_kernel, dim3((unsigned)a.N), nt, 0, stream, a, cuts);
-    hipLaunchKernelGGL(paged_ranks_kernel<false>, blocks, nt, 0, stream, a, cuts, holes, tails, moves);
+    hipLaunchKernelGGL(paged_ranks_kernel<false>, dim3((unsigned)((blocks + span - 1) / span), (unsigned)a.N), nt, 0, stream, a,
+                       cuts, holes, tails, moves, (int)span);
   }
   if (a.K > 0) {
     const int64_t per = (int64_t)a.K * a.pool.H * (a.pool.D * es / 16);

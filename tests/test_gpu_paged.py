@@ -1084,3 +1084,37 @@ def test_evict_with_numbers_beyond_64_bits(dev, keep, recent):
     q, kp, vp, table, n, g = _case(dev, 19, [40, 0, 64], H=2, R=16, D=32, blocks=2)
     w = torch.rand(3, table.shape[1] * 16, generator=g, device=dev)
     _evict(kp, vp, table, n, w, keep, recent, "huge numbers")
+
+
+@pytest.mark.parametrize("lengths,keep,recent", [([300001, 5], 292000, 40000), ([262145, 262144, 600000], 262100, 3),
+                                                 ([530000], 520000, 0)])
+def test_evict_of_very_long_sequences(dev, lengths, keep, recent):
+    # beyond 262,144 rows a workgroup ranks several blocks of 1,024 rows: many ties at the threshold, recent rows from the
+    # middle of a block on
+    q, kp, vp, table, n, g = _case(dev, 23, lengths, H=1, R=256, D=32, blocks=1)
+    w = torch.randint(0, 40, (len(lengths), table.shape[1] * 256), generator=g, device=dev).float()
+    _evict(kp, vp, table, n, w, keep, recent, "very long")
+
+
+def test_evict_time_grows_with_the_rows(dev):
+    # four times the rows in about four times the time, not sixteen (twice the linear time is allowed)
+    import tabicl_mi355_paged as paged
+
+    def us(rows):
+        pool = torch.zeros(1, 1, 1, 1024, 32, dtype=BF, device=dev)
+        table = torch.full((1, rows // 1024), -1, dtype=torch.int32, device=dev)  # the ranks' time, without moves
+        n = torch.tensor([rows], dtype=torch.int32, device=dev)
+        w = torch.rand(1, rows, device=dev)
+        best = float("inf")
+        for _ in range(4):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            paged.paged_evict(pool, pool.clone(), table, n, w, 16)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, start.elapsed_time(end) * 1e3)
+        return best
+
+    few, many = us(1 << 22), us(1 << 24)
+    print(f"[paged] eviction of 2^22 rows {few:.0f} us, of 2^24 {many:.0f}", flush=True)
+    assert many < 8 * few
