@@ -490,6 +490,7 @@ class PagedIclKVCache(_icl.IclKVCache):
             raise ValueError(f"append expects {self.keys.dtype} (cast before appending)")
         if not 0 <= block < NB:
             raise ValueError(f"block {block} out of range [0, {NB})")
+        _no_grad("PagedIclKVCache.append", k, v)
         _nat.require_device(k, v, self.keys)
         T = k.shape[2]
         new = [T] * S if rows is None else [int(r) for r in rows]

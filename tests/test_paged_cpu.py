@@ -527,3 +527,16 @@ def test_workspace_sizes_do_not_pile_up(monkeypatch):
         for T in range(1, 90):
             paged.paged_attention(torch.zeros(2, 2, T, 64), k, v, table[:, :width], n)
         assert len(paged._WS_BYTES) <= 4096
+
+
+def test_refused_append_takes_no_pages(plain):
+    c = _cache(plain)
+    k = torch.zeros(3, 2, 20, 32, requires_grad=True)
+    z = torch.zeros(3, 2, 20, 32)
+    for a, b in ((k, z), (z, k)):
+        with pytest.raises(ValueError, match="no gradient"):
+            c.append(0, a, b)
+    assert c.free_pages == 12 and (c.table == -1).all() and c.length(0, 0) == 0
+    with torch.no_grad():
+        c.append(0, k, k)
+    assert c.length(0, 2) == 20
