@@ -414,14 +414,15 @@ class PagedIclKVCache(_icl.IclKVCache):
         if page_rows < 16 or page_rows & (page_rows - 1):
             raise ValueError(f"page_rows must be a power of two from 16 on, got {page_rows}")
         width = -(-max_rows // page_rows)
-        self.keys = torch.empty(blocks, pages, heads, page_rows, head_dim, dtype=dtype, device=device)
-        self.values = torch.empty_like(self.keys)
+        with torch.inference_mode(False):  # tensors that calls in and outside of inference mode may change
+            self.keys = torch.empty(blocks, pages, heads, page_rows, head_dim, dtype=dtype, device=device)
+            self.values = torch.empty_like(self.keys)
+            self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
+            self.lengths = torch.zeros(blocks, sequences, dtype=torch.int32, device=device)
+            self.weights = torch.zeros(sequences, width * page_rows, dtype=torch.float32, device=device) if track else None
+            self._pages = torch.full((sequences, width), -1, dtype=torch.int32)  # the table's host copy
         self.page_rows = page_rows
         self.capacity = width * page_rows
-        self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
-        self.lengths = torch.zeros(blocks, sequences, dtype=torch.int32, device=device)
-        self.weights = torch.zeros(sequences, self.capacity, dtype=torch.float32, device=device) if track else None
-        self._pages = torch.full((sequences, width), -1, dtype=torch.int32)  # the table's host copy
         self._held = [0] * sequences  # pages a sequence holds
         self._rows = [[0] * sequences for _ in range(blocks)]  # the lengths' host copy
         self._free = list(range(pages - 1, -1, -1))

@@ -540,3 +540,19 @@ def test_refused_append_takes_no_pages(plain):
     with torch.no_grad():
         c.append(0, k, k)
     assert c.length(0, 2) == 20
+
+
+@pytest.mark.parametrize("inside", [True, False])
+def test_cache_built_in_inference_mode(plain, inside):
+    # built by a service's set-up in inference mode, filled and asked in or outside of it, as IclKVCache can be
+    with torch.inference_mode():
+        c = plain.PagedIclKVCache(2, 1, 2, 32, 60, 8, 16, torch.float32, "cpu", track=True)
+    g = torch.Generator().manual_seed(9)
+    with torch.inference_mode(inside):
+        k, v, q = (torch.randn(2, 2, 20, 32, generator=g) for _ in range(3))
+        c.append(0, k, v, [20, 4])
+        c.query(0, q)
+        c.evict(10)
+        c.release(1)
+        c.append(0, k, v)
+    assert c.lengths.tolist() == [[30, 20]] and c.free_pages == 8 - 2 - 2
