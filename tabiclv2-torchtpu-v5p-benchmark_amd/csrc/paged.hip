@@ -39,9 +39,15 @@ __device__ __forceinline__ int64_t pool_row(const PagedPool& c, int n, int h, in
 // One query row leaves 15 of the 16 columns empty: the products stay far below the loads all the same.
 // bf16 probabilities enter as two bf16 terms (2^-16 of each left out), so that the output is off by its own rounding
 // alone; the second product costs nothing beside the loads. fp32 runs on the fp32 matrix unit.
-// Softmax: p = 2^(s - ref) with ref the running maximum + PA_SHIFT, moved only when a score passes the maximum by more than
-// 2^PA_SLACK (one test per turn); the shift keeps sums of products with values near the largest float finite.
+// Softmax: p = 2^(s - ref), ref moved to the running maximum when a score passes it by more than PA_SLACK (one test per turn).
+// The products with V take 2^-24 p, so that sums with values near the largest float stay finite. bf16 has the 24 in ref,
+// where it costs no instruction and rounds the exponent to 2^-20; fp32 would lose four bits of a mild score by that, and
+// multiplies.
 constexpr float PA_SHIFT = 24.f, PA_SLACK = 8.f;
+template <typename T>
+struct PagedShift {
+  static constexpr float REF = sizeof(T) == 2 ? PA_SHIFT : 0.f, VALUE = sizeof(T) == 2 ? 1.f : 0x1p-24f;
+};
 constexpr float PA_REF0 = -3.4028234663852886e38f;
 
 // The work is cut on the device, by the lengths as they are: a unit is PA_UNIT rows of one item, units are counted item after
@@ -155,18 +161,29 @@ __device__ __forceinline__ void load_dwords(uint32_t* d, __amdgpu_buffer_rsrc_t 
   }
 }
 
-// The scores of 16 keys (chunks k of their rows) for 16 queries: key 4 (l / 16) + i, query l % 16.
+// The scores of 16 keys (chunks k of their rows) for 16 queries: key 4 (l / 16) + i, query l % 16. fp32 sums in four chains:
+// one of D products would be the largest rounding of all (2-norm of the output's error for sharp scores, D = 64 and 128:
+// 9.4e-7 and 1.1e-6 with one chain and the 24 in ref, 4.5e-7 this way; of mild ones 4.2e-7 and 1.8e-7).
 template <typename T, int NC>
 __device__ __forceinline__ f32x4 tile_scores(const uint4* k, const uint4* q) {
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (sizeof(T) == 2) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if constexpr (sizeof(T) == 2)
+    for (int c = 0; c < NC; ++c)
       s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[c]), __builtin_bit_cast(bf16x8, q[c]), s, 0, 0, 0);
-    else
-      s = mfma16x16x16(__builtin_bit_cast(f32x4, k[c]), __builtin_bit_cast(f32x4, q[c]), s);
+    return s;
+  } else {
+    f32x4 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, k[c])[i], __builtin_bit_cast(f32x4, q[c])[i], s[i], 0,
+                                                    0, 0);
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
   }
-  return s;
 }
 
 // A score in log2 units, rounded before the reference is taken off: the difference of the largest one is then exact, however
@@ -216,7 +233,7 @@ __device__ __forceinline__ void paged_values(const PagedTile<bf16, D>& t, const 
   }
 template <int D>
 __device__ __forceinline__ void paged_values(const PagedTile<float, D>& t, const float (*p)[4], f32x4* o) {
-  const f32x4 pv = {p[0][0], p[0][1], p[0][2], p[0][3]};
+  const f32x4 pv = f32x4{p[0][0], p[0][1], p[0][2], p[0][3]} * PagedShift<float>::VALUE;
 #pragma unroll
   for (int e = 0; e < D / 16; ++e) {
     const f32x4 va = {__uint_as_float(t.v[0][0][e]), __uint_as_float(t.v[0][1][e]), __uint_as_float(t.v[0][2][e]),
@@ -339,8 +356,8 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
                 f32x4{x[s][0], x[s][1], x[s][2], x[s][3]};
         }
       }
-      if (wave_any(top - ref[qt] > PA_SLACK - PA_SHIFT)) {
-        const float to = fmaxf(ref[qt], quad_max(top) + PA_SHIFT), f = __builtin_amdgcn_exp2f(ref[qt] - to);
+      if (wave_any(top - ref[qt] > PA_SLACK - PagedShift<T>::REF)) {
+        const float to = fmaxf(ref[qt], quad_max(top) + PagedShift<T>::REF), f = __builtin_amdgcn_exp2f(ref[qt] - to);
         ref[qt] = to;
         l[qt] *= f;
 #pragma unroll
@@ -408,12 +425,12 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
     for (int t = 0; t < QT; ++t) {
       const int r = (qt0 * QT + t) * 16 + lr;
       if (r >= rows) continue;
-      const float inv = slot >= 0 ? 1.f : l[t] == 0.f ? 0.f : 1.f / l[t];
+      const float inv = l[t] == 0.f ? 0.f : 1.f / l[t], out = slot >= 0 ? 1.f : inv * (1.f / PagedShift<T>::VALUE);
       float x[4 * DE];  // columns 4 DE lg + j of the row
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < DE; ++e) x[i * DE + e] = o[t][e][i] * inv;
+        for (int e = 0; e < DE; ++e) x[i * DE + e] = o[t][e][i] * out;
       if (slot >= 0) {
         const int64_t at = (int64_t)slot * 16 * QT + t * 16 + lr;
         store_row<float, 4 * DE>(z.part + at * D + lg * 4 * DE, x);
@@ -520,7 +537,7 @@ __device__ __forceinline__ void pa_merge_row(const PagedAttn& a, const PagedSpli
     for (int j = 0; j < 4; ++j) o[j] = o[j] * f0 + __shfl_xor(o[j], x, 64) * f1;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane < LPR) store4(op, o * inv);
+  if (lane < LPR) store4(op, o * (inv * (1.f / PagedShift<T>::VALUE)));
   if (z.stat && lane == 0) z.stat[row] = make_float2(m, inv);
 }
 

@@ -1118,3 +1118,33 @@ def test_evict_time_grows_with_the_rows(dev):
     few, many = us(1 << 22), us(1 << 24)
     print(f"[paged] eviction of 2^22 rows {few:.0f} us, of 2^24 {many:.0f}", flush=True)
     assert many < 8 * few
+
+
+@pytest.mark.parametrize("D,T,L", [(64, 4, 1381), (64, 24, 300), (128, 4, 1700), (128, 40, 2100), (32, 4, 40), (64, 2, 5)])
+@pytest.mark.parametrize("sharp", [0.5, 3.0])
+def test_fp32_accuracy(dev, D, T, L, sharp):
+    # In the 2-norm as near to float64 as scores whose products are summed in fp32 in four chains, with everything after them
+    # in float64: that is the rounding that cannot be avoided without more bits. A quarter on top for the chains' order, and
+    # 2^-23 for the exponential (one unit), the sums over the keys and the output's own rounding.
+    q, kp, vp, table, n, g = _case(dev, D + T, [L] * 4, D=D, T=T, dtype=F32, sharp=sharp)
+    import tabicl_mi355_paged as paged
+    w = torch.zeros(4, table.shape[1] * 64, device=dev)
+    out = paged.paged_attention(q, kp, vp, table, n, w)
+    want, ww, _, _ = ref.attention(q, kp, vp, table, n, D ** -0.5, torch.zeros_like(w))
+    four, fw = torch.zeros_like(want), torch.zeros_like(ww)
+    for s in range(4):
+        at, page, row = ref.rows_of(table[s], L, 64, kp.shape[0])
+        k, v = (t[page, :, row].transpose(0, 1).double() for t in (kp, vp))  # [H, L, D]
+        parts = []
+        for c in range(4):
+            acc = torch.zeros(8, T, L, device=dev)
+            for d in range(c, D, 4):
+                acc = (acc.double() + q[s, :, :, d, None].double() * k[:, None, :, d]).float()
+            parts.append(acc)
+        x = ((parts[0] + parts[1]) + (parts[2] + parts[3])).double()
+        p = torch.softmax(x * D ** -0.5, -1)
+        four[s], fw[s, :L] = torch.matmul(p, v), p.sum((0, 1))
+    for name, a, b, c in (("out", out, want, four), ("weights", w, ww, fw)):
+        err, least = (float((t.double() - b).norm() / b.norm()) for t in (a, c))
+        print(f"[paged] fp32 {name} D={D} T={T} L={L} sharp {sharp}: {err:.2e}, four chains {least:.2e}", flush=True)
+        assert err <= 1.25 * least + 2.0 ** -23, name
