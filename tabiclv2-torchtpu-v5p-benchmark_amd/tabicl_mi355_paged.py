@@ -198,7 +198,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
 
     The work is split over the cached rows, so one test row over one long table fills the GPU; a table slice
     table[:, :w] that covers the longest sequence spares the workgroups of pages nobody holds. For up to a few hundred
-    query rows (each group of 64 reads the cache again). No gradient."""
+    query rows (each group of 64 reads the cache again); with weights, more go in slices where the workspace would pass
+    1 GiB. No gradient."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, table, lengths, weights, out):
         o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
@@ -385,8 +386,10 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
 
 # PagedIclKVCache.query gathers a block's rows for the dense kernel, which shares each tile of K and V among 256 query rows,
 # from so many query rows and so many products of query rows and cached rows (per head) on. us in the pages / gathered, for
-# query rows T: 8 x 45,000 cached rows T 128 241 / 449, 256 438 / 462, 384 648 / 568, 5000 9164 / 3440; 8 x 5,000 rows 256
-# 72 / 69, 512 120 / 87; 1 x 20,000 rows 512 65 / 98, 1000 101 / 102; 8 x 700 rows 512 39 / 56, 5000 285 / 88.
+# query rows T: 8 x 45,000 cached rows T 192 419 / 450, 256 443 / 462, 257 644 / 549, 1000 1641 / 899; 40 x 100 to 20,000 256
+# 641 / 571; 8 x 5,000 256 68 / 64, 512 114 / 81; 8 x 20,000 256 208 / 207, 320 254 / 266, 384 299 / 265; 8 x 700 512 39 / 56,
+# 5000 285 / 88. One table alone has too few tiles for the dense kernel until about 1,000 rows: 1 x 45,000 384 89 / 185, 1000
+# 187 / 190.
 _DENSE_QUERY_ROWS, _DENSE_SCORES = 256, 1 << 24
 # Bytes of K and V that a gather puts side by side (more only for a single sequence of more): the sequences go in runs, each
 # padded to its own longest one. us of all at once / in runs of 2 GiB / 1 GiB, T 384: 16 x 45,000 rows 1246 / 1243 / 1262, one
@@ -515,7 +518,9 @@ class PagedIclKVCache(_icl.IclKVCache):
         """Attention of q [sequences, H, Tq, d] over `block` of the cache: each sequence's own rows, of those the ones
         below valid_kv_len if given (a number, or a tensor of one for all or one per sequence). q in the cache's dtype or one
         that widens to it, its heads as many as the cache's or a multiple (head h reads head h // (Hq // H) of the cache). No
-        gradient, however many query rows there are."""
+        gradient, however many query rows there are. The bf16 probabilities take part as two bf16 terms in the pages, and as
+        one where an untracked cache answers 256 rows and more (by many cached ones) with the dense kernel, as IclKVCache does:
+        up to 2^-8 of each value then."""
         _no_grad("PagedIclKVCache.query", q, out)
         S, (_, _, H, _, D) = self.table.shape[0], self.keys.shape
         if q.dim() != 4 or q.shape[0] != S or q.shape[1] == 0 or q.shape[1] % H or q.shape[3] != D:
@@ -577,8 +582,10 @@ class PagedIclKVCache(_icl.IclKVCache):
 
     def evict(self, keep: Union[int, Sequence[int]], recent: int = 0) -> Tensor:
         """Cuts each sequence to at most keep rows (a number, or one per sequence), in every block alike: its `recent`
-        last rows and the heaviest of the others (paged_evict by the tracked weights, which follow their rows). Pages
-        behind the kept rows, reserved ones too, go back to the pool. Returns index [sequences, K] int32: slot j now holds the old row index[s, j]."""
+        last rows and the heaviest of the others (paged_evict by the tracked weights, which follow their rows). Last are the
+        rows of the highest numbers: rows that an eviction moved into freed places are among the earlier ones from then on.
+        Pages behind the kept rows, reserved ones too, go back to the pool. Returns index [sequences, K] int32: slot j now
+        holds the old row index[s, j]."""
         self._own("evict")
         if self.weights is None:
             raise ValueError("evict needs a cache built with track=True")

@@ -1148,3 +1148,42 @@ def test_fp32_accuracy(dev, D, T, L, sharp):
         err, least = (float((t.double() - b).norm() / b.norm()) for t in (a, c))
         print(f"[paged] fp32 {name} D={D} T={T} L={L} sharp {sharp}: {err:.2e}, four chains {least:.2e}", flush=True)
         assert err <= 1.25 * least + 2.0 ** -23, name
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_cases(dev, seed):
+    # types, head layouts, page sizes, lengths, missing pages, weights, appends and budgets at random
+    import random
+    import tabicl_mi355_paged as paged
+    rng = random.Random(seed)
+    dtype, D, R = rng.choice([BF, F32]), rng.choice([32, 64, 128]), 1 << rng.randint(4, 9)
+    H, G, N = rng.choice([1, 2, 3, 8]), rng.choice([1, 1, 2, 5]), rng.choice([1, 2, 3, 7, 65, 130])
+    top = rng.choice([40, 1024, 1500, 6000, 20000]) if N < 8 else rng.choice([40, 300, 1500])
+    edges = [0, 1, 15, 16, 17, 127, 128, 129, 255, 256, 257, 1023, 1024, 1025, 2047, 2049]
+    lengths = [min(top, rng.choice(edges) if rng.random() < 0.3 else rng.randint(0, top)) for _ in range(N)]
+    T = rng.choice([1, 1, 2, 5, 17, 40, 70])
+    if max(lengths) * N * H * G * T > 3e7:
+        T = 1
+    q, kp, vp, table, n, g = _case(dev, seed, lengths, H=H, G=G, D=D, R=R, T=T, dtype=dtype, slack=rng.choice([0, 0, 3]),
+                                   sharp=rng.choice([0.3, 1.0, 4.0]))
+    whole = table.clone()
+    if rng.random() < 0.3:
+        gone = torch.randint(0, table.numel(), (max(1, table.numel() // 6),), generator=g, device=dev)
+        table.view(-1)[gone] = rng.choice([-1, kp.shape[0], 1 << 30])
+    w = torch.rand(N, table.shape[1] * R, generator=g, device=dev) * 0.1 if rng.random() < 0.6 else None
+    _attend(q, kp, vp, table, n, w, what=f"random {seed}")
+    if kp.numel() > 3e7:
+        return
+    new = rng.randint(1, 60)
+    k, v = (torch.randn(N, H, new, D, generator=g, device=dev).to(dtype) for _ in range(2))
+    want = ref.append(kp.cpu(), vp.cpu(), whole.cpu(), n.cpu(), k.cpu(), v.cpu())
+    paged.paged_append(kp, vp, whole, n, k, v)
+    torch.cuda.synchronize()
+    for got, x in zip((kp, vp), want):
+        assert torch.equal(got.cpu().view(torch.uint8), x.view(torch.uint8))
+    shape = (N, table.shape[1] * R)
+    weights = rng.choice([lambda: torch.rand(shape, generator=g, device=dev),
+                          lambda: torch.randint(0, 4, shape, generator=g, device=dev).float(),
+                          lambda: torch.exp(torch.randn(shape, generator=g, device=dev) * 20)])()
+    keep = rng.choice([rng.randint(0, top), torch.randint(-2, top + 5, (N,), generator=g, device=dev, dtype=torch.int32)])
+    _evict(kp[None], vp[None], whole, n, weights, keep, rng.choice([0, 0, 3, top]), f"random {seed}")
