@@ -579,8 +579,9 @@ class IclKVCache:
         if not chunks or chunks[0][0] != 0 or chunks[-1][1] != x.shape[0] or any(
                 a[1] != b[0] for a, b in zip(chunks, chunks[1:])):
             raise ValueError(f"chunks {chunks} do not cover the batch [0, {x.shape[0]}) in order")
-        parts = [self.estimators(a, b).query_blocks(x[a:b], blocks, valid_kv_len, q_transform, activation)
-                 for a, b in chunks]
+        each = isinstance(valid_kv_len, Tensor) and valid_kv_len.numel() == x.shape[0]  # a length per estimator
+        parts = [self.estimators(a, b).query_blocks(x[a:b], blocks, valid_kv_len.reshape(-1)[a:b] if each else valid_kv_len,
+                                                    q_transform, activation) for a, b in chunks]
         return parts[0] if len(parts) == 1 else torch.cat(parts, dim=0)
 
     def block_kv(self, block: int):

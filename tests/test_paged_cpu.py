@@ -556,3 +556,21 @@ def test_cache_built_in_inference_mode(plain, inside):
         c.release(1)
         c.append(0, k, v)
     assert c.lengths.tolist() == [[30, 20]] and c.free_pages == 8 - 2 - 2
+
+
+def test_chunks_with_a_valid_length_per_table(plain):
+    # one length per table goes to the chunks table by table, as one for all does
+    import tabicl_mi355_icl as icl
+    g = torch.Generator().manual_seed(10)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    blocks = [icl.IclBlockWeights(r(64), r(64), r(192, 64) / 8, None, r(64, 64) / 8, None, r(64), r(64), r(128, 64) / 8, None,
+                                  r(64, 128) / 11, None) for _ in range(2)]
+    c = _cache(plain, track=False)
+    for b in range(2):
+        c.append(b, r(3, 2, 20, 32), r(3, 2, 20, 32), [20, 11, 4])
+    x = r(3, 5, 64)
+    for valid in (None, 6, torch.tensor(6), torch.tensor([6]), torch.tensor([9, 2, 20]), torch.tensor([[9], [2], [20]])):
+        with torch.no_grad():
+            want = c.query_blocks(x, blocks, valid)
+            for chunks in ([(0, 3)], [(0, 1), (1, 3)], [(0, 1), (1, 2), (2, 3)]):
+                assert torch.allclose(c.query_chunked(x, blocks, chunks, valid), want, atol=1e-5), (valid, chunks)
