@@ -1187,3 +1187,26 @@ def test_random_cases(dev, seed):
                           lambda: torch.exp(torch.randn(shape, generator=g, device=dev) * 20)])()
     keep = rng.choice([rng.randint(0, top), torch.randint(-2, top + 5, (N,), generator=g, device=dev, dtype=torch.int32)])
     _evict(kp[None], vp[None], whole, n, weights, keep, rng.choice([0, 0, 3, top]), f"random {seed}")
+
+
+def test_slices_in_a_graph(dev):
+    # a call that goes in slices, captured: every replay adds its weights once
+    import tabicl_mi355_paged as paged
+    q, kp, vp, table, n, g = _case(dev, 97, [3000], H=8, T=12001)
+    w = torch.zeros(1, table.shape[1] * 64, device=dev)
+    paged.paged_attention(q, kp, vp, table, n, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged.paged_attention(q, kp, vp, table, n, w)
+    for step in range(3):
+        q.copy_(torch.randn(q.shape, generator=g, device=dev).to(BF))
+        n.fill_(3000 - 700 * step)
+        w.zero_()
+        want = paged.paged_attention(q, kp, vp, table, n, w)
+        ww = w.clone()
+        w.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(w, ww), step
