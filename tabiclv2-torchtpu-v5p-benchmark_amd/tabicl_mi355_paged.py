@@ -385,12 +385,14 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
 
 
 # PagedIclKVCache.query gathers a block's rows for the dense kernel, which shares each tile of K and V among 256 query rows,
-# from so many query rows and so many products of query rows and cached rows (per head) on. us in the pages / gathered, for
-# query rows T: 8 x 45,000 cached rows T 192 419 / 450, 256 443 / 462, 257 644 / 549, 1000 1641 / 899; 40 x 100 to 20,000 256
-# 641 / 571; 8 x 5,000 256 68 / 64, 512 114 / 81; 8 x 20,000 256 208 / 207, 320 254 / 266, 384 299 / 265; 8 x 700 512 39 / 56,
-# 5000 285 / 88. One table alone has too few tiles for the dense kernel until about 1,000 rows: 1 x 45,000 384 89 / 185, 1000
-# 187 / 190.
-_DENSE_QUERY_ROWS, _DENSE_SCORES = 256, 1 << 24
+# from so many query rows, so many of them over all sequences (it has too few tiles for the GPU below) and so many products of
+# query rows and cached rows (per head) on. us in the pages / gathered, for query rows T:
+#   8 x 45,000 cached rows T 192 419 / 450, 256 443 / 462, 257 644 / 549, 1000 1641 / 899; 40 x 100 to 20,000 256 641 / 571;
+#   8 x 5,000 256 68 / 64, 512 114 / 81; 8 x 20,000 256 208 / 207, 320 254 / 266, 384 299 / 265; 8 x 700 512 39 / 56,
+#   5000 285 / 88;
+#   1 x 45,000 384 87 / 186, 1000 184 / 192, 1500 266 / 194; 2 x 45,000 384 146 / 216, 512 184 / 217, 700 300 / 219;
+#   4 x 45,000 256 181 / 279, 384 281 / 304, 512 352 / 311; 1 x 200,000 700 674 / 808, 1000 804 / 797.
+_DENSE_QUERY_ROWS, _DENSE_ALL_ROWS, _DENSE_SCORES = 256, 1024, 1 << 24
 # Bytes of K and V that a gather puts side by side (more only for a single sequence of more): the sequences go in runs, each
 # padded to its own longest one. us of all at once / in runs of 2 GiB / 1 GiB, T 384: 16 x 45,000 rows 1246 / 1243 / 1262, one
 # table of 50,000 rows beside 63 of 500 752 (6.3 GB) / 514 / 507, 40 of 100 to 20,000 763 / 713 / 829.
@@ -519,8 +521,8 @@ class PagedIclKVCache(_icl.IclKVCache):
         below valid_kv_len if given (a number, or a tensor of one for all or one per sequence). q in the cache's dtype or one
         that widens to it, its heads as many as the cache's or a multiple (head h reads head h // (Hq // H) of the cache). No
         gradient, however many query rows there are. The bf16 probabilities take part as two bf16 terms in the pages, and as
-        one where an untracked cache answers 256 rows and more (by many cached ones) with the dense kernel, as IclKVCache does:
-        up to 2^-8 of each value then."""
+        one where an untracked cache answers 256 rows and more (1,024 over all sequences, by many cached ones) with the dense
+        kernel, as IclKVCache does: up to 2^-8 of each value then."""
         _no_grad("PagedIclKVCache.query", q, out)
         S, (_, _, H, _, D) = self.table.shape[0], self.keys.shape
         if q.dim() != 4 or q.shape[0] != S or q.shape[1] == 0 or q.shape[1] % H or q.shape[3] != D:
@@ -542,8 +544,9 @@ class PagedIclKVCache(_icl.IclKVCache):
         w = max(1, -(-longest // self.page_rows))
         if captured:
             w = self.table.shape[1]
-        elif q.shape[2] >= _DENSE_QUERY_ROWS and q.shape[0] * q.shape[2] * longest >= _DENSE_SCORES and D == 64 \
-                and q.shape[1] == H and dt == torch.bfloat16 and self.weights is None:
+        elif q.shape[2] >= _DENSE_QUERY_ROWS and S * q.shape[2] >= _DENSE_ALL_ROWS \
+                and S * q.shape[2] * longest >= _DENSE_SCORES and D == 64 and q.shape[1] == H and dt == torch.bfloat16 \
+                and self.weights is None:
             return self._gathered(block, q.to(dt), lengths, longest, out)
         weights = None if self.weights is None else self.weights[:, :w * self.page_rows]
         return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out)

@@ -964,7 +964,7 @@ def test_cache_many_query_rows_of_grouped_heads(dev, monkeypatch):
     g = torch.Generator(device=dev).manual_seed(89)
     k, v = (torch.randn(2, 2, 1100, 64, generator=g, device=dev).to(BF) for _ in range(2))
     c.append(0, k, v, [1100, 90])
-    q = torch.randn(2, 6, 400, 64, generator=g, device=dev).to(BF)
+    q = torch.randn(2, 6, 600, 64, generator=g, device=dev).to(BF)
     want, _, tol, _ = ref.attention(q, c.keys[0], c.values[0], c.table, c.lengths[0], 0.125)
     ref.near(c.query(0, q), want, tol, "grouped heads")
 

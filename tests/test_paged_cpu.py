@@ -409,7 +409,7 @@ def test_gather_of_ragged_tables_is_bounded(plain, monkeypatch):
             assert torch.equal(got[s], dense(q[s:s + 1], k[s:s + 1], v[s:s + 1], [n], None)[0]), (valid, s)
 
 
-@pytest.mark.parametrize("T", [1, 300])
+@pytest.mark.parametrize("T", [1, 600])
 def test_query_shapes(plain, monkeypatch, T):
     # the same heads at every number of query rows: groups of them too, and a refusal that names what is expected
     monkeypatch.setattr(plain, "_DENSE_SCORES", 1)
@@ -574,3 +574,17 @@ def test_chunks_with_a_valid_length_per_table(plain):
             want = c.query_blocks(x, blocks, valid)
             for chunks in ([(0, 3)], [(0, 1), (1, 3)], [(0, 1), (1, 2), (2, 3)]):
                 assert torch.allclose(c.query_chunked(x, blocks, chunks, valid), want, atol=1e-5), (valid, chunks)
+
+
+@pytest.mark.parametrize("S,T,gathered", [(1, 384, False), (1, 1023, False), (1, 1024, True), (2, 500, False), (2, 512, True),
+                                          (8, 128, False), (4, 256, True)])
+def test_few_query_rows_over_all_tables_stay_in_the_pages(plain, monkeypatch, S, T, gathered):
+    monkeypatch.setattr(plain, "_DENSE_SCORES", 1)
+    c = plain.PagedIclKVCache(S, 1, 1, 64, 16, S, 16, torch.bfloat16, "cpu")
+    z = torch.zeros(S, 1, 4, 64, dtype=torch.bfloat16)
+    c.append(0, z, z)
+    calls = []
+    monkeypatch.setattr(plain, "paged_gather", lambda kp, vp, table, n, rows: calls.append(rows) or (z[:, :, :rows],) * 2)
+    monkeypatch.setattr(plain.PagedIclKVCache, "_dense", staticmethod(lambda q, k, v, n, out: torch.zeros_like(q)))
+    q = torch.zeros(S, 1, T, 64, dtype=torch.bfloat16)
+    assert c.query(0, q).shape == q.shape and calls == [4] * gathered
