@@ -423,6 +423,7 @@ int tabicl_paged_gather(const void* k_pages, const void* v_pages, int64_t pages,
  * rows are not kept, in order; no other row moves. All blocks (element stride block_sp) move alike. Written:
  * index [N, K] (slot j holds the old row index[n, j]; -1 from kept on), kept_weights [N, max_pages * page_rows]
  * (weights of the kept rows in their slots, 0 after), kept_lengths [N]. weights, table and lengths stay as they are.
+ * Rows without a page are ranked like the others, and a kept row whose new place has no page is nowhere afterwards.
  * No page may stand in the table twice; kept_weights must not overlap weights. ws: tabicl_paged_evict_workspace_bytes(N, K)
  * bytes, 16-byte aligned (of K = 0 too).
  */

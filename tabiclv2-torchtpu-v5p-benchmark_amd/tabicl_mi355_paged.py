@@ -363,7 +363,8 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor
     below it; nothing else moves. Returns index [N, K] int32 (slot j holds the old row index[n, j], -1 from kept on; K =
     keep, or the capacity for a tensor), the weights in their new slots [N, max_pages page_rows] (0 past the cut) and
     kept [N] int32. weights, table and lengths are not changed: take over the new ones. No page may stand in the table
-    twice."""
+    twice. A row below the length whose page the pool does not have is ranked by its weight like any other; a kept row whose
+    new place has no page is nowhere afterwards."""
     if k_pages.dim() == 4 and v_pages.dim() == 4:
         k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
     keep_n = None
