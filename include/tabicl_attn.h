@@ -436,6 +436,101 @@ int tabicl_paged_evict(void* k_pages, void* v_pages, int64_t blocks, int64_t blo
 int64_t tabicl_paged_evict_workspace_bytes(int64_t N, int64_t K);
 
 /*
+ * Pools of 8-bit codes: value = code * scale, e4m3 (TABICL_CODE_E4M3) or int8 (TABICL_CODE_I8) codes in k_pages, v_pages as
+ * above (page_sp in codes), scales fp32 [pages, H, 2] (K, V), 8-byte aligned. A scale is a power of two: the smallest 2^k,
+ * k in [-60, 100], with max |x| <= Q 2^k over finite values (Q = 448 or 127). dtype: of q and out, of the rows written and read.
+ */
+#define TABICL_CODE_E4M3 0
+#define TABICL_CODE_I8 1
+
+/* tabicl_paged_attn over such a pool, without weights; the products are exact (fp32 queries and probabilities enter as three
+ * bf16 terms), the sums fp32. Any finite scales will do. */
+int tabicl_paged_attn_q8(const void* q, const void* k_pages, const void* v_pages, const float* scales, int64_t pages,
+                         int64_t page_sp, int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages,
+                         const int32_t* lengths, void* out, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t q_sn,
+                         int64_t q_sh, int64_t q_st, int64_t o_sn, int64_t o_sh, int64_t o_st, float scale, int32_t dtype,
+                         int32_t code, void* ws, int64_t ws_bytes, void* stream);
+int64_t tabicl_paged_attn_q8_workspace_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows,
+                                             int32_t dtype);
+
+/*
+ * tabicl_paged_append into such a pool: codes rounded to the nearest (ties to even), saturating; NaN stays NaN in e4m3 and
+ * becomes 0 in int8. A page that already holds rows of its sequence (lengths[n] lies inside it) takes the larger of its scale
+ * and the new rows'; where it grows, the held codes are rounded again. Other pages take the new rows' scale. starts (or NULL):
+ * k, v are packed [T, H, D] (k_sn, v_sn unused), row t of sequence n their row starts[n] + t; count is required then.
+ */
+int tabicl_paged_append_q8(void* k_pages, void* v_pages, float* scales, int64_t pages, int64_t page_sp, int64_t page_rows,
+                           const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const void* k,
+                           const void* v, const int32_t* count, const int32_t* starts, int64_t N, int64_t H, int64_t T, int64_t D,
+                           int64_t k_sn, int64_t k_sh, int64_t k_st, int64_t v_sn, int64_t v_sh, int64_t v_st, int32_t dtype,
+                           int32_t code, void* stream);
+/* tabicl_paged_gather of the values (bf16: exact). */
+int tabicl_paged_gather_q8(const void* k_pages, const void* v_pages, const float* scales, int64_t pages, int64_t page_sp,
+                           int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths,
+                           void* k, void* v, int64_t N, int64_t H, int64_t T, int64_t D, int32_t dtype, int32_t code,
+                           void* stream);
+
+/*
+ * Attention over selected pages. Pool formats: 0 bf16, 1 fp32, 2 e4m3, 3 int8 (with scales as above; NULL for 0 and 1).
+ *
+ * tabicl_paged_bounds: bounds int8 [pages, H, 2, D] (16-byte aligned) and bound_scales fp32 [pages, H] of the pages that hold
+ *   rows of the sequences, over the live rows of K: bounds[.., 0, :] = ceil(max / s), bounds[.., 1, :] = floor(min / s), s the
+ *   smallest 2^k, k in [-60, 100], with |max|, |min| <= 127 2^k where they are finite. Infinite ones become +-127; NaN does not
+ *   count. start (or NULL) [N]: only pages from row start[n] on, of up to `rows` rows from there.
+ * tabicl_paged_select: index [N, H, Tq, K] <- for each query row and K/V head the K pages (their places in the table, in
+ *   ascending order, -1 behind the last) of largest bound, ties to the lower page. bound = max over the group's heads of
+ *   sum_d (u_d hi_d where u_d > 0, else u_d lo_d) s with u = round(q / 2^j) in int8, 2^j one step of 127 for the query row (all heads of the
+ *   group; NaN 0, infinities +-127): whole numbers, so that the choice depends on no order of sums. Pages outside the pool are
+ *   not chosen. Workspace only where max_pages > 32768.
+ * tabicl_paged_sparse_attn: tabicl_paged_attn over the pages that index lists. Entries outside the table, and pages outside the
+ *   pool, hold no rows; any order will do, and a page listed twice counts twice.
+ */
+int tabicl_paged_bounds(const void* k_pages, const float* scales, int64_t pages, int64_t page_sp, int64_t page_rows,
+                        const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const int32_t* start,
+                        int64_t rows, int8_t* bounds, float* bound_scales, int64_t N, int64_t H, int64_t D, int32_t format,
+                        void* stream);
+int tabicl_paged_select(const void* q, const int8_t* bounds, const float* bound_scales, int64_t pages, int64_t page_rows,
+                        const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, int32_t* index,
+                        int64_t K, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t q_sn, int64_t q_sh,
+                        int64_t q_st, int32_t dtype, void* ws, int64_t ws_bytes, void* stream);
+int64_t tabicl_paged_select_workspace_bytes(int64_t N, int64_t H, int64_t Tq, int64_t max_pages);
+int tabicl_paged_sparse_attn(const void* q, const void* k_pages, const void* v_pages, const float* scales, int64_t pages,
+                             int64_t page_sp, int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages,
+                             const int32_t* lengths, const int32_t* index, int64_t K, void* out, int64_t N, int64_t Hq, int64_t H,
+                             int64_t Tq, int64_t D, int64_t q_sn, int64_t q_sh, int64_t q_st, int64_t o_sn, int64_t o_sh,
+                             int64_t o_st, float scale, int32_t dtype, int32_t format, void* ws, int64_t ws_bytes, void* stream);
+/* rows: K * page_rows. */
+int64_t tabicl_paged_sparse_attn_workspace_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows);
+
+/*
+ * The books of a pool on the device. free_pages [pages]: a stack of page ids, *free_count of them, the top one last.
+ *   tabicl_paged_reserve: pages for rows lengths[n] + t, t < count[n]: the table's entries from the first page behind row
+ *     lengths[n] to that of the last new row that hold no page get the pages from the top of the stack, sequence by sequence and
+ *     in order, as far as they go; granted[n] <- how many of the new rows have a place (before the first that has none).
+ *   tabicl_paged_release: the pages behind row lengths[n] of each sequence back on the stack (the last sequence's last page first: a
+ *     release of what a reserve gave out restores the stack), -1 in their place.
+ *   tabicl_paged_slots: starts [N + 1] <- running sums of the counts; slots [total] <- for row j of a packed batch, t = j -
+ *     starts[n] of sequence n, page * page_rows + row of its place lengths[n] + t in the pool, or -1 (no page; behind the last
+ *     row). The counts must add up to less than 2^31.
+ *   tabicl_paged_append_slots: row j of k, v [total, H, D] (element strides, contiguous last dim) to slot slots[j]; negative
+ *     slots, and those past the pool, are left out; no slot may stand twice. bf16 and fp32 pools.
+ * No page may stand in the tables or on the stack twice. ws of reserve and release: tabicl_paged_books_workspace_bytes(N).
+ */
+int tabicl_paged_reserve(int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const int32_t* count,
+                         const int32_t* free_pages, int32_t* free_count, int32_t* granted, int64_t pages, int64_t page_rows,
+                         int64_t N, void* ws, int64_t ws_bytes, void* stream);
+int tabicl_paged_release(int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, int32_t* free_pages,
+                         int32_t* free_count, int64_t pages, int64_t page_rows, int64_t N, void* ws, int64_t ws_bytes,
+                         void* stream);
+int64_t tabicl_paged_books_workspace_bytes(int64_t N);
+int tabicl_paged_slots(const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const int32_t* count,
+                       int64_t* slots, int32_t* starts, int64_t total, int64_t pages, int64_t page_rows, int64_t N,
+                       void* stream);
+int tabicl_paged_append_slots(void* k_pages, void* v_pages, int64_t pages, int64_t page_sp, int64_t page_rows,
+                              const int64_t* slots, const void* k, const void* v, int64_t total, int64_t H, int64_t D,
+                              int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int32_t dtype, void* stream);
+
+/*
  * Shape predicate, mirroring supported / hxq_supported / packed_supported
  * (reference scripts/tabicl_tpu_pallas_attn.py:319-320, 715-719, 762-764). Returns 1 if the op
  * accepts the shape, 0 otherwise. Lq/Lk are query/key lengths, E the merged width (ICL: head dim).

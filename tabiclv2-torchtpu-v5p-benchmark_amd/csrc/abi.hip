@@ -713,7 +713,8 @@ constexpr int64_t PAGED_MAX_ROWS = 1LL << 30;  // rows of a sequence: row number
 // The pool part of the paged entry points' arguments, checked and packed (status 0 or 1 with the message set).
 int paged_pool(const char* op, PagedPool* c, const void* k_pages, const void* v_pages, int64_t pages, int64_t page_sp,
                int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths,
-               int64_t N, int64_t H, int64_t D, int32_t dtype) {
+               int64_t N, int64_t H, int64_t D, int32_t dtype, int64_t cell = 0) {
+  if (!cell) cell = (int64_t)esize(dtype);  // bytes of a value in the pool
   if (dtype != TABICL_DTYPE_BF16 && dtype != TABICL_DTYPE_F32) return fail(1, "%s: dtype code %d not supported", op, dtype);
   if (D != 32 && D != 64 && D != 128) return fail(1, "%s: head dim must be 32, 64 or 128, got %lld", op, (long long)D);
   if (page_rows < 16 || page_rows > (1 << 20) || (page_rows & (page_rows - 1)))
@@ -721,7 +722,7 @@ int paged_pool(const char* op, PagedPool* c, const void* k_pages, const void* v_
   if (N < 0 || N > 65535 || H < 1 || H > 1024) return fail(1, "%s: needs 0 <= N <= 65535 and 1 <= H <= 1024", op);
   if (pages < 0 || pages > 0x7fffffffLL || max_pages < 0 || max_pages > PAGED_MAX_ROWS / page_rows || table_sn < 0)
     return fail(1, "%s: bad page counts (pages %lld, max_pages %lld)", op, (long long)pages, (long long)max_pages);
-  if (page_sp < H * page_rows * D || !stride_ok(page_sp, dtype) || (pages && page_sp > (1LL << 60) / pages))
+  if (page_sp < H * page_rows * D || page_sp * cell % 16 || (pages && page_sp > (1LL << 60) / pages))
     return fail(1, "%s: the page stride must be a multiple of 16 bytes and at least H * page_rows * D", op);
   if (N > 0 && (!lengths || (max_pages > 0 && !table))) return fail(1, "%s: table and lengths are required", op);
   if (!aligned16(k_pages) || !aligned16(v_pages)) return fail(1, "%s: pools must be 16-byte aligned", op);
@@ -891,4 +892,327 @@ int tabicl_paged_evict(void* k_pages, void* v_pages, int64_t blocks, int64_t blo
   a.kept_lengths = kept_lengths;
   a.N = (int)N;
   return launch_status(tabicl_launch_paged_evict(a, dtype, ws, (hipStream_t)stream), "paged_evict");
+}
+
+namespace {
+
+// dtype: of queries, rows and results; code: of the pool's values.
+int paged_code(const char* op, int32_t code, const void* scales, int64_t pages) {
+  if (code != TABICL_CODE_E4M3 && code != TABICL_CODE_I8) return fail(1, "%s: code %d not supported (0 e4m3, 1 int8)", op, code);
+  if (pages > 0 && (!scales || ((uintptr_t)scales & 7))) return fail(1, "%s: scales are required (8-byte aligned)", op);
+  return 0;
+}
+
+int paged_format(const char* op, int32_t format, int32_t dtype, const void* scales, int64_t pages) {
+  if (format < 0 || format > 3) return fail(1, "%s: pool format %d not supported (0 bf16, 1 fp32, 2 e4m3, 3 int8)", op, format);
+  if (format < 2) return format == dtype ? 0 : fail(1, "%s: a bf16 or fp32 pool takes its own dtype", op);
+  return paged_code(op, format - 2, scales, pages);
+}
+
+int64_t format_bytes(int32_t format) { return format == 0 ? 2 : format == 1 ? 4 : 1; }
+
+int strides16(const char* op, const int64_t* s, int count, int32_t dtype) {
+  for (int i = 0; i < count; ++i)
+    if (s[i] < 0 || !stride_ok(s[i], dtype)) return fail(1, "%s: strides must be non-negative multiples of 16 bytes", op);
+  return 0;
+}
+
+int paged_attn_fill(const char* op, PagedAttn* a, const void* q, void* out, int64_t N, int64_t Hq, int64_t Tq, int64_t q_sn,
+                    int64_t q_sh, int64_t q_st, int64_t o_sn, int64_t o_sh, int64_t o_st, float scale, int32_t dtype) {
+  if (!q || !out || !aligned16(q) || !aligned16(out)) return fail(1, "%s: q and out must be 16-byte aligned", op);
+  const int64_t s[6] = {q_sn, q_sh, q_st, o_sn, o_sh, o_st};
+  if (int st = strides16(op, s, 6, dtype)) return st;
+  if (!(scale > -1e30f && scale < 1e30f)) return fail(1, "%s: scale must be finite", op);
+  a->q = q;
+  a->q_sn = q_sn;
+  a->q_sh = q_sh;
+  a->q_st = q_st;
+  a->out = out;
+  a->o_sn = o_sn;
+  a->o_sh = o_sh;
+  a->o_st = o_st;
+  a->N = (int)N;
+  a->Hq = (int)Hq;
+  a->Tq = (int)Tq;
+  a->scale = scale;
+  return 0;
+}
+
+int paged_workspace(const char* op, int64_t need, const void* ws, int64_t ws_bytes) {
+  if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need))
+    return fail(1, "%s: workspace of %lld bytes (16-byte aligned) required", op, (long long)need);
+  return 0;
+}
+
+}  // namespace
+
+int64_t tabicl_paged_attn_q8_workspace_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows,
+                                             int32_t dtype) {
+  if (dtype != TABICL_DTYPE_BF16 && dtype != TABICL_DTYPE_F32)
+    return -fail(1, "paged_attn_q8_workspace_bytes: dtype code %d not supported", dtype);
+  if (int st = paged_attn_sizes("paged_attn_q8_workspace_bytes", N, Hq, H, Tq, D, rows)) return -st;
+  if (N == 0 || Tq == 0) return 0;
+  return tabicl_launch_paged_attn_q8_ws_bytes(N, Hq, H, Tq, D, rows, dtype);
+}
+
+int tabicl_paged_attn_q8(const void* q, const void* k_pages, const void* v_pages, const float* scales, int64_t pages,
+                         int64_t page_sp, int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages,
+                         const int32_t* lengths, void* out, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D,
+                         int64_t q_sn, int64_t q_sh, int64_t q_st, int64_t o_sn, int64_t o_sh, int64_t o_st, float scale,
+                         int32_t dtype, int32_t code, void* ws, int64_t ws_bytes, void* stream) {
+  PagedAttn a = {};
+  if (int st = paged_pool("paged_attn_q8", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+                          lengths, N, H, D, dtype, 1))
+    return st;
+  if (int st = paged_code("paged_attn_q8", code, scales, pages)) return st;
+  if (int st = paged_attn_sizes("paged_attn_q8", N, Hq, H, Tq, D, max_pages * page_rows)) return st;
+  if (N == 0 || Tq == 0) return 0;
+  if (int st = paged_attn_fill("paged_attn_q8", &a, q, out, N, Hq, Tq, q_sn, q_sh, q_st, o_sn, o_sh, o_st, scale, dtype)) return st;
+  if (int st = paged_workspace("paged_attn_q8",
+                               tabicl_launch_paged_attn_q8_ws_bytes(N, Hq, H, Tq, D, max_pages * page_rows, dtype), ws, ws_bytes))
+    return st;
+  a.scales = scales;
+  return launch_status(tabicl_launch_paged_attn_q8(a, dtype, code, ws, (hipStream_t)stream), "paged_attn_q8");
+}
+
+int tabicl_paged_append_q8(void* k_pages, void* v_pages, float* scales, int64_t pages, int64_t page_sp, int64_t page_rows,
+                           const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const void* k,
+                           const void* v, const int32_t* count, const int32_t* starts, int64_t N, int64_t H, int64_t T, int64_t D,
+                           int64_t k_sn, int64_t k_sh, int64_t k_st, int64_t v_sn, int64_t v_sh, int64_t v_st, int32_t dtype,
+                           int32_t code, void* stream) {
+  PagedAppend8 a = {};
+  if (int st = paged_pool("paged_append_q8", &a.rows.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+                          lengths, N, H, D, dtype, 1))
+    return st;
+  if (int st = paged_code("paged_append_q8", code, scales, pages)) return st;
+  if (T < 0 || T > PAGED_MAX_ROWS) return fail(1, "paged_append_q8: bad row count %lld", (long long)T);
+  if (starts && !count) return fail(1, "paged_append_q8: packed rows need a count per sequence");
+  if (N == 0 || T == 0 || max_pages == 0) return 0;
+  if (!k || !v || !aligned16(k) || !aligned16(v)) return fail(1, "paged_append_q8: k and v must be 16-byte aligned");
+  const int64_t s[6] = {k_sn, k_sh, k_st, v_sn, v_sh, v_st};
+  if (int st = strides16("paged_append_q8", s, 6, dtype)) return st;
+  if ((T / page_rows + 2 < max_pages ? T / page_rows + 2 : max_pages) * H > PAGED_MAX_GRID / 2)
+    return fail(1, "paged_append_q8: more than 2^22 pages and heads of a sequence to look at");
+  a.rows.k = k;
+  a.rows.v = v;
+  a.rows.k_sn = k_sn;
+  a.rows.k_sh = k_sh;
+  a.rows.k_st = k_st;
+  a.rows.v_sn = v_sn;
+  a.rows.v_sh = v_sh;
+  a.rows.v_st = v_st;
+  a.rows.count = count;
+  a.rows.N = (int)N;
+  a.rows.T = (int)T;
+  a.scales = scales;
+  a.starts = starts;
+  return launch_status(tabicl_launch_paged_append_q8(a, dtype, code, (hipStream_t)stream), "paged_append_q8");
+}
+
+int tabicl_paged_gather_q8(const void* k_pages, const void* v_pages, const float* scales, int64_t pages, int64_t page_sp,
+                           int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths,
+                           void* k, void* v, int64_t N, int64_t H, int64_t T, int64_t D, int32_t dtype, int32_t code, void* stream) {
+  PagedGather a = {};
+  if (int st = paged_pool("paged_gather_q8", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+                          lengths, N, H, D, dtype, 1))
+    return st;
+  if (int st = paged_code("paged_gather_q8", code, scales, pages)) return st;
+  if (T < 0 || T > PAGED_MAX_ROWS) return fail(1, "paged_gather_q8: bad row count %lld", (long long)T);
+  if (N == 0 || T == 0) return 0;
+  if (!k || !v || !aligned16(k) || !aligned16(v)) return fail(1, "paged_gather_q8: k and v must be 16-byte aligned");
+  a.k = k;
+  a.v = v;
+  a.N = (int)N;
+  a.T = (int)T;
+  return launch_status(tabicl_launch_paged_gather_q8(a, scales, dtype, code, (hipStream_t)stream), "paged_gather_q8");
+}
+
+int tabicl_paged_bounds(const void* k_pages, const float* scales, int64_t pages, int64_t page_sp, int64_t page_rows,
+                        const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const int32_t* start,
+                        int64_t rows, int8_t* bounds, float* bound_scales, int64_t N, int64_t H, int64_t D, int32_t format,
+                        void* stream) {
+  PagedBounds a = {};
+  if (int st = paged_format("paged_bounds", format, format < 2 ? format : 0, scales, pages)) return st;
+  if (int st = paged_pool("paged_bounds", &a.pool, k_pages, k_pages, pages, page_sp, page_rows, table, table_sn, max_pages, lengths, N,
+                          H, D, format == 1 ? 1 : 0, format_bytes(format)))
+    return st;
+  if (rows < 0) return fail(1, "paged_bounds: rows must not be negative");
+  if (pages > 0 && (!bounds || !bound_scales || !aligned16(bounds) || ((uintptr_t)bound_scales & 3)))
+    return fail(1, "paged_bounds: bounds (16-byte aligned) and bound_scales are required");
+  if (rows > max_pages * page_rows || !start) rows = max_pages * page_rows;
+  if ((max_pages < rows / page_rows + 2 ? max_pages : rows / page_rows + 2) * H > 4 * PAGED_MAX_GRID)
+    return fail(1, "paged_bounds: more than 2^25 pages and heads of a sequence to look at");
+  if (N == 0 || pages == 0) return 0;
+  a.scales = scales;
+  a.start = start;
+  a.bounds = bounds;
+  a.bound_scales = bound_scales;
+  a.N = (int)N;
+  return launch_status(tabicl_launch_paged_bounds(a, format, rows, (hipStream_t)stream), "paged_bounds");
+}
+
+int64_t tabicl_paged_select_workspace_bytes(int64_t N, int64_t H, int64_t Tq, int64_t max_pages) {
+  if (N < 0 || N > 65535 || H < 1 || H > 1024 || Tq < 0 || max_pages < 0 || max_pages > PAGED_MAX_ROWS / 16 ||
+      N * H * Tq > PAGED_MAX_QUERIES / 2)
+    return -fail(1, "paged_select_workspace_bytes: bad sizes N=%lld H=%lld Tq=%lld max_pages=%lld", (long long)N, (long long)H,
+                 (long long)Tq, (long long)max_pages);
+  return tabicl_launch_paged_select_ws_bytes(N, H, Tq, max_pages);
+}
+
+int tabicl_paged_select(const void* q, const int8_t* bounds, const float* bound_scales, int64_t pages, int64_t page_rows,
+                        const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, int32_t* index, int64_t K,
+                        int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t q_sn, int64_t q_sh, int64_t q_st,
+                        int32_t dtype, void* ws, int64_t ws_bytes, void* stream) {
+  PagedSelect a = {};
+  if (int st = paged_pool("paged_select", &a.pool, bounds, bounds, pages, H * page_rows * D, page_rows, table, table_sn, max_pages,
+                          lengths, N, H, D, dtype))
+    return st;
+  if (int st = paged_attn_sizes("paged_select", N, Hq, H, Tq, D, max_pages * page_rows)) return st;
+  if (N * H * Tq > PAGED_MAX_QUERIES / 2) return fail(1, "paged_select: more than 2^21 query rows over all sequences and K/V heads");
+  if (K < 0 || K > PAGED_MAX_ROWS / page_rows) return fail(1, "paged_select: bad page count %lld", (long long)K);
+  if (N == 0 || Tq == 0 || K == 0) return 0;
+  if (!q || !aligned16(q) || !index || ((uintptr_t)index & 3)) return fail(1, "paged_select: q (16-byte aligned) and index are required");
+  if (pages > 0 && !bound_scales) return fail(1, "paged_select: bound_scales are required");
+  const int64_t s[3] = {q_sn, q_sh, q_st};
+  if (int st = strides16("paged_select", s, 3, dtype)) return st;
+  if (int st = paged_workspace("paged_select", tabicl_launch_paged_select_ws_bytes(N, H, Tq, max_pages), ws, ws_bytes)) return st;
+  a.q = q;
+  a.q_sn = q_sn;
+  a.q_sh = q_sh;
+  a.q_st = q_st;
+  a.bounds = bounds;
+  a.bound_scales = bound_scales;
+  a.index = index;
+  a.N = (int)N;
+  a.Hq = (int)Hq;
+  a.Tq = (int)Tq;
+  a.K = (int)K;
+  return launch_status(tabicl_launch_paged_select(a, dtype, ws, (hipStream_t)stream), "paged_select");
+}
+
+namespace {
+
+int paged_sparse_sizes(const char* op, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows) {
+  if (int st = paged_attn_sizes(op, N, Hq, H, Tq, D, rows)) return st;
+  if (N * Hq * Tq > PAGED_MAX_QUERIES) return fail(1, "%s: more than 2^22 query rows over all sequences and heads", op);
+  return 0;
+}
+
+}  // namespace
+
+int64_t tabicl_paged_sparse_attn_workspace_bytes(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t rows) {
+  if (int st = paged_sparse_sizes("paged_sparse_attn_workspace_bytes", N, Hq, H, Tq, D, rows)) return -st;
+  if (N == 0 || Tq == 0) return 0;
+  return tabicl_launch_paged_sparse_ws_bytes(N, Hq, H, Tq, D, rows);
+}
+
+int tabicl_paged_sparse_attn(const void* q, const void* k_pages, const void* v_pages, const float* scales, int64_t pages,
+                             int64_t page_sp, int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages,
+                             const int32_t* lengths, const int32_t* index, int64_t K, void* out, int64_t N, int64_t Hq, int64_t H,
+                             int64_t Tq, int64_t D, int64_t q_sn, int64_t q_sh, int64_t q_st, int64_t o_sn, int64_t o_sh,
+                             int64_t o_st, float scale, int32_t dtype, int32_t format, void* ws, int64_t ws_bytes, void* stream) {
+  PagedAttn a = {};
+  if (dtype != TABICL_DTYPE_BF16 && dtype != TABICL_DTYPE_F32) return fail(1, "paged_sparse_attn: dtype code %d not supported", dtype);
+  if (int st = paged_format("paged_sparse_attn", format, dtype, scales, pages)) return st;
+  if (int st = paged_pool("paged_sparse_attn", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, table, table_sn, max_pages,
+                          lengths, N, H, D, dtype, format_bytes(format)))
+    return st;
+  if (K < 0 || K > PAGED_MAX_ROWS / page_rows) return fail(1, "paged_sparse_attn: bad page count %lld", (long long)K);
+  if (int st = paged_sparse_sizes("paged_sparse_attn", N, Hq, H, Tq, D, K * page_rows)) return st;
+  if (N == 0 || Tq == 0) return 0;
+  if (K > 0 && (!index || ((uintptr_t)index & 3))) return fail(1, "paged_sparse_attn: index is required");
+  if (int st = paged_attn_fill("paged_sparse_attn", &a, q, out, N, Hq, Tq, q_sn, q_sh, q_st, o_sn, o_sh, o_st, scale, dtype)) return st;
+  if (int st = paged_workspace("paged_sparse_attn", tabicl_launch_paged_sparse_ws_bytes(N, Hq, H, Tq, D, K * page_rows), ws, ws_bytes))
+    return st;
+  a.scales = scales;
+  a.index = index;
+  a.K = (int)K;
+  return launch_status(tabicl_launch_paged_sparse(a, format, dtype, ws, (hipStream_t)stream), "paged_sparse_attn");
+}
+
+namespace {
+
+int paged_books(const char* op, PagedBooks* a, int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths,
+                const int32_t* count, int64_t pages, int64_t page_rows, int64_t N) {
+  if (page_rows < 16 || page_rows > (1 << 20) || (page_rows & (page_rows - 1)))
+    return fail(1, "%s: page_rows must be a power of two from 16 to 2^20, got %lld", op, (long long)page_rows);
+  if (N < 0 || N > 65535) return fail(1, "%s: needs 0 <= N <= 65535", op);
+  if (pages < 0 || pages > 0x7fffffffLL || max_pages < 0 || max_pages > PAGED_MAX_ROWS / page_rows || table_sn < 0)
+    return fail(1, "%s: bad page counts (pages %lld, max_pages %lld)", op, (long long)pages, (long long)max_pages);
+  if (N > 0 && (!lengths || (max_pages > 0 && !table))) return fail(1, "%s: table and lengths are required", op);
+  a->table = table;
+  a->table_sn = table_sn;
+  a->max_pages = (int)max_pages;
+  a->pages = (int)pages;
+  a->shift = __builtin_ctzll((unsigned long long)page_rows);
+  a->N = (int)N;
+  a->lengths = lengths;
+  a->count = count;
+  return 0;
+}
+
+}  // namespace
+
+int64_t tabicl_paged_books_workspace_bytes(int64_t N) {
+  if (N < 0 || N > 65535) return -fail(1, "paged_books_workspace_bytes: needs 0 <= N <= 65535");
+  return tabicl_launch_paged_books_ws_bytes(N);
+}
+
+int tabicl_paged_reserve(int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const int32_t* count,
+                         const int32_t* free_pages, int32_t* free_count, int32_t* granted, int64_t pages, int64_t page_rows,
+                         int64_t N, void* ws, int64_t ws_bytes, void* stream) {
+  PagedBooks a = {};
+  if (int st = paged_books("paged_reserve", &a, table, table_sn, max_pages, lengths, count, pages, page_rows, N)) return st;
+  if (N == 0) return 0;
+  if (!count || !granted || !free_count || (pages > 0 && !free_pages))
+    return fail(1, "paged_reserve: count, free, free_count and granted are required");
+  if (int st = paged_workspace("paged_reserve", tabicl_launch_paged_books_ws_bytes(N), ws, ws_bytes)) return st;
+  a.free_pages = (int32_t*)free_pages;
+  a.free_count = free_count;
+  a.granted = granted;
+  return launch_status(tabicl_launch_paged_reserve(a, ws, (hipStream_t)stream), "paged_reserve");
+}
+
+int tabicl_paged_release(int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, int32_t* free_pages,
+                         int32_t* free_count, int64_t pages, int64_t page_rows, int64_t N, void* ws, int64_t ws_bytes,
+                         void* stream) {
+  PagedBooks a = {};
+  if (int st = paged_books("paged_release", &a, table, table_sn, max_pages, lengths, nullptr, pages, page_rows, N)) return st;
+  if (N == 0) return 0;
+  if (!free_count || (pages > 0 && !free_pages)) return fail(1, "paged_release: free and free_count are required");
+  if (int st = paged_workspace("paged_release", tabicl_launch_paged_books_ws_bytes(N), ws, ws_bytes)) return st;
+  a.free_pages = free_pages;
+  a.free_count = free_count;
+  return launch_status(tabicl_launch_paged_release(a, ws, (hipStream_t)stream), "paged_release");
+}
+
+int tabicl_paged_slots(const int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const int32_t* count,
+                       int64_t* slots, int32_t* starts, int64_t total, int64_t pages, int64_t page_rows, int64_t N,
+                       void* stream) {
+  PagedBooks a = {};
+  if (int st = paged_books("paged_slots", &a, (int32_t*)table, table_sn, max_pages, lengths, count, pages, page_rows, N)) return st;
+  if (total < 0 || total > 0x7fffffffLL) return fail(1, "paged_slots: bad total %lld", (long long)total);
+  if (!starts || (total > 0 && !slots) || (N > 0 && !count)) return fail(1, "paged_slots: count, slots and starts are required");
+  return launch_status(tabicl_launch_paged_slots(a, slots, starts, total, (hipStream_t)stream), "paged_slots");
+}
+
+int tabicl_paged_append_slots(void* k_pages, void* v_pages, int64_t pages, int64_t page_sp, int64_t page_rows,
+                              const int64_t* slots, const void* k, const void* v, int64_t total, int64_t H, int64_t D, int64_t k_st,
+                              int64_t k_sh, int64_t v_st, int64_t v_sh, int32_t dtype, void* stream) {
+  PagedAppend a = {};
+  if (int st = paged_pool("paged_append_slots", &a.pool, k_pages, v_pages, pages, page_sp, page_rows, nullptr, 0, 0, nullptr, 0, H, D,
+                          dtype))
+    return st;
+  if (total < 0 || total > 0x7fffffffLL) return fail(1, "paged_append_slots: bad total %lld", (long long)total);
+  if (total == 0 || pages == 0) return 0;
+  if (!k || !v || !slots || !aligned16(k) || !aligned16(v)) return fail(1, "paged_append_slots: slots, k and v (16-byte aligned) are required");
+  const int64_t s[4] = {k_st, k_sh, v_st, v_sh};
+  if (int st = strides16("paged_append_slots", s, 4, dtype)) return st;
+  a.k = k;
+  a.v = v;
+  a.k_st = k_st;
+  a.k_sh = k_sh;
+  a.v_st = v_st;
+  a.v_sh = v_sh;
+  return launch_status(tabicl_launch_paged_append_slots(a, slots, total, dtype, (hipStream_t)stream), "paged_append_slots");
 }

@@ -3,548 +3,12 @@
 //
 //   s_i = scale q . K_i  (i < len),   p = exp(s - max s),   out = sum_i p_i V_i / sum_i p_i   (len = 0: 0)
 //   weights_i += sum over heads and query rows of p_i / sum p
-#include "common.h"
 #include "launch.h"
-#include "paged.h"
+#include "paged_core.h"
 
 #include <numeric>
 
 namespace {
-
-__device__ __forceinline__ int pool_length(const PagedPool& c, int n) {
-  const int64_t cap = (int64_t)c.max_pages << c.shift;
-  const int64_t len = c.lengths[n];
-  return (int)(len < 0 ? 0 : len < cap ? len : cap);
-}
-
-// Element offset of row `row`, head h of sequence n in the pool, or -1 where its page is none of the pool's.
-__device__ __forceinline__ int64_t pool_row(const PagedPool& c, int n, int h, int row) {
-  const int32_t page = c.table[n * c.table_sn + (row >> c.shift)];
-  if (page < 0 || page >= c.pages) return -1;
-  const int R = 1 << c.shift;
-  return page * c.page_sp + ((int64_t)h * R + (row & (R - 1))) * c.D;
-}
-
-// ---------------------------------------------------------------------------------------------
-// attention
-// ---------------------------------------------------------------------------------------------
-// Bound by the bytes of K and V, which are read once (one row over 8 x 45,000 cached rows of 8 heads: 124 us, 5.9 TB/s). A
-// workgroup takes a run of rows of one item: a sequence, a K/V head and up to 16 QT query rows (the heads of a group and
-// the query rows together); its NW waves take turns of KS rows. Nothing of K and V is shared between waves, so they go from
-// memory straight into the registers of the matrix products, a turn ahead of their use; LDS only joins the waves at the end.
-//   S^T = K Q^T  (16 keys x 16 queries): the A operand is 16 bytes of a K row per lane, the result holds query l % 16,
-//                keys 4 (l / 16) + i, which is the B operand of
-//   O^T = V^T P^T with the keys in that order: the A operand holds the values of column group l % 16 (D / 16 columns, one
-//                per product) of those keys; in bf16 the halves of pairs of rows are regrouped by v_perm_b32.
-// One query row leaves 15 of the 16 columns empty: the products stay far below the loads all the same.
-// bf16 probabilities enter as two bf16 terms (2^-16 of each left out), so that the output is off by its own rounding
-// alone; the second product costs nothing beside the loads. fp32 runs on the fp32 matrix unit.
-// Softmax: p = 2^(s - ref), ref moved to the running maximum when a score passes it by more than PA_SLACK (one test per turn).
-// The products with V take 2^-24 p, so that sums with values near the largest float stay finite. bf16 has the 24 in ref,
-// where it costs no instruction and rounds the exponent to 2^-20; fp32 would lose four bits of a mild score by that, and
-// multiplies.
-constexpr float PA_SHIFT = 24.f, PA_SLACK = 8.f;
-template <typename T>
-struct PagedShift {
-  static constexpr float REF = sizeof(T) == 2 ? PA_SHIFT : 0.f, VALUE = sizeof(T) == 2 ? 1.f : 0x1p-24f;
-};
-constexpr float PA_REF0 = -3.4028234663852886e38f;
-
-// The work is cut on the device, by the lengths as they are: a unit is PA_UNIT rows of one item, units are counted item after
-// item, and G workgroups (pa_waves per CU) take equal runs of them, whatever the lengths. An item that one workgroup covers
-// is written at once; of the others each workgroup leaves a partial (at most two: one of an item begun before it, one of an
-// item it begins), which pa_merge_kernel joins. (A fixed number of rows per workgroup instead: 64 sequences of 500 to
-// 10,000 rows took 97 us at 8 workgroups per CU and 146 at 2, one sequence of 45,000 rows 39 and 27; this way 84 and 26.)
-constexpr int PA_UNIT = 128, PA_WHOLE = 1024;
-
-struct PagedSplit {
-  int groups;    // G, or 0: a workgroup of eight waves for each item
-  int least;     // units a workgroup takes at least
-  int few;       // below so many units, half of the workgroups share them
-  int qtiles;
-  float* part;   // [2 G][16 QT][D] unnormalised outputs
-  float2* ml;    // [2 G][16 QT] (ref, sum)
-  int2* ends;    // [N H qtiles] the workgroups that hold the first and the last unit of an item
-  float2* stat;  // [N Hq Tq] (ref, 1 / sum) for the weights, or null
-  float* score;  // [N Hq Tq][score_sn] scores in log2 units for the weights, or null: from K once more
-  int64_t score_sn;
-};
-
-__device__ __forceinline__ int pa_len(const PagedAttn& a, int n) { return a.pool.pages > 0 ? pool_length(a.pool, n) : 0; }
-
-__device__ __forceinline__ int pa_units(int len) { return (len + PA_UNIT - 1) / PA_UNIT; }
-
-// Inclusive sum over the lanes of a wave, in the registers.
-__device__ __forceinline__ int wave_sum_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8 within 16 lanes
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
-  return x;
-}
-
-// The units of the sequences, 64 sequences at a time, one per lane.
-struct PagedUnits {
-  const PagedAttn& a;
-  int per, lane;  // items of a sequence
-  int own, upto;  // sequence `lane`: its units, and theirs up to it
-  int total;      // of all sequences
-  __device__ __forceinline__ int load(int base) const {
-    const int n = base + lane;
-    return n < a.N ? pa_units(pa_len(a, n)) * per : 0;
-  }
-  __device__ __forceinline__ PagedUnits(const PagedAttn& args, int items, int l) : a(args), per(items), lane(l) {
-    own = load(0);
-    upto = wave_sum_scan(own);
-    total = __builtin_amdgcn_readlane(upto, 63);
-    for (int base = 64; base < a.N; base += 64) total += __builtin_amdgcn_readlane(wave_sum_scan(load(base)), 63);
-  }
-  // the sequence that unit t < total belongs to, and its first unit
-  __device__ __forceinline__ int find(int t, int* first) const {
-    int u = own, s = upto;
-    for (int base = 0;;) {
-      const uint64_t past = __ballot(s > t);
-      if (past) {
-        const int k = __builtin_ctzll(past);
-        *first = __builtin_amdgcn_readlane(s - u, k);
-        return base + k;
-      }
-      base += 64;
-      if (base >= a.N) return *first = 0;  // not reached
-      const int before = __builtin_amdgcn_readlane(s, 63);
-      u = load(base);
-      s = wave_sum_scan(u) + before;
-    }
-  }
-};
-
-// Equal shares: `groups` workgroups (half of them below `few` units, and fewer if they would get less than `least` units) of
-// `share` units, the first `more` of them one more.
-struct PagedShares {
-  int groups, share, more;
-  __device__ __forceinline__ PagedShares(const PagedSplit& z, int total) {
-    groups = total / z.least;
-    const int most = total < z.few ? z.groups / 2 : z.groups;
-    groups = groups < 1 ? 1 : groups < most ? groups : most;
-    share = total / groups;
-    more = total - share * groups;
-  }
-  __device__ __forceinline__ int first(int w) const { return w * share + (w < more ? w : more); }
-};
-
-template <typename T, int D>
-struct PagedTile {
-  static constexpr int ES = sizeof(T), SUB = ES == 2 ? 2 : 1, KS = 16 * SUB;  // 16-key subtiles, keys of a turn
-  static constexpr int NC = D * ES / 64;                                      // 16-byte chunks of a K row per lane
-  static constexpr int DE = D / 16, DW = DE * ES / 4;                         // values and dwords of a V row per lane
-  uint4 k[SUB][NC];
-  uint32_t v[SUB][4][DW];
-};
-
-typedef uint32_t u32v2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32v4 __attribute__((ext_vector_type(4)));
-template <int DW>
-__device__ __forceinline__ void load_dwords(uint32_t* d, __amdgpu_buffer_rsrc_t r, uint32_t off) {
-  if constexpr (DW == 1) {
-    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-  } else if constexpr (DW == 2) {
-    const u32v2 x = __builtin_bit_cast(u32v2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
-    d[0] = x[0], d[1] = x[1];
-  } else {
-#pragma unroll
-    for (int i = 0; i < DW; i += 4) {
-      const u32v4 x = __builtin_bit_cast(u32v4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, 0));
-      d[i] = x[0], d[i + 1] = x[1], d[i + 2] = x[2], d[i + 3] = x[3];
-    }
-  }
-}
-
-// The scores of 16 keys (chunks k of their rows) for 16 queries: key 4 (l / 16) + i, query l % 16. fp32 sums in four chains:
-// one of D products would be the largest rounding of all (2-norm of the output's error for sharp scores, D = 64 and 128:
-// 9.4e-7 and 1.1e-6 with one chain and the 24 in ref, 4.5e-7 this way; of mild ones 4.2e-7 and 1.8e-7).
-template <typename T, int NC>
-__device__ __forceinline__ f32x4 tile_scores(const uint4* k, const uint4* q) {
-  if constexpr (sizeof(T) == 2) {
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[c]), __builtin_bit_cast(bf16x8, q[c]), s, 0, 0, 0);
-    return s;
-  } else {
-    f32x4 s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, k[c])[i], __builtin_bit_cast(f32x4, q[c])[i], s[i], 0,
-                                                    0, 0);
-    }
-    return (s[0] + s[1]) + (s[2] + s[3]);
-  }
-}
-
-// A score in log2 units, rounded before the reference is taken off: the difference of the largest one is then exact, however
-// large it is, and the same wherever it is formed. (A fused product would leave the rounding of the product in the exponent:
-// at scores of 10^9 the probabilities of a row added up to 10^7.)
-__device__ __forceinline__ float log2_score(float s, float sc) {
-#pragma clang fp contract(off)
-  return s * sc;
-}
-
-// Sum over the 16 lanes of a row, in the registers (row_ror).
-template <int N>
-__device__ __forceinline__ float row_add(float x) {
-  return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 + N, 0xf, 0xf, false));
-}
-__device__ __forceinline__ float row16_sum(float x) { return row_add<1>(row_add<2>(row_add<4>(row_add<8>(x)))); }
-
-template <int D>
-__device__ __forceinline__ void paged_values(const PagedTile<bf16, D>& t, const float (*p)[4], f32x4* o) {
-  // hi: p cut to bf16, lo: the rest and 2^-18 of hi, so that neither term is 0 for a p > 0 nor of the other sign: an
-  // infinite value stays infinite
-  uint32_t hw[4];
-  bf16x4 l4[2];
-#pragma unroll
-  for (int sub = 0; sub < 2; ++sub) {
-    f32x4 lo32;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      lo32[i] = __builtin_fmaf(__uint_as_float(__float_as_uint(p[sub][i]) & 0xffff0000u), -(1.f - 0x1p-18f), p[sub][i]);
-    l4[sub] = cvt_bf16x4(lo32);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      hw[2 * sub + i] = __builtin_amdgcn_perm(__float_as_uint(p[sub][2 * i + 1]), __float_as_uint(p[sub][2 * i]), 0x07060302u);
-  }
-  const bf16x8 hi = __builtin_bit_cast(bf16x8, (uint4{hw[0], hw[1], hw[2], hw[3]}));
-  const bf16x8 lo = __builtin_shufflevector(l4[0], l4[1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e) {
-    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-    const int w = e / 2;
-    const uint4 a = {__builtin_amdgcn_perm(t.v[0][1][w], t.v[0][0][w], sel), __builtin_amdgcn_perm(t.v[0][3][w], t.v[0][2][w], sel),
-                     __builtin_amdgcn_perm(t.v[1][1][w], t.v[1][0][w], sel), __builtin_amdgcn_perm(t.v[1][3][w], t.v[1][2][w], sel)};
-    const bf16x8 va = __builtin_bit_cast(bf16x8, a);
-    o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, hi, o[e], 0, 0, 0);
-    o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, lo, o[e], 0, 0, 0);
-  }
-  }
-template <int D>
-__device__ __forceinline__ void paged_values(const PagedTile<float, D>& t, const float (*p)[4], f32x4* o) {
-  const f32x4 pv = f32x4{p[0][0], p[0][1], p[0][2], p[0][3]} * PagedShift<float>::VALUE;
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e) {
-    const f32x4 va = {__uint_as_float(t.v[0][0][e]), __uint_as_float(t.v[0][1][e]), __uint_as_float(t.v[0][2][e]),
-                      __uint_as_float(t.v[0][3][e])};
-    o[e] = mfma16x16x16(va, pv, o[e]);
-  }
-}
-
-// N values to p, 16 bytes at a time.
-template <typename T, int N>
-__device__ __forceinline__ void store_row(T* p, const float* x) {
-  constexpr int C = 16 / sizeof(T);
-#pragma unroll
-  for (int j = 0; j < N; j += C) {
-    if constexpr (C == 4) {
-      *(f32x4*)(p + j) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
-    } else {
-      const bf16x4 lo = cvt_bf16x4(f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]});
-      const bf16x4 hi = cvt_bf16x4(f32x4{x[j + 4], x[j + 5], x[j + 6], x[j + 7]});
-      *(bf16x8*)(p + j) = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-  }
-}
-
-// Rows [c0, c1) of an item by the NW waves of a workgroup: the output, or (slot >= 0) a partial of it.
-template <typename T, int D, int QT, bool W, int NW>
-__device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit& z, int n, int item, int c0, int c1, int slot) {
-  typedef PagedTile<T, D> Tile;
-  constexpr int SUB = Tile::SUB, KS = Tile::KS, NC = Tile::NC, DE = Tile::DE, ES = Tile::ES;
-  __shared__ float sh_o[NW / 2][16 * QT][D + 4];
-  __shared__ float2 sh_ml[NW / 2][16 * QT];
-  const PagedPool& c = a.pool;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
-  const int G = a.Hq / c.H, rows = G * a.Tq;
-  const float sc = a.scale * TA_LOG2E;
-  const uint32_t koff = lr * D * ES + lg * 16, voff = lg * 4 * D * ES + lr * DE * ES;
-  const int qt0 = item % z.qtiles, h = item / z.qtiles, nh = n * c.H + h;
-
-  // this lane's query rows: 16 QT of the (head of the group, query row) pairs
-  uint4 q[QT][NC];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = (qt0 * QT + t) * 16 + lr;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) q[t][i] = uint4{0, 0, 0, 0};
-    if (r < rows) {
-      const char* qp = (const char*)a.q + (n * a.q_sn + (h * G + r / a.Tq) * a.q_sh + (r % a.Tq) * a.q_st) * ES + lg * 16;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) q[t][i] = ldg16(qp + i * 64);
-    }
-  }
-  f32x4 o[QT][DE];
-  float ref[QT], l[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    ref[t] = PA_REF0;
-    l[t] = 0.f;
-#pragma unroll
-    for (int e = 0; e < DE; ++e) o[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const int32_t* table = c.table + n * c.table_sn;
-  // 64 page ids of the table at a time, one per lane
-  int pg0 = c0 >> c.shift, pg = pg0 + lane < c.max_pages ? table[pg0 + lane] : -1;
-  const int64_t head = (int64_t)h << c.shift;
-
-  // Loads the turn at `key`; returns the live rows of its subtiles, 8 bits each. The rows past c1 and those of a page the
-  // pool does not have lie behind their buffer's end: the loads return 0 for them and touch no memory, so every turn issues
-  // the same loads (waits that count them need no branch) and a value nobody wrote meets no product.
-  auto fetch = [&](Tile& t, int key) -> int {
-    int live = 0;
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      const int k0 = key + 16 * s, left = c1 - k0;
-      int i = left > 0 ? (k0 >> c.shift) - pg0 : 0;
-      if (i >= 64) {
-        pg0 += i;
-        pg = pg0 + lane < c.max_pages ? table[pg0 + lane] : -1;
-        asm volatile("" : "+v"(pg));  // waited for here, not wherever the paths join (there: for every load in flight)
-        i = 0;
-      }
-      const int page = __builtin_amdgcn_readlane(pg, i);
-      const int have = page < 0 || page >= c.pages || left <= 0 ? 0 : left < 16 ? left : 16;
-      live |= have << (8 * s);
-      const int64_t off = ((have ? page : 0) * c.page_sp + (head + (k0 & ((1 << c.shift) - 1))) * D) * ES;
-      const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((char*)c.k + off, 0, have * D * ES, TA_BUF_WORD3);
-      const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((char*)c.v + off, 0, have * D * ES, TA_BUF_WORD3);
-#pragma unroll
-      for (int i2 = 0; i2 < NC; ++i2)
-        t.k[s][i2] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, koff + i2 * 64, 0, 0));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) load_dwords<Tile::DW>(t.v[s][j], vr, voff + j * D * ES);
-    }
-    return live;
-  };
-  auto compute = [&](Tile& t, int key, int live) {
-    const bool full = live == (SUB == 2 ? 16 << 8 | 16 : 16);
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      float x[SUB][4], top = TA_NEG_INF;
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        const f32x4 sv = tile_scores<T, NC>(t.k[s], q[qt]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[s][i] = log2_score(sv[i], sc);
-      }
-      if (!full) {
-#pragma unroll
-        for (int s = 0; s < SUB; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[s][i] = lg * 4 + i < (live >> (8 * s) & 255) ? x[s][i] : TA_NEG_INF;
-      }
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[s][i]);
-        if constexpr (W) {
-          const int r = (qt0 * QT + qt) * 16 + lr;
-          if (r < rows && key < c1)
-            *(f32x4*)(z.score + ((int64_t)nh * rows + r) * z.score_sn + key + 16 * s + lg * 4) =
-                f32x4{x[s][0], x[s][1], x[s][2], x[s][3]};
-        }
-      }
-      if (wave_any(top - ref[qt] > PA_SLACK - PagedShift<T>::REF)) {
-        const float to = fmaxf(ref[qt], quad_max(top) + PagedShift<T>::REF), f = __builtin_amdgcn_exp2f(ref[qt] - to);
-        ref[qt] = to;
-        l[qt] *= f;
-#pragma unroll
-        for (int e = 0; e < DE; ++e) o[qt][e] *= f;
-      }
-      float p[SUB][4];
-#pragma unroll
-      for (int s = 0; s < SUB; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[s][i] = __builtin_amdgcn_exp2f(x[s][i] - ref[qt]);
-#pragma unroll
-      for (int s = 0; s < SUB; ++s) l[qt] += (p[s][0] + p[s][1]) + (p[s][2] + p[s][3]);
-      paged_values<D>(t, p, o[qt]);
-      // one query tile's scores and probabilities live at a time, where stored scores take the registers too (12 dwords a
-      // lane spilled without it; elsewhere the tiles overlap: 64 query rows of 64 dims over 8 x 12,000 rows 57.5 -> 56 us)
-      if constexpr (QT > 1 && W) __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-
-  int key = c0 + wave * KS;
-  if (key < c1) {
-    Tile ta, tb;
-    int la = fetch(ta, key);
-    for (; key < c1; key += 2 * NW * KS) {
-      const int lb = fetch(tb, key + NW * KS);
-      compute(ta, key, la);
-      la = fetch(ta, key + 2 * NW * KS);
-      if (key + NW * KS < c1) compute(tb, key + NW * KS, lb);
-    }
-  }
-
-  // join the waves: the upper half hands over to the lower half, until one has all
-#pragma unroll
-  for (int t = 0; t < QT; ++t) l[t] = quad_sum(l[t]);
-#pragma unroll
-  for (int half = NW / 2; half >= 1; half >>= 1) {
-    if (wave >= half && wave < 2 * half) {
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < DE; ++e) sh_o[wave - half][t * 16 + lr][(lg * 4 + i) * DE + e] = o[t][e][i];
-        if (lg == 0) sh_ml[wave - half][t * 16 + lr] = make_float2(ref[t], l[t]);
-      }
-    }
-    __syncthreads();
-    if (wave < half) {
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        const float2 ml = sh_ml[wave][t * 16 + lr];
-        const float to = fmaxf(ref[t], ml.x), f0 = __builtin_amdgcn_exp2f(ref[t] - to), f1 = __builtin_amdgcn_exp2f(ml.x - to);
-        ref[t] = to;
-        l[t] = l[t] * f0 + ml.y * f1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < DE; ++e) o[t][e][i] = o[t][e][i] * f0 + sh_o[wave][t * 16 + lr][(lg * 4 + i) * DE + e] * f1;
-      }
-    }
-    __syncthreads();
-  }
-  if (wave == 0) {
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      const int r = (qt0 * QT + t) * 16 + lr;
-      if (r >= rows) continue;
-      const float inv = l[t] == 0.f ? 0.f : 1.f / l[t], out = slot >= 0 ? 1.f : inv * (1.f / PagedShift<T>::VALUE);
-      float x[4 * DE];  // columns 4 DE lg + j of the row
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < DE; ++e) x[i * DE + e] = o[t][e][i] * out;
-      if (slot >= 0) {
-        const int64_t at = (int64_t)slot * 16 * QT + t * 16 + lr;
-        store_row<float, 4 * DE>(z.part + at * D + lg * 4 * DE, x);
-        if (lg == 0) z.ml[at] = make_float2(ref[t], l[t]);
-      } else {
-        store_row<T, 4 * DE>((T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lg * 4 * DE, x);
-        if (z.stat && lg == 0) z.stat[(int64_t)nh * rows + r] = make_float2(ref[t], inv);
-      }
-    }
-  }
-}
-
-// Waves per SIMD that the registers of a kernel allow: one for tiles of 32 and 64 query rows of 128 dims. In tiles of 16 with
-// two waves every tile reads K and V again (tiles of 16 / larger: bf16, 32 query rows a head over 8 x 5,000 rows 57 / 42 us,
-// 64 rows 104 / 48; fp32, 17 rows 102 / 70, 34 rows over 49 x 5,311 372 / 304).
-constexpr int pa_waves(int D, int QT) { return D == 128 && QT > 1 ? 1 : 2; }
-
-// Equal shares of all items' units.
-template <typename T, int D, int QT, bool W>
-__global__ __launch_bounds__(256, pa_waves(D, QT)) void pa_kernel(PagedAttn a, PagedSplit z) {
-  const int per = a.pool.H * z.qtiles;
-  const PagedUnits units(a, per, threadIdx.x & 63);
-  const PagedShares shares(z, units.total);
-  if ((int)blockIdx.x >= shares.groups) return;
-  int unit = shares.first(blockIdx.x);
-  const int end = shares.first(blockIdx.x + 1);
-  while (unit < end) {
-    int first;
-    const int n = units.find(unit, &first);
-    const int len = __builtin_amdgcn_readfirstlane(pa_len(a, n)), each = pa_units(len);
-    const int item = (unit - first) / each, u0 = unit - first - item * each;
-    const int u1 = u0 + end - unit < each ? u0 + end - unit : each;
-    if (threadIdx.x == 0 && u0 == 0) z.ends[n * per + item].x = blockIdx.x;
-    if (threadIdx.x == 0 && u1 == each) z.ends[n * per + item].y = blockIdx.x;
-    pa_segment<T, D, QT, W, 4>(a, z, n, item, u0 * PA_UNIT, u1 * PA_UNIT < len ? u1 * PA_UNIT : len,
-                               u1 - u0 < each ? 2 * blockIdx.x + (u0 == 0) : -1);
-    unit += u1 - u0;
-  }
-}
-
-// A workgroup of eight waves for each item, where no sequence is long.
-template <typename T, int D, int QT, bool W>
-__global__ __launch_bounds__(512) void pa_whole_kernel(PagedAttn a, PagedSplit z) {
-  const int per = a.pool.H * z.qtiles, n = blockIdx.x / per;
-  pa_segment<T, D, QT, W, 8>(a, z, n, blockIdx.x % per, 0, __builtin_amdgcn_readfirstlane(pa_len(a, n)), -1);
-}
-
-__device__ __forceinline__ void store4(float* p, f32x4 x) { *(f32x4*)p = x; }
-__device__ __forceinline__ void store4(bf16* p, f32x4 x) { *(bf16x4*)p = cvt_bf16x4(x); }
-
-// Where the partials of query row r (of all rows of K/V head h of sequence n) are: `parts` of them, from workgroup w0 on;
-// one: pa_kernel has written the row.
-template <int QT>
-struct PagedParts {
-  int w0, parts, at;
-  __device__ __forceinline__ PagedParts(const PagedSplit& z, int nh, int r) {
-    const int2 w = z.ends[nh * z.qtiles + r / (16 * QT)];
-    w0 = w.x;
-    parts = w.y - w0 + 1;
-    at = r % (16 * QT);
-  }
-  __device__ __forceinline__ int64_t slot(int i) const { return (int64_t)(2 * (w0 + i) + (i == 0)) * (16 * QT) + at; }
-};
-
-// Joins the partials of a query row in a wave: 4 values of a partial output per lane, 256 / D partials at a time. Rows that
-// pa_kernel has written are left alone; rows without a key become 0.
-template <typename T, int D, int QT>
-__device__ __forceinline__ void pa_merge_row(const PagedAttn& a, const PagedSplit& z, int64_t row) {
-  constexpr int LPR = D / 4, GR = 64 / LPR;
-  const int lane = threadIdx.x & 63, G = a.Hq / a.pool.H, rows = G * a.Tq;
-  if (row >= (int64_t)a.N * a.pool.H * rows) return;
-  const int r = (int)(row % rows), nh = (int)(row / rows), n = nh / a.pool.H, h = nh % a.pool.H;
-  PagedParts<QT> p(z, nh, r);
-  p.w0 = __builtin_amdgcn_readfirstlane(p.w0);
-  p.parts = __builtin_amdgcn_readfirstlane(p.parts);
-  const int len = pa_len(a, n);
-  T* op = (T*)a.out + n * a.o_sn + (h * G + r / a.Tq) * a.o_sh + (r % a.Tq) * a.o_st + lane * 4;
-  if (len == 0) {
-    if (lane < LPR) store4(op, f32x4{0.f, 0.f, 0.f, 0.f});
-    return;
-  }
-  if (p.parts == 1) return;
-  // every group of lanes joins its share of the partials by itself (their loads wait for nothing but the lengths), then
-  // the groups are joined
-  float m = PA_REF0, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = lane / LPR; i < p.parts; i += GR) {
-    const float2 v = z.ml[p.slot(i)];
-    const f32x4 x = *(const f32x4*)(z.part + p.slot(i) * D + lane % LPR * 4);
-    const float to = fmaxf(m, v.x), f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(v.x - to);
-    m = to;
-    l = l * f0 + v.y * f1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = o[j] * f0 + x[j] * f1;
-  }
-#pragma unroll
-  for (int x = LPR; x < 64; x <<= 1) {
-    const float mo = __shfl_xor(m, x, 64), lo = __shfl_xor(l, x, 64);
-    const float to = fmaxf(m, mo), f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(mo - to);
-    m = to;
-    l = l * f0 + lo * f1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = o[j] * f0 + __shfl_xor(o[j], x, 64) * f1;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane < LPR) store4(op, o * (inv * (1.f / PagedShift<T>::VALUE)));
-  if (z.stat && lane == 0) z.stat[row] = make_float2(m, inv);
-}
-
-template <typename T, int D, int QT>
-__global__ __launch_bounds__(256) void pa_merge_kernel(PagedAttn a, PagedSplit z) {
-  pa_merge_row<T, D, QT>(a, z, (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
-}
 
 // weights[n, i] += sum over the query rows of p (stat: their references and sums): the 64 keys from k0 on, 4 per thread, the
 // query rows over 16 threads (each in steps of 16), joined in a fixed order.
@@ -586,7 +50,7 @@ template <typename T, int D, int QT>
 __global__ __launch_bounds__(256) void pa_merge_weights_kernel(PagedAttn a, PagedSplit z, int merges) {
   __shared__ float2 stat[PA_JOIN];
   if ((int)blockIdx.x < merges)
-    return pa_merge_row<T, D, QT>(a, z, (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    return pa_merge_row<T, T, D, QT>(a, z, (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
   const int at = blockIdx.x - merges, blocks = (int)(z.score_sn / 64), n = at / blocks, k0 = at % blocks * 64;
   const int len = pa_len(a, n), rows = a.Hq / a.pool.H * a.Tq, all = a.Hq * a.Tq;
   if (k0 >= len) return;
@@ -953,19 +417,6 @@ __global__ __launch_bounds__(256) void paged_move_kernel(PagedEvict a, const int
   }
 }
 
-int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
-
-int cu_count() {
-  static int count[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (!count[dev]) {
-    int n = 0;
-    count[dev] = hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n > 0 ? n : 256;
-  }
-  return count[dev];
-}
-
 // Scores kept for the weights take at most this many bytes, or those of 16 query rows of every K/V head where these are
 // more (an eighth of an fp32 cache of 64 dims): tracked queries by the hundred go in slices (pa_slice), which read the cache
 // as often as one launch does where they are whole tiles (bf16, 5,000 query rows over 1 x 45,000 rows: 4.4 ms with 6.9 GB, 4.8
@@ -1045,9 +496,9 @@ template <typename T, int D, int QT, bool W>
 void launch_pa_w(const PagedAttn& a, const PagedSplit& z, hipStream_t stream) {
   if (z.groups == 0) {
     if constexpr (pa_waves(D, QT) == 2)
-      hipLaunchKernelGGL((pa_whole_kernel<T, D, QT, W>), dim3((unsigned)(a.N * a.pool.H * z.qtiles)), dim3(512), 0, stream, a, z);
+      hipLaunchKernelGGL((pa_whole_kernel<T, T, D, QT, W>), dim3((unsigned)(a.N * a.pool.H * z.qtiles)), dim3(512), 0, stream, a, z);
   } else {
-    hipLaunchKernelGGL((pa_kernel<T, D, QT, W>), dim3((unsigned)z.groups), dim3(256), 0, stream, a, z);
+    hipLaunchKernelGGL((pa_kernel<T, T, D, QT, W>), dim3((unsigned)z.groups), dim3(256), 0, stream, a, z);
     const unsigned merge = (unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4);
     // In one launch where the workgroups of the weights all fit on the GPU at once and each has few rows to join (us of the
     // whole call, apart / in one, 8 heads: one query row over 8 x 2,000 rows 17.5 / 14.5, over 8 x 15,000 60.6 / 58.1, over
@@ -1058,7 +509,7 @@ void launch_pa_w(const PagedAttn& a, const PagedSplit& z, hipStream_t stream) {
         hipLaunchKernelGGL((pa_merge_weights_kernel<T, D, QT>), dim3(merge + blocks), dim3(256), 0, stream, a, z, (int)merge);
         return;
       }
-    hipLaunchKernelGGL((pa_merge_kernel<T, D, QT>), dim3(merge), dim3(256), 0, stream, a, z);
+    hipLaunchKernelGGL((pa_merge_kernel<T, T, D, QT>), dim3(merge), dim3(256), 0, stream, a, z);
   }
   if (W)
     hipLaunchKernelGGL(pa_weights_kernel, dim3((unsigned)(z.score_sn / 64), a.N), dim3(256), 0, stream, a, z);

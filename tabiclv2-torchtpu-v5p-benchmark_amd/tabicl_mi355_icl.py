@@ -471,10 +471,18 @@ class IclKVCache:
             raise ValueError(f"in_proj_bias must be [{3 * width}], got {tuple(in_proj_bias.shape)}")
         _nat.require_device(x, in_proj_weight)
         kv = F.linear(x, in_proj_weight[width:], None if in_proj_bias is None else in_proj_bias[width:])
-        if kv.dtype != self.keys.dtype:
-            kv = kv.to(self.keys.dtype)  # the reference stores k_l.to(cache_dtype) (tabicl_tpu_bucketed.py:676, 688)
+        if kv.dtype != self._row_dtype(kv.dtype):
+            kv = kv.to(self._row_dtype(kv.dtype))  # the reference stores k_l.to(cache_dtype) (tabicl_tpu_bucketed.py:676, 688)
         kv = kv.view(E, x.shape[1], 2, H, D)
         return kv[:, :, 0].permute(0, 2, 1, 3), kv[:, :, 1].permute(0, 2, 1, 3)
+
+    def _row_dtype(self, dtype: torch.dtype) -> torch.dtype:
+        """The type that projected rows of `dtype` are appended in."""
+        return self.keys.dtype
+
+    def _attn_dtype(self, dtype: torch.dtype) -> torch.dtype:
+        """The type that queries of `dtype` are answered in."""
+        return torch.promote_types(dtype, self.keys.dtype)
 
     def attention_layer(self, block: int, x: Tensor, in_proj_weight: Tensor, in_proj_bias: Optional[Tensor],
                         out_proj_weight: Tensor, out_proj_bias: Optional[Tensor],
@@ -497,7 +505,7 @@ class IclKVCache:
         q = q.view(E, Tq, H, D).transpose(1, 2)  # heads as a strided view: the kernel takes row strides
         if q_transform is not None:
             q = q_transform(q)
-        attn_dtype = torch.promote_types(q.dtype, self.keys.dtype)
+        attn_dtype = self._attn_dtype(q.dtype)
         merged = torch.empty(E, Tq, H, D, dtype=attn_dtype, device=x.device)
         self.query(block, q, valid_kv_len, out=merged.transpose(1, 2))  # written in merged-head order
         o = merged.view(E, Tq, width)
@@ -519,7 +527,7 @@ class IclKVCache:
         # the fused layers read their operands through pointers: any other x or cache goes to attention_layer, which
         # refuses what does not fit
         E, _, H, _, D = self.shape
-        fits = self.keys.dtype == torch.bfloat16 and H * D == 512 and x.dim() == 3 and x.shape[0] == E
+        fits = self._attn_dtype(torch.bfloat16) == torch.bfloat16 and H * D == 512 and x.dim() == 3 and x.shape[0] == E
         for b, w in enumerate(blocks):
             if fits and _linear_native(x, w, activation):
                 x = self._native_block(b, x, w, valid_kv_len, q_transform)
@@ -540,7 +548,7 @@ class IclKVCache:
         q = q.view(E, Tq, H, D).transpose(1, 2)
         if q_transform is not None:
             q = q_transform(q)
-        merged = torch.empty(E, Tq, H, D, dtype=torch.promote_types(q.dtype, self.keys.dtype), device=x.device)
+        merged = torch.empty(E, Tq, H, D, dtype=self._attn_dtype(q.dtype), device=x.device)
         self.query(block, q, valid_kv_len, out=merged.transpose(1, 2))
         o = merged.view(E, Tq, width)
         if o.dtype != torch.bfloat16:  # q_transform widened q

@@ -84,6 +84,24 @@ SIGNATURES = {
     "tabicl_paged_evict": [_c_p] * 2 + [_i64] * 5 + [_c_p, _i64, _i64, _c_p, _c_p, _i64, _c_p, _i64, _i64, _c_p, _i64,
                                                      _c_p, _c_p, _i64, _i64, _i64, _i32, _c_p, _i64, _c_p],
     "tabicl_paged_evict_workspace_bytes": [_i64] * 2,
+    "tabicl_paged_attn_q8": [_c_p] * 4 + [_i64] * 3 + [_c_p, _i64, _i64, _c_p, _c_p] + [_i64] * 11
+                            + [_f32, _i32, _i32, _c_p, _i64, _c_p],
+    "tabicl_paged_attn_q8_workspace_bytes": [_i64] * 6 + [_i32],
+    "tabicl_paged_append_q8": [_c_p] * 3 + [_i64] * 3 + [_c_p, _i64, _i64] + [_c_p] * 5 + [_i64] * 10 + [_i32, _i32, _c_p],
+    "tabicl_paged_gather_q8": [_c_p] * 3 + [_i64] * 3 + [_c_p, _i64, _i64, _c_p, _c_p, _c_p] + [_i64] * 4
+                              + [_i32, _i32, _c_p],
+    "tabicl_paged_bounds": [_c_p] * 2 + [_i64] * 3 + [_c_p, _i64, _i64, _c_p, _c_p, _i64, _c_p, _c_p] + [_i64] * 3
+                           + [_i32, _c_p],
+    "tabicl_paged_select": [_c_p] * 3 + [_i64] * 2 + [_c_p, _i64, _i64, _c_p, _c_p] + [_i64] * 9 + [_i32, _c_p, _i64, _c_p],
+    "tabicl_paged_select_workspace_bytes": [_i64] * 4,
+    "tabicl_paged_sparse_attn": [_c_p] * 4 + [_i64] * 3 + [_c_p, _i64, _i64, _c_p, _c_p, _i64, _c_p] + [_i64] * 11
+                                + [_f32, _i32, _i32, _c_p, _i64, _c_p],
+    "tabicl_paged_sparse_attn_workspace_bytes": [_i64] * 6,
+    "tabicl_paged_reserve": [_c_p, _i64, _i64] + [_c_p] * 5 + [_i64] * 3 + [_c_p, _i64, _c_p],
+    "tabicl_paged_release": [_c_p, _i64, _i64] + [_c_p] * 3 + [_i64] * 3 + [_c_p, _i64, _c_p],
+    "tabicl_paged_books_workspace_bytes": [_i64],
+    "tabicl_paged_slots": [_c_p, _i64, _i64] + [_c_p] * 4 + [_i64] * 4 + [_c_p],
+    "tabicl_paged_append_slots": [_c_p] * 2 + [_i64] * 3 + [_c_p] * 3 + [_i64] * 7 + [_i32, _c_p],
     "tabicl_attn_supported": [_i32, _i64, _i64, _i64, _i32, _i32],
     "tabicl_attn_last_error": [],
     "tabicl_attn_version": [],
@@ -93,7 +111,10 @@ _RESTYPES = {"tabicl_attn_last_error": ctypes.c_char_p, "tabicl_attn_version": c
              "tabicl_smallhead_bwd_workspace_bytes": ctypes.c_int64, "tabicl_hxf_workspace_bytes": ctypes.c_int64,
              "tabicl_icl_noalloc_scratch_bytes": ctypes.c_int64, "tabicl_icl_bwd_workspace_bytes": ctypes.c_int64,
              "tabicl_layer_workspace_bytes": ctypes.c_int64, "tabicl_paged_attn_workspace_bytes": ctypes.c_int64,
-             "tabicl_paged_evict_workspace_bytes": ctypes.c_int64}
+             "tabicl_paged_evict_workspace_bytes": ctypes.c_int64,
+             "tabicl_paged_attn_q8_workspace_bytes": ctypes.c_int64, "tabicl_paged_select_workspace_bytes": ctypes.c_int64,
+             "tabicl_paged_sparse_attn_workspace_bytes": ctypes.c_int64,
+             "tabicl_paged_books_workspace_bytes": ctypes.c_int64}
 
 
 class NativeLibraryError(RuntimeError):

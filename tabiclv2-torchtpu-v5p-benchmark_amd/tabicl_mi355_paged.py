@@ -8,6 +8,9 @@ once, that gets its train rows over time or answers one test row at a time keeps
     that each cached row drew;
   * paged_append, paged_gather (ops of these names): new rows into the pages, rows out of them;
   * paged_evict (op tabicl::paged_evict_out): cuts sequences to their rows of largest weight, in place;
+  * the same over pools of 8-bit codes, with `scales` (tabicl_mi355_paged8); attention over selected pages: paged_bounds,
+    paged_select, paged_sparse_attention (tabicl_mi355_sparse); page tables and slot maps kept on the GPU: paged_reserve,
+    paged_slots, paged_append_packed, paged_release (tabicl_mi355_books);
   * PagedIclKVCache: the pool, the page table and the lengths, with the surface of IclKVCache (append, query,
     attention_layer, query_blocks, usable as cached_query's icl_cache), and evict.
 
@@ -22,53 +25,23 @@ from __future__ import annotations
 from typing import Callable, Optional, Sequence, Union
 
 import torch
-import torch.autograd.forward_ad as _fwd
 import torch.nn.functional as F
 from torch import Tensor
 
 import tabicl_mi355_icl as _icl
 import tabicl_mi355_native as _nat
+import tabicl_mi355_paged8 as _p8
+import tabicl_mi355_pool as _pool
+from tabicl_mi355_books import paged_append_packed, paged_release, paged_reserve, paged_slots  # noqa: F401
+from tabicl_mi355_sparse import paged_bounds, paged_select, paged_sparse_attention  # noqa: F401
 
 
-# A call of few rows is over in 10 us on the GPU; the checks below take 4 us of a host core (12 with a test and a generator
-# expression per property).
-def _rows16(t: Tensor, es: int):
-    """(t, its (n, h, row) element strides) of [N, H, T, D] when its last dim is contiguous and it starts, and its other
-    dims step, in multiples of 16 bytes (what the kernels' loads need), else of a contiguous copy. A dim of one entry,
-    whose stride says nothing, counts as stride 0."""
-    n, h, r, d = t.stride()
-    shape = t.shape
-    n, h, r = n if shape[0] > 1 else 0, h if shape[1] > 1 else 0, r if shape[2] > 1 else 0
-    if (d == 1 or shape[3] == 1) and ((n | h | r) * es | t.data_ptr()) & 15 == 0:
-        return t, n, h, r
-    t = t.clone(memory_format=torch.contiguous_format)
-    return t, shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3]
+_rows16, _apart, _no_grad, _fwd_level = _pool.rows16, _pool.apart, _pool.no_grad, _pool.fwd_level
 
 
 def _pool_args(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, lead: int = 0):
-    """Checks a pool [pages, H, page_rows, D] (behind `lead` more dims) with its table and lengths; returns (pages, page
-    stride, page_rows, table, table stride, max_pages) as the entry points take them, then H, D, N, device index, dtype
-    code."""
-    shape, st = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 + lead or v_pages.shape != shape or v_pages.stride() != st:
-        raise ValueError(f"k_pages and v_pages must be [{'blocks, ' * lead}pages, H, page_rows, D] of one layout, got "
-                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
-    P, H, R, D = shape[lead:]
-    if st[-1] != 1 or st[-2] != D or (st[-3] != R * D and H > 1):
-        raise ValueError("a page [H, page_rows, D] must be contiguous")
-    if k_pages.dtype is not v_pages.dtype:
-        raise ValueError("k_pages and v_pages must share a dtype")
-    ts = table.shape
-    if table.dtype is not torch.int32 or len(ts) != 2 or (table.stride(1) != 1 and ts[1] > 1):
-        raise ValueError("table must be an int32 [N, max_pages] tensor with contiguous rows")
-    N, M = ts
-    if lengths.dtype is not torch.int32 or lengths.shape != (N,) or (N > 1 and lengths.stride(0) != 1):
-        raise ValueError(f"lengths must be a contiguous int32 tensor of {N} entries")
-    dev = k_pages.get_device()
-    if v_pages.get_device() != dev or table.get_device() != dev or lengths.get_device() != dev:
-        raise ValueError("the pool, table and lengths must be on one device")
-    return (P, st[lead] if P > 1 else H * R * D, R, table.data_ptr(), table.stride(0) if N > 1 else M, M), H, D, N, dev, \
-        _nat.dtype_code(k_pages.dtype)
+    """tabicl_mi355_pool.pool_args, then the dtype code of a bf16 or fp32 pool."""
+    return *_pool.pool_args(k_pages, v_pages, table, lengths, lead), _nat.dtype_code(k_pages.dtype)
 
 
 def _check_weights(weights: Tensor, N: int, cap: int, dev: int) -> int:
@@ -129,12 +102,6 @@ def _attn_launch(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
               None if ws is None else ws.data_ptr(), nbytes, _nat.stream_of(q))
 
 
-def _apart(q: Tensor, out: Tensor) -> Tensor:
-    """q, or a copy of it where `out` may overlap it: the kernels read q again after parts of the output are written (the
-    weights, and the tiles of one item in several workgroups)."""
-    return q.clone() if q.untyped_storage().data_ptr() == out.untyped_storage().data_ptr() else q
-
-
 # Three ops, since torch.compile refuses an op that returns a tensor and may or may not change another.
 @torch.library.custom_op("tabicl::paged_attn", mutates_args=())
 def _paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float) -> Tensor:
@@ -173,20 +140,9 @@ def _(q, k_pages, v_pages, table, lengths, scale, out, weights):  # noqa: ANN001
     return None
 
 
-def _fwd_level() -> int:
-    return getattr(_fwd, "_current_level", 0)
-
-
-def _no_grad(what: str, *ts: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise ValueError(f"{what} has no gradient (a serving operator): detach its inputs or call it under no_grad")
-    # forward mode: an op without a formula would drop the tangent and say nothing
-    if _fwd_level() >= 0 and any(t is not None and _fwd.unpack_dual(t).tangent is not None for t in ts):
-        raise ValueError(f"{what} has no gradient, nor one in forward mode (a serving operator): detach its inputs")
-
-
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor,
-                    weights: Optional[Tensor] = None, scale: Optional[float] = None, out: Optional[Tensor] = None) -> Tensor:
+                    weights: Optional[Tensor] = None, scale: Optional[float] = None, out: Optional[Tensor] = None,
+                    scales: Optional[Tensor] = None) -> Tensor:
     """softmax(q k^T scale) v of q [N, Hq, Tq, D] over the first lengths[n] rows of each sequence n of a paged pool
     (k_pages, v_pages [pages, H, page_rows, D]; Hq a multiple of H, query head h reads K/V head h // (Hq // H); table
     [N, max_pages] and lengths [N] int32; scale defaults to D^-0.5). Returns [N, Hq, Tq, D] in q's dtype, the pool's;
@@ -199,7 +155,12 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     The work is split over the cached rows, so one test row over one long table fills the GPU; a table slice
     table[:, :w] that covers the longest sequence spares the workgroups of pages nobody holds. For up to a few hundred
     query rows (each group of 64 reads the cache again); with weights, more go in slices where the workspace would pass
-    1 GiB. No gradient."""
+    1 GiB. No gradient.
+
+    scales (fp32 [pages, H, 2]): the pool holds e4m3 or int8 codes (tabicl_mi355_paged8). q is bf16 or fp32 then; the products
+    are exact, the sums fp32 (bf16 probabilities take part as two bf16 terms, fp32 ones as three). No weights."""
+    if scales is not None or k_pages.dtype in _pool.CODES:
+        return _p8.attention(q, k_pages, v_pages, table, lengths, weights, scale, out, scales)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, table, lengths, weights, out):
         o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
@@ -258,12 +219,18 @@ def _(k_pages, v_pages, table, lengths, k, v, count=None):  # noqa: ANN001
 
 
 def paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: Tensor, v: Tensor,
-                 count: Optional[Tensor] = None) -> None:
+                 count: Optional[Tensor] = None, scales: Optional[Tensor] = None) -> None:
     """Rows t < count[n] (int32 [N]; default all) of k, v [N, H, T, D] into rows lengths[n] + t of each sequence of the
     pool (any strides with a contiguous last dim, e.g. the heads of a K|V projection). lengths is read, not changed: the
     other blocks of a model append at the same rows. Rows that the table has no page for are dropped. A page that
-    is written must stand in the table once."""
-    if _nat.direct(k_pages, v_pages, table, lengths, k, v, count):
+    is written must stand in the table once.
+
+    scales (fp32 [pages, H, 2], written too): the pool holds e4m3 or int8 codes; k and v are bf16 or fp32. A page that rows
+    join keeps the larger of its scale and theirs, and the codes it holds are rounded again where it grows; infinities saturate,
+    NaN stays NaN in e4m3 and becomes 0 in int8."""
+    if scales is not None or k_pages.dtype in _pool.CODES:
+        _p8.append(k_pages, v_pages, table, lengths, k, v, count, None, scales)
+    elif _nat.direct(k_pages, v_pages, table, lengths, k, v, count):
         _append_launch(k_pages, v_pages, table, lengths, k, v, count)
         torch.autograd.graph.increment_version((k_pages, v_pages))
     else:
@@ -300,13 +267,19 @@ def _(k_pages, v_pages, table, lengths, rows):  # noqa: ANN001
     return k_pages.new_empty(shape), v_pages.new_empty(shape)
 
 
-def paged_gather(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, rows: int) -> tuple[Tensor, Tensor]:
+def paged_gather(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, rows: int, scales: Optional[Tensor] = None,
+                 dtype: Optional[torch.dtype] = None) -> tuple[Tensor, Tensor]:
     """k, v [N, H, rows, D] with the first min(lengths[n], rows) rows of each sequence side by side, 0 where a row has no
     page; what lies past a sequence's length is not written. For calls that the dense kernels answer faster (many query
-    rows), or to copy a cache out of its pool."""
+    rows), or to copy a cache out of its pool. In the pool's dtype; with scales (a pool of e4m3 or int8 codes) the values in
+    `dtype`, bf16 (the default: they are bf16 numbers) or fp32."""
     _no_grad("paged_gather", k_pages, v_pages)
     if k_pages.dim() != 4 or rows < 0:
         raise ValueError(f"paged_gather needs pools [pages, H, page_rows, D] and rows >= 0, got {tuple(k_pages.shape)}, {rows}")
+    if scales is not None or k_pages.dtype in _pool.CODES:
+        return _p8.gather(k_pages, v_pages, table, lengths, int(rows), scales, dtype)
+    if dtype is not None and dtype is not k_pages.dtype:
+        raise ValueError(f"a {k_pages.dtype} pool is gathered in its own dtype")
     if _nat.direct(k_pages, v_pages, table, lengths):
         return _gather(k_pages, v_pages, table, lengths, int(rows))
     return torch.ops.tabicl.paged_gather(k_pages, v_pages, table, lengths, int(rows))
@@ -410,13 +383,25 @@ class PagedIclKVCache(_icl.IclKVCache):
     track=True adds up, over every query of every block, the attention weight that each cached row draws (`weights`, fp32
     [sequences, capacity]); evict(keep) cuts the sequences to their heaviest rows and returns the emptied pages.
 
+    dtype torch.float8_e4m3fn or torch.int8: rows are held in 8 bits with a scale for each page and head (`scales`, fp32 [blocks,
+    pages, heads, 2]; tabicl_mi355_paged8), appended in bf16 or fp32 and queried in either. Not with track.
+
+    select=K: each query row of each head attends to the K pages of its table whose keys can give it the largest scores
+    (tabicl_mi355_sparse; all of them, where a table has no more), however many rows a query has. The bounds of the keys
+    (`bounds`, `bound_scales`) follow the appends. Not with track.
+
     Pages are given out on the host; the page table and the lengths live on the GPU, so a query costs no host sync. Calls
     follow each other on one stream. Only queries can be captured in a graph and replayed as the cache grows (the other calls
     keep books on the host)."""
 
     def __init__(self, sequences: int, blocks: int, heads: int, head_dim: int, max_rows: int, pages: int,
                  page_rows: int = 64, dtype: torch.dtype = torch.bfloat16, device: Union[str, torch.device] = "cuda",
-                 track: bool = False):
+                 track: bool = False, select: Optional[int] = None):
+        q8 = dtype in _pool.CODES
+        if track and (q8 or select is not None):
+            raise ValueError("a cache of 8-bit rows, or one whose queries select pages, tracks no weights")
+        if select is not None and select < 1:
+            raise ValueError(f"select must be at least 1, got {select}")
         if page_rows < 16 or page_rows & (page_rows - 1):
             raise ValueError(f"page_rows must be a power of two from 16 on, got {page_rows}")
         width = -(-max_rows // page_rows)
@@ -427,6 +412,12 @@ class PagedIclKVCache(_icl.IclKVCache):
             self.lengths = torch.zeros(blocks, sequences, dtype=torch.int32, device=device)
             self.weights = torch.zeros(sequences, width * page_rows, dtype=torch.float32, device=device) if track else None
             self._pages = torch.full((sequences, width), -1, dtype=torch.int32)  # the table's host copy
+            self.scales = torch.zeros(blocks, pages, heads, 2, dtype=torch.float32, device=device) if q8 else None
+            self.bounds = self.bound_scales = None
+            if select is not None:
+                self.bounds = torch.zeros(blocks, pages, heads, 2, head_dim, dtype=torch.int8, device=device)
+                self.bound_scales = torch.zeros(blocks, pages, heads, dtype=torch.float32, device=device)
+        self.select = select
         self.page_rows = page_rows
         self.capacity = width * page_rows
         self._held = [0] * sequences  # pages a sequence holds
@@ -493,12 +484,7 @@ class PagedIclKVCache(_icl.IclKVCache):
         S, NB, H, cap, D = self.shape
         if k.shape != v.shape or k.dim() != 4 or k.shape[0] != S or k.shape[1] != H or k.shape[3] != D:
             raise ValueError(f"append expects k/v [{S}, {H}, T, {D}], got {tuple(k.shape)} / {tuple(v.shape)}")
-        if k.dtype != self.keys.dtype or v.dtype != self.keys.dtype:
-            raise ValueError(f"append expects {self.keys.dtype} (cast before appending)")
-        if not 0 <= block < NB:
-            raise ValueError(f"block {block} out of range [0, {NB})")
-        _no_grad("PagedIclKVCache.append", k, v)
-        _nat.require_device(k, v, self.keys)
+        self._check_rows(block, k, v)
         T = k.shape[2]
         new = [T] * S if rows is None else [int(r) for r in rows]
         if len(new) != S or any(not 0 <= r <= T for r in new):
@@ -506,9 +492,57 @@ class PagedIclKVCache(_icl.IclKVCache):
         ends = [a + n for a, n in zip(self._rows[block], new)]
         self.reserve(ends)
         count = None if rows is None else torch.tensor(new, dtype=torch.int32, device=self.table.device)
-        paged_append(self.keys[block], self.values[block], self.table, self.lengths[block], k, v, count)
-        self.lengths[block] += T if count is None else count
+        paged_append(self.keys[block], self.values[block], self.table, self.lengths[block], k, v, count, **self._scales_of(block))
+        self._grown(block, T if count is None else count, T)
         self._rows[block] = ends
+
+    def append_packed(self, block: int, k: Tensor, v: Tensor, rows: Sequence[int]) -> None:
+        """append of packed rows k, v [total, H, d]: rows[0] rows of the first sequence, then rows[1] of the second, and so
+        on; none is padded."""
+        self._own("append_packed")
+        S, NB, H, cap, D = self.shape
+        new = [int(r) for r in rows]
+        if len(new) != S or min(new, default=0) < 0:
+            raise ValueError(f"rows must be {S} counts of at least 0, got {new}")
+        total = sum(new)
+        if k.shape != v.shape or k.shape != (total, H, D):
+            raise ValueError(f"append_packed expects k/v [{total}, {H}, {D}], got {tuple(k.shape)} / {tuple(v.shape)}")
+        self._check_rows(block, k, v)
+        ends = [a + n for a, n in zip(self._rows[block], new)]
+        self.reserve(ends)
+        count = torch.tensor(new, dtype=torch.int32, device=self.table.device)
+        slots, starts = paged_slots(self.table, self.lengths[block], count, total, self.keys.shape[1], self.page_rows)
+        paged_append_packed(self.keys[block], self.values[block], self.table, self.lengths[block], count, k, v, slots, starts,
+                            **self._scales_of(block))
+        self._grown(block, count, max(new, default=0))
+        self._rows[block] = ends
+
+    def _check_rows(self, block: int, k: Tensor, v: Tensor) -> None:
+        if k.dtype != self._row_dtype(k.dtype) or v.dtype != k.dtype:
+            raise ValueError(f"append expects {self._row_dtype(k.dtype)} (cast before appending)")
+        if not 0 <= block < self.shape[1]:
+            raise ValueError(f"block {block} out of range [0, {self.shape[1]})")
+        _no_grad("PagedIclKVCache.append", k, v)
+        _nat.require_device(k, v, self.keys)
+
+    def _scales_of(self, block: int) -> dict:
+        return {} if self.scales is None else {"scales": self.scales[block]}
+
+    def _grown(self, block: int, count, most: int) -> None:  # noqa: ANN001
+        """The lengths (and bounds) of a block after an append of `count` rows per sequence, at most `most`."""
+        lengths = self.lengths[block]
+        if self.bounds is not None:
+            paged_bounds(self.keys[block], self.table, lengths + count, self.bounds[block], self.bound_scales[block], lengths, most,
+                         **self._scales_of(block))
+        lengths += count
+
+    def _row_dtype(self, dtype: torch.dtype) -> torch.dtype:
+        if self.scales is None:
+            return self.keys.dtype
+        return dtype if dtype in (torch.bfloat16, torch.float32) else torch.bfloat16
+
+    def _attn_dtype(self, dtype: torch.dtype) -> torch.dtype:
+        return super()._attn_dtype(dtype) if self.scales is None else torch.promote_types(dtype, torch.bfloat16)
 
     def append_projected(self, block: int, x: Tensor, in_proj_weight: Tensor, in_proj_bias: Optional[Tensor] = None,
                          rows: Optional[Sequence[int]] = None) -> None:
@@ -539,18 +573,23 @@ class PagedIclKVCache(_icl.IclKVCache):
         elif valid_kv_len is not None and (captured or int(valid_kv_len) < longest):
             longest = max(0, min(int(valid_kv_len), self.capacity))
             lengths = lengths.clamp(max=longest)
-        dt = self.keys.dtype
-        if torch.promote_types(q.dtype, dt) != dt:
+        dt = self.keys.dtype if self.scales is None else self._attn_dtype(q.dtype)
+        if torch.promote_types(q.dtype, dt) != dt or dt not in (torch.bfloat16, torch.float32):
             raise ValueError(f"q is {q.dtype}, wider than the {dt} cache: cast it")
         w = max(1, -(-longest // self.page_rows))
         if captured:
             w = self.table.shape[1]
-        elif q.shape[2] >= _DENSE_QUERY_ROWS and S * q.shape[2] >= _DENSE_ALL_ROWS \
+        if self.select is not None and w > self.select:
+            q, table, eight = q.to(dt), self.table[:, :w], self._scales_of(block)
+            index = paged_select(q, self.bounds[block], self.bound_scales[block], table, lengths, self.page_rows, self.select)
+            return paged_sparse_attention(q, self.keys[block], self.values[block], table, lengths, index, None, out, **eight)
+        if not captured and q.shape[2] >= _DENSE_QUERY_ROWS and S * q.shape[2] >= _DENSE_ALL_ROWS \
                 and S * q.shape[2] * longest >= _DENSE_SCORES and D == 64 and q.shape[1] == H and dt == torch.bfloat16 \
                 and self.weights is None:
             return self._gathered(block, q.to(dt), lengths, longest, out)
         weights = None if self.weights is None else self.weights[:, :w * self.page_rows]
-        return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out)
+        return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out,
+                               **self._scales_of(block))
 
     def _gathered(self, block: int, q: Tensor, lengths: Tensor, longest: int, out: Optional[Tensor]) -> Tensor:
         """query by the dense kernel, over the rows of one run of sequences after the other side by side."""
@@ -569,7 +608,7 @@ class PagedIclKVCache(_icl.IclKVCache):
             rows = max(1, rows)
             run = slice(start, stop)
             k, v = paged_gather(self.keys[block], self.values[block], self.table[run, :-(-rows // self.page_rows)], lengths[run],
-                                rows)
+                                rows, **self._scales_of(block))
             o = self._dense(q[run], k, v, lengths[run], None if out is None else out[run])
             del k, v  # before the next run's
             start = stop
