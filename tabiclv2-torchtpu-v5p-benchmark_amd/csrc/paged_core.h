@@ -4,6 +4,8 @@
 #include "common.h"
 #include "paged.h"
 
+#include <type_traits>
+
 namespace {
 
 __device__ __forceinline__ int pool_length(const PagedPool& c, int n) {
@@ -53,6 +55,13 @@ constexpr float PA_REF0 = -3.4028234663852886e38f;
 // 10,000 rows took 97 us at 8 workgroups per CU and 146 at 2, one sequence of 45,000 rows 39 and 27; this way 84 and 26.)
 constexpr int PA_UNIT = 128, PA_WHOLE = 1024;
 
+// Units that an item of 8-bit rows counts for beyond its own, where some sequence is shorter than a workgroup's share: a
+// workgroup that begins several items has the latency of each beginning, half of what a turn of bf16 rows has to hide it
+// behind (us with 0 / 2 / 4 / 6 / 8 units, one row of 64 dims: 64 sequences of 100 to 3,000 rows 47 / 33 / 27 / 22 / 22, 16 of 500
+// to 10,000 27 / 22 / 21 / 20 / 20; of 128 dims and fp32, 12 query rows, 46 / 38 / 36 / 34 / 34; where all are longer they cost up to
+// 13%: 64 query rows over 8 x 5,000 30 / 36 / 32 / 34 / 33).
+constexpr int PA_EXTRA8 = 6;
+
 struct PagedSplit {
   int groups;    // G, or 0: a workgroup of eight waves for each item
   int least;     // units a workgroup takes at least
@@ -69,6 +78,7 @@ struct PagedSplit {
 __device__ __forceinline__ int pa_len(const PagedAttn& a, int n) { return a.pool.pages > 0 ? pool_length(a.pool, n) : 0; }
 
 __device__ __forceinline__ int pa_units(int len) { return (len + PA_UNIT - 1) / PA_UNIT; }
+__device__ __forceinline__ int pa_each(int len, int extra) { return len ? pa_units(len) + extra : 0; }
 
 // Inclusive sum over the lanes of a wave, in the registers.
 __device__ __forceinline__ int wave_sum_scan(int x) {
@@ -84,18 +94,31 @@ __device__ __forceinline__ int wave_sum_scan(int x) {
 // The units of the sequences, 64 sequences at a time, one per lane.
 struct PagedUnits {
   const PagedAttn& a;
-  int per, lane;  // items of a sequence
+  int per, extra, lane;  // items of a sequence; units that an item counts for beyond its rows
   int own, upto;  // sequence `lane`: its units, and theirs up to it
   int total;      // of all sequences
   __device__ __forceinline__ int load(int base) const {
     const int n = base + lane;
-    return n < a.N ? pa_units(pa_len(a, n)) * per : 0;
+    return n < a.N ? pa_each(pa_len(a, n), extra) * per : 0;
   }
-  __device__ __forceinline__ PagedUnits(const PagedAttn& args, int items, int l) : a(args), per(items), lane(l) {
+  __device__ __forceinline__ void count() {
     own = load(0);
     upto = wave_sum_scan(own);
     total = __builtin_amdgcn_readlane(upto, 63);
     for (int base = 64; base < a.N; base += 64) total += __builtin_amdgcn_readlane(wave_sum_scan(load(base)), 63);
+  }
+  __device__ __forceinline__ PagedUnits(const PagedAttn& args, int items, int l) : a(args), per(items), extra(0), lane(l) { count(); }
+  // Counts again with `more` units for each item, if there is a sequence with rows of fewer than `share` units.
+  __device__ __forceinline__ void weigh(int share, int more) {
+    const int64_t least = (int64_t)share * per;
+    bool some = wave_any(own > 0 && own < least);
+    for (int base = 64; base < a.N && !some; base += 64) {
+      const int u = load(base);
+      some = wave_any(u > 0 && u < least);
+    }
+    if (!some) return;
+    extra = more;
+    count();
   }
   // the sequence that unit t < total belongs to, and its first unit
   __device__ __forceinline__ int find(int t, int* first) const {
@@ -282,31 +305,39 @@ __device__ __forceinline__ uint2 codes_bf16<I8>(uint32_t x) {
                __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x07060302u)};
 }
 
-// The V operands of 32 keys (subtiles s and s + 1), one for each of the D / 16 columns of a lane: bytes of four rows are
-// regrouped by column, then converted.
+// The V operands of 32 keys (subtiles s and s + 1), one for each of the D / 16 columns of a lane. e4m3: bytes of four rows are
+// regrouped by column, then converted in pairs; int8: converted byte by byte, then regrouped.
 template <typename C, int D>
 __device__ __forceinline__ void paged_operands8(const PagedTile8<D>& t, int s, bf16x8* va) {
-  constexpr int DE = D / 16;
-  uint32_t col[2][DE];
+  constexpr int DE = D / 16, VW = PagedTile8<D>::VW, DP = DE < 4 ? DE : 4;  // columns of a dword
+  uint32_t w[DE][4];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int w = 0; w < PagedTile8<D>::VW; ++w) {
-      const uint32_t *r0 = t.v[s + u][0], *r1 = t.v[s + u][1], *r2 = t.v[s + u][2], *r3 = t.v[s + u][3];
-      const uint32_t lo01 = __builtin_amdgcn_perm(r1[w], r0[w], 0x05010400u), lo23 = __builtin_amdgcn_perm(r3[w], r2[w], 0x05010400u);
-      col[u][4 * w] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
-      col[u][4 * w + 1] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
-      if constexpr (DE >= 4) {
-        const uint32_t hi01 = __builtin_amdgcn_perm(r1[w], r0[w], 0x07030602u), hi23 = __builtin_amdgcn_perm(r3[w], r2[w], 0x07030602u);
-        col[u][4 * w + 2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
-        col[u][4 * w + 3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+    for (int v = 0; v < VW; ++v) {
+      const uint32_t r[4] = {t.v[s + u][0][v], t.v[s + u][1][v], t.v[s + u][2][v], t.v[s + u][3][v]};
+      if constexpr (std::is_same<C, I8>::value) {
+#pragma unroll
+        for (int e = 0; e < DP; ++e)
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            w[4 * v + e][2 * u + p] = __builtin_amdgcn_perm(__float_as_uint((float)(int8_t)(r[2 * p + 1] >> (8 * e))),
+                                                            __float_as_uint((float)(int8_t)(r[2 * p] >> (8 * e))), 0x07060302u);
+      } else {
+#pragma unroll
+        for (int half = 0; half < DP / 2; ++half) {
+          const uint32_t sel = half ? 0x07030602u : 0x05010400u;
+          const uint32_t x01 = __builtin_amdgcn_perm(r[1], r[0], sel), x23 = __builtin_amdgcn_perm(r[3], r[2], sel);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint2 y = codes_bf16<C>(__builtin_amdgcn_perm(x23, x01, e ? 0x07060302u : 0x05040100u));
+            w[4 * v + 2 * half + e][2 * u] = y.x, w[4 * v + 2 * half + e][2 * u + 1] = y.y;
+          }
+        }
       }
     }
 #pragma unroll
-  for (int e = 0; e < DE; ++e) {
-    const uint2 x = codes_bf16<C>(col[0][e]), y = codes_bf16<C>(col[1][e]);
-    va[e] = __builtin_bit_cast(bf16x8, (uint4{x.x, x.y, y.x, y.y}));
-  }
+  for (int e = 0; e < DE; ++e) va[e] = __builtin_bit_cast(bf16x8, (uint4{w[e][0], w[e][1], w[e][2], w[e][3]}));
 }
 
 __device__ __forceinline__ float upper_half(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
@@ -757,7 +788,8 @@ constexpr int pa_waves(int D, int QT) { return D == 128 && QT > 1 ? 1 : 2; }
 template <typename T, typename C, int D, int QT, bool W>
 __global__ __launch_bounds__(256, pa_waves(D, QT)) void pa_kernel(PagedAttn a, PagedSplit z) {
   const int per = a.pool.H * z.qtiles;
-  const PagedUnits units(a, per, threadIdx.x & 63);
+  PagedUnits units(a, per, threadIdx.x & 63);
+  if constexpr (sizeof(C) == 1) units.weigh(PagedShares(z, units.total).share, PA_EXTRA8);
   const PagedShares shares(z, units.total);
   if ((int)blockIdx.x >= shares.groups) return;
   int unit = shares.first(blockIdx.x);
@@ -765,12 +797,12 @@ __global__ __launch_bounds__(256, pa_waves(D, QT)) void pa_kernel(PagedAttn a, P
   while (unit < end) {
     int first;
     const int n = units.find(unit, &first);
-    const int len = __builtin_amdgcn_readfirstlane(pa_len(a, n)), each = pa_units(len);
+    const int len = __builtin_amdgcn_readfirstlane(pa_len(a, n)), each = pa_each(len, units.extra);
     const int item = (unit - first) / each, u0 = unit - first - item * each;
     const int u1 = u0 + end - unit < each ? u0 + end - unit : each;
     if (threadIdx.x == 0 && u0 == 0) z.ends[n * per + item].x = blockIdx.x;
     if (threadIdx.x == 0 && u1 == each) z.ends[n * per + item].y = blockIdx.x;
-    pa_segment<T, C, D, QT, W, false, 4>(a, z, n, item / z.qtiles, 0, item % z.qtiles, u0 * PA_UNIT,
+    pa_segment<T, C, D, QT, W, false, 4>(a, z, n, item / z.qtiles, 0, item % z.qtiles, u0 * PA_UNIT < len ? u0 * PA_UNIT : len,
                                          u1 * PA_UNIT < len ? u1 * PA_UNIT : len,
                                          u1 - u0 < each ? 2 * blockIdx.x + (u0 == 0) : -1);
     unit += u1 - u0;

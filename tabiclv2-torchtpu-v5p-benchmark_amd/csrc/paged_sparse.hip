@@ -10,6 +10,8 @@
 #include "launch.h"
 #include "paged_core.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -58,10 +60,124 @@ __device__ __forceinline__ void values16<I8>(uint4 u, float* x) {
   for (int i = 0; i < 16; ++i) x[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
 }
 
-// One wave per page and head. Bound by the bytes of K.
+// The largest and the smallest value of each dim in a lane's 16 bytes, over the rows added. Two 16-bit numbers at a time:
+// 8-bit codes take the upper byte of one (even and odd bytes apart; what the lower byte holds decides nothing). Numbers in
+// sign and magnitude (bf16, e4m3) order as integers apart from their signs: the largest as signed is the largest value, if there
+// is one >= 0; the largest as unsigned the smallest, if there is a negative one; else the smallest as unsigned is either. A NaN
+// shows as a magnitude beyond infinity (or the e4m3 NaN), and its page is gone through again value by value. (fp32 values one
+// by one, with unpacking: 12 instructions for 16 bytes instead of 28 in bf16; 45,000 rows of 8 sequences and heads 79 -> 68 us,
+// bound by the reads of K then.)
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+template <typename F>
+__device__ __forceinline__ uint32_t across(uint32_t x, int lanes, F f) {
+  if (lanes == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return f(r[0], r[1]);
+  }
+  if (lanes == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return f(r[0], r[1]);
+  }
+  return f(x, (uint32_t)__shfl_xor((int)x, lanes, 64));
+}
+__device__ __forceinline__ uint32_t max_i16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+}
+__device__ __forceinline__ uint32_t min_i16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+}
+__device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ uint32_t min_u16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ uint32_t max_f32(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+__device__ __forceinline__ uint32_t min_f32(uint32_t a, uint32_t b) { return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b))); }
+
+// One of N registers by a number that differs between lanes (by masks: a choice between array elements would become an
+// address, and the array go to memory).
+template <int N>
+__device__ __forceinline__ uint32_t choose(const uint32_t* x, int i) {
+  if constexpr (N == 1) {
+    return x[0];
+  } else {
+    const uint32_t upper = i & (N / 2) ? 0xffffffffu : 0u;
+    return (choose<N / 2>(x + N / 2, i) & upper) | (choose<N / 2>(x, i) & ~upper);
+  }
+}
+
 template <typename C>
+struct Extremes {
+  static constexpr int ES = sizeof(C), W = ES == 1 ? 8 : 4, VPC = 16 / ES;  // registers, values of 16 bytes
+  static constexpr bool SIGNED = std::is_same<C, I8>::value, FLOAT = ES == 4;
+  uint32_t a[W], b[W], c[W];  // max signed, max unsigned, min unsigned; int8, fp32: max, min
+  __device__ __forceinline__ Extremes() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      a[i] = FLOAT ? 0xff800000u : 0x80008000u;
+      b[i] = FLOAT ? 0x7f800000u : SIGNED ? 0x7fff7fffu : 0u;
+      c[i] = 0xffffffffu;
+    }
+  }
+  __device__ __forceinline__ void merge(int i, uint32_t x, uint32_t y, uint32_t z) {
+    a[i] = FLOAT ? max_f32(a[i], x) : max_i16(a[i], x);
+    b[i] = FLOAT ? min_f32(b[i], y) : SIGNED ? min_i16(b[i], y) : max_u16(b[i], y);
+    if (!FLOAT && !SIGNED) c[i] = min_u16(c[i], z);
+  }
+  __device__ __forceinline__ void add(uint4 u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (ES == 1) {
+        const uint32_t even = w[i] << 8;
+        merge(2 * i, even, even, even);
+        merge(2 * i + 1, w[i], w[i], w[i]);
+      } else {
+        merge(i, w[i], w[i], w[i]);
+      }
+    }
+  }
+  __device__ __forceinline__ void join(int lanes) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      a[i] = across(a[i], lanes, FLOAT ? max_f32 : max_i16);
+      b[i] = across(b[i], lanes, FLOAT ? min_f32 : SIGNED ? min_i16 : max_u16);
+      if (!FLOAT && !SIGNED) c[i] = across(c[i], lanes, min_u16);
+    }
+  }
+  // The extremes of value e (of the 16 bytes; e differs between lanes); false where a NaN hides them.
+  __device__ __forceinline__ bool value(int e, float* hi, float* lo) const {
+    if constexpr (FLOAT) {
+      *hi = __uint_as_float(choose<4>(a, e)), *lo = __uint_as_float(choose<4>(b, e));
+      return true;  // fmaxf and fminf pass a NaN by
+    } else {
+      const int w = ES == 1 ? e / 4 * 2 + (e & 1) : e / 2, shift = (ES == 1 ? e >> 1 & 1 : e & 1) * 16;
+      const uint32_t x = choose<W>(a, w) >> shift & 0xffffu, y = choose<W>(b, w) >> shift & 0xffffu;
+      if constexpr (SIGNED) {
+        *hi = (float)(int8_t)(x >> 8), *lo = (float)(int8_t)(y >> 8);
+        return true;
+      } else {
+        const uint32_t z = choose<W>(c, w) >> shift & 0xffffu, p = x & 0x8000u ? z : x, m = y & 0x8000u ? y : z;
+        if constexpr (ES == 2) {
+          *hi = __uint_as_float(p << 16), *lo = __uint_as_float(m << 16);
+          return !((x & 0x8000u) == 0 && x > 0x7f80u) && y <= 0xff80u;
+        } else {
+          const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(p >> 8 | (m & 0xff00u), false);
+          *hi = v[0], *lo = v[1];
+          return x >> 8 != 0x7f && y >> 8 != 0xff;
+        }
+      }
+    }
+  }
+};
+
+// One wave per page and head. Bound by the bytes of K.
+template <typename C, int D>
 __global__ __launch_bounds__(256) void paged_bounds_kernel(PagedBounds a) {
-  constexpr int VPC = 16 / sizeof(C), ES = sizeof(C);  // values of a lane's 16 bytes
+  constexpr int ES = sizeof(C), VPC = 16 / ES, LPR = D / VPC, RPP = 64 / LPR;  // values of 16 bytes, lanes of a row, rows of a pass
+  constexpr int DPL = D < 64 ? 1 : D / 64;                                     // dims that a lane finishes
   const PagedPool& c = a.pool;
   const int n = blockIdx.y, item = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int h = item % c.H, len = pool_length(c, n), R = 1 << c.shift;
@@ -72,60 +188,69 @@ __global__ __launch_bounds__(256) void paged_bounds_kernel(PagedBounds a) {
   const int page = c.table[n * c.table_sn + p];
   if (page < 0 || page >= c.pages) return;
   const int live = len - row0 < R ? (int)(len - row0) : R;
-  const int lpr = c.D * ES / 16, rpp = 64 / lpr;  // lanes of a row, rows of a pass
-  const char* k = (const char*)c.k + (page * c.page_sp + (int64_t)h * R * c.D) * ES + lane % lpr * 16;
-  float lo[VPC], hi[VPC];
-#pragma unroll
-  for (int e = 0; e < VPC; ++e) lo[e] = -TA_NEG_INF, hi[e] = TA_NEG_INF;
-  auto add = [&](uint4 u) {
-    float x[VPC];
-    values16<C>(u, x);
-#pragma unroll
-    for (int e = 0; e < VPC; ++e) lo[e] = fminf(lo[e], x[e]), hi[e] = fmaxf(hi[e], x[e]);  // a NaN changes neither
-  };
-  int r = lane / lpr;
-  for (; r + 7 * rpp < live; r += 8 * rpp) {
+  const char* k = (const char*)c.k + (page * c.page_sp + (int64_t)h * R * D) * ES + lane % LPR * 16;
+  Extremes<C> ext;
+  int r = lane / LPR;
+  for (; r + 7 * RPP < live; r += 8 * RPP) {
     uint4 u[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = ldg16(k + (int64_t)(r + i * rpp) * c.D * ES);
+    for (int i = 0; i < 8; ++i) u[i] = ldg16(k + (int64_t)(r + i * RPP) * D * ES);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) add(u[i]);
+    for (int i = 0; i < 8; ++i) ext.add(u[i]);
   }
-  for (; r < live; r += rpp) add(ldg16(k + (int64_t)r * c.D * ES));
-  for (int x = lpr; x < 64; x <<= 1)
+  for (; r < live; r += RPP) ext.add(ldg16(k + (int64_t)r * D * ES));
 #pragma unroll
-    for (int e = 0; e < VPC; ++e) lo[e] = fminf(lo[e], __shfl_xor(lo[e], x, 64)), hi[e] = fmaxf(hi[e], __shfl_xor(hi[e], x, 64));
-  if constexpr (ES == 1) {
-    const float s = a.scales[((int64_t)page * c.H + h) * 2];
+  for (int x = LPR; x < 64; x <<= 1) ext.join(x);
+  // every lane has the extremes of its VPC dims now, and finishes DPL of them (D = 32: two lanes or more the same one)
+  const int e0 = lane / LPR * DPL % VPC, dim = lane % LPR * VPC + e0;
+  float hi[DPL], lo[DPL];
+  bool fine = true;
 #pragma unroll
-    for (int e = 0; e < VPC; ++e) lo[e] *= s, hi[e] *= s;
+  for (int i = 0; i < DPL; ++i) fine &= ext.value(e0 + i, &hi[i], &lo[i]);
+  if (wave_any(!fine)) {
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) hi[i] = TA_NEG_INF, lo[i] = -TA_NEG_INF;
+    for (int row = 0; row < live; ++row) {
+      float x[VPC];
+      values16<C>(ldg16(k + (int64_t)row * D * ES), x);
+#pragma unroll
+      for (int e = 0; e < VPC; ++e)
+#pragma unroll
+        for (int i = 0; i < DPL; ++i)
+          if (e == e0 + i) hi[i] = fmaxf(hi[i], x[e]), lo[i] = fminf(lo[i], x[e]);
+    }
   }
   uint32_t most = 0;
 #pragma unroll
-  for (int e = 0; e < VPC; ++e) {
-    if (hi[e] < lo[e]) lo[e] = hi[e] = 0.f;  // a dim of NaN alone
-    most = umax(most, umax(finite_bits(lo[e]), finite_bits(hi[e])));
+  for (int i = 0; i < DPL; ++i) {
+    if constexpr (ES == 1) {
+      const float s = a.scales[((int64_t)page * c.H + h) * 2];
+      hi[i] *= s, lo[i] *= s;
+    }
+    if (hi[i] < lo[i]) hi[i] = lo[i] = 0.f;  // a dim of NaN alone
+    most = umax(most, umax(finite_bits(lo[i]), finite_bits(hi[i])));
   }
-  for (int x = 1; x < lpr; x <<= 1) most = umax(most, (uint32_t)__shfl_xor(most, x, 64));
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) most = across(most, x, umax);
   const int e2 = step_exponent(most);
   const float inv = pow2(-e2);
-  if (lane >= lpr) return;
-  uint32_t wh[(VPC + 3) / 4], wl[(VPC + 3) / 4];
+  int8_t* out = a.bounds + ((int64_t)page * c.H + h) * 2 * D + dim;
 #pragma unroll
-  for (int e = 0; e < VPC; ++e) {
+  for (int i = 0; i < DPL; ++i) {
     // infinite bounds, and finite ones beyond the largest scale, at the end of the range
-    const int x = (int)fminf(fmaxf(ceilf(hi[e] * inv), -127.f), 127.f), y = (int)fminf(fmaxf(floorf(lo[e] * inv), -127.f), 127.f);
-    if (e % 4 == 0) wh[e / 4] = wl[e / 4] = 0;
-    wh[e / 4] |= (uint32_t)(x & 255) << (8 * (e % 4));
-    wl[e / 4] |= (uint32_t)(y & 255) << (8 * (e % 4));
-  }
-  int8_t* out = a.bounds + ((int64_t)page * c.H + h) * 2 * c.D + lane * VPC;
-#pragma unroll
-  for (int w = 0; w < VPC / 4; ++w) {
-    *(uint32_t*)(out + 4 * w) = wh[w];
-    *(uint32_t*)(out + c.D + 4 * w) = wl[w];
+    out[i] = (int8_t)(int)fminf(fmaxf(ceilf(hi[i] * inv), -127.f), 127.f);
+    out[D + i] = (int8_t)(int)fminf(fmaxf(floorf(lo[i] * inv), -127.f), 127.f);
   }
   if (lane == 0) a.bound_scales[(int64_t)page * c.H + h] = pow2(e2);
+}
+
+template <int D>
+void launch_bounds(const PagedBounds& a, int format, dim3 grid, hipStream_t stream) {
+  const dim3 nt(256);
+  if (format == 0) hipLaunchKernelGGL((paged_bounds_kernel<bf16, D>), grid, nt, 0, stream, a);
+  else if (format == 1) hipLaunchKernelGGL((paged_bounds_kernel<float, D>), grid, nt, 0, stream, a);
+  else if (format == 2) hipLaunchKernelGGL((paged_bounds_kernel<E4M3, D>), grid, nt, 0, stream, a);
+  else hipLaunchKernelGGL((paged_bounds_kernel<I8, D>), grid, nt, 0, stream, a);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -134,7 +259,10 @@ __global__ __launch_bounds__(256) void paged_bounds_kernel(PagedBounds a) {
 // A workgroup of 16 waves takes up to TT query rows of one sequence and K/V head: the bounds of 16 pages for 16 (query row,
 // head of the group) pairs at a time on the 8-bit matrix unit, kept as ordered codes [TT][pages] in LDS (0: no such page); then
 // the K-th largest code of each query row by four 8-bit digits of a histogram, 16 / TT waves a row; then the pages above it,
-// and the first ones equal to it, in order.
+// and the first ones equal to it, in order. Bound by its chain of loads and barriers (64 query rows of 704 pages: a few MB), so
+// the first tiles' table entries and bounds are on their way before the queries are looked at, the histograms of all
+// digits are cleared at once, every wave of a row finds the digit for itself (one barrier a digit), and there is little code:
+// most of it runs once, as fast as instructions come in (four tiles at a time instead of one, twice: 12.7 us for 11.8).
 constexpr int PS_NW = 16, PS_LDS = 32768;  // codes kept in LDS
 
 __device__ __forceinline__ uint32_t bound_code(float x) {  // larger bound, larger code; none is 0
@@ -146,173 +274,246 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
+// U tiles of 16 pages, a wave's every 16th: their bounds as operands, their scales and whether they are there. The table is read
+// up to its width, not the sequence's, so that its entries need not wait for the length.
+template <int KB, int U>
+struct BoundTiles {
+  int page[U];
+  i32x4 b[U][KB];
+  float scale[U];
+  uint32_t have[U];
+  __device__ __forceinline__ void pages(const PagedSelect& a, const int32_t* table, int tile, int lr) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t p = ((int64_t)tile + u * PS_NW) * 16 + lr;
+      page[u] = p < a.pool.max_pages ? table[p] : -1;
+    }
+  }
+  __device__ __forceinline__ void bounds(const PagedSelect& a, int h, int tile, int P, int lr, int lg) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = page[u] >= 0 && page[u] < a.pool.pages && (tile + u * PS_NW) * 16 + lr < P;
+      const int64_t at = (int64_t)(in ? page[u] : 0) * a.pool.H + h;
+      have[u] = (uint32_t)__ballot(in) & 0xffffu;
+      scale[u] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KB; ++i) b[u][i] = i32x4{0, 0, 0, 0};
+      if (in) {
+        scale[u] = a.bound_scales[at];
+#pragma unroll
+        for (int i = 0; i < KB; ++i) b[u][i] = *(const i32x4*)(a.bounds + (at * KB + i) * 64 + lg * 16);
+      }
+    }
+  }
+};
+
+// Grid (tiles of TT = 2^tshift query rows, H, N). per16: 256 / G, rounded up (x / G = x * per16 >> 8 for x < 16; G <= 16).
 template <typename T, int D, bool GLOBAL>
-__global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a, int TT, int qtiles, uint32_t* store) {
-  extern __shared__ uint32_t lds_codes[];
-  constexpr int KB = 2 * D / 64;  // products of 64 bounds
+__global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a, int tshift, int per16, uint32_t* store) {
+  extern __shared__ uint32_t lds[];  // [4][TT][256] histograms, [TT][max_pages] codes
+  constexpr int KB = 2 * D / 64, U = 1, NV = (D + 63) / 64;
   __shared__ __attribute__((aligned(16))) int8_t sh_q[16][2 * D];
-  __shared__ float sh_inv[16];
-  __shared__ int hist[16][256], pick[16][2], part[PS_NW][2];
+  __shared__ uint32_t sh_most[16];
+  __shared__ int2 part[PS_NW];
   const PagedPool& c = a.pool;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
-  const int qt = blockIdx.x % qtiles, nh = blockIdx.x / qtiles, n = nh / c.H, h = nh % c.H, t0 = qt * TT;
+  const int n = blockIdx.z, h = blockIdx.y, TT = 1 << tshift, t0 = blockIdx.x << tshift;
   const int G = a.Hq / c.H, R = 1 << c.shift, len = __builtin_amdgcn_readfirstlane(pool_length(c, n));
   const int P = (len + R - 1) >> c.shift, stride = c.max_pages;
-  uint32_t* codes = GLOBAL ? store + (int64_t)blockIdx.x * TT * stride : lds_codes;
+  const int32_t* table = c.table + n * c.table_sn;
+  int* hist = (int*)lds;
+  const int64_t nh = (int64_t)n * c.H + h;
+  uint32_t* codes = GLOBAL ? store + (nh * a.Tq + t0) * stride : lds + (1024 << tshift);
+  BoundTiles<KB, U> now, next;
+  now.pages(a, table, wave, lr);
+  next.pages(a, table, wave + U * PS_NW, lr);
+  now.bounds(a, h, wave, P, lr, lg);
+
+  // column `wave` of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
   const char* q = (const char*)a.q + (n * a.q_sn + (int64_t)h * G * a.q_sh) * sizeof(T);
-  auto value = [&](int g, int t, int d) {
-    return (float)*(const T*)(q + (g * a.q_sh + t * a.q_st + d) * (int64_t)sizeof(T));
-  };
-
-  // the step of each query row: wave t looks at the group's heads
-  if (wave < TT) {
-    uint32_t most = 0;
-    if (t0 + wave < a.Tq)
-      for (int i = lane; i < G * D; i += 64) most = umax(most, finite_bits(value(i / D, t0 + wave, i % D)));
+  const bool wide = G > 16;
+  const int qrow = wide ? 0 : wave * per16 >> 8, qhead = wave - qrow * G;
+  float x[NV];
+  auto column = [&](int g0) {
+    const int g = g0 + qhead;
+    const bool in = qrow < TT && t0 + qrow < a.Tq && g < G;
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) most = umax(most, (uint32_t)__shfl_xor(most, x, 64));
-    if (lane == 0) sh_inv[wave] = pow2(-step_exponent(most));
+    for (int i = 0; i < NV; ++i) {
+      const int d = lane + 64 * i;
+      x[i] = in && d < D ? (float)*(const T*)(q + (g * a.q_sh + (t0 + qrow) * a.q_st + d) * (int64_t)sizeof(T)) : 0.f;
+    }
+  };
+  uint32_t most = 0;
+#pragma unroll 1
+  for (int g0 = 0; g0 < G; g0 += 16) {
+    column(g0);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) most = umax(most, finite_bits(x[i]));
   }
-  for (int i = threadIdx.x; i < TT * P; i += PS_NW * 64) codes[i / P * stride + i % P] = 0;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < 1024 << tshift; i += PS_NW * 64) hist[i] = 0;
+  if (G > 1)
+#pragma unroll 1
+    for (int t = 0; t < TT; ++t)
+#pragma unroll 1
+      for (int i = threadIdx.x; i < P; i += PS_NW * 64) codes[t * stride + i] = 0;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) most = across(most, s, umax);
+  if (lane == 0) sh_most[wave] = most;
   __syncthreads();
+  // the step of this column's query row: the largest of its group's
+  most = 0;
+#pragma unroll 1
+  for (int w = wide ? 0 : qrow * G, end = wide || w + G > 16 ? 16 : w + G; w < end; ++w) most = umax(most, sh_most[w]);
+  const float inv = pow2(-step_exponent(most));
 
-  for (int g0 = 0; g0 < G; g0 += 16) {  // TT > 1: all heads at once
-    {
-      const int t = TT > 1 ? wave / G : 0, g = TT > 1 ? wave % G : g0 + wave;
-      const bool in = t < TT && g < G && t0 + t < a.Tq;
-      for (int d = lane; d < D; d += 64) {
-        int u = 0;
-        if (in) {
-          const float x = value(g, t0 + t, d);
-          u = x != x ? 0 : (int)fminf(fmaxf(__builtin_rintf(x * sh_inv[t]), -127.f), 127.f);
-        }
+#pragma unroll 1
+  for (int g0 = 0; g0 < G; g0 += 16) {
+    if (wide) column(g0);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int d = lane + 64 * i;
+      const int u = x[i] != x[i] ? 0 : (int)fminf(fmaxf(__builtin_rintf(x[i] * inv), -127.f), 127.f);
+      if (d < D) {
         sh_q[wave][d] = (int8_t)(u > 0 ? u : 0);
         sh_q[wave][D + d] = (int8_t)(u < 0 ? u : 0);
       }
     }
     __syncthreads();
-    const int t = TT > 1 ? lr / G : 0, g = TT > 1 ? lr % G : g0 + lr;
+    const int t = wide ? 0 : lr * per16 >> 8, g = g0 + lr - t * G;
     const bool mine = t < TT && g < G && t0 + t < a.Tq;
+    uint32_t* to = codes + t * stride + lg * 4;
     i32x4 qb[KB];
 #pragma unroll
     for (int i = 0; i < KB; ++i) qb[i] = *(const i32x4*)(&sh_q[lr][i * 64 + lg * 16]);
-    for (int p0 = wave * 16; p0 < P; p0 += PS_NW * 16) {
-      int page = p0 + lr < P ? c.table[n * c.table_sn + p0 + lr] : -1;
-      const bool have = page >= 0 && page < c.pages;
-      const int64_t at = ((int64_t)(have ? page : 0) * c.H + h);
-      i32x4 sum = {0, 0, 0, 0};
-      float scale = 0.f;
-      if (have) scale = a.bound_scales[at];
+    if (g0 > 0) {
+      now.pages(a, table, wave, lr);
+      next.pages(a, table, wave + U * PS_NW, lr);
+      now.bounds(a, h, wave, P, lr, lg);
+    }
+    // a step's bounds are loaded while the one before is multiplied, the table's entries a step earlier
+#pragma unroll 1
+    for (int tile = wave; tile * 16 < P; tile += U * PS_NW) {
+      next.bounds(a, h, tile + U * PS_NW, P, lr, lg);
 #pragma unroll
-      for (int i = 0; i < KB; ++i) {
-        i32x4 b = {0, 0, 0, 0};
-        if (have) b = *(const i32x4*)(a.bounds + at * 2 * D + i * 64 + lg * 16);
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, qb[i], sum, 0, 0, 0);
-      }
+      for (int u = 0; u < U; ++u) {
+        const int p0 = (tile + u * PS_NW) * 16;
+        i32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float s = __shfl(scale, lg * 4 + i, 64);
-        const int there = __shfl((int)have, lg * 4 + i, 64);
-        if (there && mine) {
-          const uint32_t code = bound_code((float)sum[i] * s);
-          uint32_t* to = codes + t * stride + p0 + lg * 4 + i;
-          if (G == 1) *to = code;
-          else atomicMax(to, code);
+        for (int i = 0; i < KB; ++i) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.b[u][i], qb[i], sum, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float s = __shfl(now.scale[u], lg * 4 + i, 64);
+          const bool there = now.have[u] >> (lg * 4 + i) & 1;
+          const uint32_t code = there ? bound_code((float)sum[i] * s) : 0;
+          if (mine && p0 + lg * 4 + i < P) {
+            if (G == 1) to[p0 + i] = code;
+            else atomicMax(to + p0 + i, code);
+          }
         }
       }
+      now = next;
+      next.pages(a, table, tile + 2 * U * PS_NW, lr);
     }
     __syncthreads();
   }
 
   // the rows in groups of waves
-  const int wpr = PS_NW / TT, t = wave / wpr, member = wave % wpr * 64 + lane, members = wpr * 64;
+  const int wshift = 4 - tshift, wpr = 1 << wshift, t = wave >> wshift, sub = wave & (wpr - 1), member = sub * 64 + lane, members = wpr * 64;
   const uint32_t* mycodes = codes + t * stride;
   int want = a.K < P ? a.K : 0;  // of the pages of the threshold's code, in the end; every page there is: 0
   uint32_t threshold = 0;
   if (a.K < P) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = member; i < 256; i += members) hist[t][i] = 0;
-      __syncthreads();
+    int* bins = hist + t * 256;
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8, bins += 256 << tshift) {
+#pragma unroll 1
       for (int i = member; i < P; i += members) {
-        const uint32_t x = mycodes[i];
-        if (shift == 24 || (x ^ threshold) >> (shift + 8) == 0) atomicAdd(&hist[t][x >> shift & 255], 1);
+        const uint32_t v = mycodes[i];
+        if (shift == 24 || (v ^ threshold) >> (shift + 8) == 0) atomicAdd(&bins[v >> shift & 255], 1);
       }
       __syncthreads();
-      if (wave % wpr == 0) {  // four bins a lane, counted from the top
-        int b[4], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += b[i] = hist[t][255 - 4 * lane - i];
-        int before = wave_sum_scan(sum) - sum;
-        if (before < want && before + sum >= want) {  // one lane
-          int i = 0;
-          while (before + b[i] < want) before += b[i++];
-          pick[t][0] = 255 - 4 * lane - i;
-          pick[t][1] = want - before;
+      // four bins a lane, counted from the top; the digit's bin is one lane's
+      const int4 b = *(const int4*)(bins + 252 - 4 * lane);
+      const int sum = b.x + b.y + b.z + b.w, before = wave_sum_scan(sum) - sum;
+      const uint64_t hit = __ballot(before < want && before + sum >= want);
+      const int at = hit ? __builtin_ctzll(hit) : 0;
+      const int bw = __builtin_amdgcn_readlane(b.w, at), bz = __builtin_amdgcn_readlane(b.z, at), by = __builtin_amdgcn_readlane(b.y, at);
+      int rest = want - __builtin_amdgcn_readlane(before, at), digit = 255 - 4 * at;
+      if (rest > bw) {
+        rest -= bw;
+        --digit;
+        if (rest > bz) {
+          rest -= bz;
+          --digit;
+          if (rest > by) {
+            rest -= by;
+            --digit;
+          }
         }
       }
-      __syncthreads();
-      threshold |= (uint32_t)pick[t][0] << shift;
-      want = pick[t][1];
+      threshold |= (uint32_t)digit << shift;
+      want = rest;
     }
   }
   if (threshold == 0) want = 0;  // fewer pages than K: those that are there
   // a run of pages per wave: what is taken before it, then the places
-  const int run = ((P + members - 1) / members) * 64, p0 = wave % wpr * run, p1 = p0 + run < P ? p0 + run : P;
+  const int run = ((P + members - 1) >> (6 + wshift)) * 64, p0 = sub * run, p1 = p0 + run < P ? p0 + run : P;
   int more = 0, even = 0;
+#pragma unroll 1
   for (int p = p0 + lane; p - lane < p1; p += 64) {
-    const uint32_t x = p < p1 ? mycodes[p] : 0;
-    more += __popcll(__ballot(x > threshold));
-    even += __popcll(__ballot(x == threshold && x != 0));
+    const uint32_t v = p < p1 ? mycodes[p] : 0;
+    more += __popcll(__ballot(v > threshold));
+    even += __popcll(__ballot(v == threshold && v != 0));
   }
-  if (lane == 0) part[wave][0] = more, part[wave][1] = even;
+  if (lane == 0) part[wave] = make_int2(more, even);
   __syncthreads();
   if (t0 + t >= a.Tq) return;
-  int more0 = 0, even0 = 0, all = 0, evens = 0;
-  for (int w = 0; w < wpr; ++w) {
-    const int m = part[t * wpr + w][0], e = part[t * wpr + w][1];
-    if (w < wave % wpr) more0 += m, even0 += e;
-    all += m;
-    evens += e;
-  }
-  all += evens < want ? evens : want;
-  int32_t* out = a.index + ((int64_t)nh * a.Tq + t0 + t) * a.K;
+  const int2 mine = lane < wpr ? part[(t << wshift) + lane] : make_int2(0, 0);
+  const int upm = wave_sum_scan(mine.x), upe = wave_sum_scan(mine.y);
+  int more0 = sub ? __builtin_amdgcn_readlane(upm, sub - 1) : 0, even0 = sub ? __builtin_amdgcn_readlane(upe, sub - 1) : 0;
+  const int evens = __builtin_amdgcn_readlane(upe, 63), all = __builtin_amdgcn_readlane(upm, 63) + (evens < want ? evens : want);
+  int32_t* out = a.index + (nh * a.Tq + t0 + t) * a.K;
+#pragma unroll 1
   for (int p = p0 + lane; p - lane < p1; p += 64) {
-    const uint32_t x = p < p1 ? mycodes[p] : 0;
-    const uint64_t above = __ballot(x > threshold), equal = __ballot(x == threshold && x != 0);
+    const uint32_t v = p < p1 ? mycodes[p] : 0;
+    const uint64_t above = __ballot(v > threshold), equal = __ballot(v == threshold && v != 0);
     const int rank = even0 + lanes_below(equal);
-    if (x > threshold || (x == threshold && x != 0 && rank < want)) out[more0 + lanes_below(above) + (rank < want ? rank : want)] = p;
+    if (v > threshold || (v == threshold && v != 0 && rank < want)) out[more0 + lanes_below(above) + (rank < want ? rank : want)] = p;
     more0 += __popcll(above);
     even0 += __popcll(equal);
   }
+#pragma unroll 1
   for (int i = all + member; i < a.K; i += members) out[i] = -1;
 }
 
-// Query rows of a workgroup: a power of two with up to 16 (query row, head) pairs whose codes fit in LDS.
-int select_rows(int64_t G, int64_t Tq, int64_t max_pages) {
-  int tt = 1;
-  while (tt < 16 && tt < Tq && 2 * tt * G <= 16 && 2 * tt * max_pages <= PS_LDS) tt *= 2;
-  return tt;
+// The query rows of a workgroup as a shift: a power of two with up to 16 (query row, head) pairs whose codes and histograms fit
+// in LDS.
+int select_shift(int64_t G, int64_t Tq, int64_t max_pages) {
+  int s = 0;
+  while (s < 4 && (1 << s) < Tq && (2 << s) * G <= 16 && (2 << s) * (max_pages + 1024) <= PS_LDS) ++s;
+  return s;
 }
 
 template <typename T, int D>
 void launch_select(const PagedSelect& a, void* ws, hipStream_t stream) {
   const int64_t G = a.Hq / a.pool.H, M = a.pool.max_pages;
-  const int tt = select_rows(G, a.Tq, M), qtiles = (a.Tq + tt - 1) / tt;
-  const dim3 grid((unsigned)((int64_t)a.N * a.pool.H * qtiles)), nt(PS_NW * 64);
+  const int shift = select_shift(G, a.Tq, M), per16 = (int)((256 + G - 1) / G);
+  const dim3 grid((unsigned)((a.Tq + (1 << shift) - 1) >> shift), (unsigned)a.pool.H, (unsigned)a.N), nt(PS_NW * 64);
+  const size_t bins = (size_t)4096 << shift, lds = bins + (M > PS_LDS ? 0 : ((size_t)M << shift) * 4);
   if (M > PS_LDS) {
-    hipLaunchKernelGGL((paged_select_kernel<T, D, true>), grid, nt, 0, stream, a, tt, qtiles, (uint32_t*)ws);
-  } else {
-    const size_t lds = (size_t)tt * M * 4;
-    static bool set[64];  // per device: more LDS than a kernel may have unasked
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    if (lds > 32768 && (dev < 0 || dev >= 64 || !set[dev])) {
-      (void)hipFuncSetAttribute((const void*)paged_select_kernel<T, D, false>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                PS_LDS * 4);
-      if (dev >= 0 && dev < 64) set[dev] = true;
-    }
-    hipLaunchKernelGGL((paged_select_kernel<T, D, false>), grid, nt, lds, stream, a, tt, qtiles, (uint32_t*)nullptr);
+    hipLaunchKernelGGL((paged_select_kernel<T, D, true>), grid, nt, lds, stream, a, shift, per16, (uint32_t*)ws);
+    return;
   }
+  static bool set[64];  // per device: more LDS than a kernel may have unasked
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  if (lds > 49152 && (dev < 0 || dev >= 64 || !set[dev])) {
+    (void)hipFuncSetAttribute((const void*)paged_select_kernel<T, D, false>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                              PS_LDS * 4 + 16384);
+    if (dev >= 0 && dev < 64) set[dev] = true;
+  }
+  hipLaunchKernelGGL((paged_select_kernel<T, D, false>), grid, nt, lds, stream, a, shift, per16, (uint32_t*)nullptr);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -404,11 +605,10 @@ int tabicl_launch_paged_bounds(const PagedBounds& a, int format, int64_t rows, h
     part.pool.table += n * a.pool.table_sn;
     part.pool.lengths += n;
     if (a.start) part.start += n;
-    const dim3 grid((unsigned)gx, (unsigned)(a.N - n < some ? a.N - n : some)), nt(256);
-    if (format == 0) hipLaunchKernelGGL(paged_bounds_kernel<bf16>, grid, nt, 0, stream, part);
-    else if (format == 1) hipLaunchKernelGGL(paged_bounds_kernel<float>, grid, nt, 0, stream, part);
-    else if (format == 2) hipLaunchKernelGGL(paged_bounds_kernel<E4M3>, grid, nt, 0, stream, part);
-    else hipLaunchKernelGGL(paged_bounds_kernel<I8>, grid, nt, 0, stream, part);
+    const dim3 grid((unsigned)gx, (unsigned)(a.N - n < some ? a.N - n : some));
+    if (a.pool.D == 32) launch_bounds<32>(part, format, grid, stream);
+    else if (a.pool.D == 64) launch_bounds<64>(part, format, grid, stream);
+    else launch_bounds<128>(part, format, grid, stream);
   }
   return (int)hipGetLastError();
 }
