@@ -1,4 +1,5 @@
-"""Builds libtabicl_attn.so (the C-ABI HIP library) for gfx950 with hipcc, in-tree.
+"""Builds libtabicl_attn.so (the C-ABI HIP library) for gfx950 with hipcc, and tabicl_mi355_direct.so (a Python module that
+makes the paged cache's calls of it, csrc/direct.cpp; host code alone) with g++, in-tree.
 
 Usage: python build_lib.py [-v]. Objects go to _build/ next to this file; the library is written
 next to this file, where tabicl_mi355_native.py loads it from.
@@ -15,6 +16,8 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 BUILD = HERE / "_build"
 LIB = HERE / "libtabicl_attn.so"
+DIRECT = HERE / "tabicl_mi355_direct.so"
+CXX = os.environ.get("CXX", "g++")
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 in any kernel of this library.
@@ -38,11 +41,30 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
         print(res.stderr, flush=True)
 
 
+def _direct(verbose: bool) -> None:
+    import sysconfig
+
+    import torch
+    torch_dir = Path(torch.__file__).resolve().parent
+    tmp = DIRECT.with_suffix(".so.tmp")
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{sysconfig.get_paths()['include']}", f"-isystem{torch_dir / 'include'}",
+           f"-isystem{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", str(CSRC / "direct.cpp"), "-o", str(tmp),
+           f"-L{torch_dir / 'lib'}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for direct.cpp:\n{res.stderr}")
+    os.replace(tmp, DIRECT)
+
+
 def build(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     objs = [BUILD / (Path(s).stem + ".o") for s in SOURCES]
-    with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
         futs = [ex.submit(_compile, CSRC / s, o, verbose) for s, o in zip(SOURCES, objs)]
+        futs.append(ex.submit(_direct, verbose))
         for f in futs:
             f.result()
     tmp = LIB.with_suffix(".so.tmp")

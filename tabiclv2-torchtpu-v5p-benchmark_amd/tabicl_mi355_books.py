@@ -64,8 +64,12 @@ def paged_reserve(table: Tensor, lengths: Tensor, count: Tensor, free: Tensor, f
     of the stack, request by request, as far as they go. Returns granted [N] int32: how many of the rows have a place (all,
     or those before the first page that was not to be had). lengths and count stay as they are. In place: table, free_count."""
     if _nat.direct(table, lengths, count, free, free_count):
-        granted = torch.empty(table.shape[:1], dtype=torch.int32, device=table.device)
-        _reserve_launch(table, lengths, count, free, free_count, int(page_rows), granted)
+        granted = None
+        if _nat.DIRECT is not None:
+            granted = _nat.DIRECT.reserve(table, lengths, count, free, free_count, int(page_rows), _nat.stream_of(table))
+        if granted is None:
+            granted = torch.empty(table.shape[:1], dtype=torch.int32, device=table.device)
+            _reserve_launch(table, lengths, count, free, free_count, int(page_rows), granted)
         torch.autograd.graph.increment_version((table, free_count))
         return granted
     return torch.ops.tabicl.paged_reserve(table, lengths, count, free, free_count, int(page_rows))
@@ -101,7 +105,8 @@ def paged_release(table: Tensor, lengths: Tensor, free: Tensor, free_count: Tens
     evicted, or (lengths 0) a request that is done. The last request's last page goes first, so that a release of what a
     reserve gave out leaves the stack as it was. In place: table, free, free_count."""
     if _nat.direct(table, lengths, free, free_count):
-        _release_launch(table, lengths, free, free_count, int(page_rows))
+        if _nat.DIRECT is None or not _nat.DIRECT.release(table, lengths, free, free_count, int(page_rows), _nat.stream_of(table)):
+            _release_launch(table, lengths, free, free_count, int(page_rows))
         torch.autograd.graph.increment_version((table, free, free_count))
     else:
         torch.ops.tabicl.paged_release(table, lengths, free, free_count, int(page_rows))
@@ -142,6 +147,10 @@ def paged_slots(table: Tensor, lengths: Tensor, count: Tensor, total: int, pages
     if total < 0:
         raise ValueError(f"total must not be negative, got {total}")
     if _nat.direct(table, lengths, count):
+        if _nat.DIRECT is not None:
+            r = _nat.DIRECT.slots(table, lengths, count, int(total), int(pages), int(page_rows), _nat.stream_of(table))
+            if r is not None:
+                return r
         return _slots(table, lengths, count, int(total), int(pages), int(page_rows))
     return torch.ops.tabicl.paged_slots(table, lengths, count, int(total), int(pages), int(page_rows))
 
@@ -192,7 +201,8 @@ def paged_append_packed(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths
     if scales is not None or k_pages.dtype in _pool.CODES:
         _p8.append(k_pages, v_pages, table, lengths, k, v, count, starts, scales)
     elif _nat.direct(k_pages, v_pages, slots, k, v):
-        _append_launch(k_pages, v_pages, slots, k, v)
+        if _nat.DIRECT is None or not _nat.DIRECT.append_slots(k_pages, v_pages, slots, k, v, _nat.stream_of(k)):
+            _append_launch(k_pages, v_pages, slots, k, v)
         torch.autograd.graph.increment_version((k_pages, v_pages))
     else:
         _pool.no_grad("paged_append_packed", k_pages, v_pages, k, v)

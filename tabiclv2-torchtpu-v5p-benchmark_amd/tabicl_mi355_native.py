@@ -127,6 +127,18 @@ class UnsupportedShapeError(ValueError):
 
 _LIB = None
 _LOAD_ERROR: Exception | None = None
+# tabicl_mi355_direct (csrc/direct.cpp) bound to the loaded library, or None: wrappers make their ordinary calls through it
+DIRECT = None
+
+
+def _bind_direct(lib: ctypes.CDLL) -> None:
+    global DIRECT
+    try:
+        import tabicl_mi355_direct as module
+    except ImportError:  # not built, or for another torch: the wrappers call the library by ctypes
+        return
+    module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES})
+    DIRECT = module
 
 
 def load() -> ctypes.CDLL:
@@ -146,6 +158,7 @@ def load() -> ctypes.CDLL:
         fn.argtypes = argtypes
         fn.restype = _RESTYPES.get(name, ctypes.c_int)
     _LIB = lib
+    _bind_direct(lib)
     return lib
 
 

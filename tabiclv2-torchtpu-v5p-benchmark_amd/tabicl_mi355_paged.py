@@ -273,11 +273,11 @@ def paged_gather(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tenso
     page; what lies past a sequence's length is not written. For calls that the dense kernels answer faster (many query
     rows), or to copy a cache out of its pool. In the pool's dtype; with scales (a pool of e4m3 or int8 codes) the values in
     `dtype`, bf16 (the default: they are bf16 numbers) or fp32."""
-    _no_grad("paged_gather", k_pages, v_pages)
     if k_pages.dim() != 4 or rows < 0:
         raise ValueError(f"paged_gather needs pools [pages, H, page_rows, D] and rows >= 0, got {tuple(k_pages.shape)}, {rows}")
     if scales is not None or k_pages.dtype in _pool.CODES:
         return _p8.gather(k_pages, v_pages, table, lengths, int(rows), scales, dtype)
+    _no_grad("paged_gather", k_pages, v_pages)
     if dtype is not None and dtype is not k_pages.dtype:
         raise ValueError(f"a {k_pages.dtype} pool is gathered in its own dtype")
     if _nat.direct(k_pages, v_pages, table, lengths):

@@ -70,6 +70,12 @@ def attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, length
         raise ValueError("a pool of 8-bit codes needs its scales [pages, H, 2]")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, scales, table, lengths, out):
+        if _nat.DIRECT is not None:
+            o = _nat.DIRECT.attn(q, k_pages, v_pages, scales, table, lengths, out, None, scale, _nat.stream_of(q))
+            if o is not None:
+                if out is not None:
+                    torch.autograd.graph.increment_version(out)
+                return o
         o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
         _attn_launch(q if out is None else _pool.apart(q, out), k_pages, v_pages, scales, table, lengths, scale, o)
         if out is not None:
@@ -132,7 +138,9 @@ def append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: 
     if scales is None:
         raise ValueError("a pool of 8-bit codes needs its scales [pages, H, 2]")
     if _nat.direct(k_pages, v_pages, scales, table, lengths, k, v, count, starts):
-        _append_launch(k_pages, v_pages, scales, table, lengths, k, v, count, starts)
+        if starts is not None or _nat.DIRECT is None or not _nat.DIRECT.append(k_pages, v_pages, scales, table, lengths, k, v, count,
+                                                                               _nat.stream_of(k)):
+            _append_launch(k_pages, v_pages, scales, table, lengths, k, v, count, starts)
         torch.autograd.graph.increment_version((k_pages, v_pages, scales))
     else:
         _pool.no_grad("paged_append", k_pages, v_pages, scales, k, v)
@@ -179,7 +187,11 @@ def gather(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, row
         raise ValueError("a pool of 8-bit codes needs its scales [pages, H, 2]")
     dtype = torch.bfloat16 if dtype is None else dtype
     _nat.dtype_code(dtype)
-    _pool.no_grad("paged_gather", k_pages, v_pages, scales)
     if _nat.direct(k_pages, v_pages, scales, table, lengths):
+        if _nat.DIRECT is not None:
+            kv = _nat.DIRECT.gather(k_pages, v_pages, scales, table, lengths, rows, dtype is torch.float32, _nat.stream_of(k_pages))
+            if kv is not None:
+                return kv
         return _gather(k_pages, v_pages, scales, table, lengths, rows, dtype)
+    _pool.no_grad("paged_gather", k_pages, v_pages, scales)
     return torch.ops.tabicl.paged_gather_q8(k_pages, v_pages, scales, table, lengths, rows, dtype)

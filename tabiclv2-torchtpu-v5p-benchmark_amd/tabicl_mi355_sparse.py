@@ -73,7 +73,9 @@ def paged_bounds(k_pages: Tensor, table: Tensor, lengths: Tensor, bounds: Tensor
     if rows < 0:
         raise ValueError(f"rows must not be negative, got {rows}")
     if _nat.direct(k_pages, table, lengths, bounds, bound_scales, start, scales):
-        _bounds_launch(k_pages, table, lengths, bounds, bound_scales, start, rows, scales)
+        if _nat.DIRECT is None or not _nat.DIRECT.bounds(k_pages, table, lengths, bounds, bound_scales, start, rows, scales,
+                                                         _nat.stream_of(k_pages)):
+            _bounds_launch(k_pages, table, lengths, bounds, bound_scales, start, rows, scales)
         torch.autograd.graph.increment_version((bounds, bound_scales))
     else:
         _pool.no_grad("paged_bounds", k_pages, bound_scales, scales)
@@ -133,9 +135,13 @@ def paged_select(q: Tensor, bounds: Tensor, bound_scales: Tensor, table: Tensor,
     The query heads of a group choose together, by the largest of their bounds. No gradient."""
     if pages < 0:
         raise ValueError(f"pages must not be negative, got {pages}")
-    _pool.no_grad("paged_select", q, bound_scales)
     if _nat.direct(q, bounds, bound_scales, table, lengths):
+        if _nat.DIRECT is not None:
+            index = _nat.DIRECT.select(q, bounds, bound_scales, table, lengths, int(page_rows), int(pages), _nat.stream_of(q))
+            if index is not None:
+                return index
         return _select(q, bounds, bound_scales, table, lengths, int(page_rows), int(pages))
+    _pool.no_grad("paged_select", q, bound_scales)
     return torch.ops.tabicl.paged_select(q, bounds, bound_scales, table, lengths, int(page_rows), int(pages))
 
 
@@ -199,6 +205,12 @@ def paged_sparse_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: T
     without a row to attend to is 0. Every query row reads its own pages: for one query row to a few dozen. No gradient."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, table, lengths, index, out, scales):
+        if _nat.DIRECT is not None:
+            o = _nat.DIRECT.attn(q, k_pages, v_pages, scales, table, lengths, out, index, scale, _nat.stream_of(q))
+            if o is not None:
+                if out is not None:
+                    torch.autograd.graph.increment_version(out)
+                return o
         o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
         _sparse_launch(q if out is None else _pool.apart(q, out), k_pages, v_pages, table, lengths, index, scale, scales, o)
         if out is not None:
