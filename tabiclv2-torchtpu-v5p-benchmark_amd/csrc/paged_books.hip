@@ -8,7 +8,8 @@
 //            undoes a reserve, stack and all
 //   slots:   row j of a packed batch, the t-th of sequence n: table[n, (len + t) / R] R + (len + t) % R, or -1
 //
-// All are bound by the latency of their launches (a few bytes a row).
+// All are bound by the latency of their launches (a few bytes a row): tables of up to 65,536 entries are gone through by one
+// workgroup in one launch, larger ones by many in two (the first counts).
 #include "launch.h"
 #include "paged_core.h"
 
@@ -119,30 +120,140 @@ __global__ __launch_bounds__(256) void paged_books_kernel(PagedBooks a, const in
   }
 }
 
+// One workgroup for up to 256 sequences and BOOKS_ONE entries: counts, running sums and the entries in one launch. The entries to
+// look at are cut into runs of 64 of one sequence; a wave takes 16 runs at a time, all of them in its registers at once. (us of
+// a reserve on the GPU and with the host, two launches / this: 256 requests of one row 6.3 and 10.3 / 7.9 and 7.9, 64 of up to
+// 10,000 rows 7.6 and 10.3 / 9.4 and 9.4.)
+constexpr int BOOKS_SEQS = 256, BOOKS_ONE = 65536, BOOKS_RUNS = BOOKS_ONE / 64 + BOOKS_SEQS, PB_NW = 16, PB_EACH = 16;
+
+template <bool RELEASE>
+__global__ __launch_bounds__(PB_NW * 64) void paged_books_one_kernel(PagedBooks a) {
+  __shared__ int2 run[BOOKS_RUNS], rows[BOOKS_SEQS];  // (sequence, first entry | entries - 1); the rows in place and those wanted
+  __shared__ int need[BOOKS_RUNS], miss[BOOKS_SEQS], sums[PB_NW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int claimed = *a.free_count, have = claimed < 0 ? 0 : claimed < a.pages ? claimed : a.pages;
+  // the sum of x over the threads before this one, and over all
+  auto before = [&](int x, int* all) {
+    const int upto = wave_sum_scan(x);
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    const int waves = wave_sum_scan(lane < PB_NW ? sums[lane] : 0);
+    __syncthreads();
+    *all = __builtin_amdgcn_readlane(waves, 63);
+    return (wave ? __builtin_amdgcn_readlane(waves, wave - 1) : 0) + upto - x;
+  };
+  int first = 0, last = 0, runs;
+  if (tid < a.N) {
+    const BookRange r(a, tid, RELEASE);
+    first = r.first, last = r.last > r.first ? r.last : r.first;
+    rows[tid] = make_int2((int)r.len, (int)r.add);
+    miss[tid] = a.max_pages;
+  }
+  int at = before((last - first + 63) / 64, &runs);
+#pragma unroll 1
+  for (int p = first; p < last; p += 64) run[at++] = make_int2(tid, p << 6 | ((last - p < 64 ? last - p : 64) - 1));
+  __syncthreads();
+  int32_t* entry[PB_EACH];
+  int id[PB_EACH];
+  bool moves[PB_EACH];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < PB_EACH; ++u) {
+      const int k = k0 + wave * PB_EACH + u;
+      const int2 r = k < runs ? run[k] : make_int2(0, 0);
+      const bool in = k < runs && lane <= (r.y & 63);
+      entry[u] = a.table + r.x * a.table_sn + (r.y >> 6) + lane;
+      id[u] = in ? *entry[u] : 0;
+      moves[u] = in;
+    }
+#pragma unroll
+    for (int u = 0; u < PB_EACH; ++u) moves[u] = moves[u] && book_has(a, id[u]) == RELEASE;
+  };
+#pragma unroll 1
+  for (int k0 = 0; k0 < runs; k0 += PB_NW * PB_EACH) {
+    load(k0);
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < PB_EACH; ++u) {
+      const int count = __popcll(__ballot(moves[u]));
+      mine = lane == u ? count : mine;
+    }
+    if (lane < PB_EACH && k0 + wave * PB_EACH + lane < runs) need[k0 + wave * PB_EACH + lane] = mine;
+  }
+  __syncthreads();
+  int all;
+  const int x0 = 2 * tid < runs ? need[2 * tid] : 0, x1 = 2 * tid + 1 < runs ? need[2 * tid + 1] : 0;
+  const int start = before(x0 + x1, &all);
+  if (2 * tid < runs) need[2 * tid] = start;
+  if (2 * tid + 1 < runs) need[2 * tid + 1] = start + x0;
+  __syncthreads();
+#pragma unroll 1
+  for (int k0 = 0; k0 < runs; k0 += PB_NW * PB_EACH) {
+    if (runs > PB_NW * PB_EACH) load(k0);  // else they are here
+#pragma unroll
+    for (int u = 0; u < PB_EACH; ++u) {
+      const int k = k0 + wave * PB_EACH + u, rank = (k < runs ? need[k] : 0) + below(__ballot(moves[u]));
+      if constexpr (RELEASE) {
+        const int64_t to = (int64_t)have + all - 1 - rank;
+        if (moves[u] && to < a.pages) a.free_pages[to] = id[u];
+        if (moves[u]) *entry[u] = -1;
+      } else if (moves[u] && rank < have) {
+        id[u] = a.free_pages[have - 1 - rank];
+      }
+    }
+    if constexpr (!RELEASE) {
+#pragma unroll
+      for (int u = 0; u < PB_EACH; ++u) {
+        const int k = k0 + wave * PB_EACH + u;
+        if (moves[u]) *entry[u] = id[u];  // as it was, if the stack had none left
+        if (moves[u] && !book_has(a, id[u])) atomicMin(&miss[run[k].x], (run[k].y >> 6) + lane);
+      }
+    }
+  }
+  if constexpr (!RELEASE) {  // rows up to the first page that is not there
+    __syncthreads();
+    if (tid < a.N) {
+      const int64_t there = ((int64_t)miss[tid] << a.shift) - rows[tid].x;
+      a.granted[tid] = (int)(there < 0 ? 0 : there < rows[tid].y ? there : rows[tid].y);
+    }
+  }
+  if (tid == 0) {
+    const int64_t left = RELEASE ? (int64_t)have + all : (int64_t)have - all;
+    *a.free_count = (int)(left < 0 ? 0 : left < a.pages ? left : a.pages);
+  }
+}
+
 // The slots of `per` rows of the batch by a workgroup: the counts' running sums, PS_SEQS sequences at a time in LDS, a row's
-// sequence by bisection.
-constexpr int PS_SEQS = 2048;
+// sequence by bisection, four rows of a thread side by side.
+constexpr int PS_SEQS = 1024, PS_ROWS = 4;
 
 __global__ __launch_bounds__(256) void paged_slots_kernel(PagedBooks a, int64_t* slots, int32_t* starts, int64_t total, int per) {
   __shared__ int64_t sum[PS_SEQS + 1];
   __shared__ int64_t wsum[4];
+  __shared__ int32_t held[PS_SEQS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t j0 = (int64_t)blockIdx.x * per, j1 = j0 + per < total ? j0 + per : total;
+  const int64_t j0 = (int64_t)blockIdx.x * per, j1 = j0 + per < total ? j0 + per : total, cap = (int64_t)a.max_pages << a.shift;
   constexpr int EACH = PS_SEQS / 256;
   int64_t base = 0;
   for (int s0 = 0; s0 < a.N && (base < j1 || blockIdx.x == 0); s0 += PS_SEQS) {
     int64_t c[EACH], mine = 0;
+    int x[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      const int n = s0 + tid * EACH + i, x = n < a.N ? a.count[n] : 0;
+      const int n = s0 + tid * EACH + i;
+      x[i] = n < a.N ? a.count[n] : 0;
+      held[tid * EACH + i] = n < a.N ? a.lengths[n] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
       c[i] = mine;
-      mine += x < 0 ? 0 : x;
+      mine += x[i] < 0 ? 0 : x[i];
     }
     int64_t upto = mine;
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-      const int64_t y = __shfl_up(upto, x, 64);
-      if (lane >= x) upto += y;
+    for (int y = 1; y < 64; y <<= 1) {
+      const int64_t z = __shfl_up(upto, y, 64);
+      if (lane >= y) upto += z;
     }
     if (lane == 63) wsum[wave] = upto;
     __syncthreads();
@@ -158,21 +269,28 @@ __global__ __launch_bounds__(256) void paged_slots_kernel(PagedBooks a, int64_t*
     if (tid == 0) sum[PS_SEQS] = next;
     __syncthreads();
     const int64_t lo = j0 > base ? j0 : base, hi = j1 < next ? j1 : next;
-    for (int64_t j = lo + tid; j < hi; j += 256) {
-      int l = 0, r = PS_SEQS;  // sum[l] <= j < sum[r]
-      while (r - l > 1) {
-        const int m = (l + r) / 2;
-        if (sum[m] <= j) l = m;
-        else r = m;
+    const int seqs = a.N - s0 < PS_SEQS ? a.N - s0 : PS_SEQS;  // sum[seqs] = next
+    for (int64_t j = lo + tid; j < hi; j += 256 * PS_ROWS) {
+      int l[PS_ROWS], id[PS_ROWS];
+      int64_t row[PS_ROWS];
+#pragma unroll
+      for (int i = 0; i < PS_ROWS; ++i) l[i] = 0;
+      for (int step = PS_SEQS / 2; step > 0; step >>= 1) {
+        if (step >= seqs) continue;
+#pragma unroll
+        for (int i = 0; i < PS_ROWS; ++i)
+          if (l[i] + step < seqs && sum[l[i] + step] <= j + 256 * i) l[i] += step;  // the last sum <= j + 256 i
       }
-      const int n = s0 + l;
-      const int64_t cap = (int64_t)a.max_pages << a.shift, len = a.lengths[n] < 0 ? 0 : a.lengths[n], row = len + j - sum[l];
-      int64_t slot = -1;
-      if (row < cap) {
-        const int id = a.table[n * a.table_sn + (row >> a.shift)];
-        if (book_has(a, id)) slot = ((int64_t)id << a.shift) + (row & ((1ll << a.shift) - 1));
+#pragma unroll
+      for (int i = 0; i < PS_ROWS; ++i) {
+        row[i] = (held[l[i]] < 0 ? 0 : held[l[i]]) + j + 256 * i - sum[l[i]];
+        const bool in = j + 256 * i < hi && row[i] < cap;
+        id[i] = in ? a.table[(s0 + l[i]) * a.table_sn + (row[i] >> a.shift)] : -1;
       }
-      slots[j] = slot;
+#pragma unroll
+      for (int i = 0; i < PS_ROWS; ++i)
+        if (j + 256 * i < hi)
+          slots[j + 256 * i] = book_has(a, id[i]) ? ((int64_t)id[i] << a.shift) + (row[i] & ((1ll << a.shift) - 1)) : -1;
     }
     base = next;
     __syncthreads();
@@ -199,6 +317,10 @@ __global__ __launch_bounds__(256) void paged_append_slots_kernel(PagedAppend a, 
 
 template <bool RELEASE>
 int launch_books(const PagedBooks& a, void* ws, hipStream_t stream) {
+  if (a.N <= BOOKS_SEQS && (int64_t)a.N * a.max_pages <= BOOKS_ONE) {
+    hipLaunchKernelGGL(paged_books_one_kernel<RELEASE>, dim3(1), dim3(PB_NW * 64), 0, stream, a);
+    return (int)hipGetLastError();
+  }
   const int per = (a.N + PB_GROUPS - 1) / PB_GROUPS < 4 ? 4 : (a.N + PB_GROUPS - 1) / PB_GROUPS;
   hipLaunchKernelGGL(paged_need_kernel<RELEASE>, dim3((unsigned)((a.N + 3) / 4)), dim3(256), 0, stream, a, (int32_t*)ws);
   hipLaunchKernelGGL(paged_books_kernel<RELEASE>, dim3((unsigned)((a.N + per - 1) / per)), dim3(256), 0, stream, a,

@@ -8,6 +8,12 @@
 
 namespace {
 
+// 16 bytes that are read once: nothing else of the caches has to make room for them.
+__device__ __forceinline__ uint4 ldg16_once(const void* p) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const words*)p));
+}
+
 __device__ __forceinline__ int pool_length(const PagedPool& c, int n) {
   const int64_t cap = (int64_t)c.max_pages << c.shift;
   const int64_t len = c.lengths[n];
@@ -164,17 +170,17 @@ struct PagedTile {
 
 typedef uint32_t u32v2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32v4 __attribute__((ext_vector_type(4)));
-template <int DW>
+template <int DW, int POLICY = 0>
 __device__ __forceinline__ void load_dwords(uint32_t* d, __amdgpu_buffer_rsrc_t r, uint32_t off) {
   if constexpr (DW == 1) {
-    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, POLICY);
   } else if constexpr (DW == 2) {
-    const u32v2 x = __builtin_bit_cast(u32v2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    const u32v2 x = __builtin_bit_cast(u32v2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, POLICY));
     d[0] = x[0], d[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < DW; i += 4) {
-      const u32v4 x = __builtin_bit_cast(u32v4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, 0));
+      const u32v4 x = __builtin_bit_cast(u32v4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, POLICY));
       d[i] = x[0], d[i + 1] = x[1], d[i + 2] = x[2], d[i + 3] = x[3];
     }
   }
@@ -397,6 +403,10 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
   constexpr bool Q8 = sizeof(C) == 1;
   constexpr int SUB = Tile::SUB, KS = Tile::KS, NC = Tile::NC, DE = Tile::DE, ES = sizeof(C), TS = sizeof(T);
   constexpr int NQ = Q8 ? (TS == 2 ? 1 : 3) : 1, NP = TS == 2 ? 2 : 3;  // bf16 terms of q and of p, where C has 8 bits
+  // Rows in 8 bits of up to 64 dims that one tile of query rows reads are loaded past the caches (one row over 8 x 45,000 rows 76 ->
+  // 68 us; a second tile would have to go to memory again, 64 query rows 120 -> 127, and so would the second half of a row of
+  // 128 dims).
+  constexpr int POLICY = (Q8 && !SEL && TS == 2 && QT <= 2 && D <= 64) ? 2 : 0;
   __shared__ float sh_o[NW / 2][16 * QT][D + 4];
   __shared__ float2 sh_ml[NW / 2][16 * QT];
   const PagedPool& c = a.pool;
@@ -497,22 +507,22 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
       const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((char*)c.v + off, 0, have * D * ES, TA_BUF_WORD3);
       if constexpr (Q8) {
         if constexpr (D == 128) {
-          load_dwords<4>(t.k[s], kr, koff);
-          load_dwords<4>(t.k[s] + 4, kr, koff + 64);
+          load_dwords<4, POLICY>(t.k[s], kr, koff);
+          load_dwords<4, POLICY>(t.k[s] + 4, kr, koff + 64);
         } else {
-          load_dwords<Tile::KW>(t.k[s], kr, koff);
+          load_dwords<Tile::KW, POLICY>(t.k[s], kr, koff);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if constexpr (D == 32) t.v[s][j][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vr, voff + j * D, 0, 0);
-          else load_dwords<Tile::VW>(t.v[s][j], vr, voff + j * D);
+          if constexpr (D == 32) t.v[s][j][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vr, voff + j * D, 0, POLICY);
+          else load_dwords<Tile::VW, POLICY>(t.v[s][j], vr, voff + j * D);
         }
       } else {
 #pragma unroll
         for (int i2 = 0; i2 < NC; ++i2)
-          t.k[s][i2] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, koff + i2 * 64, 0, 0));
+          t.k[s][i2] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, koff + i2 * 64, 0, POLICY));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) load_dwords<Tile::DW>(t.v[s][j], vr, voff + j * D * ES);
+        for (int j = 0; j < 4; ++j) load_dwords<Tile::DW, POLICY>(t.v[s][j], vr, voff + j * D * ES);
       }
     }
     if constexpr (Q8) {  // behind the loads: the first turn waits for its scales here

@@ -68,7 +68,7 @@ struct Raw8 {
   uint4 u[sizeof(T) / 2];
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = ldg16(p + i * (16 / sizeof(T)));
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = ldg16_once(p + i * (16 / sizeof(T)));
   }
   __device__ __forceinline__ void values(float* x) const {
 #pragma unroll
@@ -117,8 +117,9 @@ __device__ __forceinline__ uint32_t to_codes_within<I8>(const float* x, float in
 // LANES threads take the new rows of one page and head, of K or of V: the largest |x|, the scale, the codes. Up to LANES * 8
 // chunks of eight values are read once and kept; a larger page's are read again for their codes. LANES = 256 where a page has
 // more chunks than a wave keeps. Where a value is not finite, or beyond the largest scale, they are gone through value by value.
-// Bound by the bytes of the rows and codes: 8 x 45,000 rows in bf16 to int8 268 us -> 224 with magnitudes compared in pairs and
-// codes without limits (15 -> 4 instructions a value).
+// Bound by the bytes of the rows and codes: 8 x 45,000 rows in bf16 to int8 268 us -> 238 with magnitudes compared in pairs and
+// codes without limits (15 -> 4 instructions a value), 221 with loads that leave the caches alone (stores that do: 217, and what
+// reads the codes next takes 10 us more).
 constexpr int PQ_KEEP = 8;
 
 template <typename T, typename C, int LANES>

@@ -173,7 +173,8 @@ struct Extremes {
   }
 };
 
-// One wave per page and head. Bound by the bytes of K.
+// One wave per page and head. Bound by the bytes of K, which nothing reads again soon: loads that leave the caches alone (8 x
+// 45,000 rows in bf16 78 -> 62 us).
 template <typename C, int D>
 __global__ __launch_bounds__(256) void paged_bounds_kernel(PagedBounds a) {
   constexpr int ES = sizeof(C), VPC = 16 / ES, LPR = D / VPC, RPP = 64 / LPR;  // values of 16 bytes, lanes of a row, rows of a pass
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(256) void paged_bounds_kernel(PagedBounds a) {
   for (; r + 7 * RPP < live; r += 8 * RPP) {
     uint4 u[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = ldg16(k + (int64_t)(r + i * RPP) * D * ES);
+    for (int i = 0; i < 8; ++i) u[i] = ldg16_once(k + (int64_t)(r + i * RPP) * D * ES);
 #pragma unroll
     for (int i = 0; i < 8; ++i) ext.add(u[i]);
   }
@@ -274,35 +275,29 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// U tiles of 16 pages, a wave's every 16th: their bounds as operands, their scales and whether they are there. The table is read
-// up to its width, not the sequence's, so that its entries need not wait for the length.
-template <int KB, int U>
+// A tile of 16 pages (a wave takes every 16th): their bounds as operands, their scales and whether they are there. The table is
+// read up to its width, not the sequence's, so that its entries need not wait for the length.
+template <int KB>
 struct BoundTiles {
-  int page[U];
-  i32x4 b[U][KB];
-  float scale[U];
-  uint32_t have[U];
+  int page;
+  i32x4 b[KB];
+  float scale;
+  uint32_t have;
   __device__ __forceinline__ void pages(const PagedSelect& a, const int32_t* table, int tile, int lr) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t p = ((int64_t)tile + u * PS_NW) * 16 + lr;
-      page[u] = p < a.pool.max_pages ? table[p] : -1;
-    }
+    const int64_t p = (int64_t)tile * 16 + lr;
+    page = p < a.pool.max_pages ? table[p] : -1;
   }
   __device__ __forceinline__ void bounds(const PagedSelect& a, int h, int tile, int P, int lr, int lg) {
+    const bool in = page >= 0 && page < a.pool.pages && tile * 16 + lr < P;
+    const int64_t at = (int64_t)(in ? page : 0) * a.pool.H + h;
+    have = (uint32_t)__ballot(in) & 0xffffu;
+    scale = 0.f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = page[u] >= 0 && page[u] < a.pool.pages && (tile + u * PS_NW) * 16 + lr < P;
-      const int64_t at = (int64_t)(in ? page[u] : 0) * a.pool.H + h;
-      have[u] = (uint32_t)__ballot(in) & 0xffffu;
-      scale[u] = 0.f;
+    for (int i = 0; i < KB; ++i) b[i] = i32x4{0, 0, 0, 0};
+    if (in) {
+      scale = a.bound_scales[at];
 #pragma unroll
-      for (int i = 0; i < KB; ++i) b[u][i] = i32x4{0, 0, 0, 0};
-      if (in) {
-        scale[u] = a.bound_scales[at];
-#pragma unroll
-        for (int i = 0; i < KB; ++i) b[u][i] = *(const i32x4*)(a.bounds + (at * KB + i) * 64 + lg * 16);
-      }
+      for (int i = 0; i < KB; ++i) b[i] = *(const i32x4*)(a.bounds + (at * KB + i) * 64 + lg * 16);
     }
   }
 };
@@ -311,7 +306,7 @@ struct BoundTiles {
 template <typename T, int D, bool GLOBAL>
 __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a, int tshift, int per16, uint32_t* store) {
   extern __shared__ uint32_t lds[];  // [4][TT][256] histograms, [TT][max_pages] codes
-  constexpr int KB = 2 * D / 64, U = 1, NV = (D + 63) / 64;
+  constexpr int KB = 2 * D / 64, NV = (D + 63) / 64;
   __shared__ __attribute__((aligned(16))) int8_t sh_q[16][2 * D];
   __shared__ uint32_t sh_most[16];
   __shared__ int2 part[PS_NW];
@@ -324,10 +319,15 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
   int* hist = (int*)lds;
   const int64_t nh = (int64_t)n * c.H + h;
   uint32_t* codes = GLOBAL ? store + (nh * a.Tq + t0) * stride : lds + (1024 << tshift);
-  BoundTiles<KB, U> now, next;
-  now.pages(a, table, wave, lr);
-  next.pages(a, table, wave + U * PS_NW, lr);
-  now.bounds(a, h, wave, P, lr, lg);
+  BoundTiles<KB> b0, b1, b2;
+  auto first = [&]() {
+    b0.pages(a, table, wave, lr);
+    b1.pages(a, table, wave + PS_NW, lr);
+    b2.pages(a, table, wave + 2 * PS_NW, lr);
+    b0.bounds(a, h, wave, P, lr, lg);
+    b1.bounds(a, h, wave + PS_NW, P, lr, lg);
+  };
+  first();
 
   // column `wave` of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
   const char* q = (const char*)a.q + (n * a.q_sn + (int64_t)h * G * a.q_sh) * sizeof(T);
@@ -386,34 +386,28 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
     i32x4 qb[KB];
 #pragma unroll
     for (int i = 0; i < KB; ++i) qb[i] = *(const i32x4*)(&sh_q[lr][i * 64 + lg * 16]);
-    if (g0 > 0) {
-      now.pages(a, table, wave, lr);
-      next.pages(a, table, wave + U * PS_NW, lr);
-      now.bounds(a, h, wave, P, lr, lg);
-    }
-    // a step's bounds are loaded while the one before is multiplied, the table's entries a step earlier
+    if (g0 > 0) first();
+    // a tile's bounds are loaded while the two before are multiplied, the table's entries a tile earlier
 #pragma unroll 1
-    for (int tile = wave; tile * 16 < P; tile += U * PS_NW) {
-      next.bounds(a, h, tile + U * PS_NW, P, lr, lg);
+    for (int tile = wave; tile * 16 < P; tile += PS_NW) {
+      b2.bounds(a, h, tile + 2 * PS_NW, P, lr, lg);
+      const int p0 = tile * 16;
+      i32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int p0 = (tile + u * PS_NW) * 16;
-        i32x4 sum = {0, 0, 0, 0};
+      for (int i = 0; i < KB; ++i) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(b0.b[i], qb[i], sum, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < KB; ++i) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.b[u][i], qb[i], sum, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float s = __shfl(now.scale[u], lg * 4 + i, 64);
-          const bool there = now.have[u] >> (lg * 4 + i) & 1;
-          const uint32_t code = there ? bound_code((float)sum[i] * s) : 0;
-          if (mine && p0 + lg * 4 + i < P) {
-            if (G == 1) to[p0 + i] = code;
-            else atomicMax(to + p0 + i, code);
-          }
+      for (int i = 0; i < 4; ++i) {
+        const float s = __shfl(b0.scale, lg * 4 + i, 64);
+        const bool there = b0.have >> (lg * 4 + i) & 1;
+        const uint32_t code = there ? bound_code((float)sum[i] * s) : 0;
+        if (mine && p0 + lg * 4 + i < P) {
+          if (G == 1) to[p0 + i] = code;
+          else atomicMax(to + p0 + i, code);
         }
       }
-      now = next;
-      next.pages(a, table, tile + 2 * U * PS_NW, lr);
+      b0 = b1;
+      b1 = b2;
+      b2.pages(a, table, tile + 3 * PS_NW, lr);
     }
     __syncthreads();
   }
@@ -519,16 +513,18 @@ void launch_select(const PagedSelect& a, void* ws, hipStream_t stream) {
 // ---------------------------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------------------------
-// The segments of paged_core.h over the listed pages: an item is a query row with its K/V head (16 heads of the group a tile),
-// cut into `splits` runs of `chunk` rows of its list where there are too few items for the GPU.
+// The segments of paged_core.h over the listed pages: an item is a query row with its K/V head (16 heads of the group a tile), a
+// workgroup of eight waves takes one, or one of `splits` runs of `chunk` rows of its list where there are too few items for
+// the GPU: up to a quarter of the CUs (us of both launches, split / whole: 64 items of 4,096 rows of 64 dims 20 / 27, 128 of 1,536
+// rows of 128 dims 23 / 20.6, 256 of 2,048 rows in 8 bits 19 / 14.4).
 template <typename T, typename C, int D>
-__global__ __launch_bounds__(256, 2) void ps_kernel(PagedAttn a, PagedSplit z, int splits, int chunk) {
+__global__ __launch_bounds__(512, 2) void ps_kernel(PagedAttn a, PagedSplit z, int splits, int chunk) {
   const int b = xcd_remap(blockIdx.x, gridDim.x), part = b % splits;  // an XCD's workgroups share pages in its L2
   const int64_t item = b / splits;
   const int qt = (int)(item % z.qtiles), t = (int)(item / z.qtiles % a.Tq), nh = (int)(item / z.qtiles / a.Tq);
   const int64_t all = (int64_t)a.K << a.pool.shift, c0 = (int64_t)part * chunk;
   const int c1 = (int)(c0 + chunk < all ? c0 + chunk : all);
-  pa_segment<T, C, D, 1, false, true, 4>(a, z, nh / a.pool.H, nh % a.pool.H, t, qt, (int)(c0 < all ? c0 : all), c1,
+  pa_segment<T, C, D, 1, false, true, 8>(a, z, nh / a.pool.H, nh % a.pool.H, t, qt, (int)(c0 < all ? c0 : all), c1,
                                          splits > 1 ? b : -1, a.index + ((int64_t)nh * a.Tq + t) * a.K);
 }
 
@@ -552,11 +548,11 @@ struct SparseCut {
   int splits;
   SparseCut(int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows) {
     items = N * H * Tq * ((Hq / H + 15) / 16);
-    int64_t s = items > 0 ? 2 * cu_count() / items : 1;
-    const int64_t most = (rows + 255) / 256;  // 256 rows at least
+    int64_t s = items > 0 && items * 4 <= cu_count() ? cu_count() / items : 1;
+    const int64_t most = (rows + 511) / 512;  // two turns a wave at least
     s = s < 1 ? 1 : s < most ? s : most;
     if (s < 1) s = 1;
-    chunk = ((rows + s - 1) / s + 127) / 128 * 128;  // whole turns
+    chunk = ((rows + s - 1) / s + 127) / 128 * 128;
     if (chunk < 128) chunk = 128;
     splits = rows > 0 ? (int)((rows + chunk - 1) / chunk) : 1;
   }
@@ -577,7 +573,7 @@ void launch_sparse(const PagedAttn& a, void* ws, hipStream_t stream) {
   const SparseCut cut(a.N, a.Hq, a.pool.H, a.Tq, (int64_t)a.K << a.pool.shift);
   PagedSplit z;
   sparse_split(&z, (char*)ws, a.Hq, a.pool.H, D, cut);
-  hipLaunchKernelGGL((ps_kernel<T, C, D>), dim3((unsigned)(cut.items * cut.splits)), dim3(256), 0, stream, a, z, cut.splits,
+  hipLaunchKernelGGL((ps_kernel<T, C, D>), dim3((unsigned)(cut.items * cut.splits)), dim3(512), 0, stream, a, z, cut.splits,
                      (int)cut.chunk);
   if (cut.splits > 1)
     hipLaunchKernelGGL((ps_merge_kernel<T, C, D>), dim3((unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4)), dim3(256), 0, stream, a,

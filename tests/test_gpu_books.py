@@ -106,7 +106,7 @@ def test_odd_books(dev):
     _step(table, torch.zeros_like(n), torch.full_like(n, 300), free, fc, 16, what="an empty one")
 
 
-@pytest.mark.parametrize("N,most", [(1, 5000), (3, 0), (300, 40), (1023, 3), (1025, 9), (5000, 2), (2048, 70)])
+@pytest.mark.parametrize("N,most", [(1, 5000), (3, 0), (300, 40), (1023, 3), (1025, 9), (5000, 2), (2048, 70), (70, 16000)])
 def test_many_requests(dev, N, most):
     import tabicl_mi355_paged as paged
     g = torch.Generator().manual_seed(N)
