@@ -62,11 +62,11 @@ constexpr float PA_REF0 = -3.4028234663852886e38f;
 constexpr int PA_UNIT = 128, PA_WHOLE = 1024;
 
 // Units that an item of 8-bit rows counts for beyond its own, where some sequence is shorter than a workgroup's share: a
-// workgroup that begins several items has the latency of each beginning, half of what a turn of bf16 rows has to hide it
-// behind (us with 0 / 2 / 4 / 6 / 8 units, one row of 64 dims: 64 sequences of 100 to 3,000 rows 47 / 33 / 27 / 22 / 22, 16 of 500
-// to 10,000 27 / 22 / 21 / 20 / 20; of 128 dims and fp32, 12 query rows, 46 / 38 / 36 / 34 / 34; where all are longer they cost up to
-// 13%: 64 query rows over 8 x 5,000 30 / 36 / 32 / 34 / 33).
-constexpr int PA_EXTRA8 = 6;
+// workgroup that begins several items has the latency of each beginning, and a turn of 8-bit rows holds half the bytes of one of
+// bf16 to hide it behind (us with 2 / 4 / 6 units, one row of 64 dims: 64 sequences of 100 to 3,000 rows 29.0 / 23.8 / 22.8, 200 of
+// 1,100 to 2,000 over 2 heads 28.2 / 25.6 / 26.5; 40 rows over 32 of 300 to 30,000 and 4 heads 47.5 / 45.4 / 47.4; of 128 dims and
+// fp32, 12 rows over 16 of 500 to 10,000, 31.3 / 30.3 / 30.1).
+constexpr int PA_EXTRA8 = 4;
 
 struct PagedSplit {
   int groups;    // G, or 0: a workgroup of eight waves for each item
@@ -275,10 +275,12 @@ struct I8 {
   int8_t code;
 };
 
-// Turns of 64 keys: the bytes in flight of a turn of 32 keys in bf16.
+// Turns of 32 keys, as in bf16. (64 would keep as many bytes in flight; the code is twice as long then, and takes longer to come in
+// than the loads: 64 x 1,000 rows 20.2 us for 14.2, 12 query rows of 128 dims in fp32 over 16 sequences of 501 to 10,001 rows 34
+// for 26.6, where some registers do not fit either.)
 template <int D>
 struct PagedTile8 {
-  static constexpr int SUB = 4, KS = 64, NC = D / 32, DE = D / 16;
+  static constexpr int SUB = 2, KS = 32, NC = D / 32, DE = D / 16;
   static constexpr int KW = D / 16, VW = (DE + 3) / 4;  // dwords of a K and of a V row per lane
   uint32_t k[SUB][KW], v[SUB][4][VW];
   float ks[SUB], vs[SUB];
@@ -311,17 +313,17 @@ __device__ __forceinline__ uint2 codes_bf16<I8>(uint32_t x) {
                __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x07060302u)};
 }
 
-// The V operands of 32 keys (subtiles s and s + 1), one for each of the D / 16 columns of a lane. e4m3: bytes of four rows are
+// The V operands of the 32 keys, one for each of the D / 16 columns of a lane. e4m3: bytes of four rows are
 // regrouped by column, then converted in pairs; int8: converted byte by byte, then regrouped.
 template <typename C, int D>
-__device__ __forceinline__ void paged_operands8(const PagedTile8<D>& t, int s, bf16x8* va) {
+__device__ __forceinline__ void paged_operands8(const PagedTile8<D>& t, bf16x8* va) {
   constexpr int DE = D / 16, VW = PagedTile8<D>::VW, DP = DE < 4 ? DE : 4;  // columns of a dword
   uint32_t w[DE][4];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int v = 0; v < VW; ++v) {
-      const uint32_t r[4] = {t.v[s + u][0][v], t.v[s + u][1][v], t.v[s + u][2][v], t.v[s + u][3][v]};
+      const uint32_t r[4] = {t.v[u][0][v], t.v[u][1][v], t.v[u][2][v], t.v[u][3][v]};
       if constexpr (std::is_same<C, I8>::value) {
 #pragma unroll
         for (int e = 0; e < DP; ++e)
@@ -404,9 +406,9 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
   constexpr int SUB = Tile::SUB, KS = Tile::KS, NC = Tile::NC, DE = Tile::DE, ES = sizeof(C), TS = sizeof(T);
   constexpr int NQ = Q8 ? (TS == 2 ? 1 : 3) : 1, NP = TS == 2 ? 2 : 3;  // bf16 terms of q and of p, where C has 8 bits
   // Rows in 8 bits of up to 64 dims that one tile of query rows reads are loaded past the caches (one row over 8 x 45,000 rows 76 ->
-  // 68 us; a second tile would have to go to memory again, 64 query rows 120 -> 127, and so would the second half of a row of
-  // 128 dims).
-  constexpr int POLICY = (Q8 && !SEL && TS == 2 && QT <= 2 && D <= 64) ? 2 : 0;
+  // 68 us, 16 fp32 rows over 8 x 5,000 17.8 -> 16.5; a second tile would have to go to memory again, 64 query rows 120 -> 127, and
+  // so would the second half of a row of 128 dims).
+  constexpr int POLICY = (Q8 && !SEL && QT <= 2 && D <= 64) ? 2 : 0;
   __shared__ float sh_o[NW / 2][16 * QT][D + 4];
   __shared__ float2 sh_ml[NW / 2][16 * QT];
   const PagedPool& c = a.pool;
@@ -486,7 +488,7 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
     for (int s = 0; s < SUB; ++s) {
       const int k0 = key + 16 * s;
       int left = c1 - k0, i = left > 0 ? (k0 >> c.shift) - pg0 : 0;
-      if ((!Q8 || s == 0) && i >= 64) {  // 8 bits: a turn's pages are among the same 64 (c0 and the turns are multiples of 64)
+      if ((!Q8 || s == 0) && i >= 64) {  // 8 bits: a turn's pages are among the same 64 (c0 and the turns are multiples of 32)
         pg0 += i;
         pages();
         // waited for here, not wherever the paths join (there: for every load in flight)
@@ -583,69 +585,65 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
         if constexpr (QT > 1 && W) __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      // 32 keys at a time
+      const bool full = live == (16 << 8 | 16);
+      bf16x8 kb[2][NC], va[DE];
 #pragma unroll
-      for (int s0 = 0; s0 < SUB; s0 += 2) {
-        const bool full = (live >> (8 * s0) & 0xffff) == (16 << 8 | 16);
-        bf16x8 kb[2][NC], va[DE];
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const uint2 x = codes_bf16<C>(t.k[u][2 * i]), y = codes_bf16<C>(t.k[u][2 * i + 1]);
+          kb[u][i] = __builtin_bit_cast(bf16x8, (uint4{x.x, x.y, y.x, y.y}));
+        }
+      paged_operands8<C, D>(t, va);
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        float x[2][4], top = TA_NEG_INF;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          f32x4 sv = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = NQ - 1; j >= 0; --j)  // the smallest terms first
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+              sv = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[u][i], __builtin_bit_cast(bf16x8, q[qt][j][i]), sv, 0, 0, 0);
+          const float f = sc * t.ks[u];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[u][i] = log2_score(sv[i], f);
+        }
+        if (!full) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[u][i] = lg * 4 + i < (live >> (8 * u) & 255) ? x[u][i] : TA_NEG_INF;
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            const uint2 x = codes_bf16<C>(t.k[s0 + u][2 * i]), y = codes_bf16<C>(t.k[s0 + u][2 * i + 1]);
-            kb[u][i] = __builtin_bit_cast(bf16x8, (uint4{x.x, x.y, y.x, y.y}));
-          }
-        paged_operands8<C, D>(t, s0, va);
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, x[u][i]);
+        if (wave_any(top - ref[qt] > PA_SLACK)) {
+          const float to = fmaxf(ref[qt], quad_max(top)), f = __builtin_amdgcn_exp2f(ref[qt] - to);
+          ref[qt] = to;
+          l[qt] *= f;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          float x[2][4], top = TA_NEG_INF;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            f32x4 sv = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = NQ - 1; j >= 0; --j)  // the smallest terms first
-#pragma unroll
-              for (int i = 0; i < NC; ++i)
-                sv = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[u][i], __builtin_bit_cast(bf16x8, q[qt][j][i]), sv, 0, 0, 0);
-            const float f = sc * t.ks[s0 + u];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[u][i] = log2_score(sv[i], f);
-          }
-          if (!full) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) x[u][i] = lg * 4 + i < (live >> (8 * (s0 + u)) & 255) ? x[u][i] : TA_NEG_INF;
-          }
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, x[u][i]);
-          if (wave_any(top - ref[qt] > PA_SLACK)) {
-            const float to = fmaxf(ref[qt], quad_max(top)), f = __builtin_amdgcn_exp2f(ref[qt] - to);
-            ref[qt] = to;
-            l[qt] *= f;
-#pragma unroll
-            for (int e = 0; e < DE; ++e) o[qt][e] *= f;
-          }
-          float p[8];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[4 * u + i] = __builtin_amdgcn_exp2f(x[u][i] - ref[qt]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) l[qt] += (p[4 * u] + p[4 * u + 1]) + (p[4 * u + 2] + p[4 * u + 3]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[4 * u + i] *= t.vs[s0 + u] * Shift::VALUE;
-          bf16x8 pt[NP];
-          bf16_terms<NP>(p, pt);
-#pragma unroll
-          for (int e = 0; e < DE; ++e)
-#pragma unroll
-            for (int j = NP - 1; j >= 0; --j) o[qt][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[e], pt[j], o[qt][e], 0, 0, 0);
+          for (int e = 0; e < DE; ++e) o[qt][e] *= f;
         }
+        float p[8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[4 * u + i] = __builtin_amdgcn_exp2f(x[u][i] - ref[qt]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) l[qt] += (p[4 * u] + p[4 * u + 1]) + (p[4 * u + 2] + p[4 * u + 3]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[4 * u + i] *= t.vs[u] * Shift::VALUE;
+        bf16x8 pt[NP];
+        bf16_terms<NP>(p, pt);
+#pragma unroll
+        for (int e = 0; e < DE; ++e)
+#pragma unroll
+          for (int j = NP - 1; j >= 0; --j) o[qt][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[e], pt[j], o[qt][e], 0, 0, 0);
       }
     }
   };
