@@ -263,7 +263,8 @@ void launch_bounds(const PagedBounds& a, int format, dim3 grid, hipStream_t stre
 // and the first ones equal to it, in order. Bound by its chain of loads and barriers (64 query rows of 704 pages: a few MB), so
 // the first tiles' table entries and bounds are on their way before the queries are looked at, the histograms of all
 // digits are cleared at once, every wave of a row finds the digit for itself (one barrier a digit), and there is little code:
-// most of it runs once, as fast as instructions come in (four tiles at a time instead of one, twice: 12.7 us for 11.8).
+// most of it runs once, as fast as instructions come in (three tiles at a time instead of two: 10.8 us for 10.2). One row of 8
+// sequences of 704 pages and 8 heads takes 10.2 us, of which the bounds take 4 and the digits 1.7; 16 pages alone 5.5.
 constexpr int PS_NW = 16, PS_LDS = 32768;  // codes kept in LDS
 
 __device__ __forceinline__ uint32_t bound_code(float x) {  // larger bound, larger code; none is 0
@@ -277,27 +278,23 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
 
 // A tile of 16 pages (a wave takes every 16th): their bounds as operands, their scales and whether they are there. The table is
 // read up to its width, not the sequence's, so that its entries need not wait for the length.
+__device__ __forceinline__ int tile_page(const PagedSelect& a, const int32_t* table, int tile, int lr) {
+  const int64_t p = (int64_t)tile * 16 + lr;
+  return p < a.pool.max_pages ? table[p] : -1;
+}
 template <int KB>
-struct BoundTiles {
-  int page;
+struct BoundTile {
   i32x4 b[KB];
   float scale;
-  uint32_t have;
-  __device__ __forceinline__ void pages(const PagedSelect& a, const int32_t* table, int tile, int lr) {
-    const int64_t p = (int64_t)tile * 16 + lr;
-    page = p < a.pool.max_pages ? table[p] : -1;
-  }
-  __device__ __forceinline__ void bounds(const PagedSelect& a, int h, int tile, int P, int lr, int lg) {
-    const bool in = page >= 0 && page < a.pool.pages && tile * 16 + lr < P;
-    const int64_t at = (int64_t)(in ? page : 0) * a.pool.H + h;
-    have = (uint32_t)__ballot(in) & 0xffffu;
-    scale = 0.f;
-#pragma unroll
-    for (int i = 0; i < KB; ++i) b[i] = i32x4{0, 0, 0, 0};
+  bool in;
+  // bounds, scales: page 0's, from this head and lane's on
+  __device__ __forceinline__ void load(const PagedSelect& a, const int8_t* bounds, const float* scales, int page, int p, int P) {
+    in = (uint32_t)page < (uint32_t)a.pool.pages && p < P;
     if (in) {
-      scale = a.bound_scales[at];
+      const int64_t at = (int64_t)page * a.pool.H;
+      scale = scales[at];
 #pragma unroll
-      for (int i = 0; i < KB; ++i) b[i] = *(const i32x4*)(a.bounds + (at * KB + i) * 64 + lg * 16);
+      for (int i = 0; i < KB; ++i) b[i] = *(const i32x4*)(bounds + at * (KB * 64) + i * 64);
     }
   }
 };
@@ -319,20 +316,26 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
   int* hist = (int*)lds;
   const int64_t nh = (int64_t)n * c.H + h;
   uint32_t* codes = GLOBAL ? store + (nh * a.Tq + t0) * stride : lds + (1024 << tshift);
-  BoundTiles<KB> b0, b1, b2;
+  constexpr int NB = 2;
+  const int8_t* bounds = a.bounds + h * (2 * D) + lg * 16;
+  const float* scales = a.bound_scales + h;
+  BoundTile<KB> b[NB];
+  int page[NB];  // of the tiles NB rounds later
   auto first = [&]() {
-    b0.pages(a, table, wave, lr);
-    b1.pages(a, table, wave + PS_NW, lr);
-    b2.pages(a, table, wave + 2 * PS_NW, lr);
-    b0.bounds(a, h, wave, P, lr, lg);
-    b1.bounds(a, h, wave + PS_NW, P, lr, lg);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) page[i] = tile_page(a, table, wave + i * PS_NW, lr);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      b[i].load(a, bounds, scales, page[i], (wave + i * PS_NW) * 16 + lr, P);
+      page[i] = tile_page(a, table, wave + (NB + i) * PS_NW, lr);
+    }
   };
   first();
 
   // column `wave` of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
   const char* q = (const char*)a.q + (n * a.q_sn + (int64_t)h * G * a.q_sh) * sizeof(T);
   const bool wide = G > 16;
-  const int qrow = wide ? 0 : wave * per16 >> 8, qhead = wave - qrow * G;
+  const int qrow = wide ? 0 : wave * per16 >> 8, qhead = wave - qrow * G, qplace = (wave & 3) * 4 + (wave >> 2);
   float x[NV];
   auto column = [&](int g0) {
     const int g = g0 + qhead;
@@ -352,11 +355,10 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
   }
 #pragma unroll 1
   for (int i = threadIdx.x; i < 1024 << tshift; i += PS_NW * 64) hist[i] = 0;
-  if (G > 1)
 #pragma unroll 1
-    for (int t = 0; t < TT; ++t)
+  for (int t = 0; t < TT; ++t)
 #pragma unroll 1
-      for (int i = threadIdx.x; i < P; i += PS_NW * 64) codes[t * stride + i] = 0;
+    for (int i = threadIdx.x; i < P; i += PS_NW * 64) codes[t * stride + i] = 0;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) most = across(most, s, umax);
   if (lane == 0) sh_most[wave] = most;
@@ -375,40 +377,48 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
       const int d = lane + 64 * i;
       const int u = x[i] != x[i] ? 0 : (int)fminf(fmaxf(__builtin_rintf(x[i] * inv), -127.f), 127.f);
       if (d < D) {
-        sh_q[wave][d] = (int8_t)(u > 0 ? u : 0);
-        sh_q[wave][D + d] = (int8_t)(u < 0 ? u : 0);
+        sh_q[qplace][d] = (int8_t)(u > 0 ? u : 0);
+        sh_q[qplace][D + d] = (int8_t)(u < 0 ? u : 0);
       }
     }
     __syncthreads();
-    const int t = wide ? 0 : lr * per16 >> 8, g = g0 + lr - t * G;
-    const bool mine = t < TT && g < G && t0 + t < a.Tq;
-    uint32_t* to = codes + t * stride + lg * 4;
+    // this lane's products are those of page lr with columns lg, lg + 4, ...
+    const int left = wide ? G - g0 : TT * G, values = left < 16 ? (left + 3) >> 2 : 4;
+    uint32_t* to[4];
+    bool mine[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = lg + 4 * i, t = wide ? 0 : j * per16 >> 8, g = g0 + j - t * G;
+      mine[i] = t < TT && g < G && t0 + t < a.Tq;
+      to[i] = codes + t * stride;
+    }
     i32x4 qb[KB];
 #pragma unroll
     for (int i = 0; i < KB; ++i) qb[i] = *(const i32x4*)(&sh_q[lr][i * 64 + lg * 16]);
     if (g0 > 0) first();
-    // a tile's bounds are loaded while the two before are multiplied, the table's entries a tile earlier
+    // a tile's bounds are loaded while the one before is multiplied, the table's entries two tiles earlier (each in registers of
+    // its own: to pass a tile on would wait for it)
 #pragma unroll 1
-    for (int tile = wave; tile * 16 < P; tile += PS_NW) {
-      b2.bounds(a, h, tile + 2 * PS_NW, P, lr, lg);
-      const int p0 = tile * 16;
-      i32x4 sum = {0, 0, 0, 0};
+    for (int tile0 = wave; tile0 * 16 < P; tile0 += NB * PS_NW)
 #pragma unroll
-      for (int i = 0; i < KB; ++i) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(b0.b[i], qb[i], sum, 0, 0, 0);
+      for (int r = 0; r < NB; ++r) {
+        const int tile = tile0 + r * PS_NW, p0 = tile * 16;
+        if (p0 >= P) break;
+        i32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float s = __shfl(b0.scale, lg * 4 + i, 64);
-        const bool there = b0.have >> (lg * 4 + i) & 1;
-        const uint32_t code = there ? bound_code((float)sum[i] * s) : 0;
-        if (mine && p0 + lg * 4 + i < P) {
-          if (G == 1) to[p0 + i] = code;
-          else atomicMax(to + p0 + i, code);
+        for (int i = 0; i < KB; ++i) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(qb[i], b[r].b[i], sum, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i >= values) break;
+          const uint32_t code = bound_code((float)sum[i] * b[r].scale);
+          if (mine[i] && b[r].in) {
+            if (G == 1) to[i][p0 + lr] = code;
+            else atomicMax(to[i] + p0 + lr, code);
+          }
         }
+        b[r].load(a, bounds, scales, page[r], p0 + NB * PS_NW * 16 + lr, P);
+        page[r] = tile_page(a, table, tile + 2 * NB * PS_NW, lr);
       }
-      b0 = b1;
-      b1 = b2;
-      b2.pages(a, table, tile + 3 * PS_NW, lr);
-    }
     __syncthreads();
   }
 
