@@ -817,11 +817,11 @@ __global__ __launch_bounds__(256, pa_waves(D, QT)) void pa_kernel(PagedAttn a, P
   }
 }
 
-// A workgroup of eight waves for each item, where no sequence is long.
-template <typename T, typename C, int D, int QT, bool W>
-__global__ __launch_bounds__(512) void pa_whole_kernel(PagedAttn a, PagedSplit z) {
+// A workgroup of NW waves for each item, where no sequence is long.
+template <typename T, typename C, int D, int QT, bool W, int NW = 8>
+__global__ __launch_bounds__(64 * NW, 2) void pa_whole_kernel(PagedAttn a, PagedSplit z) {
   const int per = a.pool.H * z.qtiles, n = blockIdx.x / per, item = blockIdx.x % per;
-  pa_segment<T, C, D, QT, W, false, 8>(a, z, n, item / z.qtiles, 0, item % z.qtiles, 0,
+  pa_segment<T, C, D, QT, W, false, NW>(a, z, n, item / z.qtiles, 0, item % z.qtiles, 0,
                                        __builtin_amdgcn_readfirstlane(pa_len(a, n)), -1);
 }
 

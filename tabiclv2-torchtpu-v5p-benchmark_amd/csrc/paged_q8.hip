@@ -296,8 +296,16 @@ int64_t run_pa8(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, 
   z.ends = (int2*)take(z.groups ? N * H * z.qtiles * 8 : 0);
   if (!a) return at;
   if (z.groups == 0) {
-    if constexpr (pa_waves(D, QT) == 2)
-      hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false>), dim3((unsigned)(N * H * z.qtiles)), dim3(512), 0, stream, *a, z);
+    // Two waves for each item up to 256 rows and four beyond, so that many items share a CU; eight for more than 512 rows where
+    // every item has a CU (us with 2 / 4 / 8 waves: 2,048 items of one query row of 64 dims and 64 rows 7.7 / - / 18.1, of 512 rows
+    // 24 / 25 / 32; of 60 query rows 20 / - / 74 and 48 / 59 / 102; 64 items of one query row and 256 rows 6.2 / - / 6.1, of 1,024 13.2 /
+    // 9.0 / 8.2; 16 items in fp32 of 800 rows - / 9.6 / 8.1).
+    const int64_t items = N * H * z.qtiles;
+    const dim3 grid((unsigned)items);
+    if (rows <= 256) hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 2>), grid, dim3(128), 0, stream, *a, z);
+    else if (rows <= 512 || items > cu_count())
+      hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 4>), grid, dim3(256), 0, stream, *a, z);
+    else hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 8>), grid, dim3(512), 0, stream, *a, z);
   } else {
     hipLaunchKernelGGL((pa_kernel<T, C, D, QT, false>), dim3((unsigned)z.groups), dim3(256), 0, stream, *a, z);
     hipLaunchKernelGGL((pa_merge_kernel<T, C, D, QT>), dim3((unsigned)((N * Hq * Tq + 3) / 4)), dim3(256), 0, stream, *a, z);

@@ -524,17 +524,19 @@ void launch_select(const PagedSelect& a, void* ws, hipStream_t stream) {
 // attention
 // ---------------------------------------------------------------------------------------------
 // The segments of paged_core.h over the listed pages: an item is a query row with its K/V head (16 heads of the group a tile), a
-// workgroup of eight waves takes one, or one of `splits` runs of `chunk` rows of its list where there are too few items for
-// the GPU: up to a quarter of the CUs (us of both launches, split / whole: 64 items of 4,096 rows of 64 dims 20 / 27, 128 of 1,536
-// rows of 128 dims 23 / 20.6, 256 of 2,048 rows in 8 bits 19 / 14.4).
-template <typename T, typename C, int D>
-__global__ __launch_bounds__(512, 2) void ps_kernel(PagedAttn a, PagedSplit z, int splits, int chunk) {
+// workgroup takes one, or one of `splits` runs of `chunk` rows of its list where there are too few items for the GPU: up to a
+// quarter of the CUs (us of both launches, split / whole: 64 items of 4,096 rows of 64 dims 20 / 27, 128 of 1,536 rows of 128 dims
+// 23 / 20.6, 256 of 2,048 rows in 8 bits 19 / 14.4). A workgroup has eight waves, or two where the rows are few or the workgroups
+// fill the chip (us with 8 / 2 waves in bf16, in 8 bits: 1,024 items of 64 rows 10.6 / 6.8, 11.0 / 6.2, of 2,048 rows 50 / 47, 34 / 35;
+// 256 items of 256 rows 7.2 / 6.1, 6.7 / 6.7, of 1,024 rows 14.7 / 13.8, 9.7 / 15.1).
+template <typename T, typename C, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void ps_kernel(PagedAttn a, PagedSplit z, int splits, int chunk) {
   const int b = xcd_remap(blockIdx.x, gridDim.x), part = b % splits;  // an XCD's workgroups share pages in its L2
   const int64_t item = b / splits;
   const int qt = (int)(item % z.qtiles), t = (int)(item / z.qtiles % a.Tq), nh = (int)(item / z.qtiles / a.Tq);
   const int64_t all = (int64_t)a.K << a.pool.shift, c0 = (int64_t)part * chunk;
   const int c1 = (int)(c0 + chunk < all ? c0 + chunk : all);
-  pa_segment<T, C, D, 1, false, true, 8>(a, z, nh / a.pool.H, nh % a.pool.H, t, qt, (int)(c0 < all ? c0 : all), c1,
+  pa_segment<T, C, D, 1, false, true, NW>(a, z, nh / a.pool.H, nh % a.pool.H, t, qt, (int)(c0 < all ? c0 : all), c1,
                                          splits > 1 ? b : -1, a.index + ((int64_t)nh * a.Tq + t) * a.K);
 }
 
@@ -583,8 +585,11 @@ void launch_sparse(const PagedAttn& a, void* ws, hipStream_t stream) {
   const SparseCut cut(a.N, a.Hq, a.pool.H, a.Tq, (int64_t)a.K << a.pool.shift);
   PagedSplit z;
   sparse_split(&z, (char*)ws, a.Hq, a.pool.H, D, cut);
-  hipLaunchKernelGGL((ps_kernel<T, C, D>), dim3((unsigned)(cut.items * cut.splits)), dim3(512), 0, stream, a, z, cut.splits,
-                     (int)cut.chunk);
+  const dim3 grid((unsigned)(cut.items * cut.splits));
+  if (cut.chunk <= 256 || cut.items * cut.splits > 2 * cu_count())
+    hipLaunchKernelGGL((ps_kernel<T, C, D, 2>), grid, dim3(128), 0, stream, a, z, cut.splits, (int)cut.chunk);
+  else
+    hipLaunchKernelGGL((ps_kernel<T, C, D, 8>), grid, dim3(512), 0, stream, a, z, cut.splits, (int)cut.chunk);
   if (cut.splits > 1)
     hipLaunchKernelGGL((ps_merge_kernel<T, C, D>), dim3((unsigned)(((int64_t)a.N * a.Hq * a.Tq + 3) / 4)), dim3(256), 0, stream, a,
                        z, cut.splits);

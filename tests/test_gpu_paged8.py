@@ -482,7 +482,11 @@ def test_cache_together(dev, code):
             assert ((out.double() - want).abs() <= tol + 2.0 ** -8 * most).all()
     q = torch.randn(S, H, 2, D, generator=g, device=dev).to(BF)
     want = c.query(1, q)
-    assert torch.equal(c.estimators(1, 3).query(1, q[1:]), want[1:])
+    # of fewer rows a sequence's keys are shared among other waves: the same terms summed in another order, each sum within the
+    # tolerance of the exact value, so within twice of it of each other
+    k, v = paged.paged_gather(*c.block_kv(1), c.table, c.lengths[1], 501, scales=c.scales[1], dtype=F32)
+    _, _, tol, _ = paged_ref.attention(q, k, v, torch.arange(S, dtype=torch.int32, device=dev).view(S, 1), c.lengths[1], D ** -0.5)
+    assert ((c.estimators(1, 3).query(1, q[1:]).double() - want[1:].double()).abs() <= 2 * tol[1:]).all()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         got = c.query(1, q)
