@@ -115,18 +115,19 @@ __device__ __forceinline__ uint32_t to_codes_within<I8>(const float* x, float in
 // append
 // ---------------------------------------------------------------------------------------------
 // LANES threads take the new rows of one page and head, of K or of V: the largest |x|, the scale, the codes. Up to LANES * 8
-// chunks of eight values are read once and kept; a larger page's are read again for their codes. LANES = 256 where a page has
-// more chunks than a wave keeps. Where a value is not finite, or beyond the largest scale, they are gone through value by value.
+// chunks of eight values are read once and kept; a larger page's are read again for their codes. A wave takes a page of up to 64 *
+// 8 chunks, a workgroup of 256 or 512 threads a larger one (10 x 16,907 rows of 128 dims in fp32 to pages of 256 rows, which 512
+// threads keep and 256 do not: 283 -> 214 us with their way back). Where a value is not finite, or beyond the largest scale, they are gone through value by value.
 // Bound by the bytes of the rows and codes: 8 x 45,000 rows in bf16 to int8 268 us -> 238 with magnitudes compared in pairs and
 // codes without limits (15 -> 4 instructions a value), 221 with loads that leave the caches alone (stores that do: 217, and what
 // reads the codes next takes 10 us more).
 constexpr int PQ_KEEP = 8;
 
 template <typename T, typename C, int LANES>
-__global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8 a) {
+__global__ __launch_bounds__(LANES == 64 ? 256 : LANES) void paged_append8_kernel(PagedAppend8 a) {
   const PagedPool& c = a.rows.pool;
   const int n = blockIdx.y, v = blockIdx.z, D = c.D, R = 1 << c.shift;
-  const int item = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const int item = LANES == 64 ? blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x, lane = threadIdx.x % LANES;
   const int h = item % c.H, j = item / c.H;
   const int64_t cap = (int64_t)c.max_pages << c.shift;
   const int start = pool_length(c, n);
@@ -153,13 +154,13 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(PagedAppend8 a) {
       const uint32_t o = __shfl_xor(m, x, 64);
       m = o > m ? o : m;
     }
-    if constexpr (LANES == 256) {
-      __shared__ uint32_t sh[4];
+    if constexpr (LANES > 64) {
+      __shared__ uint32_t sh[LANES / 64];
       __syncthreads();
       if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m = sh[i] > m ? sh[i] : m;
+      for (int i = 0; i < LANES / 64; ++i) m = sh[i] > m ? sh[i] : m;
     }
     return m;
   };
@@ -392,7 +393,8 @@ void launch_append8(const PagedAppend8& a, hipStream_t stream) {
     }
     const dim3 grid((unsigned)gx, (unsigned)(a.rows.N - n < some ? a.rows.N - n : some), 2);
     if (wave) hipLaunchKernelGGL((paged_append8_kernel<T, C, 64>), grid, dim3(256), 0, stream, part);
-    else hipLaunchKernelGGL((paged_append8_kernel<T, C, 256>), grid, dim3(256), 0, stream, part);
+    else if (chunks <= 256 * PQ_KEEP) hipLaunchKernelGGL((paged_append8_kernel<T, C, 256>), grid, dim3(256), 0, stream, part);
+    else hipLaunchKernelGGL((paged_append8_kernel<T, C, 512>), grid, dim3(512), 0, stream, part);
   }
 }
 
