@@ -790,11 +790,14 @@ __device__ __forceinline__ void pa_merge_row(const PagedAttn& a, const PagedSpli
 // Waves per SIMD that the registers of a kernel allow: one for tiles of 32 and 64 query rows of 128 dims. In tiles of 16 with
 // two waves every tile reads K and V again (tiles of 16 / larger: bf16, 32 query rows a head over 8 x 5,000 rows 57 / 42 us,
 // 64 rows 104 / 48; fp32, 17 rows 102 / 70, 34 rows over 49 x 5,311 372 / 304).
+// Over 8-bit rows 32 bf16 query rows of 128 dims fit beside a second wave.
 constexpr int pa_waves(int D, int QT) { return D == 128 && QT > 1 ? 1 : 2; }
+template <typename T, typename C>
+constexpr int pa_waves_of(int D, int QT) { return sizeof(C) > 1 ? pa_waves(D, QT) : D == 128 && QT > 1 && sizeof(T) == 4 ? 1 : 2; }
 
 // Equal shares of all items' units.
 template <typename T, typename C, int D, int QT, bool W>
-__global__ __launch_bounds__(256, pa_waves(D, QT)) void pa_kernel(PagedAttn a, PagedSplit z) {
+__global__ __launch_bounds__(256, (pa_waves_of<T, C>(D, QT))) void pa_kernel(PagedAttn a, PagedSplit z) {
   const int per = a.pool.H * z.qtiles;
   PagedUnits units(a, per, threadIdx.x & 63);
   if constexpr (sizeof(C) == 1) units.weigh(PagedShares(z, units.total).share, PA_EXTRA8);

@@ -283,9 +283,10 @@ int64_t run_pa8(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, 
   const int64_t qrows = Hq / H * Tq;
   PagedSplit z = {};
   z.qtiles = (int)((qrows + 16 * QT - 1) / (16 * QT));
-  z.groups = rows <= PA_WHOLE ? 0 : pa_waves(D, QT) * cu_count();
+  constexpr int waves = pa_waves_of<T, C>(D, QT);
+  z.groups = rows <= PA_WHOLE && waves == 2 ? 0 : waves * cu_count();
   z.least = 2;
-  z.few = D > 32 && pa_waves(D, QT) == 2 ? 12 * z.groups : 0;
+  z.few = D > 32 && waves == 2 ? 12 * z.groups : 0;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     char* p = (char*)ws + at;
@@ -303,10 +304,12 @@ int64_t run_pa8(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, 
     // 9.0 / 8.2; 16 items in fp32 of 800 rows - / 9.6 / 8.1).
     const int64_t items = N * H * z.qtiles;
     const dim3 grid((unsigned)items);
-    if (rows <= 256) hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 2>), grid, dim3(128), 0, stream, *a, z);
-    else if (rows <= 512 || items > cu_count())
-      hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 4>), grid, dim3(256), 0, stream, *a, z);
-    else hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 8>), grid, dim3(512), 0, stream, *a, z);
+    if constexpr (waves == 2) {
+      if (rows <= 256) hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 2>), grid, dim3(128), 0, stream, *a, z);
+      else if (rows <= 512 || items > cu_count())
+        hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 4>), grid, dim3(256), 0, stream, *a, z);
+      else hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 8>), grid, dim3(512), 0, stream, *a, z);
+    }
   } else {
     hipLaunchKernelGGL((pa_kernel<T, C, D, QT, false>), dim3((unsigned)z.groups), dim3(256), 0, stream, *a, z);
     hipLaunchKernelGGL((pa_merge_kernel<T, C, D, QT>), dim3((unsigned)((N * Hq * Tq + 3) / 4)), dim3(256), 0, stream, *a, z);
@@ -318,12 +321,17 @@ template <typename T, typename C, int D>
 int64_t run_pa8_rows(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows,
                      hipStream_t stream) {
   const int64_t qrows = Hq / H * Tq;
-  // query rows of a tile: as many as the registers hold (three bf16 terms of each in fp32)
-  constexpr int most = sizeof(T) == 4 ? (D == 32 ? 32 : 16) : D == 128 ? 16 : 64;
-  if constexpr (most >= 64)
-    if (qrows > 32) return run_pa8<T, C, D, 4>(a, ws, N, Hq, H, Tq, rows, stream);
-  if constexpr (most >= 32)
-    if (qrows > 16) return run_pa8<T, C, D, 2>(a, ws, N, Hq, H, Tq, rows, stream);
+  // Tiles of 16 query rows or, up to what the registers hold, 32 or 64: every tile converts K and V again (us in tiles of 16 / 32 /
+  // 64: 64 query rows over 48 x 6,239 rows and 2 heads of 128 dims 97 / 66 / -, in fp32 104 / 83 / -, in fp32 of 64 dims 63 / 50 /
+  // 71). Up to PA_WHOLE rows only as far as the items fill the chip (64 dims, bf16: 64 rows over 8 x 300 6.9 / 8.5 / 11.9, 200 over
+  // 57 x 1,000 and 2 heads 35 / 30 / 27, 64 over 256 x 300 77 / 54 / 50).
+  constexpr int most = sizeof(T) == 4 || D == 128 ? 2 : 4;
+  auto wider = [&](int qt) {  // than 16 qt rows
+    return qrows > 16 * qt && (rows > PA_WHOLE || N * H * ((qrows + 16 * qt - 1) / (16 * qt)) > 2 * cu_count());
+  };
+  if constexpr (most == 4)
+    if (wider(1) && wider(2)) return run_pa8<T, C, D, 4>(a, ws, N, Hq, H, Tq, rows, stream);
+  if ((rows > PA_WHOLE || pa_waves_of<T, C>(D, 2) == 2) && wider(1)) return run_pa8<T, C, D, 2>(a, ws, N, Hq, H, Tq, rows, stream);
   return run_pa8<T, C, D, 1>(a, ws, N, Hq, H, Tq, rows, stream);
 }
 

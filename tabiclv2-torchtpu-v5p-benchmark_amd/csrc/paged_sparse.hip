@@ -321,104 +321,119 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
   const float* scales = a.bound_scales + h;
   BoundTile<KB> b[NB];
   int page[NB];  // of the tiles NB rounds later
-  auto first = [&]() {
+  auto pages = [&]() {
 #pragma unroll
     for (int i = 0; i < NB; ++i) page[i] = tile_page(a, table, wave + i * PS_NW, lr);
+  };
+  auto first = [&]() {
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       b[i].load(a, bounds, scales, page[i], (wave + i * PS_NW) * 16 + lr, P);
       page[i] = tile_page(a, table, wave + (NB + i) * PS_NW, lr);
     }
   };
-  first();
-
-  // column `wave` of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
-  const char* q = (const char*)a.q + (n * a.q_sn + (int64_t)h * G * a.q_sh) * sizeof(T);
-  const bool wide = G > 16;
-  const int qrow = wide ? 0 : wave * per16 >> 8, qhead = wave - qrow * G, qplace = (wave & 3) * 4 + (wave >> 2);
-  float x[NV];
-  auto column = [&](int g0) {
-    const int g = g0 + qhead;
-    const bool in = qrow < TT && t0 + qrow < a.Tq && g < G;
+  pages();
+  if (a.K < P) {
+    first();
+    // column `wave` of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
+    const char* q = (const char*)a.q + (n * a.q_sn + (int64_t)h * G * a.q_sh) * sizeof(T);
+    const bool wide = G > 16;
+    const int qrow = wide ? 0 : wave * per16 >> 8, qhead = wave - qrow * G, qplace = (wave & 3) * 4 + (wave >> 2);
+    float x[NV];
+    auto column = [&](int g0) {
+      const int g = g0 + qhead;
+      const bool in = qrow < TT && t0 + qrow < a.Tq && g < G;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int d = lane + 64 * i;
-      x[i] = in && d < D ? (float)*(const T*)(q + (g * a.q_sh + (t0 + qrow) * a.q_st + d) * (int64_t)sizeof(T)) : 0.f;
-    }
-  };
-  uint32_t most = 0;
-#pragma unroll 1
-  for (int g0 = 0; g0 < G; g0 += 16) {
-    column(g0);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) most = umax(most, finite_bits(x[i]));
-  }
-#pragma unroll 1
-  for (int i = threadIdx.x; i < 1024 << tshift; i += PS_NW * 64) hist[i] = 0;
-#pragma unroll 1
-  for (int t = 0; t < TT; ++t)
-#pragma unroll 1
-    for (int i = threadIdx.x; i < P; i += PS_NW * 64) codes[t * stride + i] = 0;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) most = across(most, s, umax);
-  if (lane == 0) sh_most[wave] = most;
-  __syncthreads();
-  // the step of this column's query row: the largest of its group's
-  most = 0;
-#pragma unroll 1
-  for (int w = wide ? 0 : qrow * G, end = wide || w + G > 16 ? 16 : w + G; w < end; ++w) most = umax(most, sh_most[w]);
-  const float inv = pow2(-step_exponent(most));
-
-#pragma unroll 1
-  for (int g0 = 0; g0 < G; g0 += 16) {
-    if (wide) column(g0);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int d = lane + 64 * i;
-      const int u = x[i] != x[i] ? 0 : (int)fminf(fmaxf(__builtin_rintf(x[i] * inv), -127.f), 127.f);
-      if (d < D) {
-        sh_q[qplace][d] = (int8_t)(u > 0 ? u : 0);
-        sh_q[qplace][D + d] = (int8_t)(u < 0 ? u : 0);
+      for (int i = 0; i < NV; ++i) {
+        const int d = lane + 64 * i;
+        x[i] = in && d < D ? (float)*(const T*)(q + (g * a.q_sh + (t0 + qrow) * a.q_st + d) * (int64_t)sizeof(T)) : 0.f;
       }
+    };
+    uint32_t most = 0;
+#pragma unroll 1
+    for (int g0 = 0; g0 < G; g0 += 16) {
+      column(g0);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) most = umax(most, finite_bits(x[i]));
     }
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 1024 << tshift; i += PS_NW * 64) hist[i] = 0;
+#pragma unroll 1
+    for (int t = 0; t < TT; ++t)
+#pragma unroll 1
+      for (int i = threadIdx.x; i < P; i += PS_NW * 64) codes[t * stride + i] = 0;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) most = across(most, s, umax);
+    if (lane == 0) sh_most[wave] = most;
     __syncthreads();
-    // this lane's products are those of page lr with columns lg, lg + 4, ...
-    const int left = wide ? G - g0 : TT * G, values = left < 16 ? (left + 3) >> 2 : 4;
-    uint32_t* to[4];
-    bool mine[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = lg + 4 * i, t = wide ? 0 : j * per16 >> 8, g = g0 + j - t * G;
-      mine[i] = t < TT && g < G && t0 + t < a.Tq;
-      to[i] = codes + t * stride;
-    }
-    i32x4 qb[KB];
-#pragma unroll
-    for (int i = 0; i < KB; ++i) qb[i] = *(const i32x4*)(&sh_q[lr][i * 64 + lg * 16]);
-    if (g0 > 0) first();
-    // a tile's bounds are loaded while the one before is multiplied, the table's entries two tiles earlier (each in registers of
-    // its own: to pass a tile on would wait for it)
+    // the step of this column's query row: the largest of its group's
+    most = 0;
 #pragma unroll 1
-    for (int tile0 = wave; tile0 * 16 < P; tile0 += NB * PS_NW)
+    for (int w = wide ? 0 : qrow * G, end = wide || w + G > 16 ? 16 : w + G; w < end; ++w) most = umax(most, sh_most[w]);
+    const float inv = pow2(-step_exponent(most));
+
+#pragma unroll 1
+    for (int g0 = 0; g0 < G; g0 += 16) {
+      if (wide) column(g0);
 #pragma unroll
-      for (int r = 0; r < NB; ++r) {
-        const int tile = tile0 + r * PS_NW, p0 = tile * 16;
-        if (p0 >= P) break;
-        i32x4 sum = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < KB; ++i) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(qb[i], b[r].b[i], sum, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i >= values) break;
-          const uint32_t code = bound_code((float)sum[i] * b[r].scale);
-          if (mine[i] && b[r].in) {
-            if (G == 1) to[i][p0 + lr] = code;
-            else atomicMax(to[i] + p0 + lr, code);
-          }
+      for (int i = 0; i < NV; ++i) {
+        const int d = lane + 64 * i;
+        const int u = x[i] != x[i] ? 0 : (int)fminf(fmaxf(__builtin_rintf(x[i] * inv), -127.f), 127.f);
+        if (d < D) {
+          sh_q[qplace][d] = (int8_t)(u > 0 ? u : 0);
+          sh_q[qplace][D + d] = (int8_t)(u < 0 ? u : 0);
         }
-        b[r].load(a, bounds, scales, page[r], p0 + NB * PS_NW * 16 + lr, P);
-        page[r] = tile_page(a, table, tile + 2 * NB * PS_NW, lr);
       }
+      __syncthreads();
+      // this lane's products are those of page lr with columns lg, lg + 4, ...
+      const int left = wide ? G - g0 : TT * G, values = left < 16 ? (left + 3) >> 2 : 4;
+      uint32_t* to[4];
+      bool mine[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = lg + 4 * i, t = wide ? 0 : j * per16 >> 8, g = g0 + j - t * G;
+        mine[i] = t < TT && g < G && t0 + t < a.Tq;
+        to[i] = codes + t * stride;
+      }
+      i32x4 qb[KB];
+#pragma unroll
+      for (int i = 0; i < KB; ++i) qb[i] = *(const i32x4*)(&sh_q[lr][i * 64 + lg * 16]);
+      if (g0 > 0) {
+        pages();
+        first();
+      }
+      // a tile's bounds are loaded while the one before is multiplied, the table's entries two tiles earlier (each in registers of
+      // its own: to pass a tile on would wait for it)
+#pragma unroll 1
+      for (int tile0 = wave; tile0 * 16 < P; tile0 += NB * PS_NW)
+#pragma unroll
+        for (int r = 0; r < NB; ++r) {
+          const int tile = tile0 + r * PS_NW, p0 = tile * 16;
+          if (p0 >= P) break;
+          i32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < KB; ++i) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(qb[i], b[r].b[i], sum, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i >= values) break;
+            const uint32_t code = bound_code((float)sum[i] * b[r].scale);
+            if (mine[i] && b[r].in) {
+              if (G == 1) to[i][p0 + lr] = code;
+              else atomicMax(to[i] + p0 + lr, code);
+            }
+          }
+          b[r].load(a, bounds, scales, page[r], p0 + NB * PS_NW * 16 + lr, P);
+          page[r] = tile_page(a, table, tile + 2 * NB * PS_NW, lr);
+        }
+      __syncthreads();
+    }
+  } else {  // every page that is there, whatever its bound
+#pragma unroll 1
+    for (int i = threadIdx.x; i < P; i += PS_NW * 64) {
+      const uint32_t there = (uint32_t)table[i] < (uint32_t)c.pages;
+#pragma unroll 1
+      for (int t = 0; t < TT; ++t) codes[t * stride + i] = there;
+    }
     __syncthreads();
   }
 
