@@ -456,7 +456,8 @@ int64_t tabicl_paged_attn_q8_workspace_bytes(int64_t N, int64_t Hq, int64_t H, i
 /*
  * tabicl_paged_append into such a pool: codes rounded to the nearest (ties to even), saturating; NaN stays NaN in e4m3 and
  * becomes 0 in int8. A page that already holds rows of its sequence (lengths[n] lies inside it) takes the larger of its scale
- * and the new rows'; where it grows, the held codes are rounded again. Other pages take the new rows' scale. starts (or NULL):
+ * and the new rows'; where it grows, the held codes are rounded again. Other pages take the new rows' scale. No page may get
+ * rows of two sequences in a call. starts (or NULL):
  * k, v are packed [T, H, D] (k_sn, v_sn unused), row t of sequence n their row starts[n] + t; count is required then.
  */
 int tabicl_paged_append_q8(void* k_pages, void* v_pages, float* scales, int64_t pages, int64_t page_sp, int64_t page_rows,
@@ -514,7 +515,7 @@ int64_t tabicl_paged_sparse_attn_workspace_bytes(int64_t N, int64_t Hq, int64_t 
  *     row). The counts must add up to less than 2^31.
  *   tabicl_paged_append_slots: row j of k, v [total, H, D] (element strides, contiguous last dim) to slot slots[j]; negative
  *     slots, and those past the pool, are left out; no slot may stand twice. bf16 and fp32 pools.
- * No page may stand in the tables or on the stack twice. ws of reserve and release: tabicl_paged_books_workspace_bytes(N).
+ * No page may stand in the tables or on the stack twice, and the rows of a table that is written to must not overlap. ws of reserve and release: tabicl_paged_books_workspace_bytes(N).
  */
 int tabicl_paged_reserve(int32_t* table, int64_t table_sn, int64_t max_pages, const int32_t* lengths, const int32_t* count,
                          const int32_t* free_pages, int32_t* free_count, int32_t* granted, int64_t pages, int64_t page_rows,

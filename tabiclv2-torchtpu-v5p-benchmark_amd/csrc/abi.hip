@@ -1163,6 +1163,7 @@ int tabicl_paged_reserve(int32_t* table, int64_t table_sn, int64_t max_pages, co
                          int64_t N, void* ws, int64_t ws_bytes, void* stream) {
   PagedBooks a = {};
   if (int st = paged_books("paged_reserve", &a, table, table_sn, max_pages, lengths, count, pages, page_rows, N)) return st;
+  if (N > 1 && table_sn < max_pages) return fail(1, "paged_reserve: rows of the table must not overlap");
   if (N == 0) return 0;
   if (!count || !granted || !free_count || (pages > 0 && !free_pages))
     return fail(1, "paged_reserve: count, free, free_count and granted are required");
@@ -1178,6 +1179,7 @@ int tabicl_paged_release(int32_t* table, int64_t table_sn, int64_t max_pages, co
                          void* stream) {
   PagedBooks a = {};
   if (int st = paged_books("paged_release", &a, table, table_sn, max_pages, lengths, nullptr, pages, page_rows, N)) return st;
+  if (N > 1 && table_sn < max_pages) return fail(1, "paged_release: rows of the table must not overlap");
   if (N == 0) return 0;
   if (!free_count || (pages > 0 && !free_pages)) return fail(1, "paged_release: free and free_count are required");
   if (int st = paged_workspace("paged_release", tabicl_launch_paged_books_ws_bytes(N), ws, ws_bytes)) return st;

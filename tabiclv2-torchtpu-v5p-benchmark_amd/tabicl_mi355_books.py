@@ -29,12 +29,18 @@ def _free_args(free: Tensor, free_count: Tensor, dev: int) -> None:
         raise ValueError("free_count must be an int32 tensor of one entry on the table's device")
 
 
+def _own_rows(table: Tensor) -> None:
+    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError("the rows of a table that is written to must not overlap")
+
+
 def _reserve_launch(table: Tensor, lengths: Tensor, count: Tensor, free: Tensor, free_count: Tensor, page_rows: int,
                     granted: Tensor) -> None:
     t, N = _pool.table_args(table, lengths)
     dev = table.get_device()
     _pool.counts(count, N, "count")
     _free_args(free, free_count, dev)
+    _own_rows(table)
     if lengths.get_device() != dev or count.get_device() != dev:
         raise ValueError("table, lengths and count must be on one device")
     if _pool.elsewhere(dev, table):
@@ -79,6 +85,7 @@ def _release_launch(table: Tensor, lengths: Tensor, free: Tensor, free_count: Te
     t, N = _pool.table_args(table, lengths)
     dev = table.get_device()
     _free_args(free, free_count, dev)
+    _own_rows(table)
     if lengths.get_device() != dev:
         raise ValueError("table and lengths must be on one device")
     if _pool.elsewhere(dev, table):

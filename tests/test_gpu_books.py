@@ -330,3 +330,88 @@ def test_ops_equal_direct_calls_and_compile(dev):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
     for name in ("paged_reserve", "paged_slots", "paged_append_slots", "paged_release"):
         assert any(name in s for s in Seen.names), (name, Seen.names)
+
+
+def test_native_calls_equal_python_ones(dev, monkeypatch):
+    # the calls that the native module makes against the same ones without it
+    import tabicl_mi355_native as nat
+    import tabicl_mi355_paged as paged
+    nat.load()
+    assert nat.DIRECT is not None, "tabicl_mi355_direct.so is built beside the library"
+
+    def step(code):
+        table, n, free, fc, _ = _books(dev, 3, [50, 300, 0, 17], 40, 16, spare=90)
+        P, H, D, R = free.numel(), 2, 64, 16
+        g = torch.Generator(device=dev).manual_seed(5)
+        kp, vp = (torch.zeros(P, H, R, D, device=dev).to(code) for _ in range(2))
+        scales = torch.ones(P, H, 2, device=dev) if code in (E4, I8) else None
+        count = torch.tensor([20, 100, 33, 1], dtype=I32, device=dev)
+        out = [paged.paged_reserve(table, n, count, free, fc, R), *paged.paged_slots(table, n, count, 160, P, R)]
+        x = torch.randn(160, H, D, generator=g, device=dev).to(BF if scales is not None else code)
+        paged.paged_append_packed(kp, vp, table, n, count, x, -x, *out[1:], scales)
+        n = n + count
+        bnd, bs = torch.zeros(P, H, 2, D, dtype=torch.int8, device=dev), torch.zeros(P, H, device=dev)
+        paged.paged_bounds(kp, table, n, bnd, bs, None, None, scales)
+        q = torch.randn(4, 2 * H, 3, D, generator=g, device=dev).to(BF if code in (E4, I8) else code)
+        out.append(paged.paged_select(q, bnd, bs, table, n, R, 5))
+        out.append(paged.paged_sparse_attention(q, kp, vp, table, n, out[-1], scales=scales))
+        if scales is not None:
+            more = torch.randn(4, H, 2, D, generator=g, device=dev)
+            paged.paged_append(kp, vp, table, n - 1, more, more * 9, scales=scales)
+            out.append(paged.paged_attention(q, kp, vp, table, n, scales=scales))
+            live = torch.arange(333, device=dev).view(1, 1, -1, 1) < n.view(-1, 1, 1, 1)  # nothing is written past a length
+            out.extend(torch.where(live, x, 0.0) for x in paged.paged_gather(kp, vp, table, n, 333, scales=scales, dtype=F32))
+        paged.paged_release(table, n - 30, free, fc, R)
+        torch.cuda.synchronize()
+        return [t for t in (*out, table, free, fc, kp, vp, scales, bnd, bs) if t is not None]
+
+    for code in (BF, F32, E4, I8):
+        with_it = step(code)
+        with monkeypatch.context() as m:
+            m.setattr(nat, "DIRECT", None)
+            without = step(code)
+        for a, b in zip(with_it, without):
+            assert a.dtype == b.dtype and torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)), code
+
+
+def test_two_graphs(dev):
+    # two captured services replayed in turn and together: nothing is shared between them
+    import tabicl_mi355_paged as paged
+    runs = []
+    for seed in (1, 2):
+        table, n, free, fc, _ = _books(dev, seed, [40, 200, 0], 30, 16, spare=60)
+        P = free.numel()
+        g = torch.Generator(device=dev).manual_seed(seed)
+        kp, vp = (torch.randn(P, 8, 16, 64, generator=g, device=dev).to(E4) for _ in range(2))
+        scales = torch.ones(P, 8, 2, device=dev)
+        q = torch.randn(3, 8, 1, 64, generator=g, device=dev).to(BF)
+        count = torch.tensor([3, 1, 9], dtype=I32, device=dev)
+        bnd, bs = torch.zeros(P, 8, 2, 64, dtype=torch.int8, device=dev), torch.zeros(P, 8, device=dev)
+
+        def step(table=table, n=n, free=free, fc=fc, kp=kp, vp=vp, scales=scales, q=q, count=count, bnd=bnd, bs=bs):
+            granted = paged.paged_reserve(table, n, count, free, fc, 16)
+            paged.paged_bounds(kp, table, n, bnd, bs, None, None, scales)
+            index = paged.paged_select(q, bnd, bs, table, n, 16, 4)
+            outs = granted, index, paged.paged_sparse_attention(q, kp, vp, table, n, index, scales=scales), \
+                paged.paged_attention(q, kp, vp, table, n, scales=scales)
+            paged.paged_release(table, n, free, fc, 16)
+            return outs
+
+        want = [t.clone() for t in step()]
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = step()
+        runs.append((graph, got, want, stream))
+    torch.cuda.synchronize()
+    for together in (False, True, True):
+        for graph, got, _, stream in runs:
+            for t in got:
+                t.view(torch.uint8).fill_(7)
+        torch.cuda.synchronize()
+        for graph, _, _, stream in runs:
+            with torch.cuda.stream(stream if together else torch.cuda.current_stream()):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, got, want, _ in runs:
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)

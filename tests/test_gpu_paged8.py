@@ -520,3 +520,34 @@ def test_cache_layers(dev):
     assert a.dtype == b.dtype and float((a - b).abs().max()) <= 2.0 ** -6 * float(b.abs().max())
     a, b = (c.attention_layer(0, t.to(BF), w.in_w, w.in_b, w.out_w, w.out_b) for c in (c8, c16))
     assert a.dtype == BF and float((a - b).abs().max()) <= 2.0 ** -6 * float(b.abs().max())
+
+
+@CODES
+@pytest.mark.parametrize("N,most,H,T,D,dtype", [
+    (600, 20, 1, 1, 64, BF), (600, 250, 1, 3, 32, F32), (40, 200, 8, 40, 64, BF), (40, 130, 8, 40, 128, BF),  # two waves an item
+    (3, 500, 2, 5, 64, BF), (70, 700, 8, 2, 64, F32), (40, 600, 8, 33, 32, BF), (20, 1000, 8, 70, 128, BF),    # four
+    (2, 1000, 8, 1, 128, F32), (1, 777, 2, 200, 64, BF),                                                       # eight
+    (3, 1500, 2, 70, 128, BF), (3, 1500, 2, 70, 128, F32), (2, 2100, 2, 33, 64, F32), (2, 1300, 2, 100, 32, F32),  # split, wide tiles
+])
+def test_items_and_tiles(dev, code, N, most, H, T, D, dtype):
+    # sequences in number and length as the variants are chosen by: waves of an item, query rows of a tile
+    g = torch.Generator().manual_seed(N + most)
+    lengths = torch.randint(0, most + 1, (N,), generator=g).tolist()
+    lengths[0] = most
+    _attend(*_case(dev, most, lengths, H=H, T=T, D=D, R=16, dtype=dtype, code=code, sharp=2.0)[:-1], what="items")
+
+
+@CODES
+@pytest.mark.parametrize("R,D", [(128, 128), (256, 128), (512, 64), (512, 128), (1024, 128)])
+def test_append_to_large_pages(dev, code, R, D):
+    # as many values of a page as 256 or 512 threads keep, and more; non-finite ones among them, rows held before
+    g = torch.Generator(device=dev).manual_seed(R + D)
+    H, T = 2, 2 * R + 3
+    kp, vp = (_pool(dev, g, 9, H, R, D, code) for _ in range(2))
+    scales = torch.exp2(torch.randint(-10, -3, (9, H, 2), generator=g, device=dev).float())
+    table = torch.tensor([[7, 0, 3, 5], [1, 8, 2, 6]], dtype=torch.int32, device=dev)
+    n = torch.tensor([R - 5, 0], dtype=torch.int32, device=dev)
+    k, v = (torch.randn(2, H, T, D, generator=g, device=dev) * 3.0 for _ in range(2))
+    k[0, 0, 2], k[1, 1, R + 1, 3], v[0, 1, R // 2, 5], v[1, 0, T - 1] = float("inf"), float("nan"), -float("inf"), float("nan")
+    for dtype in (F32, BF):
+        _append(kp, vp, scales, table, n, k.to(dtype), v.to(dtype), what=f"large pages {dtype}")

@@ -416,3 +416,39 @@ def test_cache_selects(dev, dtype):
     o, tol = ref.sparse_attention(q, _values(c.keys[1], scales, 0), _values(c.values[1], scales, 1), c.table, c.lengths[1], index,
                                   D ** -0.5)
     paged_ref.near(got, o, tol, "captured, grown")
+
+
+@FORMATS
+@pytest.mark.parametrize("N,H,T,G,D,R,K", [(90, 8, 1, 1, 64, 16, 9), (5, 2, 60, 3, 64, 32, 20), (40, 8, 2, 1, 128, 64, 9),
+                                           (3, 1, 400, 1, 32, 16, 1), (2, 2, 1, 1, 128, 64, 5)])
+def test_many_items(dev, fmt, N, H, T, G, D, R, K):
+    # items in number and length as the waves of a workgroup are chosen by; lists longer and shorter than a sequence's pages
+    g = torch.Generator().manual_seed(N)
+    lengths = torch.randint(0, 700, (N,), generator=g).tolist()
+    q, kp, vp, scales, table, n, g = _case(dev, N + T, lengths, H=H, G=G, D=D, R=R, T=T, fmt=fmt)
+    bnd, bs = _fresh(kp, g)
+    index = _check_select(q, bnd, bs, table, n, R, K, "many items")
+    _check_sparse(q, kp, vp, scales, table, n, index, what="many items")
+
+
+@pytest.mark.parametrize("pages,K", [(33000, 33000), (40, 5000), (2000, 2000)])
+def test_select_every_page(dev, pages, K):
+    # no more pages than are asked for: all of them, whatever their bounds; some are not there
+    g = torch.Generator(device=dev).manual_seed(pages)
+    P, R = pages + 7, 16
+    table = torch.randperm(P, generator=g, device=dev)[:pages].to(torch.int32).view(1, -1).repeat(2, 1)
+    table[:, 3:20] = -1
+    table[1, pages - 1] = P
+    n = torch.tensor([pages * R, pages * R - 40], dtype=torch.int32, device=dev)
+    bnd = torch.randint(-20, 21, (P, 1, 2, 32), generator=g, device=dev, dtype=torch.int8)
+    bs = torch.ones(P, 1, device=dev)
+    bs[::3] = math.nan
+    q = torch.randn(2, 1, 3, 32, generator=g, device=dev).to(BF)
+    import tabicl_mi355_paged as paged
+    got = paged.paged_select(q, bnd, bs, table, n, R, K).cpu()
+    for i, count in enumerate((pages, pages - 2)):
+        ids = table[i, :count].cpu()
+        there = torch.nonzero((ids >= 0) & (ids < P)).view(-1).int()
+        want = torch.full((K,), -1, dtype=torch.int32)
+        want[:len(there)] = there
+        assert (got[i] == want).all()

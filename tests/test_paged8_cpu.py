@@ -163,6 +163,8 @@ def test_books_refuse():
             (lambda: paged.paged_reserve(t, n, c, f, fc.long(), 16), "free_count"),
             (lambda: paged.paged_release(t, n, f, f, 16), "free_count"),
             (lambda: paged.paged_release(t.t(), n, f, fc, 16), "table"),
+            (lambda: paged.paged_reserve(t[:1].expand(2, 3), n, c, f, fc, 16), "overlap"),
+            (lambda: paged.paged_release(torch.zeros(5, dtype=I32).as_strided((2, 3), (2, 1)), n, f, fc, 16), "overlap"),
             (lambda: paged.paged_slots(t, n, c, -1, 6, 16), "negative"),
             (lambda: paged.paged_slots(t, n, c.float(), 2, 6, 16), "count"),
             (lambda: paged.paged_append_packed(torch.zeros(6, 2, 16, 64), torch.zeros(6, 2, 16, 64), t, n, c, torch.zeros(2, 2, 32),
