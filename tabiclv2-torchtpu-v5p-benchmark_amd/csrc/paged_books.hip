@@ -122,8 +122,8 @@ __global__ __launch_bounds__(256) void paged_books_kernel(PagedBooks a, const in
 
 // One workgroup for up to 256 sequences and BOOKS_ONE entries: counts, running sums and the entries in one launch. The entries to
 // look at are cut into runs of 64 of one sequence; a wave takes 16 runs at a time, all of them in its registers at once. (us of
-// a reserve on the GPU and with the host, two launches / this: 256 requests of one row 6.3 and 10.3 / 7.9 and 7.9, 64 of up to
-// 10,000 rows 7.6 and 10.3 / 9.4 and 9.4.)
+// a reserve on the GPU, two launches / this: 256 requests of one row 6.3 / 6.2, 64 of up to 10,000 rows 7.6 / 8.9; of reserve,
+// slots, a copy and release as a program calls them, host included: 32.5 / 25.4 and 32.5 / 25.2.)
 constexpr int BOOKS_SEQS = 256, BOOKS_ONE = 65536, BOOKS_RUNS = BOOKS_ONE / 64 + BOOKS_SEQS, PB_NW = 16, PB_EACH = 16;
 
 template <bool RELEASE>
@@ -154,16 +154,16 @@ __global__ __launch_bounds__(PB_NW * 64) void paged_books_one_kernel(PagedBooks 
   for (int p = first; p < last; p += 64) run[at++] = make_int2(tid, p << 6 | ((last - p < 64 ? last - p : 64) - 1));
   __syncthreads();
   int32_t* entry[PB_EACH];
-  int id[PB_EACH];
+  int id[PB_EACH], rank[PB_EACH];
   bool moves[PB_EACH];
-  auto load = [&](int k0) {
+  auto load = [&](int k0) {  // every load is issued, so that none waits for the one before
 #pragma unroll
     for (int u = 0; u < PB_EACH; ++u) {
       const int k = k0 + wave * PB_EACH + u;
       const int2 r = k < runs ? run[k] : make_int2(0, 0);
       const bool in = k < runs && lane <= (r.y & 63);
-      entry[u] = a.table + r.x * a.table_sn + (r.y >> 6) + lane;
-      id[u] = in ? *entry[u] : 0;
+      entry[u] = in ? a.table + r.x * a.table_sn + (r.y >> 6) + lane : a.table;
+      id[u] = *entry[u];
       moves[u] = in;
     }
 #pragma unroll
@@ -171,6 +171,7 @@ __global__ __launch_bounds__(PB_NW * 64) void paged_books_one_kernel(PagedBooks 
   };
 #pragma unroll 1
   for (int k0 = 0; k0 < runs; k0 += PB_NW * PB_EACH) {
+    if (k0 + wave * PB_EACH >= runs) break;  // none left for this wave
     load(k0);
     int mine = 0;
 #pragma unroll
@@ -189,17 +190,24 @@ __global__ __launch_bounds__(PB_NW * 64) void paged_books_one_kernel(PagedBooks 
   __syncthreads();
 #pragma unroll 1
   for (int k0 = 0; k0 < runs; k0 += PB_NW * PB_EACH) {
+    if (k0 + wave * PB_EACH >= runs) break;
     if (runs > PB_NW * PB_EACH) load(k0);  // else they are here
 #pragma unroll
     for (int u = 0; u < PB_EACH; ++u) {
-      const int k = k0 + wave * PB_EACH + u, rank = (k < runs ? need[k] : 0) + below(__ballot(moves[u]));
+      const int k = k0 + wave * PB_EACH + u;
+      rank[u] = (k < runs ? need[k] : 0) + below(__ballot(moves[u]));
       if constexpr (RELEASE) {
-        const int64_t to = (int64_t)have + all - 1 - rank;
+        const int64_t to = (int64_t)have + all - 1 - rank[u];
         if (moves[u] && to < a.pages) a.free_pages[to] = id[u];
         if (moves[u]) *entry[u] = -1;
-      } else if (moves[u] && rank < have) {
-        id[u] = a.free_pages[have - 1 - rank];
       }
+    }
+    if (!RELEASE && have > 0) {
+      int page[PB_EACH];
+#pragma unroll
+      for (int u = 0; u < PB_EACH; ++u) page[u] = a.free_pages[moves[u] && rank[u] < have ? have - 1 - rank[u] : 0];
+#pragma unroll
+      for (int u = 0; u < PB_EACH; ++u) id[u] = moves[u] && rank[u] < have ? page[u] : id[u];
     }
     if constexpr (!RELEASE) {
 #pragma unroll

@@ -245,10 +245,13 @@ __device__ __forceinline__ void store16(float* p, const float* x) { store_row<fl
 template <typename T, typename C>
 __global__ __launch_bounds__(256) void paged_gather8_kernel(PagedGather a, const float* scales) {
   const PagedPool& c = a.pool;
-  const int n = blockIdx.y, chunks = c.D / 16, len = pool_length(c, n), rows = len < a.T ? len : a.T;
-  const int64_t total = (int64_t)rows * c.H * chunks;
+  const int n = blockIdx.y, cpr = __builtin_ctz(c.D / 16), len = pool_length(c, n), rows = len < a.T ? len : a.T;
+  const int64_t total = (int64_t)rows * c.H << cpr;
+  const bool narrow = total >> cpr <= 0x7fffffff;  // a 64-bit division takes as long as a load
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int ch = (int)(i % chunks), row = (int)(i / chunks % rows), h = (int)(i / chunks / rows);
+    const int64_t j = i >> cpr;
+    const int h = narrow ? (int)((uint32_t)j / (uint32_t)rows) : (int)(j / rows), row = (int)(j - (int64_t)h * rows);
+    const int ch = (int)i & ((1 << cpr) - 1);
     const int page = c.table[n * c.table_sn + (row >> c.shift)];
     const int64_t to = (((int64_t)n * c.H + h) * a.T + row) * c.D + ch * 16;
     uint4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};

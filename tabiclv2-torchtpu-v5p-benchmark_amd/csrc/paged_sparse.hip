@@ -257,15 +257,15 @@ void launch_bounds(const PagedBounds& a, int format, dim3 grid, hipStream_t stre
 // ---------------------------------------------------------------------------------------------
 // selection
 // ---------------------------------------------------------------------------------------------
-// A workgroup of 16 waves takes up to TT query rows of one sequence and K/V head: the bounds of 16 pages for 16 (query row,
+// A workgroup of 16 waves (or 4) takes up to TT query rows of one sequence and K/V head: the bounds of 16 pages for 16 (query row,
 // head of the group) pairs at a time on the 8-bit matrix unit, kept as ordered codes [TT][pages] in LDS (0: no such page); then
-// the K-th largest code of each query row by four 8-bit digits of a histogram, 16 / TT waves a row; then the pages above it,
+// the K-th largest code of each query row by four 8-bit digits of a histogram, 16 / TT (4 / TT) waves a row; then the pages above it,
 // and the first ones equal to it, in order. Bound by its chain of loads and barriers (64 query rows of 704 pages: a few MB), so
 // the first tiles' table entries and bounds are on their way before the queries are looked at, the histograms of all
 // digits are cleared at once, every wave of a row finds the digit for itself (one barrier a digit), and there is little code:
 // most of it runs once, as fast as instructions come in (three tiles at a time instead of two: 10.8 us for 10.2). One row of 8
 // sequences of 704 pages and 8 heads takes 10.2 us, of which the bounds take 4 and the digits 1.7; 16 pages alone 5.5.
-constexpr int PS_NW = 16, PS_LDS = 32768;  // codes kept in LDS
+constexpr int PS_LDS = 32768;  // codes kept in LDS
 
 __device__ __forceinline__ uint32_t bound_code(float x) {  // larger bound, larger code; none is 0
   const uint32_t u = __float_as_uint(x + 0.f);
@@ -276,7 +276,7 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// A tile of 16 pages (a wave takes every 16th): their bounds as operands, their scales and whether they are there. The table is
+// A tile of 16 pages (the waves take turns): their bounds as operands, their scales and whether they are there. The table is
 // read up to its width, not the sequence's, so that its entries need not wait for the length.
 __device__ __forceinline__ int tile_page(const PagedSelect& a, const int32_t* table, int tile, int lr) {
   const int64_t p = (int64_t)tile * 16 + lr;
@@ -300,13 +300,13 @@ struct BoundTile {
 };
 
 // Grid (tiles of TT = 2^tshift query rows, H, N). per16: 256 / G, rounded up (x / G = x * per16 >> 8 for x < 16; G <= 16).
-template <typename T, int D, bool GLOBAL>
-__global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a, int tshift, int per16, uint32_t* store) {
+template <typename T, int D, bool GLOBAL, int NW>
+__global__ __launch_bounds__(NW * 64) void paged_select_kernel(PagedSelect a, int tshift, int per16, uint32_t* store) {
   extern __shared__ uint32_t lds[];  // [4][TT][256] histograms, [TT][max_pages] codes
-  constexpr int KB = 2 * D / 64, NV = (D + 63) / 64;
+  constexpr int KB = 2 * D / 64, NV = (D + 63) / 64, COLS = 16 / NW, LOGW = NW == 16 ? 4 : 2;
   __shared__ __attribute__((aligned(16))) int8_t sh_q[16][2 * D];
   __shared__ uint32_t sh_most[16];
-  __shared__ int2 part[PS_NW];
+  __shared__ int2 part[NW];
   const PagedPool& c = a.pool;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
   const int n = blockIdx.z, h = blockIdx.y, TT = 1 << tshift, t0 = blockIdx.x << tshift;
@@ -323,65 +323,82 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
   int page[NB];  // of the tiles NB rounds later
   auto pages = [&]() {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) page[i] = tile_page(a, table, wave + i * PS_NW, lr);
+    for (int i = 0; i < NB; ++i) page[i] = tile_page(a, table, wave + i * NW, lr);
   };
   auto first = [&]() {
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      b[i].load(a, bounds, scales, page[i], (wave + i * PS_NW) * 16 + lr, P);
-      page[i] = tile_page(a, table, wave + (NB + i) * PS_NW, lr);
+      b[i].load(a, bounds, scales, page[i], (wave + i * NW) * 16 + lr, P);
+      page[i] = tile_page(a, table, wave + (NB + i) * NW, lr);
     }
   };
   pages();
   if (a.K < P) {
     first();
-    // column `wave` of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
+    // columns wave, wave + NW, ... of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
     const char* q = (const char*)a.q + (n * a.q_sn + (int64_t)h * G * a.q_sh) * sizeof(T);
     const bool wide = G > 16;
-    const int qrow = wide ? 0 : wave * per16 >> 8, qhead = wave - qrow * G, qplace = (wave & 3) * 4 + (wave >> 2);
-    float x[NV];
-    auto column = [&](int g0) {
-      const int g = g0 + qhead;
-      const bool in = qrow < TT && t0 + qrow < a.Tq && g < G;
+    float x[COLS][NV];
+    auto columns = [&](int g0) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int d = lane + 64 * i;
-        x[i] = in && d < D ? (float)*(const T*)(q + (g * a.q_sh + (t0 + qrow) * a.q_st + d) * (int64_t)sizeof(T)) : 0.f;
+      for (int s = 0; s < COLS; ++s) {
+        const int col = wave + s * NW, row = wide ? 0 : col * per16 >> 8, g = g0 + col - row * G;
+        const bool in = row < TT && t0 + row < a.Tq && g < G;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int d = lane + 64 * i;
+          x[s][i] = in && d < D ? (float)*(const T*)(q + (g * a.q_sh + (t0 + row) * a.q_st + d) * (int64_t)sizeof(T)) : 0.f;
+        }
       }
     };
-    uint32_t most = 0;
+    uint32_t most[COLS] = {};
 #pragma unroll 1
     for (int g0 = 0; g0 < G; g0 += 16) {
-      column(g0);
+      columns(g0);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) most = umax(most, finite_bits(x[i]));
+      for (int s = 0; s < COLS; ++s)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) most[s] = umax(most[s], finite_bits(x[s][i]));
     }
 #pragma unroll 1
-    for (int i = threadIdx.x; i < 1024 << tshift; i += PS_NW * 64) hist[i] = 0;
+    for (int i = threadIdx.x; i < 1024 << tshift; i += NW * 64) hist[i] = 0;
 #pragma unroll 1
     for (int t = 0; t < TT; ++t)
 #pragma unroll 1
-      for (int i = threadIdx.x; i < P; i += PS_NW * 64) codes[t * stride + i] = 0;
+      for (int i = threadIdx.x; i < P; i += NW * 64) codes[t * stride + i] = 0;
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) most = across(most, s, umax);
-    if (lane == 0) sh_most[wave] = most;
+    for (int s = 0; s < COLS; ++s) {
+#pragma unroll
+      for (int y = 1; y < 64; y <<= 1) most[s] = across(most[s], y, umax);
+      if (lane == 0) sh_most[wave + s * NW] = most[s];
+    }
     __syncthreads();
-    // the step of this column's query row: the largest of its group's
-    most = 0;
+    // the step of a column's query row: the largest of its group's
+    float inv[COLS];
+#pragma unroll
+    for (int s = 0; s < COLS; ++s) {
+      uint32_t m = 0;
+      const int w0 = wide ? 0 : ((wave + s * NW) * per16 >> 8) * G, w1 = wide || w0 + G > 16 ? 16 : w0 + G;
 #pragma unroll 1
-    for (int w = wide ? 0 : qrow * G, end = wide || w + G > 16 ? 16 : w + G; w < end; ++w) most = umax(most, sh_most[w]);
-    const float inv = pow2(-step_exponent(most));
+      for (int w = w0; w < w1; ++w) m = umax(m, sh_most[w]);
+      inv[s] = pow2(-step_exponent(m));
+    }
 
 #pragma unroll 1
     for (int g0 = 0; g0 < G; g0 += 16) {
-      if (wide) column(g0);
+      if (wide) columns(g0);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int d = lane + 64 * i;
-        const int u = x[i] != x[i] ? 0 : (int)fminf(fmaxf(__builtin_rintf(x[i] * inv), -127.f), 127.f);
-        if (d < D) {
-          sh_q[qplace][d] = (int8_t)(u > 0 ? u : 0);
-          sh_q[qplace][D + d] = (int8_t)(u < 0 ? u : 0);
+      for (int s = 0; s < COLS; ++s) {
+        const int col = wave + s * NW;
+        int8_t* place = sh_q[(col & 3) * 4 + (col >> 2)];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int d = lane + 64 * i;
+          const int u = x[s][i] != x[s][i] ? 0 : (int)fminf(fmaxf(__builtin_rintf(x[s][i] * inv[s]), -127.f), 127.f);
+          if (d < D) {
+            place[d] = (int8_t)(u > 0 ? u : 0);
+            place[D + d] = (int8_t)(u < 0 ? u : 0);
+          }
         }
       }
       __syncthreads();
@@ -405,10 +422,10 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
       // a tile's bounds are loaded while the one before is multiplied, the table's entries two tiles earlier (each in registers of
       // its own: to pass a tile on would wait for it)
 #pragma unroll 1
-      for (int tile0 = wave; tile0 * 16 < P; tile0 += NB * PS_NW)
+      for (int tile0 = wave; tile0 * 16 < P; tile0 += NB * NW)
 #pragma unroll
         for (int r = 0; r < NB; ++r) {
-          const int tile = tile0 + r * PS_NW, p0 = tile * 16;
+          const int tile = tile0 + r * NW, p0 = tile * 16;
           if (p0 >= P) break;
           i32x4 sum = {0, 0, 0, 0};
 #pragma unroll
@@ -422,14 +439,14 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
               else atomicMax(to[i] + p0 + lr, code);
             }
           }
-          b[r].load(a, bounds, scales, page[r], p0 + NB * PS_NW * 16 + lr, P);
-          page[r] = tile_page(a, table, tile + 2 * NB * PS_NW, lr);
+          b[r].load(a, bounds, scales, page[r], p0 + NB * NW * 16 + lr, P);
+          page[r] = tile_page(a, table, tile + 2 * NB * NW, lr);
         }
       __syncthreads();
     }
   } else {  // every page that is there, whatever its bound
 #pragma unroll 1
-    for (int i = threadIdx.x; i < P; i += PS_NW * 64) {
+    for (int i = threadIdx.x; i < P; i += NW * 64) {
       const uint32_t there = (uint32_t)table[i] < (uint32_t)c.pages;
 #pragma unroll 1
       for (int t = 0; t < TT; ++t) codes[t * stride + i] = there;
@@ -438,7 +455,7 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
   }
 
   // the rows in groups of waves
-  const int wshift = 4 - tshift, wpr = 1 << wshift, t = wave >> wshift, sub = wave & (wpr - 1), member = sub * 64 + lane, members = wpr * 64;
+  const int wshift = LOGW - tshift, wpr = 1 << wshift, t = wave >> wshift, sub = wave & (wpr - 1), member = sub * 64 + lane, members = wpr * 64;
   const uint32_t* mycodes = codes + t * stride;
   int want = a.K < P ? a.K : 0;  // of the pages of the threshold's code, in the end; every page there is: 0
   uint32_t threshold = 0;
@@ -506,33 +523,41 @@ __global__ __launch_bounds__(PS_NW * 64) void paged_select_kernel(PagedSelect a,
   for (int i = all + member; i < a.K; i += members) out[i] = -1;
 }
 
-// The query rows of a workgroup as a shift: a power of two with up to 16 (query row, head) pairs whose codes and histograms fit
-// in LDS.
-int select_shift(int64_t G, int64_t Tq, int64_t max_pages) {
+// The query rows of a workgroup as a shift: a power of two with up to 16 (query row, head) pairs and a wave a row, whose codes and
+// histograms fit in LDS.
+int select_shift(int64_t G, int64_t Tq, int64_t max_pages, int most) {
   int s = 0;
-  while (s < 4 && (1 << s) < Tq && (2 << s) * G <= 16 && (2 << s) * (max_pages + 1024) <= PS_LDS) ++s;
+  while (s < most && (1 << s) < Tq && (2 << s) * G <= 16 && (2 << s) * (max_pages + 1024) <= PS_LDS) ++s;
   return s;
 }
 
 template <typename T, int D>
 void launch_select(const PagedSelect& a, void* ws, hipStream_t stream) {
   const int64_t G = a.Hq / a.pool.H, M = a.pool.max_pages;
-  const int shift = select_shift(G, a.Tq, M), per16 = (int)((256 + G - 1) / G);
-  const dim3 grid((unsigned)((a.Tq + (1 << shift) - 1) >> shift), (unsigned)a.pool.H, (unsigned)a.N), nt(PS_NW * 64);
+  // Four waves for tables of up to 256 pages, so that many workgroups share a CU (us with 16 / 4 waves: 8 heads of 8 sequences of 64
+  // pages 7.2 / 7.2, of 256 7.9 / 8.6, of 512 9.3 / 11.2; of 64 sequences of 64 pages 12.9 / 8.1, of 256 14.4 / 10.2; 23 query rows and 4
+  // heads a group over 51 of 11 pages 70 / 22; 32 query rows over 32 of 256 24 / 28).
+  const bool few = M <= 256;
+  const int shift = select_shift(G, a.Tq, M, few ? 2 : 4), per16 = (int)((256 + G - 1) / G);
+  const dim3 grid((unsigned)((a.Tq + (1 << shift) - 1) >> shift), (unsigned)a.pool.H, (unsigned)a.N), nt(few ? 256 : 1024);
   const size_t bins = (size_t)4096 << shift, lds = bins + (M > PS_LDS ? 0 : ((size_t)M << shift) * 4);
   if (M > PS_LDS) {
-    hipLaunchKernelGGL((paged_select_kernel<T, D, true>), grid, nt, lds, stream, a, shift, per16, (uint32_t*)ws);
+    hipLaunchKernelGGL((paged_select_kernel<T, D, true, 16>), grid, nt, lds, stream, a, shift, per16, (uint32_t*)ws);
+    return;
+  }
+  if (few) {
+    hipLaunchKernelGGL((paged_select_kernel<T, D, false, 4>), grid, nt, lds, stream, a, shift, per16, (uint32_t*)nullptr);
     return;
   }
   static bool set[64];  // per device: more LDS than a kernel may have unasked
   int dev = 0;
   (void)hipGetDevice(&dev);
   if (lds > 49152 && (dev < 0 || dev >= 64 || !set[dev])) {
-    (void)hipFuncSetAttribute((const void*)paged_select_kernel<T, D, false>, hipFuncAttributeMaxDynamicSharedMemorySize,
+    (void)hipFuncSetAttribute((const void*)paged_select_kernel<T, D, false, 16>, hipFuncAttributeMaxDynamicSharedMemorySize,
                               PS_LDS * 4 + 16384);
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
-  hipLaunchKernelGGL((paged_select_kernel<T, D, false>), grid, nt, lds, stream, a, shift, per16, (uint32_t*)nullptr);
+  hipLaunchKernelGGL((paged_select_kernel<T, D, false, 16>), grid, nt, lds, stream, a, shift, per16, (uint32_t*)nullptr);
 }
 
 // ---------------------------------------------------------------------------------------------
