@@ -263,8 +263,8 @@ void launch_bounds(const PagedBounds& a, int format, dim3 grid, hipStream_t stre
 // and the first ones equal to it, in order. Bound by its chain of loads and barriers (64 query rows of 704 pages: a few MB), so
 // the first tiles' table entries and bounds are on their way before the queries are looked at, the histograms of all
 // digits are cleared at once, every wave of a row finds the digit for itself (one barrier a digit), and there is little code:
-// most of it runs once, as fast as instructions come in (three tiles at a time instead of two: 10.8 us for 10.2). One row of 8
-// sequences of 704 pages and 8 heads takes 10.2 us, of which the bounds take 4 and the digits 1.7; 16 pages alone 5.5.
+// most of it runs once, as fast as instructions come in (three tiles at a time instead of two: 10.0 us for 9.5). One row of 8
+// sequences of 704 pages and 8 heads takes 9.5 us, of which the digits take 1.7; 64 pages 7.2, 16 of 16, unscored, 3.3.
 constexpr int PS_LDS = 32768;  // codes kept in LDS
 
 __device__ __forceinline__ uint32_t bound_code(float x) {  // larger bound, larger code; none is 0
@@ -277,25 +277,28 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
 }
 
 // A tile of 16 pages (the waves take turns): their bounds as operands, their scales and whether they are there. The table is
-// read up to its width, not the sequence's, so that its entries need not wait for the length.
+// read up to its width, not the sequence's, so that its entries need not wait for the length. Lanes without a page load another
+// one's: a load under a condition would have every wait wait for all loads.
 __device__ __forceinline__ int tile_page(const PagedSelect& a, const int32_t* table, int tile, int lr) {
-  const int64_t p = (int64_t)tile * 16 + lr;
-  return p < a.pool.max_pages ? table[p] : -1;
+  const uint32_t p = tile * 16 + lr, last = a.pool.max_pages - 1, at = p < last ? p : last;
+  const int id = table[at];
+  return p <= last ? id : -1;
 }
+// The bounds come in with four lanes side by side on 64 bytes of a page (16 lanes on 16 pages, as the operands lie, are 16 lines
+// of the cache for every 16 lanes: 8 heads of a sequence of 3,125 pages 22.8 us for 17.2) and are passed on through LDS.
 template <int KB>
 struct BoundTile {
-  i32x4 b[KB];
-  float scale;
+  i32x4 b[KB];  // 16 bytes from 16 (lane % 4) on of each 64, of page lane / 4
+  float scale;  // of page lane % 16
   bool in;
-  // bounds, scales: page 0's, from this head and lane's on
+  // bounds, scales: page 0's, from this head and lane's on; page: page lane % 16
   __device__ __forceinline__ void load(const PagedSelect& a, const int8_t* bounds, const float* scales, int page, int p, int P) {
     in = (uint32_t)page < (uint32_t)a.pool.pages && p < P;
-    if (in) {
-      const int64_t at = (int64_t)page * a.pool.H;
-      scale = scales[at];
+    const uint32_t at = in ? page : 0, mine = __shfl((int)at, (threadIdx.x & 63) >> 2, 64);
+    scale = *(const float*)((const char*)scales + (uint64_t)at * (uint32_t)(a.pool.H * 4));
+    const int8_t* from = bounds + (uint64_t)mine * (uint32_t)(a.pool.H * (KB * 64));
 #pragma unroll
-      for (int i = 0; i < KB; ++i) b[i] = *(const i32x4*)(bounds + at * (KB * 64) + i * 64);
-    }
+    for (int i = 0; i < KB; ++i) b[i] = *(const i32x4*)(from + i * 64);
   }
 };
 
@@ -304,20 +307,23 @@ template <typename T, int D, bool GLOBAL, int NW>
 __global__ __launch_bounds__(NW * 64) void paged_select_kernel(PagedSelect a, int tshift, int per16, uint32_t* store) {
   extern __shared__ uint32_t lds[];  // [4][TT][256] histograms, [TT][max_pages] codes
   constexpr int KB = 2 * D / 64, NV = (D + 63) / 64, COLS = 16 / NW, LOGW = NW == 16 ? 4 : 2;
-  __shared__ __attribute__((aligned(16))) int8_t sh_q[16][2 * D];
+  __shared__ __attribute__((aligned(16))) int8_t sh_q[16][2 * D], sh_b[NW][1024];
   __shared__ uint32_t sh_most[16];
   __shared__ int2 part[NW];
   const PagedPool& c = a.pool;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
   const int n = blockIdx.z, h = blockIdx.y, TT = 1 << tshift, t0 = blockIdx.x << tshift;
   const int G = a.Hq / c.H, R = 1 << c.shift, len = __builtin_amdgcn_readfirstlane(pool_length(c, n));
-  const int P = (len + R - 1) >> c.shift, stride = c.max_pages;
+  const int P = c.pages > 0 ? (len + R - 1) >> c.shift : 0, stride = c.max_pages;
   const int32_t* table = c.table + n * c.table_sn;
   int* hist = (int*)lds;
   const int64_t nh = (int64_t)n * c.H + h;
   uint32_t* codes = GLOBAL ? store + (nh * a.Tq + t0) * stride : lds + (1024 << tshift);
   constexpr int NB = 2;
-  const int8_t* bounds = a.bounds + h * (2 * D) + lg * 16;
+  const int8_t* bounds = a.bounds + h * (2 * D) + (lane & 3) * 16;
+  // 64 bytes of a tile's pages in LDS, their sixteenths in an order by which neither side meets itself in a bank
+  int8_t* const put = sh_b[wave] + (lane >> 2) * 64 + ((lane ^ lane >> 3) & 3) * 16;
+  const int8_t* const get = sh_b[wave] + lr * 64 + ((lg ^ lr >> 1) & 3) * 16;
   const float* scales = a.bound_scales + h;
   BoundTile<KB> b[NB];
   int page[NB];  // of the tiles NB rounds later
@@ -332,7 +338,7 @@ __global__ __launch_bounds__(NW * 64) void paged_select_kernel(PagedSelect a, in
       page[i] = tile_page(a, table, wave + (NB + i) * NW, lr);
     }
   };
-  pages();
+  if (c.max_pages > 0) pages();
   if (a.K < P) {
     first();
     // columns wave, wave + NW, ... of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
@@ -404,13 +410,13 @@ __global__ __launch_bounds__(NW * 64) void paged_select_kernel(PagedSelect a, in
       __syncthreads();
       // this lane's products are those of page lr with columns lg, lg + 4, ...
       const int left = wide ? G - g0 : TT * G, values = left < 16 ? (left + 3) >> 2 : 4;
-      uint32_t* to[4];
+      int to[4];
       bool mine[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = lg + 4 * i, t = wide ? 0 : j * per16 >> 8, g = g0 + j - t * G;
         mine[i] = t < TT && g < G && t0 + t < a.Tq;
-        to[i] = codes + t * stride;
+        to[i] = t * stride + lr;
       }
       i32x4 qb[KB];
 #pragma unroll
@@ -429,16 +435,18 @@ __global__ __launch_bounds__(NW * 64) void paged_select_kernel(PagedSelect a, in
           if (p0 >= P) break;
           i32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < KB; ++i) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(qb[i], b[r].b[i], sum, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i >= values) break;
-            const uint32_t code = bound_code((float)sum[i] * b[r].scale);
-            if (mine[i] && b[r].in) {
-              if (G == 1) to[i][p0 + lr] = code;
-              else atomicMax(to[i] + p0 + lr, code);
-            }
+          for (int i = 0; i < KB; ++i) {
+            *(i32x4*)put = b[r].b[i];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // what other lanes of the wave wrote, in order
+            const i32x4 operand = *(const i32x4*)get;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(qb[i], operand, sum, 0, 0, 0);
           }
+          if (mine[0] && b[r].in) atomicMax(codes + to[0] + p0, bound_code((float)sum[0] * b[r].scale));
+          if (values > 1)
+#pragma unroll
+            for (int i = 1; i < 4; ++i)
+              if (mine[i] && b[r].in) atomicMax(codes + to[i] + p0, bound_code((float)sum[i] * b[r].scale));
           b[r].load(a, bounds, scales, page[r], p0 + NB * NW * 16 + lr, P);
           page[r] = tile_page(a, table, tile + 2 * NB * NW, lr);
         }
