@@ -261,10 +261,10 @@ void launch_bounds(const PagedBounds& a, int format, dim3 grid, hipStream_t stre
 // head of the group) pairs at a time on the 8-bit matrix unit, kept as ordered codes [TT][pages] in LDS (0: no such page); then
 // the K-th largest code of each query row by four 8-bit digits of a histogram, 16 / TT (4 / TT) waves a row; then the pages above it,
 // and the first ones equal to it, in order. Bound by its chain of loads and barriers (64 query rows of 704 pages: a few MB), so
-// the first tiles' table entries and bounds are on their way before the queries are looked at, the histograms of all
+// the first tile's table entries and bounds are on their way before the queries are looked at, the histograms of all
 // digits are cleared at once, every wave of a row finds the digit for itself (one barrier a digit), and there is little code:
-// most of it runs once, as fast as instructions come in (three tiles at a time instead of two: 10.0 us for 9.5). One row of 8
-// sequences of 704 pages and 8 heads takes 9.5 us, of which the digits take 1.7; 64 pages 7.2, 16 of 16, unscored, 3.3.
+// most of it runs once, as fast as instructions come in (two tiles of bounds on their way instead of one: 9.5 us for 9.1). One row of 8
+// sequences of 704 pages and 8 heads takes 9.1 us, of which the digits take 1.7; 64 pages 7.0, 16 of 16, unscored, 3.5.
 constexpr int PS_LDS = 32768;  // codes kept in LDS
 
 __device__ __forceinline__ uint32_t bound_code(float x) {  // larger bound, larger code; none is 0
@@ -285,7 +285,7 @@ __device__ __forceinline__ int tile_page(const PagedSelect& a, const int32_t* ta
   return p <= last ? id : -1;
 }
 // The bounds come in with four lanes side by side on 64 bytes of a page (16 lanes on 16 pages, as the operands lie, are 16 lines
-// of the cache for every 16 lanes: 8 heads of a sequence of 3,125 pages 22.8 us for 17.2) and are passed on through LDS.
+// of the cache for every 16 lanes: 8 heads of a sequence of 3,125 pages 22.8 us for 16.6) and are passed on through LDS.
 template <int KB>
 struct BoundTile {
   i32x4 b[KB];  // 16 bytes from 16 (lane % 4) on of each 64, of page lane / 4
@@ -319,26 +319,17 @@ __global__ __launch_bounds__(NW * 64) void paged_select_kernel(PagedSelect a, in
   int* hist = (int*)lds;
   const int64_t nh = (int64_t)n * c.H + h;
   uint32_t* codes = GLOBAL ? store + (nh * a.Tq + t0) * stride : lds + (1024 << tshift);
-  constexpr int NB = 2;
   const int8_t* bounds = a.bounds + h * (2 * D) + (lane & 3) * 16;
   // 64 bytes of a tile's pages in LDS, their sixteenths in an order by which neither side meets itself in a bank
   int8_t* const put = sh_b[wave] + (lane >> 2) * 64 + ((lane ^ lane >> 3) & 3) * 16;
   const int8_t* const get = sh_b[wave] + lr * 64 + ((lg ^ lr >> 1) & 3) * 16;
   const float* scales = a.bound_scales + h;
-  BoundTile<KB> b[NB];
-  int page[NB];  // of the tiles NB rounds later
-  auto pages = [&]() {
-#pragma unroll
-    for (int i = 0; i < NB; ++i) page[i] = tile_page(a, table, wave + i * NW, lr);
-  };
+  BoundTile<KB> b;
+  int page = c.max_pages > 0 ? tile_page(a, table, wave, lr) : -1;  // of the tile after b's
   auto first = [&]() {
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      b[i].load(a, bounds, scales, page[i], (wave + i * NW) * 16 + lr, P);
-      page[i] = tile_page(a, table, wave + (NB + i) * NW, lr);
-    }
+    b.load(a, bounds, scales, page, wave * 16 + lr, P);
+    page = tile_page(a, table, wave + NW, lr);
   };
-  if (c.max_pages > 0) pages();
   if (a.K < P) {
     first();
     // columns wave, wave + NW, ... of the queries: with up to 16 heads in the group (query row, head), else 16 heads at a time
@@ -422,34 +413,32 @@ __global__ __launch_bounds__(NW * 64) void paged_select_kernel(PagedSelect a, in
 #pragma unroll
       for (int i = 0; i < KB; ++i) qb[i] = *(const i32x4*)(&sh_q[lr][i * 64 + lg * 16]);
       if (g0 > 0) {
-        pages();
+        page = tile_page(a, table, wave, lr);
         first();
       }
-      // a tile's bounds are loaded while the one before is multiplied, the table's entries two tiles earlier (each in registers of
-      // its own: to pass a tile on would wait for it)
+      // a tile's bounds are on their way while the one before becomes codes, its table entries a tile earlier
 #pragma unroll 1
-      for (int tile0 = wave; tile0 * 16 < P; tile0 += NB * NW)
+      for (int tile = wave; tile * 16 < P; tile += NW) {
+        const int p0 = tile * 16;
+        i32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-        for (int r = 0; r < NB; ++r) {
-          const int tile = tile0 + r * NW, p0 = tile * 16;
-          if (p0 >= P) break;
-          i32x4 sum = {0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < KB; ++i) {
-            *(i32x4*)put = b[r].b[i];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // what other lanes of the wave wrote, in order
-            const i32x4 operand = *(const i32x4*)get;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(qb[i], operand, sum, 0, 0, 0);
-          }
-          if (mine[0] && b[r].in) atomicMax(codes + to[0] + p0, bound_code((float)sum[0] * b[r].scale));
-          if (values > 1)
-#pragma unroll
-            for (int i = 1; i < 4; ++i)
-              if (mine[i] && b[r].in) atomicMax(codes + to[i] + p0, bound_code((float)sum[i] * b[r].scale));
-          b[r].load(a, bounds, scales, page[r], p0 + NB * NW * 16 + lr, P);
-          page[r] = tile_page(a, table, tile + 2 * NB * NW, lr);
+        for (int i = 0; i < KB; ++i) {
+          *(i32x4*)put = b.b[i];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // what other lanes of the wave wrote, in order
+          const i32x4 operand = *(const i32x4*)get;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(qb[i], operand, sum, 0, 0, 0);
         }
+        const bool in = b.in;
+        const float scale = b.scale;
+        b.load(a, bounds, scales, page, p0 + NW * 16 + lr, P);
+        page = tile_page(a, table, tile + 2 * NW, lr);
+        if (mine[0] && in) atomicMax(codes + to[0] + p0, bound_code((float)sum[0] * scale));
+        if (values > 1)
+#pragma unroll
+          for (int i = 1; i < 4; ++i)
+            if (mine[i] && in) atomicMax(codes + to[i] + p0, bound_code((float)sum[i] * scale));
+      }
       __syncthreads();
     }
   } else {  // every page that is there, whatever its bound
