@@ -551,7 +551,7 @@ void launch_select(const PagedSelect& a, void* ws, hipStream_t stream) {
   (void)hipGetDevice(&dev);
   if (lds > 49152 && (dev < 0 || dev >= 64 || !set[dev])) {
     (void)hipFuncSetAttribute((const void*)paged_select_kernel<T, D, false, 16>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                              PS_LDS * 4 + 16384);
+                              PS_LDS * 4 + 4096);  // one row's codes and histograms; 20 KB more for the queries and bounds
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
   hipLaunchKernelGGL((paged_select_kernel<T, D, false, 16>), grid, nt, lds, stream, a, shift, per16, (uint32_t*)nullptr);

@@ -452,3 +452,14 @@ def test_select_every_page(dev, pages, K):
         want = torch.full((K,), -1, dtype=torch.int32)
         want[:len(there)] = there
         assert (got[i] == want).all()
+
+
+@pytest.mark.parametrize("pages", [32768, 15000])
+def test_select_of_many_wide_pages(dev, pages):
+    # the most LDS that a workgroup takes: all codes of the longest table beside the queries and bounds of 128 dims
+    g = torch.Generator(device=dev).manual_seed(pages)
+    table = torch.randperm(pages, generator=g, device=dev).to(torch.int32).view(1, -1)
+    n = torch.tensor([pages * 16 - 3], dtype=torch.int32, device=dev)
+    bnd = torch.randint(-20, 21, (pages, 1, 2, 128), generator=g, device=dev, dtype=torch.int8)
+    q = torch.randn(1, 2, 2, 128, generator=g, device=dev).to(BF)
+    _check_select(q, bnd, torch.ones(pages, 1, device=dev), table, n, 16, 100, "many wide pages")
