@@ -462,7 +462,7 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
   const int32_t* table = c.table + n * c.table_sn;
   // 64 page ids of the table at a time, one per lane; with a selection the rows that each has, for 8 bits its scales
   int pg0 = c0 >> c.shift, pg, has = 0;
-  float2 cs = make_float2(0.f, 0.f);
+  float2 cs;
   const int len = SEL ? __builtin_amdgcn_readfirstlane(pa_len(a, n)) : 0;
   auto pages = [&]() {
     if constexpr (!SEL) {
@@ -473,8 +473,11 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
       pg = in ? table[at] : -1;
       has = in ? len - (at << c.shift) : 0;
     }
-    if constexpr (Q8)
-      if (pg >= 0 && pg < c.pages) cs = *(const float2*)(a.scales + ((int64_t)pg * c.H + h) * 2);
+    if constexpr (Q8) {
+      // 0 for a page without rows: nobody may have written its scales, and the probabilities of its rows, 0, are multiplied by them
+      cs = make_float2(0.f, 0.f);
+      if (pg >= 0 && pg < c.pages && (!SEL || has > 0)) cs = *(const float2*)(a.scales + ((int64_t)pg * c.H + h) * 2);
+    }
   };
   pages();
   const int64_t head = (int64_t)h << c.shift;
