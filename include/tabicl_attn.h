@@ -507,7 +507,8 @@ int64_t tabicl_paged_sparse_attn_workspace_bytes(int64_t N, int64_t Hq, int64_t 
  * The books of a pool on the device. free_pages [pages]: a stack of page ids, *free_count of them, the top one last.
  *   tabicl_paged_reserve: pages for rows lengths[n] + t, t < count[n]: the table's entries from the first page behind row
  *     lengths[n] to that of the last new row that hold no page get the pages from the top of the stack, sequence by sequence and
- *     in order, as far as they go; granted[n] <- how many of the new rows have a place (before the first that has none).
+ *     in order, as far as they go; granted[n] <- how many of the new rows have a place (before the first that has none;
+ *     the page that row lengths[n] joins may be missing too).
  *   tabicl_paged_release: the pages behind row lengths[n] of each sequence back on the stack (the last sequence's last page first: a
  *     release of what a reserve gave out restores the stack), -1 in their place.
  *   tabicl_paged_slots: starts [N + 1] <- running sums of the counts; slots [total] <- for row j of a packed batch, t = j -

@@ -3,7 +3,8 @@
 // on the device, so that a step of a serving loop can be captured and replayed while the requests grow.
 //
 //   reserve: entries p of the table, ceil(len / R) <= p < ceil((len + count) / R), that hold no page get one: the r-th such
-//            entry (by sequence, then p) the r-th page from the top of the stack, as far as it goes
+//            entry (by sequence, then p) the r-th page from the top of the stack, as far as it goes; granted: the rows before
+//            the first without a page, none where row len joins a page (len / R, not among those) that is not there
 //   release: entries p >= ceil(len / R) that hold a page give it back and become -1: the last one first, so that a release
 //            undoes a reserve, stack and all
 //   slots:   row j of a packed batch, the t-th of sequence n: table[n, (len + t) / R] R + (len + t) % R, or -1
@@ -37,6 +38,11 @@ struct BookRange {
 };
 
 __device__ __forceinline__ bool book_has(const PagedBooks& a, int id) { return id >= 0 && id < a.pages; }
+
+// The page that row `len` of sequence n joins, 0 where it begins one.
+__device__ __forceinline__ int book_joins(const PagedBooks& a, int n, int64_t len) {
+  return len & ((1ll << a.shift) - 1) ? a.table[n * a.table_sn + (len >> a.shift)] : 0;
+}
 
 // need[n]: the entries of sequence n that get (or give back) a page; need[N]: the pages on the stack. A wave per sequence.
 template <bool RELEASE>
@@ -82,6 +88,7 @@ __global__ __launch_bounds__(256) void paged_books_kernel(PagedBooks a, const in
     const int mine = need[n];
     if ((n - n0) % 4 == wave) {
       const BookRange r(a, n, RELEASE);
+      const int joins = RELEASE ? 0 : book_joins(a, n, r.len);
       int64_t rank = before;
       int missing = a.max_pages;
       for (int p = r.first; p < r.last; p += 64) {
@@ -109,7 +116,7 @@ __global__ __launch_bounds__(256) void paged_books_kernel(PagedBooks a, const in
       }
       if (!RELEASE && lane == 0) {  // rows up to the first page that is not there
         const int64_t rows = ((int64_t)missing << a.shift) - r.len;
-        a.granted[n] = (int)(rows < 0 ? 0 : rows < r.add ? rows : r.add);
+        a.granted[n] = (int)(rows < 0 || !book_has(a, joins) ? 0 : rows < r.add ? rows : r.add);
       }
     }
     before += mine;
@@ -142,12 +149,13 @@ __global__ __launch_bounds__(PB_NW * 64) void paged_books_one_kernel(PagedBooks 
     *all = __builtin_amdgcn_readlane(waves, 63);
     return (wave ? __builtin_amdgcn_readlane(waves, wave - 1) : 0) + upto - x;
   };
-  int first = 0, last = 0, runs;
+  int first = 0, last = 0, runs, joins = 0;
   if (tid < a.N) {
     const BookRange r(a, tid, RELEASE);
     first = r.first, last = r.last > r.first ? r.last : r.first;
     rows[tid] = make_int2((int)r.len, (int)r.add);
     miss[tid] = a.max_pages;
+    if (!RELEASE) joins = book_joins(a, tid, r.len);
   }
   int at = before((last - first + 63) / 64, &runs);
 #pragma unroll 1
@@ -222,7 +230,7 @@ __global__ __launch_bounds__(PB_NW * 64) void paged_books_one_kernel(PagedBooks 
     __syncthreads();
     if (tid < a.N) {
       const int64_t there = ((int64_t)miss[tid] << a.shift) - rows[tid].x;
-      a.granted[tid] = (int)(there < 0 ? 0 : there < rows[tid].y ? there : rows[tid].y);
+      a.granted[tid] = (int)(there < 0 || !book_has(a, joins) ? 0 : there < rows[tid].y ? there : rows[tid].y);
     }
   }
   if (tid == 0) {

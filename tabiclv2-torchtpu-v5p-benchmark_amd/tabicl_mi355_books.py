@@ -68,7 +68,8 @@ def paged_reserve(table: Tensor, lengths: Tensor, count: Tensor, free: Tensor, f
     """Gives each request n pages for count[n] rows behind its lengths[n] (int32 [N] on the GPU): the entries of table
     [N, max_pages] from the first page behind row lengths[n] to that of the last new row that hold no page get pages from the top
     of the stack, request by request, as far as they go. Returns granted [N] int32: how many of the rows have a place (all,
-    or those before the first page that was not to be had). lengths and count stay as they are. In place: table, free_count."""
+    or those before the first page that was not to be had; none, where row lengths[n] joins a page that the table does not have).
+    lengths and count stay as they are. In place: table, free_count."""
     if _nat.direct(table, lengths, count, free, free_count):
         granted = None
         if _nat.DIRECT is not None:

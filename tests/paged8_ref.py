@@ -177,7 +177,7 @@ class Books:
             for p in span:
                 if not self.has(row[p]) and self.stack:
                     row[p] = self.stack.pop()
-            first = next((p for p in span if not self.has(row[p])), len(row))
+            first = next((p for p in range(length // self.R, span.stop) if not self.has(row[p])), len(row))
             granted.append(max(0, min(add, first * self.R - length)))
         return granted
 
