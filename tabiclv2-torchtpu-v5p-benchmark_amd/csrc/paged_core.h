@@ -356,7 +356,7 @@ __device__ __forceinline__ uint32_t pack_upper(float a, float b) {
 }
 
 // Eight fp32 values as the sum of N bf16 terms (the first ones cut, so that nothing is lost up to the last; it is rounded where
-// N < 3). The rest of an infinite value counts as 0.
+// N < 3). The rest of an infinite value is NaN.
 template <int N>
 __device__ __forceinline__ void bf16_terms(const float* x, bf16x8* term) {
   float r[8];
@@ -420,6 +420,9 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
 
   // this lane's query rows: 16 QT of the (head of the group, query row) pairs
   uint4 q[QT][NQ][NC];
+  auto row = [&](int r) { return (const char*)a.q + (n * a.q_sn + (h * G + r / Tn) * a.q_sh + (t0 + r % Tn) * a.q_st) * TS; };
+  auto dims = [&](int i) { return D == 32 ? lg * 8 : i / 2 * 64 + lg * 16 + i % 2 * 8; };  // Q8: as the chunks of a K row lie
+  float finite = 0.f;  // neither infinite nor NaN while no value is (fp32 queries over 8 bits)
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int r = (qt0 * QT + t) * 16 + lr;
@@ -428,19 +431,21 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
 #pragma unroll
       for (int i = 0; i < NC; ++i) q[t][j][i] = uint4{0, 0, 0, 0};
     if (r < rows) {
-      const char* qp = (const char*)a.q + (n * a.q_sn + (h * G + r / Tn) * a.q_sh + (t0 + r % Tn) * a.q_st) * TS;
+      const char* qp = row(r);
       if constexpr (!Q8) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) q[t][0][i] = ldg16(qp + lg * 16 + i * 64);
       } else {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-          const int dim = D == 32 ? lg * 8 : i / 2 * 64 + lg * 16 + i % 2 * 8;  // as the chunks of a K row lie
+          const int dim = dims(i);
           if constexpr (TS == 2) {
             q[t][0][i] = ldg16(qp + dim * 2);
           } else {
             const f32x4 x = *(const f32x4*)(qp + dim * 4), y = *(const f32x4*)(qp + dim * 4 + 16);
             const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) finite = __builtin_fmaf(v[e], v[e + 1], finite);
             bf16x8 term[3];
             bf16_terms<3>(v, term);
 #pragma unroll
@@ -655,6 +660,29 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
   if (key < c1) {
     Tile ta, tb;
     int la = fetch(ta, key);
+    // The first term of an infinite value is all of it: NaN from the others would hide scores of -inf, which take no part. Looked
+    // for in products of pairs, and behind the first loads, so that they need not wait for the queries (16 sequences of 501 to
+    // 10,001 rows 31.0 us as without it; 31.6 before the loads, or with a choice for each value).
+    if constexpr (NQ == 3)
+      if (wave_any(!(__builtin_fabsf(finite) < -TA_NEG_INF))) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const int r = (qt0 * QT + t) * 16 + lr;
+          if (r >= rows) continue;
+#pragma unroll
+          for (int i = 0; i < NC; ++i) {
+            const uint32_t* v = (const uint32_t*)(row(r) + dims(i) * 4);
+            uint32_t keep[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              keep[e] = ((v[2 * e] & 0x7fffffffu) == 0x7f800000u ? 0u : 0xffffu) | ((v[2 * e + 1] & 0x7fffffffu) == 0x7f800000u ? 0u : 0xffff0000u);
+#pragma unroll
+            for (int j = 1; j < NQ; ++j) {
+              q[t][j][i].x &= keep[0], q[t][j][i].y &= keep[1], q[t][j][i].z &= keep[2], q[t][j][i].w &= keep[3];
+            }
+          }
+        }
+      }
     for (; key < c1; key += 2 * NW * KS) {
       const int lb = fetch(tb, key + NW * KS);
       compute(ta, key, la);
