@@ -371,6 +371,9 @@ _DENSE_QUERY_ROWS, _DENSE_ALL_ROWS, _DENSE_SCORES = 256, 1024, 1 << 24
 # padded to its own longest one. us of all at once / in runs of 2 GiB / 1 GiB, T 384: 16 x 45,000 rows 1246 / 1243 / 1262, one
 # table of 50,000 rows beside 63 of 500 752 (6.3 GB) / 514 / 507, 40 of 100 to 20,000 763 / 713 / 829.
 _GATHER_BYTES = 2 << 30
+# What paged_select (query rows over sequences and K/V heads) and paged_sparse_attention (over sequences and query heads) take in a
+# call, and the bytes of the list of pages and of selection's workspace that a query over selected pages keeps at a time.
+_SELECT_ROWS, _SPARSE_ROWS, _SELECT_BYTES = 1 << 21, 1 << 22, 1 << 30
 
 
 class PagedIclKVCache(_icl.IclKVCache):
@@ -387,7 +390,7 @@ class PagedIclKVCache(_icl.IclKVCache):
     pages, heads, 2]; tabicl_mi355_paged8), appended in bf16 or fp32 and queried in either. Not with track.
 
     select=K: each query row of each head attends to the K pages of its table whose keys can give it the largest scores
-    (tabicl_mi355_sparse; all of them, where a table has no more), however many rows a query has. The bounds of the keys
+    (tabicl_mi355_sparse; all of them, where a table has no more), however many rows a query has (they go in slices). The bounds of the keys
     (`bounds`, `bound_scales`) follow the appends. Not with track.
 
     Pages are given out on the host; the page table and the lengths live on the GPU, so a query costs no host sync. Calls
@@ -580,9 +583,7 @@ class PagedIclKVCache(_icl.IclKVCache):
         if captured:
             w = self.table.shape[1]
         if self.select is not None and w > self.select:
-            q, table, eight = q.to(dt), self.table[:, :w], self._scales_of(block)
-            index = paged_select(q, self.bounds[block], self.bound_scales[block], table, lengths, self.page_rows, self.select)
-            return paged_sparse_attention(q, self.keys[block], self.values[block], table, lengths, index, None, out, **eight)
+            return self._selected(block, q.to(dt), self.table[:, :w], lengths, out)
         if not captured and q.shape[2] >= _DENSE_QUERY_ROWS and S * q.shape[2] >= _DENSE_ALL_ROWS \
                 and S * q.shape[2] * longest >= _DENSE_SCORES and D == 64 and q.shape[1] == H and dt == torch.bfloat16 \
                 and self.weights is None:
@@ -590,6 +591,31 @@ class PagedIclKVCache(_icl.IclKVCache):
         weights = None if self.weights is None else self.weights[:, :w * self.page_rows]
         return paged_attention(q.to(dt), self.keys[block], self.values[block], self.table[:, :w], lengths, weights, None, out,
                                **self._scales_of(block))
+
+    def _selected(self, block: int, q: Tensor, table: Tensor, lengths: Tensor, out: Optional[Tensor]) -> Tensor:
+        """query over selected pages, in slices of what the operators take at once and _SELECT_BYTES hold."""
+        (S, Hq, T, _), H = q.shape, self.keys.shape[2]
+        pairs = min(_SELECT_ROWS // H, _SPARSE_ROWS // Hq)  # (sequence, query row) pairs of a slice
+        if 4 * S * H * T * (self.select + table.shape[1]) > _SELECT_BYTES:
+            each = 4 * H * self.select + max(0, int(_nat.load().tabicl_paged_select_workspace_bytes(1, H, 1, table.shape[1])))
+            pairs = max(1, min(pairs, _SELECT_BYTES // each))
+        ns = min(S, max(1, pairs // max(1, T)))
+        nt = pairs // ns
+        whole = ns == S and nt >= T
+        if not whole:
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q = _apart(q, out)
+        for s in range(0, S, ns):
+            for t in range(0, max(1, T), nt):
+                part = q if whole else q[s:s + ns, :, t:t + nt]
+                to = out if whole else out[s:s + ns, :, t:t + nt]
+                index = paged_select(part, self.bounds[block], self.bound_scales[block], table[s:s + ns], lengths[s:s + ns],
+                                     self.page_rows, self.select)
+                to = paged_sparse_attention(part, self.keys[block], self.values[block], table[s:s + ns], lengths[s:s + ns], index, None,
+                                            to, **self._scales_of(block))
+                del index  # before the next slice's
+        return to if whole else out
 
     def _gathered(self, block: int, q: Tensor, lengths: Tensor, longest: int, out: Optional[Tensor]) -> Tensor:
         """query by the dense kernel, over the rows of one run of sequences after the other side by side."""

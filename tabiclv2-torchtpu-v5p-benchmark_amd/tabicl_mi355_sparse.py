@@ -132,7 +132,8 @@ def paged_select(q: Tensor, bounds: Tensor, bound_scales: Tensor, table: Tensor,
     """The `pages` pages of largest bound for each query row of q [N, Hq, Tq, D] (bf16 or fp32) and K/V head, as their places
     in the sequence's row of the table: int32 [N, H, Tq, pages], ascending, -1 behind the last (a sequence of fewer
     pages). Ties go to the lower page; pages that the pool has not got are not chosen. bounds, bound_scales: paged_bounds'.
-    The query heads of a group choose together, by the largest of their bounds. No gradient."""
+    The query heads of a group choose together, by the largest of their bounds. At most 2^21 query rows over all sequences and K/V
+    heads. No gradient."""
     if pages < 0:
         raise ValueError(f"pages must not be negative, got {pages}")
     if _nat.direct(q, bounds, bound_scales, table, lengths):
@@ -202,7 +203,8 @@ def paged_sparse_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: T
     """tabicl_mi355_paged.paged_attention of each query row and K/V head over the pages that index [N, H, Tq, pages] lists
     (paged_select's, or any other: places in the table in any order, entries outside of it are skipped, a page listed
     twice counts twice). Rows past a sequence's length, and pages that the pool has not got, hold nothing; a query row
-    without a row to attend to is 0. Every query row reads its own pages: for one query row to a few dozen. No gradient."""
+    without a row to attend to is 0. Every query row reads its own pages: for one query row to a few dozen (at most 2^22
+    over all sequences and query heads). No gradient."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, table, lengths, index, out, scales):
         if _nat.DIRECT is not None:
