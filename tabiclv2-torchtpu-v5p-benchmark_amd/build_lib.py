@@ -1,5 +1,7 @@
 """Builds libtabicl_attn.so (the C-ABI HIP library) for gfx950 with hipcc, and tabicl_mi355_direct.so (a Python module that
-makes the paged cache's calls of it, csrc/direct.cpp; host code alone) with g++, in-tree.
+makes the paged cache's calls of it, csrc/direct.cpp; host code alone) with g++, in-tree. The library needs neither torch nor
+Python; where these, their headers or g++ are missing, a warning says so and the module is left out (the wrappers call the library
+by ctypes then).
 
 Usage: python build_lib.py [-v]. Objects go to _build/ next to this file; the library is written
 next to this file, where tabicl_mi355_native.py loads it from.
@@ -10,6 +12,7 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import warnings
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -41,7 +44,7 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
         print(res.stderr, flush=True)
 
 
-def _direct(verbose: bool) -> None:
+def _direct(verbose: bool) -> Path:
     import sysconfig
 
     import torch
@@ -56,7 +59,7 @@ def _direct(verbose: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for direct.cpp:\n{res.stderr}")
-    os.replace(tmp, DIRECT)
+    return tmp
 
 
 def build(verbose: bool = False) -> Path:
@@ -64,7 +67,7 @@ def build(verbose: bool = False) -> Path:
     objs = [BUILD / (Path(s).stem + ".o") for s in SOURCES]
     with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
         futs = [ex.submit(_compile, CSRC / s, o, verbose) for s, o in zip(SOURCES, objs)]
-        futs.append(ex.submit(_direct, verbose))
+        direct = ex.submit(_direct, verbose)
         for f in futs:
             f.result()
     tmp = LIB.with_suffix(".so.tmp")
@@ -75,6 +78,11 @@ def build(verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
+    try:
+        os.replace(direct.result(), DIRECT)
+    except (ImportError, OSError, RuntimeError) as e:
+        DIRECT.unlink(missing_ok=True)  # one of another library would call it by other signatures
+        warnings.warn(f"{DIRECT.name} was not built, the paged cache's calls go by ctypes: {e}", RuntimeWarning)
     return LIB
 
 
