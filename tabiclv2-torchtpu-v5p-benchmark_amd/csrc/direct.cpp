@@ -131,6 +131,11 @@ at::Tensor workspace(int64_t bytes, const at::Tensor& like) {
   return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
 }
 void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// The interpreter's lock, let go over an allocation and a launch: either may wait for the GPU, and other threads go on meanwhile.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
 void* stream_arg(PyObject* o) { return PyLong_AsVoidPtr(o); }
 
 // attn(q, k_pages, v_pages, scales, table, lengths, out, index, scale, stream) -> out; index None: every page (8-bit pools)
@@ -159,34 +164,41 @@ PyObject* attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     index = (const int32_t*)x.data_ptr();
     K = x.size(3);
   }
-  at::Tensor made;
-  if (a[6] == Py_None) {
-    made = at::empty(q.sizes(), q.options());
-  } else {
+  const bool make = a[6] == Py_None;
+  if (!make) {
     if (!is_tensor(a[6])) Py_RETURN_NONE;
     const at::Tensor& o = T(a[6]);
-    if (o.dim() != 4 || o.sizes() != q.sizes() || o.scalar_type() != q.scalar_type() || o.storage().data() == q.storage().data())
+    if (o.dim() != 4 || o.sizes() != q.sizes() || o.scalar_type() != q.scalar_type() || o.storage().data() == q.storage().data() ||
+        !ro.read(o, t.dev) || (t.N > 1 && !ro.n) || (Hq > 1 && !ro.h) || (Tq > 1 && !ro.r))
       Py_RETURN_NONE;
   }
-  const at::Tensor& o = made.defined() ? made : T(a[6]);
-  if (!ro.read(o, t.dev) || (t.N > 1 && !ro.n) || (Hq > 1 && !ro.h) || (Tq > 1 && !ro.r)) Py_RETURN_NONE;
   const float scale = (float)PyFloat_AsDouble(a[8]);
   void* stream = stream_arg(a[9]);
   if (PyErr_Occurred()) return nullptr;
   const int64_t bytes = a[7] != Py_None ? lib.sparse_ws(t.N, Hq, p.H, Tq, p.D, K * p.R)
                                         : lib.attn_q8_ws(t.N, Hq, p.H, Tq, p.D, t.M * p.R, dt);
   if (bytes < 0) Py_RETURN_NONE;
-  const at::Tensor ws = workspace(bytes, q);
-  const int st =
-      a[7] != Py_None
-          ? lib.sparse(q.data_ptr(), k.data_ptr(), v.data_ptr(), scales, p.P, p.sp, p.R, t.p, t.sn, t.M,
-                       (const int32_t*)lengths.data_ptr(), index, K, o.data_ptr(), t.N, Hq, p.H, Tq, p.D, rq.n, rq.h, rq.r, ro.n, ro.h,
-                       ro.r, scale, dt, p.format, pointer(ws), bytes, stream)
-          : lib.attn_q8(q.data_ptr(), k.data_ptr(), v.data_ptr(), scales, p.P, p.sp, p.R, t.p, t.sn, t.M,
-                        (const int32_t*)lengths.data_ptr(), o.data_ptr(), t.N, Hq, p.H, Tq, p.D, rq.n, rq.h, rq.r, ro.n, ro.h, ro.r,
-                        scale, dt, p.format - 2, pointer(ws), bytes, stream);
+  const bool listed = a[7] != Py_None;
+  at::Tensor o, ws;
+  if (!make) o = T(a[6]);
+  int st;
+  {
+    Unlocked u;
+    if (make) {
+      o = at::empty(q.sizes(), q.options());
+      ro.read(o, t.dev);
+    }
+    ws = workspace(bytes, q);
+    st = listed
+             ? lib.sparse(q.data_ptr(), k.data_ptr(), v.data_ptr(), scales, p.P, p.sp, p.R, t.p, t.sn, t.M,
+                          (const int32_t*)lengths.data_ptr(), index, K, o.data_ptr(), t.N, Hq, p.H, Tq, p.D, rq.n, rq.h, rq.r, ro.n, ro.h,
+                          ro.r, scale, dt, p.format, pointer(ws), bytes, stream)
+             : lib.attn_q8(q.data_ptr(), k.data_ptr(), v.data_ptr(), scales, p.P, p.sp, p.R, t.p, t.sn, t.M,
+                          (const int32_t*)lengths.data_ptr(), o.data_ptr(), t.N, Hq, p.H, Tq, p.D, rq.n, rq.h, rq.r, ro.n, ro.h, ro.r,
+                          scale, dt, p.format - 2, pointer(ws), bytes, stream);
+  }
   if (st) Py_RETURN_NONE;
-  if (made.defined()) return THPVariable_Wrap(made);
+  if (make) return THPVariable_Wrap(o);
   Py_INCREF(a[6]);
   return a[6];
   END_HANDLE_TH_ERRORS
@@ -214,10 +226,14 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   void* stream = stream_arg(a[8]);
   if (PyErr_Occurred()) return nullptr;
-  if (lib.append_q8(kp.data_ptr(), vp.data_ptr(), (float*)scales, p.P, p.sp, p.R, t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(),
-                    k.data_ptr(), v.data_ptr(), count, nullptr, t.N, p.H, k.size(2), p.D, rk.n, rk.h, rk.r, rv.n, rv.h, rv.r, dt,
-                    p.format - 2, stream))
-    Py_RETURN_NONE;
+  int st;
+  {
+    Unlocked u;
+    st = lib.append_q8(kp.data_ptr(), vp.data_ptr(), (float*)scales, p.P, p.sp, p.R, t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(),
+                       k.data_ptr(), v.data_ptr(), count, nullptr, t.N, p.H, k.size(2), p.D, rk.n, rk.h, rk.r, rv.n, rv.h, rv.r, dt,
+                       p.format - 2, stream);
+  }
+  if (st) Py_RETURN_NONE;
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -238,10 +254,15 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   if (rows < 0) Py_RETURN_NONE;
   const auto options = kp.options().dtype(dt ? at::kFloat : at::kBFloat16);
-  const at::Tensor k = at::empty({t.N, p.H, rows, p.D}, options), v = at::empty({t.N, p.H, rows, p.D}, options);
-  if (lib.gather_q8(kp.data_ptr(), vp.data_ptr(), scales, p.P, p.sp, p.R, t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(),
-                    k.data_ptr(), v.data_ptr(), t.N, p.H, rows, p.D, dt, p.format - 2, stream))
-    Py_RETURN_NONE;
+  at::Tensor k, v;
+  int st;
+  {
+    Unlocked u;
+    k = at::empty({t.N, p.H, rows, p.D}, options), v = at::empty({t.N, p.H, rows, p.D}, options);
+    st = lib.gather_q8(kp.data_ptr(), vp.data_ptr(), scales, p.P, p.sp, p.R, t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(),
+                       k.data_ptr(), v.data_ptr(), t.N, p.H, rows, p.D, dt, p.format - 2, stream);
+  }
+  if (st) Py_RETURN_NONE;
   return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
   END_HANDLE_TH_ERRORS
 }
@@ -274,9 +295,13 @@ PyObject* bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyErr_Clear();  // a number beyond 64 bits
     Py_RETURN_NONE;
   }
-  if (lib.bounds(kp.data_ptr(), scales, p.P, p.sp, p.R, t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(), start,
-                 rows < most ? rows : most, (int8_t*)b.data_ptr(), (float*)s.data_ptr(), t.N, p.H, p.D, p.format, stream))
-    Py_RETURN_NONE;
+  int st;
+  {
+    Unlocked u;
+    st = lib.bounds(kp.data_ptr(), scales, p.P, p.sp, p.R, t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(), start,
+                    rows < most ? rows : most, (int8_t*)b.data_ptr(), (float*)s.data_ptr(), t.N, p.H, p.D, p.format, stream);
+  }
+  if (st) Py_RETURN_NONE;
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -298,11 +323,16 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   const int64_t Hq = q.size(1), Tq = q.size(2), bytes = lib.select_ws(t.N, H, Tq, t.M);
   if (bytes < 0) Py_RETURN_NONE;
-  const at::Tensor index = at::empty({t.N, H, Tq, K}, q.options().dtype(at::kInt)), ws = workspace(bytes, q);
-  if (lib.select(q.data_ptr(), (const int8_t*)b.data_ptr(), (const float*)s.data_ptr(), P, R, t.p, t.sn, t.M,
-                 (const int32_t*)lengths.data_ptr(), (int32_t*)index.data_ptr(), K, t.N, Hq, H, Tq, D, rq.n, rq.h, rq.r, dt, pointer(ws),
-                 bytes, stream))
-    Py_RETURN_NONE;
+  at::Tensor index, ws;
+  int st;
+  {
+    Unlocked u;
+    index = at::empty({t.N, H, Tq, K}, q.options().dtype(at::kInt)), ws = workspace(bytes, q);
+    st = lib.select(q.data_ptr(), (const int8_t*)b.data_ptr(), (const float*)s.data_ptr(), P, R, t.p, t.sn, t.M,
+                    (const int32_t*)lengths.data_ptr(), (int32_t*)index.data_ptr(), K, t.N, Hq, H, Tq, D, rq.n, rq.h, rq.r, dt, pointer(ws),
+                    bytes, stream);
+  }
+  if (st) Py_RETURN_NONE;
   return THPVariable_Wrap(index);
   END_HANDLE_TH_ERRORS
 }
@@ -323,11 +353,16 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = stream_arg(a[6]);
   if (PyErr_Occurred()) return nullptr;
   if (bytes < 0) Py_RETURN_NONE;
-  const at::Tensor granted = at::empty({t.N}, lengths.options()), ws = workspace(bytes, lengths);
-  if (lib.reserve((int32_t*)t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(), (const int32_t*)count.data_ptr(),
-                  (const int32_t*)f.data_ptr(), (int32_t*)c.data_ptr(), (int32_t*)granted.data_ptr(), f.size(0), R, t.N, pointer(ws), bytes,
-                  stream))
-    Py_RETURN_NONE;
+  at::Tensor granted, ws;
+  int st;
+  {
+    Unlocked u;
+    granted = at::empty({t.N}, lengths.options()), ws = workspace(bytes, lengths);
+    st = lib.reserve((int32_t*)t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(), (const int32_t*)count.data_ptr(),
+                     (const int32_t*)f.data_ptr(), (int32_t*)c.data_ptr(), (int32_t*)granted.data_ptr(), f.size(0), R, t.N, pointer(ws),
+                     bytes, stream);
+  }
+  if (st) Py_RETURN_NONE;
   return THPVariable_Wrap(granted);
   END_HANDLE_TH_ERRORS
 }
@@ -343,10 +378,15 @@ PyObject* release(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = stream_arg(a[5]);
   if (PyErr_Occurred()) return nullptr;
   if (bytes < 0) Py_RETURN_NONE;
-  const at::Tensor ws = workspace(bytes, lengths);
-  if (lib.release((int32_t*)t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(), (int32_t*)f.data_ptr(), (int32_t*)c.data_ptr(), f.size(0), R,
-                  t.N, pointer(ws), bytes, stream))
-    Py_RETURN_NONE;
+  at::Tensor ws;
+  int st;
+  {
+    Unlocked u;
+    ws = workspace(bytes, lengths);
+    st = lib.release((int32_t*)t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(), (int32_t*)f.data_ptr(), (int32_t*)c.data_ptr(),
+                     f.size(0), R, t.N, pointer(ws), bytes, stream);
+  }
+  if (st) Py_RETURN_NONE;
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -362,10 +402,15 @@ PyObject* slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = stream_arg(a[6]);
   if (PyErr_Occurred()) return nullptr;
   if (total < 0) Py_RETURN_NONE;
-  const at::Tensor out = at::empty({total}, lengths.options().dtype(at::kLong)), starts = at::empty({t.N + 1}, lengths.options());
-  if (lib.slots(t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(), (const int32_t*)count.data_ptr(), (int64_t*)out.data_ptr(),
-                (int32_t*)starts.data_ptr(), total, pages, R, t.N, stream))
-    Py_RETURN_NONE;
+  at::Tensor out, starts;
+  int st;
+  {
+    Unlocked u;
+    out = at::empty({total}, lengths.options().dtype(at::kLong)), starts = at::empty({t.N + 1}, lengths.options());
+    st = lib.slots(t.p, t.sn, t.M, (const int32_t*)lengths.data_ptr(), (const int32_t*)count.data_ptr(), (int64_t*)out.data_ptr(),
+                   (int32_t*)starts.data_ptr(), total, pages, R, t.N, stream);
+  }
+  if (st) Py_RETURN_NONE;
   return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(starts));
   END_HANDLE_TH_ERRORS
 }
@@ -393,9 +438,13 @@ PyObject* append_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   void* stream = stream_arg(a[5]);
   if (PyErr_Occurred()) return nullptr;
-  if (lib.append_slots(kp.data_ptr(), vp.data_ptr(), p.P, p.sp, p.R, (const int64_t*)s.data_ptr(), k.data_ptr(), v.data_ptr(), k.size(0),
-                       p.H, p.D, st[0][0], st[0][1], st[1][0], st[1][1], p.format, stream))
-    Py_RETURN_NONE;
+  int done;
+  {
+    Unlocked u;
+    done = lib.append_slots(kp.data_ptr(), vp.data_ptr(), p.P, p.sp, p.R, (const int64_t*)s.data_ptr(), k.data_ptr(), v.data_ptr(),
+                            k.size(0), p.H, p.D, st[0][0], st[0][1], st[1][0], st[1][1], p.format, stream);
+  }
+  if (done) Py_RETURN_NONE;
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
