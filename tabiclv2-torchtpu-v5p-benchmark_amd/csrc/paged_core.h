@@ -396,8 +396,8 @@ __device__ __forceinline__ void store_row(T* p, const float* x) {
 
 // Rows [c0, c1) of an item (query tile qt0 of K/V head h of sequence n) by the NW waves of a workgroup: the output, or
 // (slot >= 0) a partial of it. SEL: the rows of the pages that `index` lists for query row t0, R for each of its entries;
-// the query rows are those of the group's heads.
-template <typename T, typename C, int D, int QT, bool W, bool SEL, int NW>
+// the query rows are those of the group's heads. ONCE: nothing reads these rows again.
+template <typename T, typename C, int D, int QT, bool W, bool SEL, int NW, bool ONCE>
 __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit& z, int n, int h, int t0, int qt0, int c0, int c1,
                                            int slot, const int32_t* index = nullptr) {
   typedef typename PagedTileOf<T, C, D>::type Tile;
@@ -405,10 +405,10 @@ __device__ __forceinline__ void pa_segment(const PagedAttn& a, const PagedSplit&
   constexpr bool Q8 = sizeof(C) == 1;
   constexpr int SUB = Tile::SUB, KS = Tile::KS, NC = Tile::NC, DE = Tile::DE, ES = sizeof(C), TS = sizeof(T);
   constexpr int NQ = Q8 ? (TS == 2 ? 1 : 3) : 1, NP = TS == 2 ? 2 : 3;  // bf16 terms of q and of p, where C has 8 bits
-  // Rows in 8 bits of up to 64 dims that one tile of query rows reads are loaded past the caches (one row over 8 x 45,000 rows 76 ->
-  // 68 us, 16 fp32 rows over 8 x 5,000 17.8 -> 16.5; a second tile would have to go to memory again, 64 query rows 120 -> 127, and
-  // so would the second half of a row of 128 dims).
-  constexpr int POLICY = (Q8 && !SEL && QT <= 2 && D <= 64) ? 2 : 0;
+  // Rows in 8 bits of up to 64 dims that one tile of query rows reads are loaded past the caches (from them / past them: one row over
+  // 8 x 45,000 rows 72.8 / 66.7 us, 32 fp32 rows 104.3 / 101.9; a second tile would have to go to memory again, 64 fp32 rows 187 / 195,
+  // 200 over 8 x 5,000 80 / 87, over 64 x 300 66 / 73, and so would the second half of a row of 128 dims).
+  constexpr int POLICY = ONCE ? 2 : 0;
   __shared__ float sh_o[NW / 2][16 * QT][D + 4];
   __shared__ float2 sh_ml[NW / 2][16 * QT];
   const PagedPool& c = a.pool;
@@ -827,7 +827,7 @@ template <typename T, typename C>
 constexpr int pa_waves_of(int D, int QT) { return sizeof(C) > 1 ? pa_waves(D, QT) : D == 128 && QT > 1 && sizeof(T) == 4 ? 1 : 2; }
 
 // Equal shares of all items' units.
-template <typename T, typename C, int D, int QT, bool W>
+template <typename T, typename C, int D, int QT, bool W, bool ONCE = false>
 __global__ __launch_bounds__(256, (pa_waves_of<T, C>(D, QT))) void pa_kernel(PagedAttn a, PagedSplit z) {
   const int per = a.pool.H * z.qtiles;
   PagedUnits units(a, per, threadIdx.x & 63);
@@ -844,19 +844,19 @@ __global__ __launch_bounds__(256, (pa_waves_of<T, C>(D, QT))) void pa_kernel(Pag
     const int u1 = u0 + end - unit < each ? u0 + end - unit : each;
     if (threadIdx.x == 0 && u0 == 0) z.ends[n * per + item].x = blockIdx.x;
     if (threadIdx.x == 0 && u1 == each) z.ends[n * per + item].y = blockIdx.x;
-    pa_segment<T, C, D, QT, W, false, 4>(a, z, n, item / z.qtiles, 0, item % z.qtiles, u0 * PA_UNIT < len ? u0 * PA_UNIT : len,
-                                         u1 * PA_UNIT < len ? u1 * PA_UNIT : len,
-                                         u1 - u0 < each ? 2 * blockIdx.x + (u0 == 0) : -1);
+    pa_segment<T, C, D, QT, W, false, 4, ONCE>(a, z, n, item / z.qtiles, 0, item % z.qtiles, u0 * PA_UNIT < len ? u0 * PA_UNIT : len,
+                                               u1 * PA_UNIT < len ? u1 * PA_UNIT : len,
+                                               u1 - u0 < each ? 2 * blockIdx.x + (u0 == 0) : -1);
     unit += u1 - u0;
   }
 }
 
 // A workgroup of NW waves for each item, where no sequence is long.
-template <typename T, typename C, int D, int QT, bool W, int NW = 8>
+template <typename T, typename C, int D, int QT, bool W, int NW = 8, bool ONCE = false>
 __global__ __launch_bounds__(64 * NW, 2) void pa_whole_kernel(PagedAttn a, PagedSplit z) {
   const int per = a.pool.H * z.qtiles, n = blockIdx.x / per, item = blockIdx.x % per;
-  pa_segment<T, C, D, QT, W, false, NW>(a, z, n, item / z.qtiles, 0, item % z.qtiles, 0,
-                                       __builtin_amdgcn_readfirstlane(pa_len(a, n)), -1);
+  pa_segment<T, C, D, QT, W, false, NW, ONCE>(a, z, n, item / z.qtiles, 0, item % z.qtiles, 0,
+                                             __builtin_amdgcn_readfirstlane(pa_len(a, n)), -1);
 }
 
 template <typename T, typename C, int D, int QT>

@@ -281,7 +281,8 @@ __global__ __launch_bounds__(256) void paged_gather8_kernel(PagedGather a, const
 // attention: the kernels of paged_core.h; the codes become bf16 operands in the registers (exactly), K's scale goes into the
 // scores and V's into the probabilities. fp32 queries and probabilities enter as three bf16 terms: nothing of them is lost.
 // ---------------------------------------------------------------------------------------------
-template <typename T, typename C, int D, int QT>
+// ONCE: the query rows are one tile.
+template <typename T, typename C, int D, int QT, bool ONCE>
 int64_t run_pa8(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, hipStream_t stream) {
   const int64_t qrows = Hq / H * Tq;
   PagedSplit z = {};
@@ -308,16 +309,24 @@ int64_t run_pa8(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, 
     const int64_t items = N * H * z.qtiles;
     const dim3 grid((unsigned)items);
     if constexpr (waves == 2) {
-      if (rows <= 256) hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 2>), grid, dim3(128), 0, stream, *a, z);
+      if (rows <= 256) hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 2, ONCE>), grid, dim3(128), 0, stream, *a, z);
       else if (rows <= 512 || items > cu_count())
-        hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 4>), grid, dim3(256), 0, stream, *a, z);
-      else hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 8>), grid, dim3(512), 0, stream, *a, z);
+        hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 4, ONCE>), grid, dim3(256), 0, stream, *a, z);
+      else hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 8, ONCE>), grid, dim3(512), 0, stream, *a, z);
     }
   } else {
-    hipLaunchKernelGGL((pa_kernel<T, C, D, QT, false>), dim3((unsigned)z.groups), dim3(256), 0, stream, *a, z);
+    hipLaunchKernelGGL((pa_kernel<T, C, D, QT, false, ONCE>), dim3((unsigned)z.groups), dim3(256), 0, stream, *a, z);
     hipLaunchKernelGGL((pa_merge_kernel<T, C, D, QT>), dim3((unsigned)((N * Hq * Tq + 3) / 4)), dim3(256), 0, stream, *a, z);
   }
   return at;
+}
+
+// Tiles of 16 QT query rows; a single one in the form that loads past the caches.
+template <typename T, typename C, int D, int QT>
+int64_t run_pa8_tiles(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, hipStream_t stream) {
+  if constexpr (D <= 64 && QT <= 2)
+    if (Hq / H * Tq <= 16 * QT) return run_pa8<T, C, D, QT, true>(a, ws, N, Hq, H, Tq, rows, stream);
+  return run_pa8<T, C, D, QT, false>(a, ws, N, Hq, H, Tq, rows, stream);
 }
 
 template <typename T, typename C, int D>
@@ -333,9 +342,9 @@ int64_t run_pa8_rows(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_
     return qrows > 16 * qt && (rows > PA_WHOLE || N * H * ((qrows + 16 * qt - 1) / (16 * qt)) > 2 * cu_count());
   };
   if constexpr (most == 4)
-    if (wider(1) && wider(2)) return run_pa8<T, C, D, 4>(a, ws, N, Hq, H, Tq, rows, stream);
-  if ((rows > PA_WHOLE || pa_waves_of<T, C>(D, 2) == 2) && wider(1)) return run_pa8<T, C, D, 2>(a, ws, N, Hq, H, Tq, rows, stream);
-  return run_pa8<T, C, D, 1>(a, ws, N, Hq, H, Tq, rows, stream);
+    if (wider(1) && wider(2)) return run_pa8_tiles<T, C, D, 4>(a, ws, N, Hq, H, Tq, rows, stream);
+  if ((rows > PA_WHOLE || pa_waves_of<T, C>(D, 2) == 2) && wider(1)) return run_pa8_tiles<T, C, D, 2>(a, ws, N, Hq, H, Tq, rows, stream);
+  return run_pa8_tiles<T, C, D, 1>(a, ws, N, Hq, H, Tq, rows, stream);
 }
 
 // The query rows in slices of what a launch counts, one after the other over one workspace.

@@ -573,8 +573,8 @@ __global__ __launch_bounds__(64 * NW, 2) void ps_kernel(PagedAttn a, PagedSplit 
   const int qt = (int)(item % z.qtiles), t = (int)(item / z.qtiles % a.Tq), nh = (int)(item / z.qtiles / a.Tq);
   const int64_t all = (int64_t)a.K << a.pool.shift, c0 = (int64_t)part * chunk;
   const int c1 = (int)(c0 + chunk < all ? c0 + chunk : all);
-  pa_segment<T, C, D, 1, false, true, NW>(a, z, nh / a.pool.H, nh % a.pool.H, t, qt, (int)(c0 < all ? c0 : all), c1,
-                                         splits > 1 ? b : -1, a.index + ((int64_t)nh * a.Tq + t) * a.K);
+  pa_segment<T, C, D, 1, false, true, NW, false>(a, z, nh / a.pool.H, nh % a.pool.H, t, qt, (int)(c0 < all ? c0 : all), c1,
+                                                splits > 1 ? b : -1, a.index + ((int64_t)nh * a.Tq + t) * a.K);
 }
 
 // A wave joins a query row's partials.
