@@ -281,6 +281,10 @@ __global__ __launch_bounds__(256) void paged_gather8_kernel(PagedGather a, const
 // attention: the kernels of paged_core.h; the codes become bf16 operands in the registers (exactly), K's scale goes into the
 // scores and V's into the probabilities. fp32 queries and probabilities enter as three bf16 terms: nothing of them is lost.
 // ---------------------------------------------------------------------------------------------
+// The widest tile of query rows, in sixteens.
+template <typename T>
+constexpr int pa8_most(int D) { return sizeof(T) == 4 || D == 128 ? 2 : 4; }
+
 // ONCE: the query rows are one tile.
 template <typename T, typename C, int D, int QT, bool ONCE>
 int64_t run_pa8(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t rows, hipStream_t stream) {
@@ -288,7 +292,8 @@ int64_t run_pa8(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, 
   PagedSplit z = {};
   z.qtiles = (int)((qrows + 16 * QT - 1) / (16 * QT));
   constexpr int waves = pa_waves_of<T, C>(D, QT);
-  z.groups = rows <= PA_WHOLE && waves == 2 ? 0 : waves * cu_count();
+  constexpr bool splits = ONCE || D == 128 || QT == pa8_most<T>(D);  // several narrow tiles: over short caches alone
+  z.groups = !splits || (rows <= PA_WHOLE && waves == 2) ? 0 : waves * cu_count();
   z.least = 2;
   z.few = D > 32 && waves == 2 ? 12 * z.groups : 0;
   int64_t at = 0;
@@ -314,7 +319,7 @@ int64_t run_pa8(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_t H, 
         hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 4, ONCE>), grid, dim3(256), 0, stream, *a, z);
       else hipLaunchKernelGGL((pa_whole_kernel<T, C, D, QT, false, 8, ONCE>), grid, dim3(512), 0, stream, *a, z);
     }
-  } else {
+  } else if constexpr (splits) {
     hipLaunchKernelGGL((pa_kernel<T, C, D, QT, false, ONCE>), dim3((unsigned)z.groups), dim3(256), 0, stream, *a, z);
     hipLaunchKernelGGL((pa_merge_kernel<T, C, D, QT>), dim3((unsigned)((N * Hq * Tq + 3) / 4)), dim3(256), 0, stream, *a, z);
   }
@@ -337,7 +342,7 @@ int64_t run_pa8_rows(const PagedAttn* a, void* ws, int64_t N, int64_t Hq, int64_
   // 64: 64 query rows over 48 x 6,239 rows and 2 heads of 128 dims 97 / 66 / -, in fp32 104 / 83 / -, in fp32 of 64 dims 63 / 50 /
   // 71). Up to PA_WHOLE rows only as far as the items fill the chip (64 dims, bf16: 64 rows over 8 x 300 6.9 / 8.5 / 11.9, 200 over
   // 57 x 1,000 and 2 heads 35 / 30 / 27, 64 over 256 x 300 77 / 54 / 50).
-  constexpr int most = sizeof(T) == 4 || D == 128 ? 2 : 4;
+  constexpr int most = pa8_most<T>(D);
   auto wider = [&](int qt) {  // than 16 qt rows
     return qrows > 16 * qt && (rows > PA_WHOLE || N * H * ((qrows + 16 * qt - 1) / (16 * qt)) > 2 * cu_count());
   };
