@@ -444,7 +444,8 @@ int64_t tabicl_paged_evict_workspace_bytes(int64_t N, int64_t K);
 #define TABICL_CODE_I8 1
 
 /* tabicl_paged_attn over such a pool, without weights; the products are exact (fp32 queries and probabilities enter as three
- * bf16 terms), the sums fp32. Any finite scales will do. */
+ * bf16 terms), the sums fp32. Scales need not be powers of two; those of V from 2^-80 on (below, the least probabilities meet the
+ * end of fp32's range: the products with V take 2^-24 of them). Scales of pages without rows are not read into the result. */
 int tabicl_paged_attn_q8(const void* q, const void* k_pages, const void* v_pages, const float* scales, int64_t pages,
                          int64_t page_sp, int64_t page_rows, const int32_t* table, int64_t table_sn, int64_t max_pages,
                          const int32_t* lengths, void* out, int64_t N, int64_t Hq, int64_t H, int64_t Tq, int64_t D, int64_t q_sn,

@@ -263,8 +263,9 @@ void launch_bounds(const PagedBounds& a, int format, dim3 grid, hipStream_t stre
 // and the first ones equal to it, in order. Bound by its chain of loads and barriers (64 query rows of 704 pages: a few MB), so
 // the first tile's table entries and bounds are on their way before the queries are looked at, the histograms of all
 // digits are cleared at once, every wave of a row finds the digit for itself (one barrier a digit), and there is little code:
-// most of it runs once, as fast as instructions come in (two tiles of bounds on their way instead of one: 9.5 us for 9.1). One row of 8
-// sequences of 704 pages and 8 heads takes 9.1 us, of which the digits take 1.7; 64 pages 7.0, 16 of 16, unscored, 3.5.
+// most of it runs once, as fast as instructions come in (two tiles of bounds on their way instead of one: 0.4 us more). One row of 8
+// sequences of 704 pages and 8 heads takes 8.4 us call after call in a graph (10.3 between other kernels, which leave it neither the
+// bounds nor its code in the caches), of which the digits take 1.7; 64 pages 6.3, 16 of 16, unscored, 2.5.
 constexpr int PS_LDS = 32768;  // codes kept in LDS
 
 __device__ __forceinline__ uint32_t bound_code(float x) {  // larger bound, larger code; none is 0

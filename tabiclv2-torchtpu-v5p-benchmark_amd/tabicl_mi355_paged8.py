@@ -5,7 +5,9 @@ when they are given scales (ops tabicl::paged_attn_q8, paged_attn_q8_out, paged_
 A scale is a power of two, the smallest 2^k (k in [-60, 100]) with max |x| <= Q 2^k, Q = 448 (e4m3) or 127 (int8). Rows that
 join a page of smaller scale raise it, and the codes that the page holds are rounded to the new step: at most once per
 doubling. Values are bf16 numbers, so a gather in bf16 is exact. e4m3 keeps four significant bits of each value, int8 seven
-of the largest value of a page and head, which is more for values of one size. No counterpart in the reference."""
+of the largest value of a page and head (a power of two as the scale may leave one of them unused), which is more for values of one
+size: outputs over 5,000 normal rows are off by 3 to 8 % of their size in e4m3 and 1.4 to 2.7 % in int8, by as much and 9 to 35 %
+where every sixteenth dim is 16 times as large. No counterpart in the reference."""
 from __future__ import annotations
 
 from typing import Optional
