@@ -36,12 +36,7 @@ from tabicl_mi355_books import paged_append_packed, paged_release, paged_reserve
 from tabicl_mi355_sparse import paged_bounds, paged_select, paged_sparse_attention  # noqa: F401
 
 
-_rows16, _apart, _no_grad, _fwd_level = _pool.rows16, _pool.apart, _pool.no_grad, _pool.fwd_level
-
-
-def _pool_args(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, lead: int = 0):
-    """tabicl_mi355_pool.pool_args, then the dtype code of a bf16 or fp32 pool."""
-    return *_pool.pool_args(k_pages, v_pages, table, lengths, lead), _nat.dtype_code(k_pages.dtype)
+_rows16, _apart, _no_grad, _fwd_level, _pool_args = _pool.rows16, _pool.apart, _pool.no_grad, _pool.fwd_level, _pool.pool_args
 
 
 def _check_weights(weights: Tensor, N: int, cap: int, dev: int) -> int:
@@ -69,7 +64,8 @@ def _ws_bytes(key: tuple, N: int, Hq: int, H: int, Tq: int, D: int, rows: int, w
 
 def _attn_launch(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Optional[Tensor],
                  scale: float, out: Tensor) -> None:
-    pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths)
+    pool, H, D, N, dev = _pool_args(k_pages, v_pages, table, lengths)
+    code = _pool.dense_code(k_pages.dtype)
     shape = q.shape
     if len(shape) != 4 or shape[0] != N or shape[3] != D or shape[1] % max(1, H):
         raise ValueError(f"q must be [{N}, a multiple of {H} heads, Tq, {D}], got {tuple(shape)}")
@@ -159,7 +155,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
 
     scales (fp32 [pages, H, 2]): the pool holds e4m3 or int8 codes (tabicl_mi355_paged8). q is bf16 or fp32 then; the products
     are exact, the sums fp32 (bf16 probabilities take part as two bf16 terms, fp32 ones as three). No weights."""
-    if scales is not None or k_pages.dtype in _pool.CODES:
+    if scales is not None:
         return _p8.attention(q, k_pages, v_pages, table, lengths, weights, scale, out, scales)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, table, lengths, weights, out):
@@ -183,7 +179,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
 
 def _append_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: Tensor, v: Tensor,
                    count: Optional[Tensor]) -> None:
-    pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths)
+    pool, H, D, N, dev = _pool_args(k_pages, v_pages, table, lengths)
+    code = _pool.dense_code(k_pages.dtype)
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or shape[0] != N or shape[1] != H or shape[3] != D:
         raise ValueError(f"k and v must be [{N}, {H}, T, {D}], got {tuple(shape)} and {tuple(v.shape)}")
@@ -228,7 +225,7 @@ def paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tenso
     scales (fp32 [pages, H, 2], written too): the pool holds e4m3 or int8 codes; k and v are bf16 or fp32. A page that rows
     join keeps the larger of its scale and theirs, and the codes it holds are rounded again where it grows; infinities saturate,
     NaN stays NaN in e4m3 and becomes 0 in int8."""
-    if scales is not None or k_pages.dtype in _pool.CODES:
+    if scales is not None:
         _p8.append(k_pages, v_pages, table, lengths, k, v, count, None, scales)
     elif _nat.direct(k_pages, v_pages, table, lengths, k, v, count):
         _append_launch(k_pages, v_pages, table, lengths, k, v, count)
@@ -239,7 +236,8 @@ def paged_append(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tenso
 
 
 def _gather_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, k: Tensor, v: Tensor) -> None:
-    pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths)
+    pool, H, D, N, dev = _pool_args(k_pages, v_pages, table, lengths)
+    code = _pool.dense_code(k_pages.dtype)
     if dev != torch.cuda.current_device() if dev >= 0 else True:
         _nat.require_device(k_pages)
         with torch.cuda.device(dev):
@@ -287,7 +285,8 @@ def paged_gather(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tenso
 
 def _evict_launch(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Tensor, keep: int,
                   recent: int, keep_n: Optional[Tensor], index: Tensor, kept_weights: Tensor, kept: Tensor) -> None:
-    pool, H, D, N, dev, code = _pool_args(k_pages, v_pages, table, lengths, 1)
+    pool, H, D, N, dev = _pool_args(k_pages, v_pages, table, lengths, 1)
+    code = _nat.dtype_code(k_pages.dtype)
     w_sn = _check_weights(weights, N, pool[2] * pool[5], dev)
     if keep < 0 or recent < 0:
         raise ValueError(f"keep and recent must not be negative, got {keep} and {recent}")

@@ -64,12 +64,10 @@ def _(q, k_pages, v_pages, scales, table, lengths, scale, out):  # noqa: ANN001
 
 
 def attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, weights: Optional[Tensor],
-              scale: Optional[float], out: Optional[Tensor], scales: Optional[Tensor]) -> Tensor:
+              scale: Optional[float], out: Optional[Tensor], scales: Tensor) -> Tensor:
     """tabicl_mi355_paged.paged_attention of a pool of 8-bit codes."""
     if weights is not None:
         raise ValueError("paged_attention over 8-bit codes adds up no weights")
-    if scales is None:
-        raise ValueError("a pool of 8-bit codes needs its scales [pages, H, 2]")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _nat.direct(q, k_pages, v_pages, scales, table, lengths, out):
         if _nat.DIRECT is not None:

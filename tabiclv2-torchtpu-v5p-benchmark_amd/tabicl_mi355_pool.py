@@ -56,11 +56,25 @@ def pool_args(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, 
         raise ValueError("a page [H, page_rows, D] must be contiguous")
     if k_pages.dtype is not v_pages.dtype:
         raise ValueError("k_pages and v_pages must share a dtype")
-    t, N = table_args(table, lengths)
+    ts = table.shape  # table_args' checks in place: a call of it takes as long as half of the checks here
+    if table.dtype is not torch.int32 or len(ts) != 2 or (table.stride(1) != 1 and ts[1] > 1):
+        raise ValueError("table must be an int32 [N, max_pages] tensor with contiguous rows")
+    N, M = ts
+    if lengths.dtype is not torch.int32 or lengths.shape != (N,) or (N > 1 and lengths.stride(0) != 1):
+        raise ValueError(f"lengths must be a contiguous int32 tensor of {N} entries")
     dev = k_pages.get_device()
     if v_pages.get_device() != dev or table.get_device() != dev or lengths.get_device() != dev:
         raise ValueError("the pool, table and lengths must be on one device")
-    return (P, st[lead] if P > 1 else H * R * D, R, *t), H, D, N, dev
+    return (P, st[lead] if P > 1 else H * R * D, R, table.data_ptr(), table.stride(0) if N > 1 else M, M), H, D, N, dev
+
+
+def dense_code(dtype: torch.dtype) -> int:
+    """The library's code of a bf16 or fp32 pool."""
+    if dtype is torch.bfloat16:
+        return _nat.DTYPE_BF16
+    if dtype in CODES:
+        raise ValueError("a pool of 8-bit codes needs its scales [pages, H, 2]")
+    return _nat.dtype_code(dtype)
 
 
 def check_scales(scales: Optional[Tensor], P: int, H: int, dev: int) -> None:
