@@ -584,7 +584,10 @@ class PagedIclKVCache(_icl.IclKVCache):
         if captured:
             w = self.table.shape[1]
         if self.select is not None and w > self.select:
-            return self._selected(block, q.to(dt), self.table[:, :w], lengths, out)
+            q, table, n = q.to(dt), self.table[:, :w], q.numel()
+            if n > 32 * _SELECT_ROWS or n > 32 * _SPARSE_ROWS or n * (self.select + w) > 8 * _SELECT_BYTES:  # n: 32 a query row at least
+                return self._selected_in_slices(block, q, table, lengths, out)
+            return self._selected(block, q, table, lengths, out)
         if not captured and q.shape[2] >= _DENSE_QUERY_ROWS and S * q.shape[2] >= _DENSE_ALL_ROWS \
                 and S * q.shape[2] * longest >= _DENSE_SCORES and D == 64 and q.shape[1] == H and dt == torch.bfloat16 \
                 and self.weights is None:
@@ -594,29 +597,26 @@ class PagedIclKVCache(_icl.IclKVCache):
                                **self._scales_of(block))
 
     def _selected(self, block: int, q: Tensor, table: Tensor, lengths: Tensor, out: Optional[Tensor]) -> Tensor:
-        """query over selected pages, in slices of what the operators take at once and _SELECT_BYTES hold."""
+        """query over selected pages."""
+        eight = self._scales_of(block)
+        index = paged_select(q, self.bounds[block], self.bound_scales[block], table, lengths, self.page_rows, self.select)
+        return paged_sparse_attention(q, self.keys[block], self.values[block], table, lengths, index, None, out, **eight)
+
+    def _selected_in_slices(self, block: int, q: Tensor, table: Tensor, lengths: Tensor, out: Optional[Tensor]) -> Tensor:
+        """_selected, as much at a time as the operators take and _SELECT_BYTES hold: runs of sequences, of one sequence runs of
+        query rows."""
         (S, Hq, T, _), H = q.shape, self.keys.shape[2]
-        pairs = min(_SELECT_ROWS // H, _SPARSE_ROWS // Hq)  # (sequence, query row) pairs of a slice
-        if 4 * S * H * T * (self.select + table.shape[1]) > _SELECT_BYTES:
-            each = 4 * H * self.select + max(0, int(_nat.load().tabicl_paged_select_workspace_bytes(1, H, 1, table.shape[1])))
-            pairs = max(1, min(pairs, _SELECT_BYTES // each))
-        ns = min(S, max(1, pairs // max(1, T)))
+        each = 4 * H * self.select + max(0, int(_nat.load().tabicl_paged_select_workspace_bytes(1, H, 1, table.shape[1])))
+        pairs = max(1, min(_SELECT_ROWS // H, _SPARSE_ROWS // Hq, _SELECT_BYTES // each))  # (sequence, query row) pairs of a slice
+        ns = min(S, max(1, pairs // T))
         nt = pairs // ns
-        whole = ns == S and nt >= T
-        if not whole:
-            if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            q = _apart(q, out)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q = _apart(q, out)
         for s in range(0, S, ns):
-            for t in range(0, max(1, T), nt):
-                part = q if whole else q[s:s + ns, :, t:t + nt]
-                to = out if whole else out[s:s + ns, :, t:t + nt]
-                index = paged_select(part, self.bounds[block], self.bound_scales[block], table[s:s + ns], lengths[s:s + ns],
-                                     self.page_rows, self.select)
-                to = paged_sparse_attention(part, self.keys[block], self.values[block], table[s:s + ns], lengths[s:s + ns], index, None,
-                                            to, **self._scales_of(block))
-                del index  # before the next slice's
-        return to if whole else out
+            for t in range(0, T, nt):
+                self._selected(block, q[s:s + ns, :, t:t + nt], table[s:s + ns], lengths[s:s + ns], out[s:s + ns, :, t:t + nt])
+        return out
 
     def _gathered(self, block: int, q: Tensor, lengths: Tensor, longest: int, out: Optional[Tensor]) -> Tensor:
         """query by the dense kernel, over the rows of one run of sequences after the other side by side."""
