@@ -1,113 +1,87 @@
-"""GPU tests of the native module that makes the paged cache's short calls: it makes them (a wrapper goes on in Python, with the same
-result, where it does not), and other threads run while a call waits for the GPU."""
-import ctypes
-import subprocess
-import threading
-import time
-
+"""The wrappers' direct launches (tabicl_mi355_native.direct): taken for plain GPU tensors, left to the
+torch.library op wherever something watches or transforms op calls, with the same bits either way."""
 import pytest
 import torch
-
-from test_gpu_books import _books
+from torch.utils._python_dispatch import TorchDispatchMode
 
 pytestmark = pytest.mark.gpu
-BF, F32, E4, I8, I32 = torch.bfloat16, torch.float32, torch.float8_e4m3fn, torch.int8, torch.int32
 
 
-def _calls(dev, code):
-    """{what: a call by the public functions} of each function of the module over a pool of `code`."""
-    import tabicl_mi355_paged as paged
-    table, n, free, fc, _ = _books(dev, 3, [50, 300, 0, 17], 40, 16, spare=90)
-    P, H, D, R = free.numel(), 2, 64, 16
-    eight = code in (E4, I8)
-    kp, vp = (torch.zeros(P, H, R, D, device=dev).to(code) for _ in range(2))
-    scales = torch.ones(P, H, 2, device=dev) if eight else None
-    count = torch.tensor([20, 100, 33, 1], dtype=I32, device=dev)
-    dtype = BF if eight else code
-    x = torch.ones(160, H, D, dtype=dtype, device=dev)
-    slots, starts = paged.paged_slots(table, n, count, 160, P, R)
-    bnd, bs = torch.zeros(P, H, 2, D, dtype=I8, device=dev), torch.zeros(P, H, device=dev)
-    q = torch.ones(4, 2 * H, 3, D, dtype=dtype, device=dev)
-    out = torch.empty(4, 3, 2 * H, D, dtype=dtype, device=dev).transpose(1, 2)
-    index = torch.zeros(4, H, 3, 2, dtype=I32, device=dev)
-    calls = {"reserve": lambda: paged.paged_reserve(table, n, count, free, fc, R),
-             "slots": lambda: paged.paged_slots(table, n, count, 160, P, R),
-             "release": lambda: paged.paged_release(table, n, free, fc, R),
-             "bounds": lambda: paged.paged_bounds(kp, table, n, bnd, bs, scales=scales),
-             "bounds of part": lambda: paged.paged_bounds(kp, table, n, bnd, bs, n - 1, 9, scales),
-             "select": lambda: paged.paged_select(q, bnd, bs, table, n, R, 5),
-             "attn": lambda: paged.paged_sparse_attention(q, kp, vp, table, n, index, scales=scales),
-             "attn into out": lambda: paged.paged_sparse_attention(q, kp, vp, table, n, index, 0.3, out, scales)}
-    if not eight:
-        calls["append_slots"] = lambda: paged.paged_append_packed(kp, vp, table, n, count, x, x, slots, starts)
-        return calls
-    more = torch.ones(4, H, 2, D, device=dev)
-    calls.update({"attn of all pages": lambda: paged.paged_attention(q.float(), kp, vp, table, n, scales=scales),
-                  "append": lambda: paged.paged_append(kp, vp, table, n, more, more, scales=scales),
-                  "append with counts": lambda: paged.paged_append(kp, vp, table, n, more, more, count, scales),
-                  "gather": lambda: paged.paged_gather(kp, vp, table, n, 33, scales=scales),
-                  "gather in fp32": lambda: paged.paged_gather(kp, vp, table, n, 33, scales, F32)})
-    return calls
+class _Seen(TorchDispatchMode):
+    """Records the op calls it sees."""
+
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(str(func))
+        return func(*args, **(kwargs or {}))
 
 
-@pytest.mark.parametrize("code", [BF, F32, E4, I8], ids=["bf16", "fp32", "e4m3", "int8"])
-def test_module_makes_the_calls(dev, monkeypatch, code):
-    import tabicl_mi355_native as nat
-    nat.load()
-    real, seen = nat.DIRECT, []
+def _calls(dev):
+    import tabicl_mi355_attn as pk
+    import tabicl_mi355_icl as icl
+    from query_ref import Rope
+    g = torch.Generator(device=dev).manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev).to(torch.bfloat16)  # noqa: E731
+    q, kv, qkv, x, ind = r(3, 40, 128), r(3, 200, 256), r(3, 24, 384), r(3, 300, 128), r(16, 128)
+    kb = torch.zeros(24, device=dev)
+    kb[20:] = -1e30
+    iq, ik, iv = r(2, 8, 30, 64), r(2, 8, 100, 64), r(2, 8, 100, 64)
+    rope = Rope()
+    valid = torch.tensor(150, device=dev)
+    return {
+        "hx_fwd": lambda: pk.hx_attention(q, kv[..., :128], kv[..., 128:], 8),
+        "hxq_fwd": lambda: pk.hxq_attention(q, kv, valid, 8),
+        "pk_self_fwd": lambda: pk.pk_self_attention(qkv, 8, kb, rope, 0.25),
+        "pk_cross_fwd": lambda: pk.pk_cross_attention(q, kv, 8, None, None, 0.25),
+        "hxf_fwd": lambda: pk.hxf_attention(ind, x, 250),
+        "icl_cached_attn": lambda: icl.icl_sdpa(iq, ik, iv, 90),
+    }
 
-    class Recorder:
-        def __getattr__(self, name):
-            def call(*a):
-                r = getattr(real, name)(*a)
-                seen.append((name, r is not None))
-                return r
-            return call
 
-    calls = _calls(dev, code)
-    monkeypatch.setattr(nat, "DIRECT", Recorder())
-    for what, call in calls.items():
-        seen.clear()
-        call()
+def test_direct_equals_op_and_modes_see_the_op(dev):
+    for name, call in _calls(dev).items():
+        print(f"[direct] {name}", flush=True)
+        out = call()
+        with _Seen() as seen:
+            want = call()
         torch.cuda.synchronize()
-        assert seen == [(what.split()[0], True)], (what, seen)
+        assert any(name in n for n in seen.names), (name, seen.names)
+        assert torch.equal(out, want), name
 
 
-def test_other_threads_run_meanwhile(dev, tmp_path):
-    # stand-ins for the library's functions that sleep without the interpreter: a thread counts on all the while
+def test_direct_conditions(dev):
     import tabicl_mi355_native as nat
-    lib = nat.load()
-    src, so = tmp_path / "sleep.c", tmp_path / "sleep.so"
-    src.write_text("#include <unistd.h>\nlong none(void) { return 0; }\nint pause_(void) { usleep(200000); return 0; }\n")
-    subprocess.run(["gcc", "-shared", "-fPIC", str(src), "-o", str(so)], check=True)
-    fake = ctypes.CDLL(str(so))
-    at = {f: ctypes.cast(getattr(fake, f), ctypes.c_void_p).value for f in ("none", "pause_")}
-    calls = {**_calls(dev, BF), **_calls(dev, I8)}
-    for call in calls.values():  # whatever is built on a first call
-        call()
-    torch.cuda.synchronize()
-    ticks, stop = [0], threading.Event()
+    t = torch.zeros(2, device=dev)
+    w = torch.zeros(2, device=dev, requires_grad=True)
+    assert nat.direct(t, None)
+    assert not nat.direct(t, w)
+    assert not nat.direct(t, torch.zeros(2))
+    with torch.no_grad():
+        assert nat.direct(t, w)
+    seen = []
+    torch.func.vmap(lambda a: (seen.append(nat.direct(a)), a)[1])(t)
+    torch.func.grad(lambda a: (seen.append(nat.direct(a)), a.sum())[1])(t)
+    with torch.autograd.forward_ad.dual_level():
+        seen.append(nat.direct(t))
+    with torch.device("cuda"):  # a function mode
+        seen.append(nat.direct(t))
+    torch.jit.trace(lambda a: (seen.append(nat.direct(a)), a + 1)[1], t, check_trace=False)
+    assert seen and not any(seen), seen
+    assert nat.direct(t)
 
-    def count():
-        while not stop.is_set():
-            ticks[0] += 1
-            time.sleep(0.002)
 
-    thread = threading.Thread(target=count)
-    try:
-        nat.DIRECT.bind({name: at["none" if name.endswith("_bytes") else "pause_"] for name in nat.SIGNATURES})
-        thread.start()
-        for what, call in calls.items():
-            before, t0 = ticks[0], time.monotonic()
-            call()
-            took = time.monotonic() - t0
-            assert took >= 0.2, (what, took)
-            assert ticks[0] - before >= 5, what
-    finally:
-        stop.set()
-        nat._bind_direct(lib)
-        if thread.is_alive():
-            thread.join()
-    for call in calls.values():
-        call()
+def test_query_out_bumps_version(dev):
+    # the direct launch writes `out` as the op does: autograd's version check sees it
+    import tabicl_mi355_icl as icl
+    cache = icl.IclKVCache(1, 1, 8, 64, 64, torch.bfloat16, dev)
+    k = torch.randn(1, 8, 64, 64, device=dev).to(torch.bfloat16)
+    cache.append(0, k, k)
+    out = torch.empty(1, 8, 10, 64, dtype=torch.bfloat16, device=dev)
+    v0 = out._version
+    with torch.no_grad():
+        cache.query(0, k[:, :, :10], out=out)
     torch.cuda.synchronize()
+    assert out._version > v0
